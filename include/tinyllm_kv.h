@@ -172,6 +172,22 @@ int tl_kv_batch_attention(tl_kv_batch *batch, int layer, const void *q, void *ou
  * attended = write position + 1, in one stream-ordered call. */
 int tl_kv_batch_decode(tl_kv_batch *batch, int layer, const void *q, const void *new_k,
                        const void *new_v, void *out, float scale, void *stream);
+/* tl_kv_batch_decode (new_k and new_v null: tl_kv_batch_attention) that also
+ * keeps account of the cached tokens' attention weights (build addition):
+ *   weights_out[slot][g][t] = (weights_in ? weights_in[slot][g][t] : 0)
+ *                             + sum over the query heads h of kv head g of
+ *                               softmax_t(scale * q_h . k_t)
+ * for every attended token t of the batch's sequences; the token that this step
+ * appends (the last one after prepare) starts from zero, and all else of
+ * weights_out stays as it is.  fp32 [max_batch_size][num_heads][max_seq_len], by
+ * slot (tl_kv_slot_of) and cache index, the caller's, one per layer; weights_out
+ * may be weights_in and must not overlap it otherwise.  q, out, new_k and new_v
+ * 16-byte aligned.  K and V are read once.  The outputs follow the same formula
+ * as tl_kv_batch_decode, not its bits.  The scores pass through a workspace of the
+ * batch, which the first call of a size allocates: one such call before a
+ * captured one, and one batch is used from one stream at a time. */
+int tl_kv_batch_decode_weights(tl_kv_batch *batch, int layer, const void *q, const void *new_k, const void *new_v,
+                               void *out, float scale, const float *weights_in, float *weights_out, void *stream);
 /* Gather of the attended tokens into compact head-major layout (the K/V
  * layout attention_decode reads, kernels/attention.cuh:10-13):
  * k_out/v_out are [n][num_heads][s_max][head_dim]; tokens at or beyond a
@@ -295,6 +311,83 @@ int  tl_kv_prefill_attention(tl_kv_prefill *p, int layer, const void *q, void *o
 int  tl_kv_prefill_run(tl_kv_prefill *p, int layer, const void *q, const void *new_k,
                        const void *new_v, void *out, float scale, void *stream);
 int  tl_kv_prefill_commit(tl_kv_prefill *p);
+/* The account of the step's attention weights (see tl_kv_batch_decode_weights, the
+ * same arrays), by the last min(window, num_tokens[i]) new tokens of each
+ * sequence, window 0 meaning all of them; causal, the new tokens' keys already in
+ * the cache (append or run):
+ *   weights_out[slot][g][t] = (weights_in and t < getSeqLen ? weights_in[slot][g][t] : 0)
+ *                             + sum over those tokens j and the query heads h of
+ *                               kv head g of softmax_t(scale * q_hj . k_t)
+ * for every t < getSeqLen + num_tokens[i]; all else stays.  q as for attention,
+ * 16-byte aligned.  Outputs are not computed.  The workspace rule of
+ * tl_kv_batch_decode_weights holds. */
+int  tl_kv_prefill_weights(tl_kv_prefill *p, int layer, const void *q, float scale, int window,
+                           const float *weights_in, float *weights_out, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Eviction from the cache by accumulated attention weight (build addition: the
+ * reference's caches only grow, src/kv_cache.cpp:240-259).  Accounts of the
+ * cached tokens' attention weights come from tl_kv_batch_decode_weights and
+ * tl_kv_prefill_weights.  An eviction is one step over all layers:
+ *   prepare: of seq_ids[i] (distinct, live) every kv head keeps
+ *            min(tl_kv_seq_len, budgets[i]) tokens, budgets[i] >= 1: those whose
+ *            position is among the `recent` newest (0 <= recent <= every
+ *            budget), and of the rest those with the largest account (equal
+ *            ones: the lower cache index; NaN counts as the smallest);
+ *   run:     one layer.  Kept tokens below the budget stay in place; the kept
+ *            ones behind it move, in order, to the indices that became free.
+ *            weights and positions: [max_batch_size][num_heads][max_seq_len]
+ *            fp32 / int32, by slot (tl_kv_slot_of) and cache index, the caller's,
+ *            one pair per layer.  Written are the first min(length, budget) of
+ *            each kv head; outputs may be the inputs, and must not overlap
+ *            them otherwise.  positions_in is read only below the length that
+ *            the sequence's last eviction left (the tokens after that came in
+ *            order), so it needs no initial value.  A layer that ran in place is
+ *            not run again before commit;
+ *   commit:  when every layer has run: the sequences are as long as what they
+ *            kept, and a block pool gets the blocks behind it back.  Other
+ *            batches must be prepared again.  Nothing changes when it fails.
+ * head_dim in {32, 64, 128, 256}.  Everything a launch needs travels in its
+ * arguments; the selection's lists are in a workspace of the batch, sized by
+ * prepare, so one batch is used from one stream at a time. */
+typedef struct tl_kv_evict tl_kv_evict;
+int  tl_kv_evict_create(tl_kv_manager *mgr, int max_seqs, tl_kv_evict **out);
+void tl_kv_evict_destroy(tl_kv_evict *e);
+int  tl_kv_evict_prepare(tl_kv_evict *e, const int *seq_ids, const int *budgets, int n, int recent, void *stream);
+/* Sequences of the last prepare, and tokens (per layer and kv head) that its commit evicts. */
+int  tl_kv_evict_info(const tl_kv_evict *e, int *n, long long *evicted);
+int  tl_kv_evict_run(tl_kv_evict *e, int layer, const float *weights_in, float *weights_out,
+                     const int32_t *positions_in, int32_t *positions_out, void *stream);
+int  tl_kv_evict_commit(tl_kv_evict *e);
+/* Tokens of the sequence that evictions took so far: its next token has position
+ * tl_kv_seq_len + tl_kv_evicted.  0 for an unknown sequence. */
+int tl_kv_evicted(const tl_kv_manager *mgr, int seq_id);
+
+/* ------------------------------------------------------------------------
+ * Attention to cached states of another sequence (build addition: the reference
+ * is decoder-only): query tokens over an encoder's states, or over a document that
+ * several sequences share.  The states are a sequence of the manager like any
+ * other, appended once (tl_kv_append or tl_kv_prefill_append, then
+ * tl_kv_advance).
+ *   prepare:   entry i has num_queries[i] >= 1 query tokens, every one of which
+ *              attends to the first attended[i] tokens of seq_ids[i] (0 <=
+ *              attended[i] <= tl_kv_seq_len, the rest is padding; attended NULL:
+ *              all of them).  seq_ids may repeat: several entries, the same states;
+ *   attention: q/out [T][num_q_heads][head_dim] fp16, the entries' tokens back to
+ *              back, T = the sum of num_queries; 16-byte aligned.  Query head h
+ *              reads kv head h / (num_q_heads / num_heads), softmax with
+ *              1/(sum+1e-6), fp32 accumulation; a query over no states gets zeros.
+ * num_q_heads / num_heads in {1,2,4,8}; head_dim in {32,64,128,256}.  Partial
+ * results pass through a workspace of the batch, which the first call of a size
+ * allocates: one such call before a captured one, and one batch is used from
+ * one stream at a time. */
+typedef struct tl_kv_cross tl_kv_cross;
+int  tl_kv_cross_create(tl_kv_manager *mgr, int max_entries, int num_q_heads, tl_kv_cross **out);
+void tl_kv_cross_destroy(tl_kv_cross *c);
+int  tl_kv_cross_prepare(tl_kv_cross *c, const int *seq_ids, const int *num_queries, const int *attended, int n,
+                         void *stream);
+int  tl_kv_cross_info(const tl_kv_cross *c, int *n, int *tokens);
+int  tl_kv_cross_attention(tl_kv_cross *c, int layer, const void *q, void *out, float scale, void *stream);
 
 /* Waves per prefill-attention workgroup, process-wide: 0 = auto, 4 or 8
  * (8: one 256-row workgroup per CU; 4: two 128-row workgroups per CU, one's
@@ -463,7 +556,8 @@ int tl_fill_normal_f16(uint64_t seed, uint64_t first, float stddev, void *out, s
  * include/tiny_llm/cuda_streams.h:67-99).  When enabled, every launch of the
  * named kernels is bracketed by hipEvents on its own stream.
  * Names: "attn_chunk", "attn_merge", "kv_append", "kv_gather", "w8a16"
- * (the W8A16 GEMM kernel), "w8a16_reduce" (its split-K reduction).
+ * (the W8A16 GEMM kernel), "w8a16_reduce" (its split-K reduction),
+ * "attn_prefill", "kv_evict", "attn_stream", "attn_account".
  * ---------------------------------------------------------------------- */
 void tl_profile_enable(int on);
 void tl_profile_reset(void);

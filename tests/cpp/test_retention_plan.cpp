@@ -1,0 +1,144 @@
+// How the work of the account and cross attention kernels is cut
+// (tiny-llm_amd/csrc/stream_plan.cpp), and the block allocator's shrink, on random
+// and extreme inputs under the address and undefined-behaviour sanitizers (built by
+// tests/test_retention_cpu.py with g++, no GPU).
+#include "block_allocator.h"
+#include "stream_plan.h"
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <set>
+#include <vector>
+
+using namespace tiny_llm::detail;
+
+#define CHECK(c)                                                                                                       \
+    do {                                                                                                               \
+        if (!(c)) {                                                                                                    \
+            std::fprintf(stderr, "check failed: %s (%s:%d)\n", #c, __FILE__, __LINE__);                              \
+            std::abort();                                                                                              \
+        }                                                                                                              \
+    } while (0)
+
+static void stream_random() {
+    std::mt19937_64 rng(1);
+    for (int it = 0; it < 500; ++it) {
+        StreamPlan p;
+        const int  n = (int)(rng() % 400), most = 1 << (rng() % 17);
+        for (int i = 0; i < n; ++i) p.entries.push_back({i, rng() % 9 ? (int32_t)(rng() % most) : 0, i, 1, -1, -1});
+        if (it % 50 == 0 && n) p.entries[0].S = INT32_MAX;
+        plan_stream(p, 1 << (rng() % 6), 1 + (int)(rng() % 300));
+        CHECK(p.chunk >= 4);
+        size_t next = 0;
+        for (const auto &l : p.launches) {
+            CHECK((size_t)l.first == next && l.n > 0 && l.n <= kStreamBatch);
+            int     items = 0, longest = 0, most_items = 0;
+            int64_t tiles = 0;
+            for (int i = l.first; i < l.first + l.n; ++i) {
+                const StreamEntry &e = p.entries[(size_t)i];
+                const int          t = stream_tiles(e.S), k = stream_items(e.S, p.chunk);
+                CHECK(e.item0 == items && e.tile0 == tiles);
+                CHECK((int64_t)t * kStreamTile >= e.S && (int64_t)(t - 1) * kStreamTile < e.S);
+                CHECK((k == 0) == (e.S == 0));
+                // the kernel's chunks: every tile once, none empty
+                int64_t at = 0;
+                for (int c = 0; c < std::min(k, 50); ++c) {
+                    const int64_t lo = (int64_t)c * t / k, hi = (int64_t)(c + 1) * t / k;
+                    CHECK(lo == at && hi > lo && hi - lo <= p.chunk);
+                    at = hi;
+                }
+                if (k <= 50) CHECK(at == t);
+                items += k;
+                tiles += t;
+                longest = std::max(longest, (int)e.S);
+                most_items = std::max(most_items, k);
+            }
+            // the kernel's search: the last entry that starts at or before the item
+            for (int item = 0; item < std::min(items, 200); ++item) {
+                int found = -1;
+                for (int j = l.first; j < l.first + l.n; ++j)
+                    if (p.entries[(size_t)j].item0 <= item) found = j;
+                const StreamEntry &e = p.entries[(size_t)found];
+                CHECK(item - e.item0 >= 0 && item - e.item0 < stream_items(e.S, p.chunk));
+            }
+            CHECK(l.items == items && l.tiles == tiles && l.max_len == longest && l.max_items == most_items);
+            next += (size_t)l.n;
+        }
+        CHECK(next == p.entries.size());
+    }
+    std::puts("ok stream_random");
+}
+
+static void account_random() {
+    std::mt19937_64 rng(2);
+    for (int it = 0; it < 500; ++it) {
+        AccountPlan p;
+        const int   n = (int)(rng() % 250), most = 1 << (rng() % 14), G = 1 << (rng() % 4);
+        for (int i = 0; i < n; ++i) {
+            const int nt = 1 + (int)(rng() % most), w = rng() % 2 ? nt : 1 + (int)(rng() % nt);
+            p.entries.push_back({i, (int32_t)(rng() % most), nt, w, 0, -1, -1, -1, -1});
+        }
+        CHECK(plan_account(p, G, 1 << (rng() % 6), 1 + (int)(rng() % 300)));
+        size_t next = 0;
+        for (const auto &l : p.launches) {
+            CHECK((size_t)l.first == next && l.n > 0 && l.n <= kAccountBatch);
+            int64_t items = 0, sums = 0, stats = 0;
+            for (int i = l.first; i < l.first + l.n; ++i) {
+                const AccountEntry &e = p.entries[(size_t)i];
+                CHECK(e.item0 == items && e.sum0 == sums && e.stat0 == stats);
+                CHECK(e.nch >= 1 && e.nch <= std::max(1, stream_tiles(e.p0 + e.n)));
+                items += ((int64_t)e.w * G + kAccountRows - 1) / kAccountRows * e.nch;
+                sums += (e.p0 + e.n + kAccountKeys - 1) / kAccountKeys;
+                stats += (int64_t)e.w * G * e.nch;
+            }
+            CHECK(l.items == items && l.sums == sums && l.stats == stats);
+            next += (size_t)l.n;
+        }
+        CHECK(next == p.entries.size());
+    }
+    AccountPlan big; // statistics that do not fit 31 bits
+    for (int i = 0; i < 5; ++i) big.entries.push_back({i, 0, 1 << 26, 1 << 26, 0, 0, 0, 0, 0});
+    CHECK(!plan_account(big, 8, 8, 256));
+    std::puts("ok account_random");
+}
+
+static void allocator_shrink() {
+    std::mt19937_64 rng(3);
+    BlockAllocator  a(5, 9, 20);
+    for (int it = 0; it < 4000; ++it) {
+        const int row = (int)(rng() % 7) - 1, k = (int)(rng() % 11) - 1;
+        const int had = row >= 0 && row < 5 ? a.mapped(row) : 0, free_before = a.freeBlocks();
+        if (rng() % 2) {
+            a.shrink(row, k);
+            const bool acts = row >= 0 && row < 5 && k >= 0 && k < had;
+            CHECK(a.freeBlocks() == free_before + (acts ? had - k : 0));
+            if (row >= 0 && row < 5) CHECK(a.mapped(row) == (acts ? k : had));
+        } else {
+            a.ensure(row, k);
+        }
+        std::set<int32_t> used;
+        for (int r = 0; r < 5; ++r)
+            for (int j = 0; j < 9; ++j) {
+                const int32_t b = a.table()[(size_t)(r * 9 + j)];
+                if (j < a.mapped(r)) CHECK(b >= 0 && b < 20 && used.insert(b).second);
+                else CHECK(b == a.spare());
+            }
+        CHECK((int)used.size() + a.freeBlocks() == 20);
+        // the device copy follows by the updates alone
+        static std::vector<int32_t> copy(45, a.spare());
+        for (const auto &u : a.takeUpdates()) copy[(size_t)u.first] = u.second;
+        CHECK(copy == a.table());
+    }
+    std::puts("ok allocator_shrink");
+}
+
+int main() {
+    stream_random();
+    account_random();
+    allocator_shrink();
+    return 0;
+}

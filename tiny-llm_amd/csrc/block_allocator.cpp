@@ -49,16 +49,18 @@ int64_t BlockAllocator::shortfall(const int *rows, const int *blocks, int n) con
     return need - freeBlocks();
 }
 
-void BlockAllocator::release(int row) {
-    if (row < 0 || row >= rows_) return;
+void BlockAllocator::release(int row) { shrink(row, 0); }
+
+void BlockAllocator::shrink(int row, int blocks) {
+    if (row < 0 || row >= rows_ || blocks < 0 || blocks >= mapped_[static_cast<size_t>(row)]) return;
     const size_t base = static_cast<size_t>(row) * static_cast<size_t>(bpr_);
     // Push in reverse so the row's first block is handed out first again.
-    for (int j = mapped_[static_cast<size_t>(row)] - 1; j >= 0; --j) {
+    for (int j = mapped_[static_cast<size_t>(row)] - 1; j >= blocks; --j) {
         free_.push_back(table_[base + static_cast<size_t>(j)]);
         table_[base + static_cast<size_t>(j)] = num_blocks_;
         touch(base + static_cast<size_t>(j));
     }
-    mapped_[static_cast<size_t>(row)] = 0;
+    mapped_[static_cast<size_t>(row)] = blocks;
 }
 
 std::vector<std::pair<int32_t, int32_t>> BlockAllocator::takeUpdates() {

@@ -47,6 +47,8 @@ class BlockAllocator {
     // Return every block of `row` to the free list; its entries go back to
     // the spare block.
     void release(int row);
+    // The same for the blocks of `row` from entry `blocks` on.
+    void shrink(int row, int blocks);
 
     // Host mirror of the table, [rows][blocks_per_row].
     const std::vector<int32_t> &table() const noexcept { return table_; }

@@ -31,7 +31,9 @@ void        w8a16_force_generic(int on);
 } // namespace detail
 } // namespace tiny_llm
 
+using tiny_llm::CrossBatch;
 using tiny_llm::DecodeBatch;
+using tiny_llm::EvictBatch;
 using tiny_llm::PrefillBatch;
 using tiny_llm::KVCacheManager;
 using tiny_llm::Result;
@@ -45,6 +47,13 @@ struct tl_kv_batch {
 
 struct tl_kv_prefill {
     std::unique_ptr<PrefillBatch> b;
+};
+
+struct tl_kv_cross {
+    std::unique_ptr<CrossBatch> b;
+};
+struct tl_kv_evict {
+    std::unique_ptr<EvictBatch> b;
 };
 
 namespace {
@@ -279,6 +288,15 @@ int tl_kv_batch_decode(tl_kv_batch *batch, int layer, const void *q, const void 
     });
 }
 
+int tl_kv_batch_decode_weights(tl_kv_batch *batch, int layer, const void *q, const void *new_k, const void *new_v,
+                               void *out, float scale, const float *weights_in, float *weights_out, void *stream) {
+    if (!batch) return fail(TL_ERR_INVALID, "tl_kv_batch_decode_weights: null batch");
+    return guarded([&] {
+        return status(batch->b->decodeWeights(layer, as_half(q), as_half(new_k), as_half(new_v), as_half(out), scale,
+                                              weights_in, weights_out, as_stream(stream)));
+    });
+}
+
 int tl_kv_batch_gather(tl_kv_batch *batch, int layer, void *k_out, void *v_out, int s_max,
                        void *stream) {
     if (!batch) return fail(TL_ERR_INVALID, "tl_kv_batch_gather: null batch");
@@ -475,6 +493,14 @@ int tl_kv_prefill_run(tl_kv_prefill *p, int layer, const void *q, const void *ne
     });
 }
 
+int tl_kv_prefill_weights(tl_kv_prefill *p, int layer, const void *q, float scale, int window, const float *weights_in,
+                          float *weights_out, void *stream) {
+    if (!p) return fail(TL_ERR_INVALID, "tl_kv_prefill_weights: null batch");
+    return guarded([&] {
+        return status(p->b->weights(layer, as_half(q), scale, window, weights_in, weights_out, as_stream(stream)));
+    });
+}
+
 int tl_kv_prefill_commit(tl_kv_prefill *p) {
     if (!p) return fail(TL_ERR_INVALID, "tl_kv_prefill_commit: null batch");
     return guarded([&] { return status(p->b->commit()); });
@@ -640,6 +666,79 @@ int tl_attn_plan(const int32_t *seq_lens, int n, int num_kv_heads, int head_dim,
     });
 }
 
+int tl_kv_evicted(const tl_kv_manager *mgr, int seq_id) { return mgr ? mgr->m->getEvicted(seq_id) : 0; }
+
+int tl_kv_evict_create(tl_kv_manager *mgr, int max_seqs, tl_kv_evict **out) {
+    if (!mgr || !out) return fail(TL_ERR_INVALID, "tl_kv_evict_create: null argument");
+    *out = nullptr;
+    return guarded([&] {
+        auto r = EvictBatch::create(*mgr->m, max_seqs);
+        if (r.isErr()) return fail(TL_ERR_INVALID, r.error());
+        *out = new tl_kv_evict{std::move(r.value())};
+        g_last_error.clear();
+        return TL_OK;
+    });
+}
+
+void tl_kv_evict_destroy(tl_kv_evict *e) { delete e; }
+
+int tl_kv_evict_prepare(tl_kv_evict *e, const int *seq_ids, const int *budgets, int n, int recent, void *stream) {
+    if (!e) return fail(TL_ERR_INVALID, "tl_kv_evict_prepare: null batch");
+    return guarded([&] { return status(e->b->prepare(seq_ids, budgets, n, recent, as_stream(stream))); });
+}
+
+int tl_kv_evict_info(const tl_kv_evict *e, int *n, long long *evicted) {
+    if (!e) return fail(TL_ERR_INVALID, "tl_kv_evict_info: null batch");
+    if (n) *n = e->b->size();
+    if (evicted) *evicted = e->b->evicted();
+    return TL_OK;
+}
+
+int tl_kv_evict_run(tl_kv_evict *e, int layer, const float *weights_in, float *weights_out,
+                    const int32_t *positions_in, int32_t *positions_out, void *stream) {
+    if (!e) return fail(TL_ERR_INVALID, "tl_kv_evict_run: null batch");
+    return guarded([&] {
+        return status(e->b->run(layer, weights_in, weights_out, positions_in, positions_out, as_stream(stream)));
+    });
+}
+
+int tl_kv_evict_commit(tl_kv_evict *e) {
+    if (!e) return fail(TL_ERR_INVALID, "tl_kv_evict_commit: null batch");
+    return guarded([&] { return status(e->b->commit()); });
+}
+
+int tl_kv_cross_create(tl_kv_manager *mgr, int max_entries, int num_q_heads, tl_kv_cross **out) {
+    if (!mgr || !out) return fail(TL_ERR_INVALID, "tl_kv_cross_create: null argument");
+    *out = nullptr;
+    return guarded([&] {
+        auto r = CrossBatch::create(*mgr->m, max_entries, num_q_heads);
+        if (r.isErr()) return fail(TL_ERR_INVALID, r.error());
+        *out = new tl_kv_cross{std::move(r.value())};
+        g_last_error.clear();
+        return TL_OK;
+    });
+}
+
+void tl_kv_cross_destroy(tl_kv_cross *c) { delete c; }
+
+int tl_kv_cross_prepare(tl_kv_cross *c, const int *seq_ids, const int *num_queries, const int *attended, int n,
+                        void *stream) {
+    if (!c) return fail(TL_ERR_INVALID, "tl_kv_cross_prepare: null batch");
+    return guarded([&] { return status(c->b->prepare(seq_ids, num_queries, attended, n, as_stream(stream))); });
+}
+
+int tl_kv_cross_info(const tl_kv_cross *c, int *n, int *tokens) {
+    if (!c) return fail(TL_ERR_INVALID, "tl_kv_cross_info: null batch");
+    if (n) *n = c->b->size();
+    if (tokens) *tokens = c->b->tokens();
+    return TL_OK;
+}
+
+int tl_kv_cross_attention(tl_kv_cross *c, int layer, const void *q, void *out, float scale, void *stream) {
+    if (!c) return fail(TL_ERR_INVALID, "tl_kv_cross_attention: null batch");
+    return guarded([&] { return status(c->b->attention(layer, as_half(q), as_half(out), scale, as_stream(stream))); });
+}
+
 int tl_fill_normal_f16(uint64_t seed, uint64_t first, float stddev, void *out, size_t n,
                        void *stream) {
     if (n == 0) return TL_OK;
@@ -657,7 +756,8 @@ void tl_profile_reset(void) { tiny_llm::detail::profile_reset(); }
 
 int tl_profile_query(const char *kernel, double *total_ms, long long *launches) {
     static const char *names[] = {"attn_chunk", "attn_merge",   "kv_append",   "kv_gather",
-                                  "w8a16",      "w8a16_reduce", "attn_prefill"};
+                                  "w8a16",      "w8a16_reduce", "attn_prefill", "kv_evict",
+                                  "attn_stream",  "attn_account"};
     constexpr int      kNames = static_cast<int>(sizeof(names) / sizeof(names[0]));
     static_assert(kNames == static_cast<int>(tiny_llm::detail::KernelId::Count), "profile names");
     if (!kernel || !total_ms || !launches) return fail(TL_ERR_INVALID, "tl_profile_query: null argument");

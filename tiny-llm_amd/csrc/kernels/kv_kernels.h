@@ -193,7 +193,10 @@ enum class KernelId {
     W8A16 = 4,       // main GEMM kernel (either path)
     W8A16Reduce = 5, // split-K reduction + epilogue
     AttnPrefill = 6,
-    Count = 7
+    Evict = 7, // selection and moves of one launch
+    AttnStream = 8, // with its finish
+    AttnAccount = 9, // statistics and sums of one launch
+    Count = 10
 };
 void profile_begin(KernelId id, hipStream_t stream);
 void profile_end(KernelId id, hipStream_t stream);

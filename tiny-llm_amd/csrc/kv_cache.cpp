@@ -11,6 +11,7 @@
 #include "block_allocator.h"
 #include "kernels/kv_kernels.h"
 #include "kernels/prefill.h"
+#include "kernels/stream.h"
 #include "kernels/w8a16.h"
 #include "runtime.h"
 #include "tl_log.h"
@@ -112,6 +113,7 @@ Result<std::unique_ptr<KVCacheManager>> KVCacheManager::build(const KVCacheConfi
     }
 
     manager->slots_.resize(static_cast<size_t>(config.max_batch_size));
+    manager->evictions_.resize(static_cast<size_t>(config.max_batch_size));
     for (auto &slot : manager->slots_) {
         slot.active = false;
         slot.seq_id = -1;
@@ -165,6 +167,7 @@ Result<int> KVCacheManager::allocateSequence(int max_len) {
     slot.current_len = 0;
     slot.max_len = max_len;
     slot.active = true;
+    evictions_[static_cast<size_t>(slot_idx)] = Eviction();
     seq_to_slot_[seq_id] = slot_idx;
     return Result<int>::ok(seq_id);
 }
@@ -322,6 +325,21 @@ int KVCacheManager::getSeqLen(int seq_id) const noexcept {
 bool KVCacheManager::hasSequence(int seq_id) const noexcept {
     return seq_to_slot_.find(seq_id) != seq_to_slot_.end();
 }
+int KVCacheManager::getEvicted(int seq_id) const noexcept {
+    const int s = slotOf(seq_id);
+    return s < 0 ? 0 : evictions_[static_cast<size_t>(s)].gone;
+}
+
+// The end of an eviction: the slot's sequence holds its first `keep` tokens.
+void KVCacheManager::truncate(int slot, int keep) {
+    SequenceCache &sc = slots_[static_cast<size_t>(slot)];
+    Eviction      &ev = evictions_[static_cast<size_t>(slot)];
+    ev.gone += sc.current_len - keep;
+    ev.base = keep;
+    sc.current_len = keep;
+    if (blocks_) blocks_->shrink(slot, (keep + block_tokens_ - 1) / block_tokens_);
+}
+
 size_t KVCacheManager::getUsedMemory() const noexcept {
     if (blocks_) return static_cast<size_t>(blocks_->usedBlocks()) * blockBytes();
     return static_cast<size_t>(getActiveSequenceCount()) * slot_size_;
@@ -475,7 +493,8 @@ DecodeBatch::DecodeBatch(KVCacheManager &mgr, int max_seqs, int num_q_heads)
       meta_(new detail::MetaRing(4, 2 * sizeof(int32_t) * detail::kDecRows, sizeof(int32_t) * detail::kGatherStore)),
       work_(new detail::Workspace()), gemm_work_(new detail::Workspace()),
       plan_(new detail::WorkList()),
-      inl_(new detail::InlineMeta()) {}
+      inl_(new detail::InlineMeta()), account_plan_(new detail::StreamPlan()),
+      account_work_(new detail::Workspace()) {}
 
 DecodeBatch::~DecodeBatch() = default;
 
@@ -514,6 +533,7 @@ Result<void> DecodeBatch::upload(const int *seq_ids, const int *attended, int n,
     n_ = 0;
     appendable_ = false;
     d_rows_ = d_gather_ = nullptr;
+    account_plan_->clear();
     ids_.clear();
     const KVCacheConfig &cfg = mgr_.getConfig();
     std::vector<char>    taken(static_cast<size_t>(cfg.max_batch_size), 0);
@@ -791,7 +811,8 @@ Result<void> DecodeBatch::project(int layer_idx, const half *x, int hidden, int 
 PrefillBatch::PrefillBatch(KVCacheManager &mgr, int max_seqs, int num_q_heads)
     : mgr_(mgr), max_seqs_(max_seqs), num_q_heads_(num_q_heads), meta_(new detail::MetaRing(4)),
       inl_(new detail::PrefillInline),
-      records_(new detail::DeviceRing(sizeof(int32_t) * detail::kPrefillItemWords * detail::kPrefillInlineWords)) {}
+      records_(new detail::DeviceRing(sizeof(int32_t) * detail::kPrefillItemWords * detail::kPrefillInlineWords)),
+      account_plan_(new detail::AccountPlan()), account_work_(new detail::Workspace()) {}
 
 PrefillBatch::~PrefillBatch() = default;
 
@@ -822,6 +843,7 @@ Result<void> PrefillBatch::prepare(const int *seq_ids, const int *num_tokens, in
     uploaded_ = false;
     inline_ok_ = false;
     launched_ = false;
+    account_plan_->clear();
     ids_.clear();
     counts_.clear();
     slots_.clear();

@@ -90,6 +90,7 @@ class Workspace {
     Workspace(const Workspace &) = delete;
     Workspace &operator=(const Workspace &) = delete;
     float *get(size_t floats);
+    bool   holds(size_t floats) const { return floats <= cap_; }
     // Grow-only ints that are zero between uses (the attention merge
     // counters: the kernels that count in them leave them zero).  A new
     // buffer is cleared on `stream`, ahead of whatever is queued there after

@@ -1,0 +1,64 @@
+#include "stream_plan.h"
+
+#include <algorithm>
+#include <climits>
+
+namespace tiny_llm {
+namespace detail {
+
+void plan_stream(StreamPlan &plan, int Hkv, int cus) {
+    // A workgroup's four waves take tiles in turn, so a chunk has at least
+    // four; two workgroups fit a CU, and eight rounds of them even out what
+    // the lengths leave uneven.
+    int64_t total = 0;
+    for (const auto &e : plan.entries) total += stream_tiles(e.S);
+    const int64_t slots = 4 * (int64_t)std::max(1, cus);
+    plan.chunk = (int)std::min<int64_t>(std::max<int64_t>(4, (total * Hkv + slots - 1) / slots), 1 << 20);
+    plan.launches.clear();
+    for (size_t i = 0; i < plan.entries.size();) {
+        StreamLaunch l{(int)i, 0, 0, 0, 0, 0};
+        for (; i < plan.entries.size() && l.n < kStreamBatch; ++i, ++l.n) {
+            StreamEntry &e = plan.entries[i];
+            const int    items = stream_items(e.S, plan.chunk);
+            e.item0 = l.items;
+            e.tile0 = (int32_t)l.tiles;
+            l.items += items;
+            l.tiles += stream_tiles(e.S);
+            l.max_items = std::max(l.max_items, items);
+            l.max_len = std::max(l.max_len, e.S);
+        }
+        plan.launches.push_back(l);
+    }
+}
+
+bool plan_account(AccountPlan &plan, int G, int Hkv, int cus) {
+    // Row tiles of all entries fill the chip by themselves, or their keys are
+    // split, into chunks of at least four tiles.
+    int64_t tiles = 0;
+    for (const auto &e : plan.entries) tiles += ((int64_t)e.w * G + kAccountRows - 1) / kAccountRows;
+    const int64_t want = 4 * (int64_t)std::max(1, cus);
+    const int64_t split = std::max<int64_t>(1, want / std::max<int64_t>(1, tiles * Hkv));
+    plan.launches.clear();
+    for (size_t i = 0; i < plan.entries.size();) {
+        AccountLaunch l{(int)i, 0, 0, 0, 0};
+        for (; i < plan.entries.size() && l.n < kAccountBatch; ++i, ++l.n) {
+            AccountEntry &e = plan.entries[i];
+            const int     keys = e.p0 + e.n;
+            const int64_t rows = (int64_t)e.w * G, rt = (rows + kAccountRows - 1) / kAccountRows;
+            e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(split, stream_tiles(keys) / 4));
+            e.stat0 = (int32_t)l.stats;
+            e.item0 = l.items;
+            e.sum0 = l.sums;
+            l.stats += rows * e.nch;
+            const int64_t items = l.items + rt * e.nch;
+            if (l.stats > INT32_MAX || items > INT32_MAX) return false;
+            l.items = (int)items;
+            l.sums += keys / kAccountKeys + (keys % kAccountKeys != 0);
+        }
+        plan.launches.push_back(l);
+    }
+    return true;
+}
+
+} // namespace detail
+} // namespace tiny_llm

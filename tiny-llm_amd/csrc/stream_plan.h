@@ -1,0 +1,69 @@
+// How the work of attn_stream_kernel (kernels/attention_stream.hip) and of the
+// prompt's account (kernels/attention_account.hip) is cut: plain C++, unit-tested
+// on the host.
+#pragma once
+
+#include <cstdint>
+#include <vector>
+
+namespace tiny_llm {
+namespace detail {
+
+constexpr int kStreamTile = 64;    // keys
+constexpr int kStreamRows = 16;    // query rows (tokens x heads of one kv head) of an entry at most
+constexpr int kStreamBatch = 144;  // entries per launch: they travel in the kernel arguments
+
+// Query tokens tok0 .. tok0 + nq - 1 attend to the first S tokens of cache row
+// `row`.  item0, tile0: work items and tiles of the entries before it in its
+// launch.
+struct StreamEntry {
+    int32_t row, S, tok0, nq, item0, tile0;
+};
+
+// Launch `first`..: n entries, `items` work items (per kv head), `tiles` tiles.
+// Entry e has ceil(tiles_e / chunk) work items of equal size (in tiles, to one).
+struct StreamLaunch {
+    int     first, n, items, max_items, max_len;
+    int64_t tiles;
+};
+struct StreamPlan {
+    std::vector<StreamEntry>  entries;
+    std::vector<StreamLaunch> launches;
+    int                       chunk = 1; // tiles
+    void                      clear() { entries.clear(), launches.clear(); }
+};
+
+inline int stream_tiles(int S) { return S / kStreamTile + (S % kStreamTile != 0); }
+inline int stream_items(int S, int chunk) { return (stream_tiles(S) + chunk - 1) / chunk; }
+
+// Sets item0 and tile0 of plan.entries, the launches and the chunk length.
+void plan_stream(StreamPlan &plan, int Hkv, int cus);
+
+constexpr int kAccountRows = 128;  // query rows of a workgroup of account_stats_kernel
+constexpr int kAccountKeys = 256;  // keys of a workgroup of account_sum_kernel
+constexpr int kAccountBatch = 96;  // entries per launch
+
+// The last w of the n new tokens of cache row `row` (positions p0 .. p0 + n - 1; tok0:
+// the first one's index in the call's tokens) attend causally.  nch: chunks of
+// its keys in account_stats_kernel, stat0: its first row of partial statistics
+// (per kv head), item0 / sum0: work items of the entries before it in its launch.
+struct AccountEntry {
+    int32_t row, p0, n, w, tok0, nch, stat0, item0, sum0;
+};
+struct AccountLaunch {
+    int first, n, items, sums;
+    int64_t stats; // rows of partial statistics, per kv head
+};
+struct AccountPlan {
+    std::vector<AccountEntry>  entries;
+    std::vector<AccountLaunch> launches;
+    int                        window = -1;
+    void                       clear() { entries.clear(), launches.clear(), window = -1; }
+};
+
+// Sets nch, stat0, item0 and sum0 of plan.entries, and the launches.  False when
+// a launch's statistics do not fit 31 bits.
+bool plan_account(AccountPlan &plan, int G, int Hkv, int cus);
+
+} // namespace detail
+} // namespace tiny_llm

@@ -21,6 +21,7 @@
 
 #include <cstdint>
 #include <memory>
+#include <string>
 #include <unordered_map>
 #include <utility>
 #include <vector>
@@ -34,6 +35,9 @@ class BlockAllocator;
 struct InlineMeta;
 struct PrefillEntry;
 struct PrefillInline;
+struct EvictEntry;
+struct StreamPlan;
+struct AccountPlan;
 class MetaRing;
 class DeviceRing;
 class Workspace;
@@ -102,6 +106,9 @@ class KVCacheManager {
     // Maps blocks so that every listed slot holds tokens[i] tokens: all or
     // nothing.
     Result<void> reserveSlots(const int32_t *slots, const int32_t *tokens, int n);
+    // Tokens of the sequence that evictions took from the cache (EvictBatch): the
+    // next token's position is getSeqLen + getEvicted.  0 for an unknown sequence.
+    int getEvicted(int seq_id) const noexcept;
     // Elements from layer l's K base to layer l+1's.
     int64_t layerStride() const noexcept { return layer_stride_; }
 
@@ -126,10 +133,20 @@ class KVCacheManager {
     size_t calculateOffset(int slot_idx, int layer_idx, bool is_value) const;
     int    findFreeSlot() const;
 
+    // What evictions did to a slot's sequence: tokens gone, and its length right
+    // after the last one (the tokens from there on came since, in order).
+    struct Eviction {
+        int gone = 0;
+        int base = 0;
+    };
+    friend class EvictBatch;
+    void truncate(int slot, int keep);
+
     KVCacheConfig config_;
     half         *memory_pool_ = nullptr;
     size_t        pool_size_ = 0;
     std::vector<SequenceCache>   slots_;
+    std::vector<Eviction>        evictions_;
     std::unordered_map<int, int> seq_to_slot_;
     int                          next_seq_id_ = 0;
     size_t                       slot_size_ = 0;
@@ -163,6 +180,14 @@ class DecodeBatch {
     Result<void> attention(int layer_idx, const half *q, half *out, float scale, hipStream_t stream);
     Result<void> decode(int layer_idx, const half *q, const half *new_k, const half *new_v, half *out,
                         float scale, hipStream_t stream);
+    // decode() (new_k and new_v null: attention()) that also keeps account of the
+    // cached tokens' attention weights: weights_out[slot][kv head][t] = the running
+    // sum weights_in[..][t] (null: zeros) + the step's softmax weights of token t,
+    // summed over the query heads of the kv head, for the attended tokens; a token
+    // that this step appends starts from zero.  fp32 [max_batch_size][num_heads]
+    // [max_seq_len], weights_out may be weights_in.  What EvictBatch chooses by.
+    Result<void> decodeWeights(int layer_idx, const half *q, const half *new_k, const half *new_v, half *out,
+                               float scale, const float *weights_in, float *weights_out, hipStream_t stream);
     Result<void> gather(int layer_idx, half *k_out, half *v_out, int s_max, hipStream_t stream);
     // The K/V projections of the decode step with the append fused into their
     // epilogue: for every entry i, K_i = x_i @ dequant(wk, sk) and V_i likewise
@@ -221,6 +246,9 @@ class DecodeBatch {
     // The same for its first gather: lengths and rows.
     const int32_t  *d_gather_ = nullptr;
     hipStream_t     gather_stream_ = nullptr;
+    // decodeWeights: its plan, made by the first call of a prepared step, and workspace.
+    std::unique_ptr<detail::StreamPlan> account_plan_;
+    std::unique_ptr<detail::Workspace>  account_work_;
 };
 
 // A prefill step over n sequences of one manager: sequence i brings
@@ -253,6 +281,14 @@ class PrefillBatch {
     // those rows into the cache (the bytes of append()).
     Result<void> prefill(int layer_idx, const half *q, const half *new_k, const half *new_v,
                          half *out, float scale, hipStream_t stream);
+    // The account of the step's attention weights (see DecodeBatch::decodeWeights),
+    // by the last `window` new tokens of each sequence (0: all of them), causal:
+    // weights_out[slot][kv head][t] = the running sum weights_in[..][t] (null:
+    // zeros) for the tokens before the step, zero for the new ones, + the softmax
+    // weights of t.  The new tokens' keys are in the cache already (append or
+    // prefill); attention's outputs are not computed.
+    Result<void> weights(int layer_idx, const half *q, float scale, int window, const float *weights_in,
+                         float *weights_out, hipStream_t stream);
     // advanceSeqLen(seq, num_tokens[i]) for every sequence of the last prepare.
     Result<void> commit();
 
@@ -288,6 +324,101 @@ class PrefillBatch {
     std::unique_ptr<detail::DeviceRing>    records_;
     hipStream_t                            work_stream_ = nullptr;
     bool                                   launched_ = false;
+    // weights: its plan, made by the first call of a prepared step and window, and workspace.
+    std::unique_ptr<detail::AccountPlan> account_plan_;
+    std::unique_ptr<detail::Workspace>   account_work_;
+};
+
+// Eviction from the caches of n sequences of one manager by accumulated
+// attention weight (DecodeBatch::decodeWeights, PrefillBatch::weights), one step
+// over all layers like the other batches: prepare() snapshots the sequences, run()
+// evicts at one layer, commit() -- when every layer has run -- shortens the
+// sequences to what they kept and returns the blocks of a block pool.
+//
+// Of a sequence's tokens, every kv head of a layer keeps min(length, budget): the
+// tokens whose position is among the `recent` newest, and of the rest those with
+// the largest account (equal ones: the lower cache index; NaN counts as the
+// smallest).  Kept tokens stay where they are when their index is below the
+// budget; the others move, in order, to the indices there that became free.
+// Cached keys hold their rotary phase, so attention does not depend on their
+// order; `positions` remembers it.
+//
+// Accounts (fp32) and positions (int32) are the caller's, one pair per layer,
+// [max_batch_size][num_heads][max_seq_len] by slot (slotOf) and cache index.  A
+// position is read only below the length that the sequence's last eviction left
+// (tokens after that came in order), so the memory needs no initial value.
+// run() writes the first min(length, budget) of both, and may work in place; an
+// output that is not its input must not overlap it.  A layer that ran in place
+// is not run again before commit().
+class EvictBatch {
+  public:
+    static Result<std::unique_ptr<EvictBatch>> create(KVCacheManager &mgr, int max_seqs);
+    ~EvictBatch();
+    EvictBatch(const EvictBatch &) = delete;
+    EvictBatch &operator=(const EvictBatch &) = delete;
+
+    // budgets[i] >= 1 tokens of seq_ids[i] (distinct, live) stay, the `recent`
+    // newest (0 <= recent <= every budget) among them.
+    Result<void> prepare(const int *seq_ids, const int *budgets, int n, int recent, hipStream_t stream);
+    Result<void> run(int layer_idx, const float *weights_in, float *weights_out, const int32_t *positions_in,
+                     int32_t *positions_out, hipStream_t stream);
+    Result<void> commit();
+
+    int size() const noexcept { return static_cast<int>(ids_.size()); }
+    // Tokens that commit() takes from the caches (per kv head and layer).
+    int64_t evicted() const noexcept { return evicted_; }
+
+  private:
+    EvictBatch(KVCacheManager &mgr, int max_seqs);
+    // "" while the sequences are as prepare() found them.
+    std::string changed() const;
+
+    KVCacheManager  &mgr_;
+    int              max_seqs_;
+    int              recent_ = 0;
+    int64_t          evicted_ = 0;
+    std::vector<int> ids_;
+    std::vector<char> ran_; // per layer: 0 not yet, 1 with other outputs, 2 in place
+    std::vector<detail::EvictEntry>    entries_;
+    std::unique_ptr<detail::Workspace> work_;
+    int32_t                           *lists_ = nullptr;
+};
+
+// Attention of query tokens to cached states that are not their own sequence's --
+// an encoder's states, a document that several sequences share -- of any length
+// beside the queries': every query of an entry attends to all of the states.
+// The states are a sequence of `mgr` like any other, appended once (appendKV or
+// PrefillBatch::append, then advanceSeqLen); several entries may name the same
+// one.  prepare() snapshots a step, attention() runs a layer of it.
+class CrossBatch {
+  public:
+    static Result<std::unique_ptr<CrossBatch>> create(KVCacheManager &mgr, int max_entries, int num_q_heads);
+    ~CrossBatch();
+    CrossBatch(const CrossBatch &) = delete;
+    CrossBatch &operator=(const CrossBatch &) = delete;
+
+    // Entry i: num_queries[i] >= 1 query tokens over the first attended[i] tokens
+    // of seq_ids[i] (0 <= attended[i] <= getSeqLen, the rest is padding; null: all).
+    Result<void> prepare(const int *seq_ids, const int *num_queries, const int *attended, int n, hipStream_t stream);
+    // q and out: [T][num_q_heads][head_dim], the entries' tokens back to back.  A
+    // query over no states gets zeros.
+    Result<void> attention(int layer_idx, const half *q, half *out, float scale, hipStream_t stream);
+
+    int size() const noexcept { return n_; }
+    int tokens() const noexcept { return tokens_; }
+
+  private:
+    CrossBatch(KVCacheManager &mgr, int max_entries, int num_q_heads);
+
+    KVCacheManager      &mgr_;
+    int                  max_entries_;
+    int                  num_q_heads_;
+    int                  n_ = 0;
+    int                  tokens_ = 0;
+    std::vector<int>     ids_;
+    std::vector<int32_t> lens_;
+    std::unique_ptr<detail::StreamPlan> stream_plan_;
+    std::unique_ptr<detail::Workspace>  work_;
 };
 
 } // namespace tiny_llm

@@ -133,6 +133,7 @@ def _declare(L: C.CDLL) -> None:
         "tl_kv_batch_append": (i, [vp, i, i, vp, vp, vp]),
         "tl_kv_batch_attention": (i, [vp, i, vp, vp, f, vp]),
         "tl_kv_batch_decode": (i, [vp, i, vp, vp, vp, vp, f, vp]),
+        "tl_kv_batch_decode_weights": (i, [vp, i, vp, vp, vp, vp, f, vp, vp, vp]),
         "tl_kv_batch_gather": (i, [vp, i, vp, vp, i, vp]),
         "tl_kv_batch_commit": (i, [vp, i]),
         "tl_kv_batch_project": (i, [vp, i, vp, i, i, vp, vp, vp, vp, vp, vp, vp, i, vp]),
@@ -155,7 +156,20 @@ def _declare(L: C.CDLL) -> None:
         "tl_kv_prefill_append": (i, [vp, i, vp, vp, vp]),
         "tl_kv_prefill_attention": (i, [vp, i, vp, vp, f, vp]),
         "tl_kv_prefill_run": (i, [vp, i, vp, vp, vp, vp, f, vp]),
+        "tl_kv_prefill_weights": (i, [vp, i, vp, f, i, vp, vp, vp]),
         "tl_kv_prefill_commit": (i, [vp]),
+        "tl_kv_evicted": (i, [vp, i]),
+        "tl_kv_evict_create": (i, [vp, i, C.POINTER(vp)]),
+        "tl_kv_evict_destroy": (None, [vp]),
+        "tl_kv_evict_prepare": (i, [vp, vp, vp, i, i, vp]),
+        "tl_kv_evict_info": (i, [vp, ip, C.POINTER(C.c_longlong)]),
+        "tl_kv_evict_run": (i, [vp, i, vp, vp, vp, vp, vp]),
+        "tl_kv_evict_commit": (i, [vp]),
+        "tl_kv_cross_create": (i, [vp, i, i, C.POINTER(vp)]),
+        "tl_kv_cross_destroy": (None, [vp]),
+        "tl_kv_cross_prepare": (i, [vp, vp, vp, vp, i, vp]),
+        "tl_kv_cross_info": (i, [vp, ip, ip]),
+        "tl_kv_cross_attention": (i, [vp, i, vp, vp, f, vp]),
         "tl_prefill_set_waves": (i, [i]),
         "tl_prefill_get_waves": (i, []),
         "tl_prefill_plan_waves": (i, [vp, vp, i, i, i, i, i, ip]),
@@ -293,6 +307,11 @@ class KVCacheManager:
     def hasSequence(self, seq_id):
         return bool(load().tl_kv_has_sequence(self._h, seq_id))
 
+    def getEvicted(self, seq_id):
+        """Tokens that evictions took from the sequence's cache: its next token
+        has position getSeqLen + getEvicted."""
+        return load().tl_kv_evicted(self._h, seq_id)
+
     def getUsedMemory(self):
         return load().tl_kv_used_memory(self._h)
 
@@ -370,6 +389,12 @@ class DecodeBatch:
     def decode(self, layer, q, new_k, new_v, out, scale, stream=0):
         _check(load().tl_kv_batch_decode(self._h, layer, q, new_k, new_v, out, scale, stream))
 
+    def decode_weights(self, layer, q, new_k, new_v, out, scale, weights_in, weights_out, stream=0):
+        """decode (new_k and new_v None: attention) that adds every attended token's
+        weight to its account (tl_kv_batch_decode_weights); weights_in None: from zero."""
+        _check(load().tl_kv_batch_decode_weights(self._h, layer, q, new_k or None, new_v or None, out, scale,
+                                                 weights_in or None, weights_out, stream))
+
     def gather(self, layer, k_out, v_out, s_max, stream=0):
         _check(load().tl_kv_batch_gather(self._h, layer, k_out or None, v_out or None, s_max, stream))
 
@@ -422,8 +447,90 @@ class PrefillBatch:
     def run(self, layer, q, new_k, new_v, out, scale, stream=0):
         _check(load().tl_kv_prefill_run(self._h, layer, q, new_k, new_v, out, scale, stream))
 
+    def weights(self, layer, q, scale, window, weights_in, weights_out, stream=0):
+        """The account of the step's attention weights by the last `window` new
+        tokens of each sequence, 0: all (tl_kv_prefill_weights); weights_in None:
+        from zero."""
+        _check(load().tl_kv_prefill_weights(self._h, layer, q, scale, window, weights_in or None, weights_out, stream))
+
     def commit(self):
         _check(load().tl_kv_prefill_commit(self._h))
+
+
+class EvictBatch:
+    """tiny_llm::EvictBatch: eviction from the caches of several sequences by
+    accumulated attention weight (tl_kv_evict_*).  weights (fp32) and positions
+    (int32) are device addresses of [max_batch_size][num_heads][max_seq_len], one
+    pair per layer, by slot and cache index."""
+
+    def __init__(self, mgr: KVCacheManager, max_seqs: int):
+        self.mgr = mgr
+        self._h = C.c_void_p()
+        self._destroy = load().tl_kv_evict_destroy  # usable at interpreter shutdown
+        _check(load().tl_kv_evict_create(mgr._h, max_seqs, C.byref(self._h)))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+    def prepare(self, seq_ids, budgets, recent=0, stream=0):
+        ids, n = _int_array(seq_ids)
+        bud, m = _int_array(budgets)
+        if n != m:
+            raise ValueError(f"{n} seq_ids and {m} budgets")
+        _check(load().tl_kv_evict_prepare(self._h, ids, bud, n, recent, stream))
+
+    def info(self):
+        n, e = C.c_int(), C.c_longlong()
+        _check(load().tl_kv_evict_info(self._h, C.byref(n), C.byref(e)))
+        return {"n": n.value, "evicted": e.value}
+
+    def run(self, layer, weights_in, weights_out, positions_in, positions_out, stream=0):
+        _check(load().tl_kv_evict_run(self._h, layer, weights_in, weights_out, positions_in, positions_out, stream))
+
+    def commit(self):
+        _check(load().tl_kv_evict_commit(self._h))
+
+
+class CrossBatch:
+    """tiny_llm::CrossBatch: query tokens over cached states of another sequence,
+    not causal (tl_kv_cross_*)."""
+
+    def __init__(self, mgr: KVCacheManager, max_entries: int, num_q_heads: int):
+        self.mgr = mgr
+        self._h = C.c_void_p()
+        self._destroy = load().tl_kv_cross_destroy  # usable at interpreter shutdown
+        _check(load().tl_kv_cross_create(mgr._h, max_entries, num_q_heads, C.byref(self._h)))
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+    def prepare(self, seq_ids, num_queries, attended=None, stream=0):
+        """Entry i: num_queries[i] tokens over the first attended[i] (None: all)
+        tokens of seq_ids[i]; seq_ids may repeat."""
+        ids, n = _int_array(seq_ids)
+        nq, m = _int_array(num_queries)
+        att, k = _int_array(attended) if attended is not None else (None, n)
+        if n != m or n != k:
+            raise ValueError(f"{n} seq_ids, {m} num_queries and {k} attended lengths")
+        _check(load().tl_kv_cross_prepare(self._h, ids, nq, att, n, stream))
+
+    def info(self):
+        n, t = C.c_int(), C.c_int()
+        _check(load().tl_kv_cross_info(self._h, C.byref(n), C.byref(t)))
+        return {"n": n.value, "tokens": t.value}
+
+    def attention(self, layer, q, out, scale, stream=0):
+        _check(load().tl_kv_cross_attention(self._h, layer, q, out, scale, stream))
 
 
 def attention_prefill(q, k, v, out, scale, batch, num_heads, seq_len, head_dim, stream=0):
