@@ -16,7 +16,11 @@
 // keep-th largest lies, the next digit within that bin.  Then one pass in index
 // order ranks the free places and the movers, writes their pairs, and brings
 // accounts and positions up to date.
-// evict_move_kernel: the K and V rows of the pairs, 16 bytes a lane.
+// evict_move_kernel: the K and V rows of the pairs, 16 bytes a lane, every row on
+// its way before the first is written: 8 x 8192 tokens to 2048 (8 heads of 128,
+// 100 MB read and written) 17 us.
+// evict_one_kernel: sequences that lose one token, in one launch: 16 x 32 heads of
+// 1025 tokens 25.5 -> 6.4 us against the two launches above.
 #include "evict.h"
 
 #include "tiny_llm/hip_utils.h"
@@ -31,10 +35,11 @@ namespace detail {
 
 namespace {
 
-constexpr int kSelThreads = 1024;
 constexpr int kBins = 2048;      // 11 bits of the key
 constexpr int kMoveThreads = 256;
 constexpr int kMovePairs = 32;   // pairs of a workgroup of evict_move_kernel
+constexpr int kOneThreads = 256;
+constexpr int kList = 2048;      // candidates that the second digit finds in a list
 constexpr uint32_t kNewest = 0xFFFFFFFFu; // above every account's key
 
 struct EvictArgs {
@@ -86,124 +91,390 @@ template <int NT> __device__ __forceinline__ uint32_t block_rank(bool flag, uint
     return before + __popcll(b & ((1ull << lane) - 1ull));
 }
 
-template <int NT> __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
+template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+    return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+// Sum over the wave's lanes up to this one (row_shr 1, 2, 4, 8, then the rows' last
+// lanes to the rows behind them).
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+    v = dpp_add<0x111, 0xF>(v);
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);
+    return dpp_add<0x143, 0xC>(v);
+}
+
+// Four consecutive words; the rows of accounts begin at any multiple of 4 bytes.
+struct __attribute__((packed, aligned(4))) Words {
+    uint32_t x[4];
+};
+__device__ __forceinline__ Words load4(const void *p, int i, int n) { // words past the end: 0
+    const uint32_t *w = static_cast<const uint32_t *>(p);
+    if (i + 4 <= n) return *reinterpret_cast<const Words *>(w + i);
+    Words r;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) r.x[u] = i + u < n ? w[i + u] : 0u;
+    return r;
+}
+
+// The addresses of one (sequence, kv head).
+struct Head {
+    EvictEntry     e;
+    int            ei, g, newest;
+    const float   *w_in;
+    const int32_t *p_in;
+    float         *w_out;
+    int32_t       *p_out;
+    __device__ __forceinline__ int position(int i) const { return i < e.base ? p_in[i] : i + e.gone; }
+    __device__ __forceinline__ uint32_t key(int i) const { return position(i) >= newest ? kNewest : account_key(w_in[i]); }
+};
+#define EVICT_HEAD(a, h)                                                                                               \
+    Head h;                                                                                                            \
+    do {                                                                                                               \
+        h.ei = blockIdx.x / (a).Hkv;                                                                                   \
+        h.g = blockIdx.x - h.ei * (a).Hkv;                                                                             \
+        h.e = (a).e[h.ei];                                                                                             \
+        h.newest = h.e.len + h.e.gone - (a).recent; /* positions from here on stay */                                  \
+        const int64_t base_ = ((int64_t)h.e.row * (a).Hkv + h.g) * (a).st.room;                                        \
+        h.w_in = (a).st.w_in + base_;                                                                                  \
+        h.p_in = (a).st.pos_in + base_;                                                                                \
+        h.w_out = (a).st.w_out + base_;                                                                                \
+        h.p_out = (a).st.pos_out + base_;                                                                              \
+    } while (0)
+
+// The bin, of `bins` from the top, in which the need-th largest lies: pick = {bin, how
+// many of it, its count}.  lds: NT / 64 words.
+template <int NT> __device__ __forceinline__ void pick_bin(const uint32_t *hist, uint32_t need, uint32_t *lds, uint32_t *pick) {
+    constexpr int P = kBins / NT;
+    const int     tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t      c[P], own = 0;
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+        c[u] = hist[kBins - 1 - (tid * P + u)];
+        own += c[u];
+    }
+    const uint32_t inc = wave_scan(own);
+    if (lane == 63) lds[wave] = inc;
+    __syncthreads();
+    uint32_t above = inc - own;
+#pragma unroll
+    for (int w = 0; w < NT / 64; ++w) above += w < wave ? lds[w] : 0u;
+#pragma unroll
+    for (int u = 0; u < P; ++u) {
+        if (above < need && need <= above + c[u]) { // one bin
+            pick[0] = (uint32_t)(kBins - 1 - (tid * P + u));
+            pick[1] = need - above;
+            pick[2] = c[u];
+        }
+        above += c[u];
+    }
+    __syncthreads();
+}
+
+// Up to NT * 4 * IT tokens, their keys in registers: thread t has tokens (it * NT + t)
+// * 4 .. + 3.  Where the first digit leaves up to kList candidates, the next ones are
+// found among a list of them.  Bound by the instructions of the one workgroup that
+// a (sequence, kv head) has, not by memory.  Four tokens a step, with one scan per
+// step, instead of one with its ballots, and no token looked at again after the
+// first digit: 8192 tokens 14.4 -> 11.1 us, 32768 39.8 -> 24.9.  Accounts in registers
+// beside or instead of the keys cost more instructions than they saved (34 us).
+template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
+    constexpr int NW = NT / 64;
+    // Histogram and list, then the free places (half of the tokens at most).
+    __shared__ uint32_t buf[kBins + kList > NT * IT * 2 ? kBins + kList : NT * IT * 2];
+    uint32_t *const hist = buf, *const list = buf + kBins, *const places = buf;
+    __shared__ uint32_t lds[NW];
+    __shared__ uint32_t pick[3];
+    __shared__ uint32_t before[IT * NW]; // flags of step it's wave w, then of those before it
+    __shared__ uint32_t s_total, s_listed;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    EVICT_HEAD(a, h);
+    const EvictEntry &e = h.e;
+    const int cap = min(e.len - e.keep, e.keep);
+    int2     *pairs = reinterpret_cast<int2 *>(a.pairs) + (int64_t)e.list * a.Hkv + (int64_t)h.g * cap;
+    auto      token = [&](int it) { return (it * NT + tid) * 4; };
+
+    // The keys stay in registers: 0 past the end, which is below or equal to every
+    // other and last in order.
+    uint32_t keys[IT][4], held = 0;
+    for (int b = tid; b < kBins; b += NT) hist[b] = 0u;
+    if (tid == 0) s_listed = 0;
+    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        const Words x = load4(h.w_in, token(it), e.len);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) keys[it][u] = x.x[u];
+    }
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        const int i = token(it);
+        if (i < e.len) {
+            Words p = {};
+            if (i < e.base) p = load4(h.p_in, i, e.base);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int pos = i + u < e.base ? (int)p.x[u] : i + u + e.gone;
+                uint32_t  k = account_key(__uint_as_float(keys[it][u]));
+                k = pos >= h.newest ? kNewest : k;
+                k = i + u < e.len ? k : 0u;
+                keys[it][u] = k;
+                held += k == kNewest;
+                if (k != kNewest) atomicAdd(&hist[k >> 21], 1u);
+            }
+        }
+    }
+    held = block_sum<NT>(held, lds); // (its barriers also order hist)
+
+    // The threshold: the tokens with keys above it stay, and of the `equal` ones that
+    // agree with it down to bit `shift`, `need`.
+    uint32_t thr = kNewest, need = (uint32_t)e.keep, equal = held;
+    int      shift = 0;
+    if (held < need) {
+        need -= held;
+        pick_bin<NT>(hist, need, lds, pick);
+        thr = pick[0] << 21;
+        need = pick[1];
+        equal = pick[2];
+        shift = 21;
+        const bool     listed = equal <= (uint32_t)kList;
+        const uint32_t n = equal;
+        if (listed && equal != need) {
+#pragma unroll
+            for (int it = 0; it < IT; ++it)
+                if (token(it) < e.len) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        if (keys[it][u] - thr < 1u << 21) list[atomicAdd(&s_listed, 1u)] = keys[it][u];
+                }
+        }
+        while (shift > 0 && equal != need) { // (all of a bin stay: no need to look into it)
+            const int bits = min(11, shift), lo = shift - bits;
+            __syncthreads();
+            for (int b = tid; b < kBins; b += NT) hist[b] = 0u;
+            __syncthreads();
+            auto count = [&](uint32_t k) {
+                if ((k >> shift) == (thr >> shift)) atomicAdd(&hist[(k >> lo) & ((1u << bits) - 1u)], 1u);
+            };
+            if (listed) {
+                for (uint32_t x = tid; x < n; x += NT) count(list[x]);
+            } else {
+#pragma unroll
+                for (int it = 0; it < IT; ++it)
+                    if (token(it) < e.len) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) count(keys[it][u]);
+                    }
+            }
+            __syncthreads();
+            pick_bin<NT>(hist, need, lds, pick);
+            thr |= pick[0] << lo;
+            need = pick[1];
+            equal = pick[2];
+            shift = lo;
+        }
+    }
+
+    // Flags of all tokens -> before[]: how many precede a step's wave; s_total.
+    uint32_t scan[IT]; // flags in the wave's lanes before this one
+    auto     rank_all = [&](auto &&flags) __attribute__((always_inline)) {
+        __syncthreads();
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+            const uint32_t c = __popc(flags(it)), inc = wave_scan(c);
+            scan[it] = inc - c;
+            if (lane == 63) before[it * NW + wave] = inc;
+        }
+        __syncthreads();
+        if (wave == 0) {
+            constexpr int N = IT * NW, P = (N + 63) / 64;
+            uint32_t      c[P], own = 0;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                c[u] = lane * P + u < N ? before[lane * P + u] : 0u;
+                own += c[u];
+            }
+            const uint32_t inc = wave_scan(own);
+            uint32_t       run = inc - own;
+            if (lane == 63) s_total = inc;
+#pragma unroll
+            for (int u = 0; u < P; ++u) {
+                if (lane * P + u < N) before[lane * P + u] = run;
+                run += c[u];
+            }
+        }
+        __syncthreads();
+    };
+    // (all of the bin stay, or none of it yet; not all tokens do, so thr is above 0 then)
+    const uint32_t limit = equal == need ? thr - 1u : thr;
+    uint32_t       stays[IT]; // bit u: token(it) + u stays
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        stays[it] = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) stays[it] |= (uint32_t)(keys[it][u] > limit) << u;
+    }
+    if (equal != need) { // the first `need` tokens at the threshold
+        auto at = [&](int it) {
+            uint32_t f = 0;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) f |= (uint32_t)(keys[it][u] == thr) << u;
+            return f;
+        };
+        rank_all(at);
+#pragma unroll
+        for (int it = 0; it < IT; ++it) {
+            uint32_t f = at(it);
+            for (uint32_t r = before[it * NW + wave] + scan[it]; f && r < need; ++r) {
+                stays[it] |= f & -f;
+                f &= f - 1;
+            }
+        }
+    }
+#pragma unroll
+    for (int it = 0; it < IT; ++it) // tokens past the end do not stay
+        stays[it] &= token(it) < e.len ? 0xFu >> max(0, token(it) + 4 - e.len) : 0u;
+
+    // What stays in place, and the free places and movers in index order.
+    auto moving = [&](int it) { // free places below keep, kept tokens from there on
+        const int      i = token(it);
+        const uint32_t low = i >= e.keep ? 0u : 0xFu >> max(0, i + 4 - e.keep); // the tokens below keep
+        return (~stays[it] & low) | (stays[it] & ~low);
+    };
+    rank_all(moving);
+    const uint32_t moved = s_total / 2; // as many free places as movers
+    const bool     copy_w = h.w_out != h.w_in, copy_p = h.p_out != h.p_in;
+    // The accounts of a step's tokens from their keys; of the newest, whose keys do
+    // not hold them, from memory.
+    auto accounts = [&](int it) __attribute__((always_inline)) {
+        Words x;
+        bool  any = false;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t k = keys[it][u];
+            x.x[u] = k == 0u ? 0x7FC00000u : k ^ (k >> 31 ? 0x80000000u : 0xFFFFFFFFu);
+            any |= k == kNewest;
+        }
+        if (any) x = load4(h.w_in, token(it), e.len);
+        return x;
+    };
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        const int      i = token(it);
+        const uint32_t f = moving(it);
+        uint32_t       r = before[it * NW + wave] + scan[it];
+        if (i >= e.keep) continue;
+        Words p = {}, x = {};
+        if (copy_w) x = accounts(it);
+        if (copy_p && i < e.base) p = load4(h.p_in, i, e.base);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (i + u >= e.keep) continue;
+            if (f >> u & 1) {
+                places[r++] = (uint32_t)(i + u);
+            } else {
+                if (copy_w) h.w_out[i + u] = __uint_as_float(x.x[u]);
+                if (i + u >= e.base) h.p_out[i + u] = i + u + e.gone;
+                else if (copy_p) h.p_out[i + u] = (int32_t)p.x[u];
+            }
+        }
+    }
+    if (tid == 0) a.counts[(int64_t)h.ei * a.Hkv + h.g] = (int32_t)moved;
+    __syncthreads();
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
+        const int      i = token(it);
+        const uint32_t f = moving(it);
+        uint32_t       r = before[it * NW + wave] + scan[it];
+        if (!f || i + 3 < e.keep) continue;
+        const Words x = accounts(it);
+        Words       p = {};
+        if (i < e.base) p = load4(h.p_in, i, e.base);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            if (!(f >> u & 1)) continue;
+            if (i + u >= e.keep) {
+                const int to = (int)places[r - moved];
+                pairs[r - moved] = make_int2(i + u, to);
+                h.w_out[to] = __uint_as_float(x.x[u]);
+                h.p_out[to] = i + u < e.base ? (int32_t)p.x[u] : i + u + e.gone;
+            }
+            ++r;
+        }
+    }
+}
+
+// The same for any number of tokens, their keys computed anew in every pass.
+template <int NT> __global__ __launch_bounds__(NT) void evict_select_any_kernel(EvictArgs a) {
     __shared__ uint32_t hist[kBins];
     __shared__ uint32_t lds[NT / 64];
     __shared__ uint32_t pick[3];
-    const int        tid = threadIdx.x;
-    const int        ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv;
-    const EvictEntry e = a.e[ei];
-    const int64_t    base = ((int64_t)e.row * a.Hkv + g) * a.st.room;
-    const float     *w_in = a.st.w_in + base;
-    const int32_t   *p_in = a.st.pos_in + base;
-    float           *w_out = a.st.w_out + base;
-    int32_t         *p_out = a.st.pos_out + base;
-    const int        newest = e.len + e.gone - a.recent; // positions from here on stay
-    auto position = [&](int i) { return i < e.base ? p_in[i] : i + e.gone; };
-    auto key_of = [&](int i) { return position(i) >= newest ? kNewest : account_key(w_in[i]); };
+    const int tid = threadIdx.x;
+    EVICT_HEAD(a, h);
+    const EvictEntry &e = h.e;
     const int cap = min(e.len - e.keep, e.keep);
-    int2     *pairs = reinterpret_cast<int2 *>(a.pairs) + (int64_t)e.list * a.Hkv + (int64_t)g * cap;
-
-    // The threshold: the key of the keep-th token, and how many tokens with it stay.
-    uint32_t thr = 0u, need = (uint32_t)e.keep, equal = 0u;
-    if (e.keep < e.len) {
-        uint32_t mine = 0;
-        for (int i = tid; i < e.len; i += NT) mine += key_of(i) == kNewest;
-        const uint32_t held = block_sum<NT>(mine, lds);
-        if (held >= need) {
-            thr = kNewest;
-            equal = held;
-        } else {
-            need -= held;
-            int shift = 32;
-            for (int pass = 0; pass < 3; ++pass) {
-                const int bits = pass < 2 ? 11 : 10, lo = shift - bits;
-                for (int b = tid; b < kBins; b += NT) hist[b] = 0u;
-                __syncthreads();
-                for (int i = tid; i < e.len; i += NT) {
-                    const uint32_t k = key_of(i);
-                    if (k != kNewest && (shift == 32 || (k >> shift) == (thr >> shift)))
-                        atomicAdd(&hist[(k >> lo) & ((1u << bits) - 1u)], 1u);
-                }
-                __syncthreads();
-                // Bins from the top: thread t sums bins kBins-1 - t*P .. - P + 1.
-                constexpr int P = kBins / NT;
-                uint32_t      own = 0;
-#pragma unroll
-                for (int u = 0; u < P; ++u) own += hist[kBins - 1 - (tid * P + u)];
-                uint32_t       inc = own; // inclusive over the wave
-                const int      lane = tid & 63, wave = tid >> 6;
-#pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const uint32_t v = __shfl_up(inc, o);
-                    inc += lane >= o ? v : 0u;
-                }
-                if (lane == 63) lds[wave] = inc;
-                __syncthreads();
-                uint32_t above = inc - own;
-                for (int w = 0; w < wave; ++w) above += lds[w];
-#pragma unroll
-                for (int u = 0; u < P; ++u) {
-                    const int      b = kBins - 1 - (tid * P + u);
-                    const uint32_t c = hist[b];
-                    if (above < need && need <= above + c) { // one bin
-                        pick[0] = (uint32_t)b;
-                        pick[1] = need - above;
-                        pick[2] = c;
-                    }
-                    above += c;
-                }
-                __syncthreads();
-                thr |= pick[0] << lo;
-                need = pick[1];
-                equal = pick[2];
-                shift = lo;
-                __syncthreads();
+    int2     *pairs = reinterpret_cast<int2 *>(a.pairs) + (int64_t)e.list * a.Hkv + (int64_t)h.g * cap;
+    uint32_t  mine = 0;
+    for (int i = tid; i < e.len; i += NT) mine += h.key(i) == kNewest;
+    const uint32_t held = block_sum<NT>(mine, lds);
+    uint32_t       thr = kNewest, need = (uint32_t)e.keep, equal = held;
+    int            shift = 0;
+    if (held < need) {
+        need -= held;
+        thr = 0u;
+        shift = 32;
+        do {
+            const int bits = min(11, shift), lo = shift - bits;
+            for (int b = tid; b < kBins; b += NT) hist[b] = 0u;
+            __syncthreads();
+            for (int i = tid; i < e.len; i += NT) {
+                const uint32_t k = h.key(i);
+                if (k != kNewest && (shift == 32 || (k >> shift) == (thr >> shift)))
+                    atomicAdd(&hist[(k >> lo) & ((1u << bits) - 1u)], 1u);
             }
-        }
+            __syncthreads();
+            pick_bin<NT>(hist, need, lds, pick);
+            thr |= pick[0] << lo;
+            need = pick[1];
+            equal = pick[2];
+            shift = lo;
+            __syncthreads();
+        } while (shift > 0 && equal != need);
     }
-
-    // In index order: which stay, the free places and the movers.
-    uint32_t ties = 0, done = 0; // so far: tokens at the threshold, free places and movers
-    uint32_t free_places = 0;
+    uint32_t done = 0, ties = 0, moved = 0;
     for (int i0 = 0; i0 < e.len; i0 += NT) {
         const int      i = i0 + tid;
         const bool     in = i < e.len;
-        const uint32_t k = in ? key_of(i) : 0u;
-        bool           stays = in && (e.keep == e.len || k > thr);
-        if (e.keep < e.len) {
-            const bool at = in && k == thr;
-            if (equal == need) {
-                stays |= at;
-            } else {
-                uint32_t       total;
-                const uint32_t r = block_rank<NT>(at, lds, total);
-                stays |= at && ties + r < need;
-                ties += total;
-            }
-            const bool     flag = in && (i < e.keep ? !stays : stays);
-            uint32_t       total;
-            const uint32_t r = done + block_rank<NT>(flag, lds, total);
-            // Free places come first in index order, as many as movers.
-            const uint32_t nf = block_sum<NT>(flag && i < e.keep, lds);
-            free_places += nf;
-            if (flag && i < e.keep && r < (uint32_t)cap) pairs[r].y = i;
-            if (flag && i >= e.keep && r - free_places < (uint32_t)cap) pairs[r - free_places].x = i;
-            done += total;
+        const uint32_t k = in ? h.key(i) : 0u;
+        const bool     at = in && (k >> shift) == (thr >> shift);
+        bool           stay = in && k > thr;
+        uint32_t       total;
+        if (equal == need) {
+            stay |= at;
+        } else {
+            const uint32_t r = block_rank<NT>(at, lds, total);
+            stay |= at && ties + r < need;
+            ties += total;
         }
-        if (in && i < e.keep && stays) {
-            if (w_out != w_in) w_out[i] = w_in[i];
-            if (p_out != p_in || i >= e.base) p_out[i] = position(i);
+        const bool     flag = in && (i < e.keep ? !stay : stay);
+        const uint32_t r = done + block_rank<NT>(flag, lds, total);
+        moved += block_sum<NT>(flag && i < e.keep, lds); // free places come first
+        if (flag && i < e.keep) pairs[r].y = i;
+        if (flag && i >= e.keep) pairs[r - moved].x = i;
+        done += total;
+        if (i < e.keep && stay) {
+            if (h.w_out != h.w_in) h.w_out[i] = h.w_in[i];
+            if (h.p_out != h.p_in || i >= e.base) h.p_out[i] = h.position(i);
         }
     }
-    if (e.keep == e.len) return;
-    if (tid == 0) a.counts[(int64_t)ei * a.Hkv + g] = (int32_t)free_places;
+    if (tid == 0) a.counts[(int64_t)h.ei * a.Hkv + h.g] = (int32_t)moved;
     __threadfence_block();
     __syncthreads();
-    for (uint32_t r = tid; r < free_places; r += NT) {
+    for (uint32_t r = tid; r < moved; r += NT) {
         const int2 p = pairs[r];
-        w_out[p.y] = w_in[p.x];
-        p_out[p.y] = position(p.x);
+        h.w_out[p.y] = h.w_in[p.x];
+        h.p_out[p.y] = h.position(p.x);
     }
 }
 
@@ -215,7 +486,68 @@ __device__ __forceinline__ int64_t row_off(const KvView &v, int row, int t) {
     return (int64_t)row * v.blk_stride + (int64_t)t * v.tok_stride;
 }
 
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
+// Sequences that lose one token, as a bounded cache does at every step (or none): the
+// smallest key goes, of equal ones the last; its place, unless it is the last one,
+// takes the last token, whose row is on its way before the search ends.  One
+// launch, no lists.
+__global__ __launch_bounds__(kOneThreads) void evict_one_kernel(EvictArgs a) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+    __shared__ uint64_t s_min[kOneThreads / 64];
+    const int tid = threadIdx.x;
+    EVICT_HEAD(a, h);
+    const EvictEntry &e = h.e;
+    const int last = e.len - 1, pieces = a.D / 8; // a K or V row's 16-byte pieces, 32 at most
+    int       gone = e.len;                       // no token
+    if (e.len > e.keep) {
+        __half *b = const_cast<__half *>(tid >= pieces ? a.kv.v_base : a.kv.k_base) + (int64_t)h.g * a.kv.head_stride +
+                    8 * (tid % pieces);
+        u32x4   v = {0u, 0u, 0u, 0u};
+        if (tid < 2 * pieces) v = *reinterpret_cast<const u32x4 *>(b + row_off(a.kv, e.row, last));
+        uint64_t best = ~0ull;
+        for (int i = 4 * tid; i < e.len; i += 4 * kOneThreads) {
+            const Words w = load4(h.w_in, i, e.len);
+            Words       p = {};
+            if (i < e.base) p = load4(h.p_in, i, e.base);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int      pos = i + u < e.base ? (int)p.x[u] : i + u + e.gone;
+                const uint32_t key = pos >= h.newest ? kNewest : account_key(__uint_as_float(w.x[u]));
+                const uint64_t k = (uint64_t)key << 32 | (uint32_t)(0x7FFFFFFF - (i + u));
+                best = i + u < e.len && k < best ? k : best;
+            }
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) {
+            const uint64_t k = __shfl_xor(best, o);
+            best = k < best ? k : best;
+        }
+        if ((tid & 63) == 0) s_min[tid >> 6] = best;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kOneThreads / 64; ++w) best = s_min[w] < best ? s_min[w] : best;
+        gone = 0x7FFFFFFF - (int)(uint32_t)best;
+        if (tid < 2 * pieces && gone < last) *reinterpret_cast<u32x4 *>(b + row_off(a.kv, e.row, gone)) = v;
+    }
+    if (h.w_out == h.w_in && h.p_out == h.p_in) { // in place: the mover, and the positions that are new
+        for (int i = e.base + tid; i < e.keep; i += kOneThreads)
+            if (i != gone) h.p_out[i] = i + e.gone;
+        if (tid == 0 && gone < last) {
+            h.w_out[gone] = h.w_in[last];
+            h.p_out[gone] = h.position(last);
+        }
+        return;
+    }
+    for (int i = tid; i < e.keep; i += kOneThreads) {
+        const int from = i == gone ? last : i;
+        if (h.w_out != h.w_in || from != i) h.w_out[i] = h.w_in[from];
+        if (h.p_out != h.p_in || from != i || i >= e.base) h.p_out[i] = h.position(from);
+    }
+}
+
+template <int D> __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
+    constexpr int PIECES = D / 8;
+    constexpr int N = kMovePairs * 2 * PIECES / kMoveThreads; // pieces per thread
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     const int        ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv;
     const EvictEntry e = a.e[ei];
     const int        cap = min(e.len - e.keep, e.keep);
@@ -223,15 +555,28 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
     if (first >= cap) return; // (before the count: none of the entry's workgroups behind its list reads it)
     const int   cnt = a.counts[(int64_t)ei * a.Hkv + g];
     const int2 *pairs = reinterpret_cast<const int2 *>(a.pairs) + (int64_t)e.list * a.Hkv + (int64_t)g * cap;
-    const int   pieces = a.D / 8;
-    const int   last = min(first + kMovePairs, cnt);
-    for (int x = threadIdx.x; x < (last - first) * 2 * pieces; x += kMoveThreads) {
-        const int     piece = x % pieces, which = x / pieces & 1;
-        const int2    p = pairs[first + x / (2 * pieces)];
-        __half       *b = const_cast<__half *>(which ? a.kv.v_base : a.kv.k_base) + (int64_t)g * a.kv.head_stride + 8 * piece;
-        const uint4   v = *reinterpret_cast<const uint4 *>(b + row_off(a.kv, e.row, p.x));
-        *reinterpret_cast<uint4 *>(b + row_off(a.kv, e.row, p.y)) = v;
+    u32x4       v[N];
+    __half     *to[N];
+#pragma unroll
+    for (int u = 0; u < N; ++u) { // every row on its way before the first is written
+        const int x = u * kMoveThreads + (int)threadIdx.x;
+        const int r = first + x / (2 * PIECES);
+        to[u] = nullptr;
+        const int2 p = pairs[min(r, cap - 1)]; // (on its way with the count)
+        if (r < cnt) {
+            __half    *b = const_cast<__half *>(x / PIECES & 1 ? a.kv.v_base : a.kv.k_base) + (int64_t)g * a.kv.head_stride +
+                        8 * (x % PIECES);
+            v[u] = *reinterpret_cast<const u32x4 *>(b + row_off(a.kv, e.row, p.x));
+            to[u] = b + row_off(a.kv, e.row, p.y);
+        }
     }
+#pragma unroll
+    for (int u = 0; u < N; ++u)
+        if (to[u]) *reinterpret_cast<u32x4 *>(to[u]) = v[u];
+}
+
+template <int NT, int IT> void launch_select(const EvictArgs &a, dim3 grid, hipStream_t stream) {
+    hipLaunchKernelGGL((evict_select_kernel<NT, IT>), grid, dim3(NT), 0, stream, a);
 }
 
 } // namespace
@@ -258,28 +603,48 @@ void launch_evict(const KvView &kv, const std::vector<EvictEntry> &entries, cons
     a.Hkv = Hkv;
     a.D = D;
     size_t launched = 0;
-    for (size_t i = 0; i < entries.size();) {
-        a.n = 0;
-        int cap = 0;
-        a.counts = workspace + 2 * pairs * Hkv + (int64_t)launched * Hkv;
-        for (; i < entries.size() && a.n < kEvictBatch; ++i) {
-            const EvictEntry &e = entries[i];
-            if (e.keep == e.len && !copies) continue; // all stays, where it is
-            a.e[a.n++] = e;
-            cap = std::max(cap, std::min(e.len - e.keep, e.keep));
-        }
-        if (a.n == 0) break;
-        launched += (size_t)a.n;
-        profile_begin(KernelId::Evict, stream);
-        hipLaunchKernelGGL((evict_select_kernel<kSelThreads>), dim3((unsigned)(a.n * Hkv)), dim3(kSelThreads), 0, stream, a);
-        HIP_CHECK(hipGetLastError());
-        if (cap > 0) {
-            const dim3 grid((unsigned)(a.n * Hkv), (unsigned)((cap + kMovePairs - 1) / kMovePairs));
-            hipLaunchKernelGGL(evict_move_kernel, grid, dim3(kMoveThreads), 0, stream, a);
+    // Entries that lose at most one token, then the others.
+    for (const bool one : {true, false})
+        for (size_t i = 0; i < entries.size();) {
+            a.n = 0;
+            int cap = 0, len = 0;
+            a.counts = workspace + 2 * pairs * Hkv + (int64_t)launched * Hkv;
+            for (; i < entries.size() && a.n < kEvictBatch; ++i) {
+                const EvictEntry &e = entries[i];
+                if ((e.len - e.keep <= 1) != one) continue;
+                if (e.keep == e.len && (!copies || e.len == 0)) continue; // all stays, where it is
+                a.e[a.n++] = e;
+                cap = std::max(cap, std::min(e.len - e.keep, e.keep));
+                len = std::max(len, e.len);
+            }
+            if (a.n == 0) break;
+            launched += (size_t)a.n;
+            profile_begin(KernelId::Evict, stream);
+            const dim3 heads((unsigned)(a.n * Hkv));
+            if (one) {
+                hipLaunchKernelGGL(evict_one_kernel, heads, dim3(kOneThreads), 0, stream, a);
+                HIP_CHECK(hipGetLastError());
+                profile_end(KernelId::Evict, stream);
+                continue;
+            }
+            if (len <= 1024) launch_select<256, 1>(a, heads, stream);
+            else if (len <= 2048) launch_select<256, 2>(a, heads, stream);
+            else if (len <= 4096) launch_select<512, 2>(a, heads, stream);
+            else if (len <= 8192) launch_select<1024, 2>(a, heads, stream);
+            else if (len <= 16384) launch_select<1024, 4>(a, heads, stream);
+            else if (len <= 32768) launch_select<1024, 8>(a, heads, stream);
+            else hipLaunchKernelGGL((evict_select_any_kernel<1024>), heads, dim3(1024), 0, stream, a);
             HIP_CHECK(hipGetLastError());
+            const dim3 grid(heads.x, (unsigned)((cap + kMovePairs - 1) / kMovePairs));
+            switch (D) {
+            case 32: hipLaunchKernelGGL((evict_move_kernel<32>), grid, dim3(kMoveThreads), 0, stream, a); break;
+            case 64: hipLaunchKernelGGL((evict_move_kernel<64>), grid, dim3(kMoveThreads), 0, stream, a); break;
+            case 128: hipLaunchKernelGGL((evict_move_kernel<128>), grid, dim3(kMoveThreads), 0, stream, a); break;
+            default: hipLaunchKernelGGL((evict_move_kernel<256>), grid, dim3(kMoveThreads), 0, stream, a); break;
+            }
+            HIP_CHECK(hipGetLastError());
+            profile_end(KernelId::Evict, stream);
         }
-        profile_end(KernelId::Evict, stream);
-    }
 }
 
 } // namespace detail
