@@ -557,7 +557,7 @@ int tl_fill_normal_f16(uint64_t seed, uint64_t first, float stddev, void *out, s
  * named kernels is bracketed by hipEvents on its own stream.
  * Names: "attn_chunk", "attn_merge", "kv_append", "kv_gather", "w8a16"
  * (the W8A16 GEMM kernel), "w8a16_reduce" (its split-K reduction),
- * "attn_prefill", "kv_evict", "attn_stream", "attn_account".
+ * "attn_prefill", "kv_evict", "attn_stream", "attn_account", "attn_cross".
  * ---------------------------------------------------------------------- */
 void tl_profile_enable(int on);
 void tl_profile_reset(void);

@@ -106,6 +106,46 @@ static void account_random() {
     std::puts("ok account_random");
 }
 
+static void cross_random() {
+    std::mt19937_64 rng(4);
+    const int       dims[] = {32, 64, 128, 256};
+    for (int it = 0; it < 500; ++it) {
+        CrossPlan p;
+        const int n = (int)(rng() % 300), most = 1 << (rng() % 17), longest = 1 << (rng() % 12);
+        const int G = 1 << (rng() % 4), D = dims[rng() % 4], hkv = 1 << (rng() % 6);
+        for (int i = 0; i < n; ++i)
+            p.entries.push_back({i, 1 + (int32_t)(rng() % most), i, 1 + (int32_t)(rng() % longest), -1, -1});
+        CHECK(plan_cross(p, D, G, hkv, 1 + (int)(rng() % 300)));
+        CHECK(p.waves == 4 || (p.waves == 8 && D <= 128));
+        std::set<int> rows;
+        size_t        next = 0;
+        for (const auto &l : p.launches) {
+            CHECK((size_t)l.first == next && l.n > 0 && l.n <= kCrossBatch);
+            int64_t items = 0;
+            bool    split = false;
+            for (int i = l.first; i < l.first + l.n; ++i) {
+                const CrossEntry &e = p.entries[(size_t)i];
+                CHECK(rows.insert(e.row).second && e.tok0 == e.row);
+                CHECK(e.item0 == items && e.nch >= 1 && e.nch <= stream_tiles(e.S)); // no chunk is empty
+                if (i > 0) {
+                    const CrossEntry &b = p.entries[(size_t)i - 1];
+                    CHECK((int64_t)b.S * e.nch >= (int64_t)e.S * b.nch);
+                }
+                const int tile = cross_rows(D, p.waves);
+                items += ((int64_t)e.nq * G + tile - 1) / tile * e.nch;
+                split |= e.nch > 1;
+            }
+            CHECK(l.items == items && l.split == split);
+            next += (size_t)l.n;
+        }
+        CHECK(next == p.entries.size());
+    }
+    CrossPlan big;
+    for (int i = 0; i < 3; ++i) big.entries.push_back({i, 1, 0, 1 << 28, 1, 0});
+    CHECK(!plan_cross(big, 256, 8, 1024, 256));
+    std::puts("ok cross_random");
+}
+
 static void allocator_shrink() {
     std::mt19937_64 rng(3);
     BlockAllocator  a(5, 9, 20);
@@ -139,6 +179,7 @@ static void allocator_shrink() {
 int main() {
     stream_random();
     account_random();
+    cross_random();
     allocator_shrink();
     return 0;
 }

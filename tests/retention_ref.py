@@ -91,7 +91,7 @@ def attend(q, k, v, scale, last=None):
         kh, vh = k64[:, h // g], v64[:, h // g]
         s = q64[:, h] @ kh.T * scale
         # |fp32 score - exact| <= (d + 4) roundings of the sum of absolute products
-        err[:, h] = (np.abs(q64[:, h]) @ np.abs(kh).T).max(axis=1, initial=0) * scale * (d + 4) * 2.0 ** -24
+        err[:, h] = (np.abs(q64[:, h]) @ np.abs(kh).T).max(axis=1, initial=0) * abs(scale) * (d + 4) * 2.0 ** -24
         if last is not None:
             s[np.arange(s_len)[None, :] > np.asarray(last)[:, None]] = -np.inf
         if s_len:

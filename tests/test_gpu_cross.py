@@ -78,6 +78,34 @@ def test_cross_layers_scales_and_another_stream(tl):
         cross(tl, c, 2, [1, 0], [2, 2], layer=1, scale=-0.5)
 
 
+@pytest.mark.parametrize("scale", [-0.5, 1e-30, 2.0])
+@pytest.mark.parametrize("nq", [[2, 1], [90, 300]])
+def test_cross_scales_of_either_sign(tl, nq, scale):
+    c = Cache(tl, [100, 333], 2, 64, seed=15, hq=4)
+    cross(tl, c, 2, [1, 0], nq, scale=scale)
+
+
+@pytest.mark.parametrize("nq", [2, 200])
+def test_cross_scale_of_zero(tl, nq):
+    """Every state has the same weight, and those past the end none."""
+    c = Cache(tl, [100], 1, 64, seed=16, hq=2)
+    q = torch.randn((nq, 2, 64), device="cuda").half()
+    out = torch.empty_like(q)
+    b = tl.CrossBatch(c.mgr, 1, 2)
+    b.prepare(c.ids, [nq])
+    b.attention(0, q.data_ptr(), out.data_ptr(), 0.0)
+    torch.cuda.synchronize()
+    mean = c.v[0][0][:, 0].astype(np.float64).mean(axis=0)
+    # the output's rounding, values below 1
+    assert np.abs(out.cpu().numpy().astype(np.float64) - mean).max() <= 2.0 ** -11
+
+
+def test_cross_neighbours_over_the_same_states(tl):
+    """They are worked on as one, also where a padded or another one is between."""
+    c = Cache(tl, [300, 40], 2, 128, seed=17, hq=8)
+    cross(tl, c, 4, [0] * 7 + [1, 0, 0], [1, 1, 2, 1, 1, 1, 1, 1, 3, 90], [300, 300, 300, 10, 300, 300, 0, 40, 300, 300])
+
+
 @pytest.mark.parametrize("nq", [[2, 1], [70, 300]])
 def test_cross_captured(tl, nq):
     c = Cache(tl, [700, 90], 2, 64, seed=6, hq=4)

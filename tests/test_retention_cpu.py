@@ -25,7 +25,7 @@ def test_plans_and_allocator_under_sanitizers(tmp_path):
                     os.path.join(CSRC, "block_allocator.cpp"), "-o", exe], check=True, capture_output=True, text=True)
     r = subprocess.run([exe], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
-    assert r.stdout.split("\n")[:3] == ["ok stream_random", "ok account_random", "ok allocator_shrink"]
+    assert r.stdout.split("\n")[:4] == ["ok stream_random", "ok account_random", "ok cross_random", "ok allocator_shrink"]
 
 
 @pytest.fixture(scope="module")
@@ -65,7 +65,7 @@ def test_lists_of_different_lengths(tlc):
         cr.prepare([1], [3], [4, 5])
 
 
-@pytest.mark.parametrize("obj", ["evict.o", "attention_stream.o", "attention_account.o"])
+@pytest.mark.parametrize("obj", ["evict.o", "attention_stream.o", "attention_account.o", "attention_cross.o"])
 def test_kernels_use_no_scratch(obj, tmp_path):
     """Registers hold the tiles and the work lists stay in the kernel arguments."""
     for name, r in kernels(obj, tmp_path).items():

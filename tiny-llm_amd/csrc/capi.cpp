@@ -757,7 +757,7 @@ void tl_profile_reset(void) { tiny_llm::detail::profile_reset(); }
 int tl_profile_query(const char *kernel, double *total_ms, long long *launches) {
     static const char *names[] = {"attn_chunk", "attn_merge",   "kv_append",   "kv_gather",
                                   "w8a16",      "w8a16_reduce", "attn_prefill", "kv_evict",
-                                  "attn_stream",  "attn_account"};
+                                  "attn_stream",  "attn_account", "attn_cross"};
     constexpr int      kNames = static_cast<int>(sizeof(names) / sizeof(names[0]));
     static_assert(kNames == static_cast<int>(tiny_llm::detail::KernelId::Count), "profile names");
     if (!kernel || !total_ms || !launches) return fail(TL_ERR_INVALID, "tl_profile_query: null argument");

@@ -1,4 +1,5 @@
 // CrossBatch: attention to cached states of another length (tiny_llm/kv_cache.h).
+#include "kernels/cross.h"
 #include "kernels/stream.h"
 #include "runtime.h"
 #include "tiny_llm/kv_cache.h"
@@ -13,7 +14,7 @@ namespace tiny_llm {
 
 CrossBatch::CrossBatch(KVCacheManager &mgr, int max_entries, int num_q_heads)
     : mgr_(mgr), max_entries_(max_entries), num_q_heads_(num_q_heads), stream_plan_(new detail::StreamPlan()),
-      work_(new detail::Workspace()) {}
+      cross_plan_(new detail::CrossPlan()), work_(new detail::Workspace()) {}
 
 CrossBatch::~CrossBatch() = default;
 
@@ -38,6 +39,7 @@ Result<void> CrossBatch::prepare(const int *seq_ids, const int *num_queries, con
     ids_.clear();
     lens_.clear();
     stream_plan_->clear();
+    cross_plan_->clear();
     if (n < 0 || n > max_entries_)
         return Result<void>::err("CrossBatch: n=" + std::to_string(n) + " outside [0, " +
                                  std::to_string(max_entries_) + "]");
@@ -65,16 +67,31 @@ Result<void> CrossBatch::prepare(const int *seq_ids, const int *num_queries, con
     }
     if (total > INT32_MAX / 2) return Result<void>::err("CrossBatch: too many query tokens in one step");
     mgr_.syncTable(stream);
-    const int step = detail::kStreamRows / group; // tokens of an entry of the plan
-    int64_t   tok = 0;
-    for (int i = 0; i < n; ++i) {
+    // Neighbours over the same states are one entry of the plans: their rows share
+    // every key.  Up to 16 rows (and entries over nothing) take attn_stream_kernel,
+    // which reads the states once at the memory's rate; more take attn_cross_kernel.
+    int64_t tok = 0;
+    for (int i = 0; i < n;) {
         const int slot = mgr_.slotOf(seq_ids[i]);
-        for (int t = 0; t < num_queries[i]; t += step)
-            stream_plan_->entries.push_back({slot, lens[static_cast<size_t>(i)], static_cast<int32_t>(tok + t),
-                                             std::min(step, num_queries[i] - t), 0, 0});
-        tok += num_queries[i];
+        const int len = lens[static_cast<size_t>(i)];
+        int       nq = 0;
+        for (const int id = seq_ids[i]; i < n && seq_ids[i] == id && lens[static_cast<size_t>(i)] == len; ++i)
+            nq += num_queries[i];
+        if (len > 0 && nq * static_cast<int64_t>(group) > detail::kStreamRows) {
+            cross_plan_->entries.push_back({slot, len, static_cast<int32_t>(tok), nq, 1, 0});
+        } else {
+            const int step = detail::kStreamRows / group;
+            for (int t = 0; t < nq; t += step)
+                stream_plan_->entries.push_back({slot, len, static_cast<int32_t>(tok + t), std::min(step, nq - t), 0, 0});
+        }
+        tok += nq;
     }
     detail::plan_stream(*stream_plan_, cfg.num_heads, detail::device_cus());
+    if (!detail::plan_cross(*cross_plan_, cfg.head_dim, group, cfg.num_heads, detail::device_cus())) {
+        stream_plan_->clear();
+        cross_plan_->clear();
+        return Result<void>::err("CrossBatch: too many query rows in one step");
+    }
     ids_.assign(seq_ids, seq_ids + n);
     lens_ = std::move(lens);
     n_ = n;
@@ -99,18 +116,34 @@ Result<void> CrossBatch::attention(int layer_idx, const half *q, half *out, floa
         if (sc->current_len < lens_[i])
             return Result<void>::err("CrossBatch: sequence " + std::to_string(ids_[i]) + " is shorter than prepare found it");
     }
-    const size_t floats = detail::stream_workspace_floats(*stream_plan_, num_q_heads_, cfg.num_heads, cfg.head_dim, false);
+    const size_t floats = std::max(
+        detail::stream_workspace_floats(*stream_plan_, num_q_heads_, cfg.num_heads, cfg.head_dim, false),
+        detail::cross_workspace_floats(*cross_plan_, cfg.num_heads, cfg.head_dim));
     if (!work_->holds(floats) && detail::stream_capturing(stream))
         return Result<void>::err("CrossBatch: the workspace cannot grow while the stream is captured: make one call "
                                  "of this size before");
-    detail::StreamCall c;
-    c.q = q;
-    c.out = out;
-    c.scale = scale;
-    c.Hq = num_q_heads_;
-    c.Hkv = cfg.num_heads;
-    c.D = cfg.head_dim;
-    detail::launch_attn_stream(c, mgr_.layerView(layer_idx, nullptr), *stream_plan_, work_->get(floats), stream);
+    float               *ws = work_->get(floats);
+    const detail::KvView view = mgr_.layerView(layer_idx, nullptr);
+    if (!stream_plan_->entries.empty()) {
+        detail::StreamCall c;
+        c.q = q;
+        c.out = out;
+        c.scale = scale;
+        c.Hq = num_q_heads_;
+        c.Hkv = cfg.num_heads;
+        c.D = cfg.head_dim;
+        detail::launch_attn_stream(c, view, *stream_plan_, ws, stream);
+    }
+    if (!cross_plan_->entries.empty()) {
+        detail::CrossCall c;
+        c.q = q;
+        c.out = out;
+        c.scale = scale;
+        c.Hq = num_q_heads_;
+        c.Hkv = cfg.num_heads;
+        c.D = cfg.head_dim;
+        detail::launch_attn_cross(c, view, *cross_plan_, ws, stream);
+    }
     return Result<void>::ok();
 }
 

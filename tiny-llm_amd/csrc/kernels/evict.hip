@@ -181,6 +181,7 @@ template <int NT> __device__ __forceinline__ void pick_bin(const uint32_t *hist,
 // beside or instead of the keys cost more instructions than they saved (34 us).
 template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
     constexpr int NW = NT / 64;
+    static_assert(IT <= 8, "a bit per token");
     // Histogram and list, then the free places (half of the tokens at most).
     __shared__ uint32_t buf[kBins + kList > NT * IT * 2 ? kBins + kList : NT * IT * 2];
     uint32_t *const hist = buf, *const list = buf + kBins, *const places = buf;
@@ -207,6 +208,7 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
 #pragma unroll
         for (int u = 0; u < 4; ++u) keys[it][u] = x.x[u];
     }
+    if (IT > 4) __builtin_amdgcn_sched_barrier(0); // (few registers are left: no positions loaded with these)
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
         const int i = token(it);
@@ -308,13 +310,11 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
     };
     // (all of the bin stay, or none of it yet; not all tokens do, so thr is above 0 then)
     const uint32_t limit = equal == need ? thr - 1u : thr;
-    uint32_t       stays[IT]; // bit u: token(it) + u stays
+    uint32_t       stays = 0; // bit 4 it + u: token(it) + u stays
 #pragma unroll
-    for (int it = 0; it < IT; ++it) {
-        stays[it] = 0;
+    for (int it = 0; it < IT; ++it)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) stays[it] |= (uint32_t)(keys[it][u] > limit) << u;
-    }
+        for (int u = 0; u < 4; ++u) stays |= (uint32_t)(keys[it][u] > limit) << (4 * it + u);
     if (equal != need) { // the first `need` tokens at the threshold
         auto at = [&](int it) {
             uint32_t f = 0;
@@ -327,20 +327,20 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
         for (int it = 0; it < IT; ++it) {
             uint32_t f = at(it);
             for (uint32_t r = before[it * NW + wave] + scan[it]; f && r < need; ++r) {
-                stays[it] |= f & -f;
+                stays |= (f & -f) << 4 * it;
                 f &= f - 1;
             }
         }
     }
 #pragma unroll
     for (int it = 0; it < IT; ++it) // tokens past the end do not stay
-        stays[it] &= token(it) < e.len ? 0xFu >> max(0, token(it) + 4 - e.len) : 0u;
+        stays &= ~((token(it) < e.len ? ~(0xFu >> max(0, token(it) + 4 - e.len)) & 0xFu : 0xFu) << 4 * it);
 
     // What stays in place, and the free places and movers in index order.
     auto moving = [&](int it) { // free places below keep, kept tokens from there on
         const int      i = token(it);
-        const uint32_t low = i >= e.keep ? 0u : 0xFu >> max(0, i + 4 - e.keep); // the tokens below keep
-        return (~stays[it] & low) | (stays[it] & ~low);
+        const uint32_t low = i >= e.keep ? 0u : 0xFu >> max(0, i + 4 - e.keep);
+        return ((stays >> 4 * it) ^ low) & 0xFu; // below keep: those that go, behind it: those that stay
     };
     rank_all(moving);
     const uint32_t moved = s_total / 2; // as many free places as movers
@@ -361,6 +361,7 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
     };
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
+        if (IT > 4) __builtin_amdgcn_sched_barrier(0);
         const int      i = token(it);
         const uint32_t f = moving(it);
         uint32_t       r = before[it * NW + wave] + scan[it];
@@ -384,6 +385,7 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
     __syncthreads();
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
+        if (IT > 4) __builtin_amdgcn_sched_barrier(0);
         const int      i = token(it);
         const uint32_t f = moving(it);
         uint32_t       r = before[it * NW + wave] + scan[it];

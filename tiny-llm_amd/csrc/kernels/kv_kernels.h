@@ -196,7 +196,8 @@ enum class KernelId {
     Evict = 7, // selection and moves of one launch
     AttnStream = 8, // with its finish
     AttnAccount = 9, // statistics and sums of one launch
-    Count = 10
+    AttnCross = 10, // with its merge
+    Count = 11
 };
 void profile_begin(KernelId id, hipStream_t stream);
 void profile_end(KernelId id, hipStream_t stream);

@@ -60,5 +60,41 @@ bool plan_account(AccountPlan &plan, int G, int Hkv, int cus) {
     return true;
 }
 
+bool plan_cross(CrossPlan &plan, int D, int G, int Hkv, int cus) {
+    // 8 waves share a key tile among 256 rows and have a CU to themselves; 4 waves waste
+    // fewer rows of a short entry, two workgroups to a CU.
+    int64_t rows = 0;
+    for (const auto &e : plan.entries) rows += (int64_t)e.nq * G;
+    const bool wide = D <= 128 && D != 64 && !plan.entries.empty() && rows >= 512 * (int64_t)plan.entries.size();
+    plan.waves = wide ? 8 : 4;
+    const int tile = cross_rows(D, plan.waves);
+    int64_t   tiles = 0;
+    for (const auto &e : plan.entries) tiles += ((int64_t)e.nq * G + tile - 1) / tile;
+    // Row tiles that do not fill the chip twice have their keys split, into chunks of
+    // at least four tiles.
+    const int64_t want = (wide ? 2 : 4) * (int64_t)std::max(1, cus);
+    const int64_t split = std::max<int64_t>(1, want / std::max<int64_t>(1, tiles * Hkv));
+    for (auto &e : plan.entries)
+        e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(split, stream_tiles(e.S) / 4));
+    std::stable_sort(plan.entries.begin(), plan.entries.end(), [](const CrossEntry &x, const CrossEntry &y) {
+        return (int64_t)x.S * y.nch > (int64_t)y.S * x.nch;
+    });
+    plan.launches.clear();
+    for (size_t i = 0; i < plan.entries.size();) {
+        CrossLaunch l{(int)i, 0, 0, false};
+        int64_t     items = 0;
+        for (; i < plan.entries.size() && l.n < kCrossBatch; ++i, ++l.n) {
+            CrossEntry &e = plan.entries[i];
+            e.item0 = (int32_t)items;
+            items += ((int64_t)e.nq * G + tile - 1) / tile * e.nch;
+            l.split |= e.nch > 1;
+            if (items * Hkv > INT32_MAX) return false;
+        }
+        l.items = (int)items;
+        plan.launches.push_back(l);
+    }
+    return true;
+}
+
 } // namespace detail
 } // namespace tiny_llm

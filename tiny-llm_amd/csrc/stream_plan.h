@@ -1,6 +1,6 @@
-// How the work of attn_stream_kernel (kernels/attention_stream.hip) and of the
-// prompt's account (kernels/attention_account.hip) is cut: plain C++, unit-tested
-// on the host.
+// How the work of attn_stream_kernel (kernels/attention_stream.hip), of the prompt's
+// account (kernels/attention_account.hip) and of attn_cross_kernel
+// (kernels/attention_cross.hip) is cut: plain C++, unit-tested on the host.
 #pragma once
 
 #include <cstdint>
@@ -64,6 +64,31 @@ struct AccountPlan {
 // Sets nch, stat0, item0 and sum0 of plan.entries, and the launches.  False when
 // a launch's statistics do not fit 31 bits.
 bool plan_account(AccountPlan &plan, int G, int Hkv, int cus);
+
+// Query tokens tok0 .. tok0 + nq - 1 attend to the first S >= 1 tokens of cache row
+// `row`: row tiles (of tokens x heads of one kv head) x nch chunks of its keys are
+// the work items of attn_cross_kernel, item0 those of the entries before it in its
+// launch.
+constexpr int kCrossBatch = 144;
+struct CrossEntry {
+    int32_t row, S, tok0, nq, nch, item0;
+};
+struct CrossLaunch {
+    int  first, n, items;
+    bool split; // some entry has several chunks
+};
+struct CrossPlan {
+    std::vector<CrossEntry>  entries;
+    std::vector<CrossLaunch> launches;
+    int                      waves = 4; // per workgroup
+    void                     clear() { entries.clear(), launches.clear(); }
+};
+// Rows of a workgroup: 32 per wave up to head_dim 128, 16 at 256.
+constexpr int cross_rows(int D, int waves) { return waves * (D <= 128 ? 32 : 16); }
+
+// Sets the waves, nch and item0 of plan.entries and the launches (and orders the
+// entries, longest items first).  False when a launch's items exceed 31 bits.
+bool plan_cross(CrossPlan &plan, int D, int G, int Hkv, int cus);
 
 } // namespace detail
 } // namespace tiny_llm

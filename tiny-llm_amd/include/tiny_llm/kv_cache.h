@@ -38,6 +38,7 @@ struct PrefillInline;
 struct EvictEntry;
 struct StreamPlan;
 struct AccountPlan;
+struct CrossPlan;
 class MetaRing;
 class DeviceRing;
 class Workspace;
@@ -417,7 +418,8 @@ class CrossBatch {
     int                  tokens_ = 0;
     std::vector<int>     ids_;
     std::vector<int32_t> lens_;
-    std::unique_ptr<detail::StreamPlan> stream_plan_;
+    std::unique_ptr<detail::StreamPlan> stream_plan_; // entries of few rows, or over no states
+    std::unique_ptr<detail::CrossPlan>  cross_plan_;  // the others
     std::unique_ptr<detail::Workspace>  work_;
 };
 
