@@ -31,12 +31,16 @@ static void stream_random() {
         const int  n = (int)(rng() % 400), most = 1 << (rng() % 17);
         for (int i = 0; i < n; ++i) p.entries.push_back({i, rng() % 9 ? (int32_t)(rng() % most) : 0, i, 1, -1, -1});
         if (it % 50 == 0 && n) p.entries[0].S = INT32_MAX;
-        plan_stream(p, 1 << (rng() % 6), 1 + (int)(rng() % 300));
-        CHECK(p.chunk >= 4);
+        const int D = 32 << (rng() % 4);
+        const int rows = (int)(rng() % 2) ? 1 << (rng() % 4) : 0;
+        plan_stream(p, 1 << (rng() % 6), D, rows, 1 + (int)(rng() % 300));
+        CHECK(p.chunk >= 1 && (p.waves == 4 || (p.waves == 8 && D <= 128)));
+        for (size_t i = 1; i < p.entries.size(); ++i) CHECK(p.entries[i].S <= p.entries[i - 1].S);
         size_t next = 0;
         for (const auto &l : p.launches) {
             CHECK((size_t)l.first == next && l.n > 0 && l.n <= kStreamBatch);
-            int     items = 0, longest = 0, most_items = 0;
+            int     items = 0, longest = 0;
+            bool    finish = false;
             int64_t tiles = 0;
             for (int i = l.first; i < l.first + l.n; ++i) {
                 const StreamEntry &e = p.entries[(size_t)i];
@@ -54,8 +58,8 @@ static void stream_random() {
                 if (k <= 50) CHECK(at == t);
                 items += k;
                 tiles += t;
-                longest = std::max(longest, (int)e.S);
-                most_items = std::max(most_items, k);
+                if (k > 1) longest = std::max(longest, (int)e.S);
+                finish |= k != 1;
             }
             // the kernel's search: the last entry that starts at or before the item
             for (int item = 0; item < std::min(items, 200); ++item) {
@@ -65,10 +69,18 @@ static void stream_random() {
                 const StreamEntry &e = p.entries[(size_t)found];
                 CHECK(item - e.item0 >= 0 && item - e.item0 < stream_items(e.S, p.chunk));
             }
-            CHECK(l.items == items && l.tiles == tiles && l.max_len == longest && l.max_items == most_items);
+            CHECK(l.items == items && l.tiles == tiles && l.max_len == longest && l.finish == finish);
             next += (size_t)l.n;
         }
         CHECK(next == p.entries.size());
+        // what the kernel keeps in LDS fits
+        int item = 0;
+        for (const auto &e : p.entries) {
+            const int64_t t = stream_tiles(e.S), k = stream_items(e.S, p.chunk);
+            for (int64_t c = 0; c < std::min<int64_t>(k, 50); ++c) item = std::max(item, (int)((c + 1) * t / k - c * t / k));
+        }
+        CHECK(item <= p.most && p.most <= p.chunk && (p.depth == 1 || (p.depth == 2 && p.waves == 4 && D <= 128)));
+        if (rows) CHECK((int64_t)p.waves * stream_stage_bytes(D, true) + (int64_t)p.most * kStreamTile * rows * 4 <= kStreamLds);
     }
     std::puts("ok stream_random");
 }

@@ -86,7 +86,7 @@ Result<void> CrossBatch::prepare(const int *seq_ids, const int *num_queries, con
         }
         tok += nq;
     }
-    detail::plan_stream(*stream_plan_, cfg.num_heads, detail::device_cus());
+    detail::plan_stream(*stream_plan_, cfg.num_heads, cfg.head_dim, 0, detail::device_cus());
     if (!detail::plan_cross(*cross_plan_, cfg.head_dim, group, cfg.num_heads, detail::device_cus())) {
         stream_plan_->clear();
         cross_plan_->clear();

@@ -13,10 +13,10 @@
 // workspace.  They and the sums are fp32: an account is compared with others of
 // like size.
 //
-// attn_stream_kernel: a workgroup of 4 waves per (entry, chunk of tiles, kv head);
-// wave w takes every fourth tile of 64 tokens (32 at head_dim 256) and keeps its own
-// running maximum, sum and output; the next tile's rows are on their way while
-// one is computed.
+// attn_stream_kernel: a workgroup of 4 or 8 waves per (entry, chunk of tiles, kv
+// head); wave w takes every 4th (8th) tile of 64 tokens (32 at head_dim 256) and keeps
+// its own running maximum, sum and output; the next tile's rows are on their way
+// while one is computed.  A workgroup that has a whole entry finishes it.
 //   S^T = K Q^T      v_mfma_f32_16x16x32_f16: A = K rows (token l%16, dims
 //                    8(l/16)..+7) straight from memory, B = Q (row l%16),
 //                    D = S^T (tokens 4(l/16)+i, row l%16)
@@ -26,7 +26,8 @@
 //                    stays fp32)
 //   O^T += V^T P^T   over 32 tokens; V^T from the wave's row-major LDS stage by
 //                    the transposing ds_read_b64_tr_b16
-// stream_finish_kernel: merges the chunks' outputs and turns scores into the account.
+// stream_finish_kernel: merges the outputs of entries with several chunks and turns
+// their scores into the account.
 #include "stream.h"
 
 #include "tiny_llm/hip_utils.h"
@@ -35,6 +36,7 @@
 
 #include <algorithm>
 #include <cstring>
+#include <mutex>
 #include <stdexcept>
 
 namespace tiny_llm {
@@ -42,12 +44,12 @@ namespace detail {
 
 namespace {
 
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float    f32x4 __attribute__((ext_vector_type(4)));
 typedef short    s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int   kWaves = 4;
 constexpr float kLazyMax = 8.0f;
 
 struct StreamArgs {
@@ -58,12 +60,12 @@ struct StreamArgs {
     float        *w_out;
     float        *part_o;  // [item][Hkv][16 rows at most][D]
     float        *part_ml; // [item][Hkv][rows][2]
-    float        *scores;  // [tile0 * Hkv + g * tiles][rows][tiles * 64]
+    float        *scores;  // [tile0 * Hkv + g * tiles + tile][rows][64]
     KvView        kv;
     int64_t       room;
     int           fresh;
     float         scale_log2;
-    int           Hq, Hkv, G, n, chunk, entry0, rows; // rows: of the partials, nq * G at most
+    int           Hq, Hkv, G, n, chunk, rows; // rows: of the partials, nq * G at most
     StreamEntry   e[kStreamBatch];
 };
 static_assert(sizeof(StreamArgs) <= 4096, "kernel arguments");
@@ -90,17 +92,60 @@ __device__ __forceinline__ void wave_sync_lds() {
         out = __builtin_amdgcn_readfirstlane(seen_ - 1);                                                               \
     } while (0)
 
-template <int D, bool PAGED, bool SCORES>
-__global__ __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(StreamArgs a) {
+// Four consecutive fp32 values; the rows of accounts begin at any multiple of 4 bytes.
+struct __attribute__((packed, aligned(4))) Four {
+    float x[4];
+};
+
+// The account of tokens [t_lo, t_hi) of entry ei and kv head g, t_lo a multiple of a
+// tile, from their scores (sc: [tile][rows][64], in LDS or memory), the rows' final
+// maxima and the inverse of their sums (in LDS).
+template <int NT>
+__device__ __forceinline__ void account_tokens(const StreamArgs &a, int ei, int g, int rows, int t_lo, int t_hi,
+                                               const float *sc, const float *m, const float *inv) {
+    const int     old = a.e[ei].S - a.fresh;
+    const int64_t base = ((int64_t)a.e[ei].row * a.Hkv + g) * a.room;
+    for (int t = t_lo + 4 * (int)threadIdx.x; t < t_hi; t += 4 * NT) {
+        Four w = {};
+        if (a.w_in && t + 4 <= old) w = *reinterpret_cast<const Four *>(a.w_in + base + t);
+        else if (a.w_in) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (t + i < old) w.x[i] = a.w_in[base + t + i];
+        }
+        const float *st = sc + (int64_t)((t - t_lo) / kStreamTile) * rows * kStreamTile + t % kStreamTile;
+        f32x4        sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int r = 0; r < rows; ++r) { // (scores past the end are -infinity)
+            const f32x4 s = *reinterpret_cast<const f32x4 *>(st + r * kStreamTile);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sum[i] = fmaf(__builtin_amdgcn_exp2f(s[i] - m[r]), inv[r], sum[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.x[i] += sum[i];
+        if (t + 4 <= t_hi) *reinterpret_cast<Four *>(a.w_out + base + t) = w;
+        else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (t + i < t_hi) a.w_out[base + t + i] = w.x[i];
+        }
+    }
+}
+
+// DEPTH steps' rows are on their way at once.  Dynamic LDS: the waves' V stages, then
+// with SCORES the chunk's scores.
+template <int D, bool PAGED, bool SCORES, int NW, int DEPTH>
+__global__ __launch_bounds__(NW * 64, D <= 128 && DEPTH == 1 ? 2 : 1) void attn_stream_kernel(StreamArgs a) {
     constexpr int TK = D <= 128 ? 64 : 32; // tokens of a wave's step
     constexpr int SUB = kStreamTile / TK;  // steps per tile
     constexpr int TT = TK / 16;
     constexpr int KS = D / 32, DT = D / 16, KP = D / 8;
     constexpr int NV = TK * KP / 64;       // V pieces per lane
+    constexpr int NQ = NV / TT;            // ... of 16 tokens
     constexpr int RPI = 64 / KP;           // V rows per load instruction
-    constexpr int STAGE = TK * D > 16 * D * 2 ? TK * D : 16 * D * 2; // halves: V rows, then o[16][D] fp32
-    __shared__ __align__(16) uint16_t stage[kWaves][STAGE];
-    __shared__ float sm[kWaves][16], sl[kWaves][16];
+    constexpr int ROWS = SCORES ? kStreamRows / 2 : kStreamRows;
+    constexpr int STAGE = stream_stage_bytes(D, SCORES) / 2; // halves: 16 V rows, then o[ROWS][D] fp32
+    extern __shared__ __align__(16) uint16_t smem[];
+    __shared__ float sm[NW][16], sl[NW][16], s_m[16], s_l[16], s_inv[16];
     // 16-byte piece x of row r at slot x ^ swz(r): the transposing reads of rows
     // 4 apart and of neighbours fall on distinct banks.
     auto swz = [](int r) {
@@ -125,16 +170,14 @@ __global__ __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) void attn_stream_ker
     const int64_t  blk_bytes = a.kv.blk_stride * 2, tokb = a.kv.tok_stride * 2;
     const int32_t *bt = PAGED ? a.kv.block_table + (int64_t)row * a.kv.bt_stride : nullptr;
     const int      mask = (1 << a.kv.log2_blk) - 1;
-    auto token_off = [&](int t) -> int64_t {
-        if constexpr (PAGED) return (int64_t)bt[t >> a.kv.log2_blk] * blk_bytes + (int64_t)(t & mask) * tokb;
-        else return (int64_t)row * blk_bytes + (int64_t)t * tokb;
-    };
 
     if (a.new_k && ch == nch - 1) { // the new token's row, then read like any other
         if ((int)threadIdx.x < 2 * KP) {
-            const int     which = threadIdx.x / KP, x = threadIdx.x - which * KP;
-            const __half *src = (which ? a.new_v : a.new_k) + ((int64_t)(a.entry0 + ei) * a.Hkv + g) * D + 8 * x;
-            char         *dst = const_cast<char *>(which ? vb : kb) + token_off(S - 1) + 16 * x;
+            const int     which = threadIdx.x / KP, x = threadIdx.x - which * KP, t = S - 1;
+            const __half *src = (which ? a.new_v : a.new_k) + ((int64_t)tok0 * a.Hkv + g) * D + 8 * x;
+            const int64_t off = PAGED ? (int64_t)bt[t >> a.kv.log2_blk] * blk_bytes + (int64_t)(t & mask) * tokb
+                                      : (int64_t)row * blk_bytes + (int64_t)t * tokb;
+            char         *dst = const_cast<char *>(which ? vb : kb) + off + 16 * x;
             *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
         }
         __threadfence_block();
@@ -154,77 +197,84 @@ __global__ __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) void attn_stream_ker
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = -INFINITY, l_run = 0.0f;
 
-    // Offset of the 16 tokens from t on, and how many of them may be read past the first.
-    auto quarter = [&](int t, int &more) -> int64_t {
-        const int tq = min(t, last);
-        more = min(15, last - tq);
-        return token_off(tq);
+    // The wave's steps: step x of the chunk's tiles, tile tile_lo + x / SUB * NW + wave.
+    const int steps = max(0, (tile_hi - tile_lo - wave + NW - 1) / NW) * SUB;
+    auto start = [&](int x) { return (tile_lo + x / SUB * NW + wave) * kStreamTile + x % SUB * TK; };
+    // Block ids of a step's quarters of 16 tokens, lane k that of quarter k (paged
+    // views): loaded a step before the rows they address, which so wait for nothing.
+    auto blocks = [&](int x) -> int {
+        if constexpr (PAGED) return lane < TT ? bt[min(start(x) + 16 * lane, last) >> a.kv.log2_blk] : 0;
+        else return 0;
     };
-    f16x8 kf[TT][KS];
-    u32x4 vr[NV];
-    auto load_k = [&](int t0) __attribute__((always_inline)) {
+    // Offset of the 16 tokens from quarter k on (its first token clamped to the last
+    // one), and how many of them may be read past the first.
+    auto quarter = [&](int t0, int k, int ids, int &more) __attribute__((always_inline)) -> int64_t {
+        const int tq = min(t0 + 16 * k, last);
+        more = min(15, last - tq);
+        if constexpr (PAGED)
+            return (int64_t)__builtin_amdgcn_readlane(ids, k) * blk_bytes + (int64_t)(tq & mask) * tokb;
+        else return (int64_t)row * blk_bytes + (int64_t)tq * tokb;
+    };
+    f16x8 kf[DEPTH][TT][KS];
+    u32x4 vr[DEPTH][NV];
+    auto load_k = [&](int x, int ids, f16x8(&k)[TT][KS]) __attribute__((always_inline)) {
+        const int t0 = __builtin_amdgcn_readfirstlane(start(x));
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
             int            more;
-            const char    *p = kb + quarter(t0 + 16 * tt, more);
+            const char    *p = kb + quarter(t0, tt, ids, more);
             const uint32_t off = (uint32_t)min(c, more) * (uint32_t)tokb + 16 * qg;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) kf[tt][s] = *reinterpret_cast<const f16x8 *>(p + off + 64 * s);
+            for (int s = 0; s < KS; ++s) k[tt][s] = *reinterpret_cast<const f16x8 *>(p + off + 64 * s);
         }
     };
-    auto load_v = [&](int t0) __attribute__((always_inline)) {
+    auto load_v = [&](int x, int ids, u32x4(&v)[NV]) __attribute__((always_inline)) {
+        const int t0 = __builtin_amdgcn_readfirstlane(start(x));
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
             const int      r = (u * RPI) % 16 + lane / KP; // in its quarter
             int            more;
-            const char    *p = vb + quarter(t0 + u * RPI / 16 * 16, more);
+            const char    *p = vb + quarter(t0, u * RPI / 16, ids, more);
             const uint32_t off = (uint32_t)min(r, more) * (uint32_t)tokb + 16 * (lane % KP);
-            vr[u] = *reinterpret_cast<const u32x4 *>(p + off);
+            // (whole lines, read once; K's lines are read in halves, which the hint made slower)
+            v[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + off));
         }
     };
-    uint16_t *vst = stage[wave];
+    uint16_t *vst = smem + wave * STAGE;
+    float    *lsc = reinterpret_cast<float *>(smem + NW * STAGE); // [tile of the chunk][rows][64]
     const int vrow = 4 * qg + (c >> 2);
-    const int vxor = ((c & 3) >> 1) ^ swz(vrow);
-    const int vlane = vrow * KP * 8 + 4 * (c & 1);
-    auto vt_read = [&](int r0, int dt) __attribute__((always_inline)) {
-        return __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr(&vst[vlane + ((2 * dt) ^ vxor) * 8 + r0 * KP * 8]));
-    };
-    float *srow = nullptr;
-    if constexpr (SCORES)
-        srow = a.scores + (((int64_t)a.e[ei].tile0 * a.Hkv + (int64_t)g * tiles) * a.rows + (int64_t)c * tiles) * kStreamTile;
+    const int vlane = vrow * KP * 8 + 4 * (c & 1), vxor = ((c & 3) >> 1) ^ swz(vrow);
 
-    // The wave's steps: step x of the chunk's tiles, tile tile_lo + x / SUB * kWaves + wave.
-    const int steps = max(0, (tile_hi - tile_lo - wave + kWaves - 1) / kWaves) * SUB;
-    auto start = [&](int x) { return (tile_lo + x / SUB * kWaves + wave) * kStreamTile + x % SUB * TK; };
-    if (steps > 0) {
-        load_k(start(0));
-        load_v(start(0));
-    }
-    for (int x = 0; x < steps; ++x) {
-        const int t0 = start(x);
-        f32x4     s[TT];
+    // One step: its rows are in k and v; those of step x + DEPTH take their place.
+    int  ids_next = 0;
+    auto step = [&](int x, f16x8(&k)[TT][KS], u32x4(&v)[NV]) __attribute__((always_inline)) {
+        const int  t0 = start(x);
+        const bool more = x + DEPTH < steps;
+        const int  ids = ids_next;
+        if (PAGED && x + DEPTH + 1 < steps) ids_next = blocks(x + DEPTH + 1);
+        f32x4 s[TT];
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
             s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int k = 0; k < KS; ++k) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tt][k], qb[k], s[tt], 0, 0, 0);
+            for (int i = 0; i < KS; ++i) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[tt][i], qb[i], s[tt], 0, 0, 0);
         }
-        if (x + 1 < steps) load_k(start(x + 1));
+        if (more) load_k(x + DEPTH, ids, k);
         const int tb = t0 + 4 * qg;
         float     mloc = -INFINITY;
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float v = s[tt][i] * a.scale_log2;
-                s[tt][i] = tb + 16 * tt + i <= last ? v : -INFINITY;
+                const float y = s[tt][i] * a.scale_log2;
+                s[tt][i] = tb + 16 * tt + i <= last ? y : -INFINITY;
                 mloc = fmaxf(mloc, s[tt][i]);
             }
         if constexpr (SCORES) {
+            float *dst = lsc + (t0 / kStreamTile - tile_lo) * rows * kStreamTile + t0 % kStreamTile + c * kStreamTile + 4 * qg;
             if (c < rows)
 #pragma unroll
-                for (int tt = 0; tt < TT; ++tt)
-                    *reinterpret_cast<f32x4 *>(srow + tb + 16 * tt) = s[tt];
+                for (int tt = 0; tt < TT; ++tt) *reinterpret_cast<f32x4 *>(dst + 16 * tt) = s[tt];
         }
         if (__any(mloc > m_run + kLazyMax)) {
             mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
@@ -236,116 +286,142 @@ __global__ __launch_bounds__(kWaves * 64, D <= 128 ? 2 : 1) void attn_stream_ker
             l_run *= alpha;
             m_run = m_new;
         }
-        f16x8 pf[TT / 2];
+        f16x4 pf[TT];
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float p = s[tt][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[tt][i] - m_run);
                 l_run += p;
-                pf[tt >> 1][4 * (tt & 1) + i] = (_Float16)p;
+                pf[tt][i] = (_Float16)p;
             }
+        // 16 tokens at a time through the stage (a wave's LDS operations keep their order).
 #pragma unroll
-        for (int u = 0; u < NV; ++u) {
-            const int r = u * RPI + lane / KP;
-            *reinterpret_cast<u32x4 *>(&vst[(r * KP + ((lane % KP) ^ swz(r))) * 8]) = vr[u];
-        }
-        if (x + 1 < steps) load_v(start(x + 1));
-        wave_sync_lds();
+        for (int q = 0; q < TT; ++q) {
 #pragma unroll
-        for (int tp = 0; tp < TT / 2; ++tp)
+            for (int u = 0; u < NQ; ++u) {
+                const int r = u * RPI + lane / KP;
+                *reinterpret_cast<u32x4 *>(&vst[(r * KP + ((lane % KP) ^ swz(r))) * 8]) = v[q * NQ + u];
+            }
+            wave_sync_lds();
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const uint2 v0 = __builtin_bit_cast(uint2, vt_read(32 * tp, dt));
-                const uint2 v1 = __builtin_bit_cast(uint2, vt_read(32 * tp + 16, dt));
-                const f16x8 vf = __builtin_bit_cast(f16x8, make_uint4(v0.x, v0.y, v1.x, v1.y));
-                acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[tp], acc[dt], 0, 0, 0);
+                const s16x4 vt = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr(&vst[vlane + ((2 * dt) ^ vxor) * 8]));
+                acc[dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, vt), pf[q], acc[dt], 0, 0, 0);
             }
-        wave_sync_lds(); // the stage is rewritten by the next step
+            wave_sync_lds();
+        }
+        if (more) load_v(x + DEPTH, ids, v);
+    };
+#pragma unroll
+    for (int d = 0; d < DEPTH; ++d)
+        if (d < steps) {
+            const int ids = blocks(d);
+            load_k(d, ids, kf[d]);
+            load_v(d, ids, vr[d]);
+        }
+    if (PAGED && DEPTH < steps) ids_next = blocks(DEPTH);
+    for (int x = 0; x < steps; x += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d)
+            if (x + d < steps) step(x + d, kf[d], vr[d]);
     }
 
     // The waves' (m, l, o) through LDS.
     l_run += __shfl_xor(l_run, 16);
     l_run += __shfl_xor(l_run, 32);
     float *so = reinterpret_cast<float *>(vst);
+    if (c < ROWS)
 #pragma unroll
-    for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(so + c * D + 16 * dt + 4 * qg) = acc[dt];
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(so + c * D + 16 * dt + 4 * qg) = acc[dt];
     if (qg == 0) {
         sm[wave][c] = m_run;
         sl[wave][c] = l_run;
     }
     __syncthreads();
-    for (int idx = threadIdx.x; idx < rows * D; idx += kWaves * 64) {
-        const int r = idx / D, d = idx - r * D;
-        float     m = sm[0][r];
+    if ((int)threadIdx.x < rows) {
+        const int r = threadIdx.x;
+        float     m = sm[0][r], l = 0.0f;
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) m = fmaxf(m, sm[w][r]);
-        float o = 0.0f, l = 0.0f;
+        for (int w = 1; w < NW; ++w) m = fmaxf(m, sm[w][r]);
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < NW; ++w) { // sm: the waves' weights
             const float wgt = sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][r] - m);
-            o = fmaf(wgt, reinterpret_cast<const float *>(stage[w])[idx], o);
             l = fmaf(wgt, sl[w][r], l);
+            sm[w][r] = wgt;
         }
-        const int64_t pr = ((int64_t)item * a.Hkv + g) * a.rows + r;
+        s_m[r] = m;
+        s_l[r] = l;
+        s_inv[r] = 1.0f / l;
+        if (nch > 1)
+            *reinterpret_cast<float2 *>(a.part_ml + (((int64_t)item * a.Hkv + g) * a.rows + r) * 2) = make_float2(m, l);
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < rows * D; idx += NW * 64) {
+        const int r = idx / D, d = idx - r * D;
+        float     o = 0.0f;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) o = fmaf(sm[w][r], reinterpret_cast<const float *>(smem + w * STAGE)[idx], o);
+        if (nch == 1)
+            a.out[((int64_t)(tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D + d] = __float2half(o * (1.0f / (s_l[r] + 1e-6f)));
+        else a.part_o[(((int64_t)item * a.Hkv + g) * a.rows + r) * D + d] = o;
+    }
+    if constexpr (SCORES) {
         if (nch == 1) {
-            a.out[((int64_t)(tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D + d] = __float2half(o * (1.0f / (l + 1e-6f)));
-        } else {
-            a.part_o[pr * D + d] = o;
+            account_tokens<NW * 64>(a, ei, g, rows, 0, S, lsc, s_m, s_inv);
+        } else { // the chunk's scores in one go
+            float *dst = a.scores + ((int64_t)a.e[ei].tile0 * a.Hkv + (int64_t)g * tiles + tile_lo) * a.rows * kStreamTile;
+            for (int k = threadIdx.x; k < (tile_hi - tile_lo) * rows * (kStreamTile / 4); k += NW * 64)
+                *reinterpret_cast<f32x4 *>(dst + 4 * k) = *reinterpret_cast<const f32x4 *>(lsc + 4 * k);
         }
-        if (d == 0) *reinterpret_cast<float2 *>(a.part_ml + pr * 2) = make_float2(m, l);
     }
 }
 
 constexpr int kFinishThreads = 256;
 constexpr int kFinishTokens = 1024; // tokens of a workgroup
 
-// Workgroup (entry, kv head, block of tokens): the rows' maxima and sums over the
-// entry's chunks, the account of the block's tokens, and in block 0 the
-// outputs of an entry with several chunks (or none: zeros).
+// Entries of several chunks (or none: zero rows).  Workgroup (entry, kv head, block
+// of tokens): the rows' maxima and sums over the chunks, the account of the
+// block's tokens, and in block 0 the outputs.
 __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArgs a, int D) {
     __shared__ float s_m[kStreamRows], s_l[kStreamRows], s_inv[kStreamRows];
     const int ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv;
-    const int row = a.e[ei].row, S = a.e[ei].S, tok0 = a.e[ei].tok0, rows = a.e[ei].nq * a.G;
+    const int S = a.e[ei].S, tok0 = a.e[ei].tok0, rows = a.e[ei].nq * a.G;
     const int tiles = (S + kStreamTile - 1) / kStreamTile;
     const int nch = (tiles + a.chunk - 1) / a.chunk;
     const int t_lo = blockIdx.y * kFinishTokens, t_hi = min(S, t_lo + kFinishTokens);
-    const bool merge = blockIdx.y == 0 && nch != 1;
-    if (t_lo >= t_hi && !merge) return;
+    if (nch == 1 || (blockIdx.y > 0 && t_lo >= t_hi)) return;
     const int64_t p0 = ((int64_t)a.e[ei].item0 * a.Hkv + g) * a.rows; // row 0 of chunk 0
     const int64_t pc = (int64_t)a.Hkv * a.rows;                      // from chunk to chunk
     const int     lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int r = wave; r < rows; r += kFinishThreads / 64) {
         float m = -INFINITY, l = 0.0f;
-        for (int ch = lane; ch < nch; ch += 64) m = fmaxf(m, a.part_ml[(p0 + ch * pc + r) * 2]);
-        for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
         for (int ch = lane; ch < nch; ch += 64) {
             const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (p0 + ch * pc + r) * 2);
-            l = fmaf(ml.y, __builtin_amdgcn_exp2f(ml.x - m), l);
+            const float  mn = fmaxf(m, ml.x);
+            l = fmaf(l, __builtin_amdgcn_exp2f(m - mn), ml.y * __builtin_amdgcn_exp2f(ml.x - mn));
+            m = mn;
         }
+        float mx = m;
+        for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+        l = m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - mx);
         for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
         if (lane == 0) {
-            s_m[r] = m;
+            s_m[r] = mx;
             s_l[r] = l;
             s_inv[r] = 1.0f / l;
         }
     }
     __syncthreads();
-    if (a.w_out) {
-        const float  *sc = a.scores + ((int64_t)a.e[ei].tile0 * a.Hkv + (int64_t)g * tiles) * a.rows * kStreamTile;
-        const int64_t base = ((int64_t)row * a.Hkv + g) * a.room;
-        for (int t = t_lo + (int)threadIdx.x; t < t_hi; t += kFinishThreads) {
-            float w = 0.0f;
-            for (int r = 0; r < rows; ++r)
-                w = fmaf(__builtin_amdgcn_exp2f(sc[(int64_t)r * tiles * kStreamTile + t] - s_m[r]), s_inv[r], w);
-            if (a.w_in && t < S - a.fresh) w += a.w_in[base + t];
-            a.w_out[base + t] = w;
-        }
+    if (a.w_out) { // (a launch with accounts has entries of one query: rows = a.rows)
+        const float *sc = a.scores + ((int64_t)a.e[ei].tile0 * a.Hkv + (int64_t)g * tiles + t_lo / kStreamTile) * a.rows * kStreamTile;
+        account_tokens<kFinishThreads>(a, ei, g, rows, t_lo, t_hi, sc, s_m, s_inv);
     }
-    if (!merge) return;
+    if (blockIdx.y > 0) return;
     for (int idx = threadIdx.x; idx < rows * D; idx += kFinishThreads) {
         const int r = idx / D, d = idx - r * D;
         float     o = 0.0f;
+#pragma unroll 4
         for (int ch = 0; ch < nch; ++ch) {
             const int64_t pr = p0 + ch * pc + r;
             o = fmaf(a.part_o[pr * D + d], __builtin_amdgcn_exp2f(a.part_ml[pr * 2] - s_m[r]), o);
@@ -355,15 +431,35 @@ __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArg
     }
 }
 
-template <int D> void launch_d(const StreamArgs &a, int items, bool paged, bool scores, hipStream_t stream) {
-    const dim3 grid((unsigned)items * (unsigned)a.Hkv), block(kWaves * 64);
-    if (paged) {
-        if (scores) hipLaunchKernelGGL((attn_stream_kernel<D, true, true>), grid, block, 0, stream, a);
-        else hipLaunchKernelGGL((attn_stream_kernel<D, true, false>), grid, block, 0, stream, a);
-    } else {
-        if (scores) hipLaunchKernelGGL((attn_stream_kernel<D, false, true>), grid, block, 0, stream, a);
-        else hipLaunchKernelGGL((attn_stream_kernel<D, false, false>), grid, block, 0, stream, a);
+template <int D, bool PAGED, bool SCORES, int NW, int DEPTH>
+void launch_one(const StreamArgs &a, int items, int lds, hipStream_t stream) {
+    auto                 *fn = attn_stream_kernel<D, PAGED, SCORES, NW, DEPTH>;
+    static std::once_flag once;
+    std::call_once(once, [&] {
+        HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      kStreamLds));
+    });
+    hipLaunchKernelGGL(fn, dim3((unsigned)items * (unsigned)a.Hkv), dim3(NW * 64), lds, stream, a);
+}
+template <int D, bool SCORES> void launch_ds(const StreamArgs &a, int items, bool paged, const StreamPlan &plan, hipStream_t stream) {
+    const int lds = plan.waves * stream_stage_bytes(D, SCORES) + (SCORES ? plan.most * kStreamTile * a.rows * 4 : 0);
+#define TL_STREAM(NW, DEPTH)                                                                                           \
+    do {                                                                                                               \
+        if (paged) launch_one<D, true, SCORES, NW, DEPTH>(a, items, lds, stream);                                      \
+        else launch_one<D, false, SCORES, NW, DEPTH>(a, items, lds, stream);                                           \
+        return;                                                                                                        \
+    } while (0)
+    if constexpr (D <= 128) {
+        if (plan.waves == 8) TL_STREAM(8, 1);
+        if constexpr (SCORES)
+            if (plan.depth == 2) TL_STREAM(4, 2);
     }
+    TL_STREAM(4, 1);
+#undef TL_STREAM
+}
+template <int D> void launch_d(const StreamArgs &a, int items, bool paged, const StreamPlan &plan, hipStream_t stream) {
+    if (a.w_out) launch_ds<D, true>(a, items, paged, plan, stream);
+    else launch_ds<D, false>(a, items, paged, plan, stream);
 }
 
 int plan_rows(const StreamPlan &plan, int first, int n, int G) {
@@ -406,7 +502,6 @@ void launch_attn_stream(const StreamCall &c, const KvView &kv, const StreamPlan 
     for (const auto &l : plan.launches) {
         if (l.n == 0) continue;
         a.n = l.n;
-        a.entry0 = l.first;
         a.rows = plan_rows(plan, l.first, l.n, a.G);
         if (a.rows > kStreamRows) throw std::invalid_argument("attention: too many query rows per entry");
         if ((int64_t)l.items * c.Hkv > INT32_MAX) throw std::invalid_argument("attention: too many work items");
@@ -417,17 +512,15 @@ void launch_attn_stream(const StreamCall &c, const KvView &kv, const StreamPlan 
         profile_begin(KernelId::AttnStream, stream);
         if (l.items > 0) {
             switch (c.D) {
-            case 32: launch_d<32>(a, l.items, paged, c.w_out != nullptr, stream); break;
-            case 64: launch_d<64>(a, l.items, paged, c.w_out != nullptr, stream); break;
-            case 128: launch_d<128>(a, l.items, paged, c.w_out != nullptr, stream); break;
-            case 256: launch_d<256>(a, l.items, paged, c.w_out != nullptr, stream); break;
+            case 32: launch_d<32>(a, l.items, paged, plan, stream); break;
+            case 64: launch_d<64>(a, l.items, paged, plan, stream); break;
+            case 128: launch_d<128>(a, l.items, paged, plan, stream); break;
+            case 256: launch_d<256>(a, l.items, paged, plan, stream); break;
             default: throw std::invalid_argument("attention: unsupported head_dim");
             }
             HIP_CHECK(hipGetLastError());
         }
-        bool none = false;
-        for (int i = l.first; i < l.first + l.n; ++i) none |= plan.entries[(size_t)i].S == 0;
-        if (c.w_out || none || l.max_items > 1) {
+        if (l.finish) {
             const unsigned blocks = c.w_out ? (unsigned)std::max(1, (l.max_len + kFinishTokens - 1) / kFinishTokens) : 1u;
             hipLaunchKernelGGL(stream_finish_kernel, dim3((unsigned)(l.n * c.Hkv), blocks), dim3(kFinishThreads), 0, stream,
                                a, c.D);

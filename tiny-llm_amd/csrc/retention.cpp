@@ -70,7 +70,7 @@ Result<void> DecodeBatch::decodeWeights(int layer_idx, const half *q, const half
     if (plan.entries.empty()) {
         for (int i = 0; i < n_; ++i)
             plan.entries.push_back({slot_[static_cast<size_t>(i)], lens_[static_cast<size_t>(i)], i, 1, 0, 0});
-        detail::plan_stream(plan, cfg.num_heads, detail::device_cus());
+        detail::plan_stream(plan, cfg.num_heads, cfg.head_dim, num_q_heads_ / cfg.num_heads, detail::device_cus());
     }
     const size_t floats = detail::stream_workspace_floats(plan, num_q_heads_, cfg.num_heads, cfg.head_dim, true);
     if (!account_work_->holds(floats) && detail::stream_capturing(stream))

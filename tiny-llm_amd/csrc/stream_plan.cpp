@@ -6,17 +6,48 @@
 namespace tiny_llm {
 namespace detail {
 
-void plan_stream(StreamPlan &plan, int Hkv, int cus) {
-    // A workgroup's four waves take tiles in turn, so a chunk has at least
-    // four; two workgroups fit a CU, and eight rounds of them even out what
-    // the lengths leave uneven.
-    int64_t total = 0;
-    for (const auto &e : plan.entries) total += stream_tiles(e.S);
-    const int64_t slots = 4 * (int64_t)std::max(1, cus);
-    plan.chunk = (int)std::min<int64_t>(std::max<int64_t>(4, (total * Hkv + slots - 1) / slots), 1 << 20);
+void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
+    std::stable_sort(plan.entries.begin(), plan.entries.end(),
+                     [](const StreamEntry &x, const StreamEntry &y) { return x.S > y.S; });
+    int64_t total = 0, some = 0;
+    for (const auto &e : plan.entries) {
+        total += stream_tiles(e.S);
+        some += e.S > 0;
+    }
+    total *= Hkv;
+    const int64_t longest = plan.entries.empty() ? 0 : stream_tiles(plan.entries.front().S);
+    const int64_t n = std::max(1, cus);
+    int64_t       chunk;
+    // An entry in one chunk is finished by its own workgroup: no partial results, no
+    // second launch, and its scores never leave the LDS.  That pays while no entry is
+    // much longer than a workgroup's share of all tiles; short ones are not worth
+    // splitting at all.
+    if (D <= 128 && some * Hkv <= n) { // few entries: eight waves each, one workgroup per CU
+        plan.waves = 8;
+        chunk = std::max<int64_t>(kStreamWhole, (total + n - 1) / n);
+    } else {
+        plan.waves = 4;
+        const int64_t share = (total + 2 * n - 1) / (2 * n);
+        chunk = longest <= std::max<int64_t>(kStreamWhole, 2 * share + share / 2) ? longest : std::max<int64_t>(8, (share + 1) / 2);
+    }
+    if (account_rows > 0) {
+        const int64_t fits = stream_most_tiles(D, plan.waves, account_rows);
+        if (chunk > fits) // (equal chunks)
+            chunk = std::min(fits, (longest + (longest + fits - 1) / fits - 1) / std::max<int64_t>(1, (longest + fits - 1) / fits));
+    }
+    plan.chunk = (int)std::max<int64_t>(1, std::min<int64_t>(chunk, 1 << 24));
+    plan.most = 0;
+    for (const auto &e : plan.entries) {
+        const int t = stream_tiles(e.S), k = stream_items(e.S, plan.chunk);
+        if (k) plan.most = std::max(plan.most, (t + k - 1) / k);
+    }
+    // Where the scores leave room for one workgroup per CU, its four waves have twice
+    // the registers, for twice the rows on their way.
+    const int64_t lds = plan.waves * stream_stage_bytes(D, true) + (int64_t)plan.most * kStreamTile * account_rows * 4;
+    plan.depth = account_rows > 0 && D <= 128 && plan.waves == 4 && lds > kStreamLds / 2 ? 2 : 1;
     plan.launches.clear();
     for (size_t i = 0; i < plan.entries.size();) {
-        StreamLaunch l{(int)i, 0, 0, 0, 0, 0};
+        StreamLaunch l{(int)i, 0, 0, 0, false, 0};
         for (; i < plan.entries.size() && l.n < kStreamBatch; ++i, ++l.n) {
             StreamEntry &e = plan.entries[i];
             const int    items = stream_items(e.S, plan.chunk);
@@ -24,8 +55,8 @@ void plan_stream(StreamPlan &plan, int Hkv, int cus) {
             e.tile0 = (int32_t)l.tiles;
             l.items += items;
             l.tiles += stream_tiles(e.S);
-            l.max_items = std::max(l.max_items, items);
-            l.max_len = std::max(l.max_len, e.S);
+            l.finish |= items != 1;
+            if (items > 1) l.max_len = std::max(l.max_len, e.S);
         }
         plan.launches.push_back(l);
     }

@@ -10,6 +10,7 @@ namespace tiny_llm {
 namespace detail {
 
 constexpr int kStreamTile = 64;    // keys
+constexpr int kStreamWhole = 32;   // tiles that one workgroup takes whatever else there is
 constexpr int kStreamRows = 16;    // query rows (tokens x heads of one kv head) of an entry at most
 constexpr int kStreamBatch = 144;  // entries per launch: they travel in the kernel arguments
 
@@ -23,21 +24,37 @@ struct StreamEntry {
 // Launch `first`..: n entries, `items` work items (per kv head), `tiles` tiles.
 // Entry e has ceil(tiles_e / chunk) work items of equal size (in tiles, to one).
 struct StreamLaunch {
-    int     first, n, items, max_items, max_len;
+    int     first, n, items, max_len;
+    bool    finish; // some entry has several chunks, or no tokens
     int64_t tiles;
 };
 struct StreamPlan {
     std::vector<StreamEntry>  entries;
     std::vector<StreamLaunch> launches;
     int                       chunk = 1; // tiles
+    int                       most = 0;  // tiles of the longest work item
+    int                       waves = 4; // per workgroup
+    int                       depth = 1; // steps whose rows are on their way at once
     void                      clear() { entries.clear(), launches.clear(); }
 };
+
+// LDS of a workgroup: at most kStreamLds of dynamic memory (160 KB a CU, less the
+// kernel's own arrays).  Per wave, a stage of 16 V rows that later holds the rows'
+// fp32 outputs (half of kStreamRows rows where scores are kept); with scores, also 4
+// bytes for each token and row of the work item.
+constexpr int kStreamLds = 160 * 1024 - 2048;
+constexpr int stream_stage_bytes(int D, bool scores) { return kStreamRows / (scores ? 2 : 1) * D * 4; }
+constexpr int stream_most_tiles(int D, int waves, int rows) { // with scores
+    return (kStreamLds - waves * stream_stage_bytes(D, true)) / (kStreamTile * rows * 4);
+}
 
 inline int stream_tiles(int S) { return S / kStreamTile + (S % kStreamTile != 0); }
 inline int stream_items(int S, int chunk) { return (stream_tiles(S) + chunk - 1) / chunk; }
 
-// Sets item0 and tile0 of plan.entries, the launches and the chunk length.
-void plan_stream(StreamPlan &plan, int Hkv, int cus);
+// Sets item0 and tile0 of plan.entries (and orders them, longest first), the
+// launches, the waves and the chunk length.  account_rows: query rows of every entry
+// when their scores are kept (at most kStreamRows / 2), 0: they are not.
+void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus);
 
 constexpr int kAccountRows = 128;  // query rows of a workgroup of account_stats_kernel
 constexpr int kAccountKeys = 256;  // keys of a workgroup of account_sum_kernel
