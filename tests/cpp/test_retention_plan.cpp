@@ -35,7 +35,11 @@ static void stream_random() {
         const int rows = (int)(rng() % 2) ? 1 << (rng() % 4) : 0;
         plan_stream(p, 1 << (rng() % 6), D, rows, 1 + (int)(rng() % 300));
         CHECK(p.chunk >= 1 && (p.waves == 4 || (p.waves == 8 && D <= 128)));
-        for (size_t i = 1; i < p.entries.size(); ++i) CHECK(p.entries[i].S <= p.entries[i - 1].S);
+        auto length = [&](const StreamEntry &e) {
+            const int k = stream_items(e.S, p.chunk);
+            return k ? (stream_tiles(e.S) + k - 1) / k : 0;
+        };
+        for (size_t i = 1; i < p.entries.size(); ++i) CHECK(length(p.entries[i]) <= length(p.entries[i - 1]));
         size_t next = 0;
         for (const auto &l : p.launches) {
             CHECK((size_t)l.first == next && l.n > 0 && l.n <= kStreamBatch);
@@ -79,7 +83,7 @@ static void stream_random() {
             const int64_t t = stream_tiles(e.S), k = stream_items(e.S, p.chunk);
             for (int64_t c = 0; c < std::min<int64_t>(k, 50); ++c) item = std::max(item, (int)((c + 1) * t / k - c * t / k));
         }
-        CHECK(item <= p.most && p.most <= p.chunk && (p.depth == 1 || (p.depth == 2 && p.waves == 4 && D <= 128)));
+        CHECK(item <= p.most && p.most <= p.chunk);
         if (rows) CHECK((int64_t)p.waves * stream_stage_bytes(D, true) + (int64_t)p.most * kStreamTile * rows * 4 <= kStreamLds);
     }
     std::puts("ok stream_random");

@@ -308,25 +308,48 @@ attn_cross_kernel(CrossArgs a) {
 
 constexpr int kMergeThreads = 256;
 
-// The chunks of each row tile of the entries that have several: four dims a thread.
-template <int ROWS> __global__ __launch_bounds__(kMergeThreads) void cross_merge_kernel(CrossArgs a, int D) {
+// The chunks of the entries that have several.  A thread has four dims of a row and
+// every groups-th chunk (groups: a power of two, up to what a workgroup holds of a
+// row), their sums meet in LDS.  128 chunks of 32 rows x 8 heads, one thread for all
+// chunks: 64 us, so: 7.
+template <int ROWS> __global__ __launch_bounds__(kMergeThreads) void cross_merge_kernel(CrossArgs a, int D, int groups) {
+    __shared__ f32x4 s_o[kMergeThreads];
+    __shared__ float s_ml[kMergeThreads][2];
     const int ei = blockIdx.z, g = blockIdx.y;
     const int nch = a.e[ei].nch, rows = a.e[ei].nq * a.G;
-    if (nch == 1) return;
-    const int per = D / 4;
-    const int x = blockIdx.x * kMergeThreads + threadIdx.x, r = x / per, d = 4 * (x - r * per);
-    if (r >= rows) return;
-    const int     rt = r / ROWS;
-    const int64_t p0 = ((int64_t)(a.e[ei].item0 + rt * nch) * a.Hkv + g) * ROWS + r % ROWS, step = (int64_t)a.Hkv * ROWS;
+    const int per = D / 4, tid = threadIdx.x;
+    const int grp = tid / per % groups, d = 4 * (tid % per);
+    const int r = blockIdx.x * (kMergeThreads / (per * groups)) + tid / (per * groups);
+    if (nch == 1 || (int)blockIdx.x * (kMergeThreads / (per * groups)) >= rows) return; // (the whole workgroup)
+    const int     rc = min(r, rows - 1), rt = rc / ROWS;
+    const int64_t p0 = ((int64_t)(a.e[ei].item0 + rt * nch) * a.Hkv + g) * ROWS + rc % ROWS, step = (int64_t)a.Hkv * ROWS;
     float         m = -INFINITY, l = 0.0f;
     f32x4         o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int ch = 0; ch < nch; ++ch) m = fmaxf(m, a.part_ml[(p0 + ch * step) * 2]);
-    for (int ch = 0; ch < nch; ++ch) {
+    for (int ch = grp; ch < nch; ch += groups) m = fmaxf(m, a.part_ml[(p0 + ch * step) * 2]);
+#pragma unroll 4
+    for (int ch = grp; ch < nch; ch += groups) {
         const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (p0 + ch * step) * 2);
         const float  w = __builtin_amdgcn_exp2f(ml.x - m);
         l = fmaf(ml.y, w, l);
         o += w * *reinterpret_cast<const f32x4 *>(a.part_o + (p0 + ch * step) * D + d);
     }
+    if (groups > 1) {
+        s_o[tid] = o;
+        s_ml[tid][0] = m;
+        s_ml[tid][1] = l;
+        __syncthreads();
+        if (grp > 0) return;
+        float mx = m;
+        for (int k = 1; k < groups; ++k) mx = fmaxf(mx, s_ml[tid + k * per][0]);
+        o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        l = 0.0f;
+        for (int k = 0; k < groups; ++k) {
+            const float w = __builtin_amdgcn_exp2f(s_ml[tid + k * per][0] - mx); // (0 for a group without chunks)
+            l = fmaf(s_ml[tid + k * per][1], w, l);
+            o += w * s_o[tid + k * per];
+        }
+    }
+    if (r >= rows) return;
     const float   inv = 1.0f / (l + 1e-6f);
     const __half2 lo = __floats2half2_rn(o[0] * inv, o[1] * inv), hi = __floats2half2_rn(o[2] * inv, o[3] * inv);
     uint2         w;
@@ -389,14 +412,19 @@ void launch_attn_cross(const CrossCall &c, const KvView &kv, const CrossPlan &pl
         HIP_CHECK(hipGetLastError());
         if (l.split) {
             int64_t rows = 0;
-            for (int i = l.first; i < l.first + l.n; ++i)
-                if (plan.entries[(size_t)i].nch > 1) rows = std::max(rows, (int64_t)plan.entries[(size_t)i].nq * a.G);
-            const dim3 grid((unsigned)((rows * (c.D / 4) + kMergeThreads - 1) / kMergeThreads), (unsigned)c.Hkv,
-                            (unsigned)l.n);
+            int     chunks = 1, groups = 1;
+            for (int i = l.first; i < l.first + l.n; ++i) {
+                const CrossEntry &e = plan.entries[(size_t)i];
+                chunks = std::max(chunks, (int)e.nch);
+                if (e.nch > 1) rows = std::max(rows, (int64_t)e.nq * a.G);
+            }
+            while (2 * groups <= chunks && 2 * groups * (c.D / 4) <= kMergeThreads) groups *= 2;
+            const int  per_block = kMergeThreads / (groups * (c.D / 4)); // rows
+            const dim3 grid((unsigned)((rows + per_block - 1) / per_block), (unsigned)c.Hkv, (unsigned)l.n);
             switch (tile) {
-            case 64: hipLaunchKernelGGL((cross_merge_kernel<64>), grid, dim3(kMergeThreads), 0, stream, a, c.D); break;
-            case 128: hipLaunchKernelGGL((cross_merge_kernel<128>), grid, dim3(kMergeThreads), 0, stream, a, c.D); break;
-            default: hipLaunchKernelGGL((cross_merge_kernel<256>), grid, dim3(kMergeThreads), 0, stream, a, c.D); break;
+            case 64: hipLaunchKernelGGL((cross_merge_kernel<64>), grid, dim3(kMergeThreads), 0, stream, a, c.D, groups); break;
+            case 128: hipLaunchKernelGGL((cross_merge_kernel<128>), grid, dim3(kMergeThreads), 0, stream, a, c.D, groups); break;
+            default: hipLaunchKernelGGL((cross_merge_kernel<256>), grid, dim3(kMergeThreads), 0, stream, a, c.D, groups); break;
             }
             HIP_CHECK(hipGetLastError());
         }

@@ -105,36 +105,46 @@ __device__ __forceinline__ void account_tokens(const StreamArgs &a, int ei, int 
                                                const float *sc, const float *m, const float *inv) {
     const int     old = a.e[ei].S - a.fresh;
     const int64_t base = ((int64_t)a.e[ei].row * a.Hkv + g) * a.room;
-    for (int t = t_lo + 4 * (int)threadIdx.x; t < t_hi; t += 4 * NT) {
-        Four w = {};
-        if (a.w_in && t + 4 <= old) w = *reinterpret_cast<const Four *>(a.w_in + base + t);
-        else if (a.w_in) {
+    constexpr int U = NT > 256 ? 1 : 8; // accounts of so many fours on their way at once (8 waves: short entries)
+    for (int t0 = t_lo + 4 * (int)threadIdx.x; t0 < t_hi; t0 += 4 * NT * U) {
+        Four w[U];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (t + i < old) w.x[i] = a.w_in[base + t + i];
+        for (int u = 0; u < U; ++u) {
+            const int t = t0 + u * 4 * NT;
+            w[u] = Four{};
+            if (a.w_in && t + 4 <= old) w[u] = *reinterpret_cast<const Four *>(a.w_in + base + t);
+            else if (a.w_in) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t + i < old) w[u].x[i] = a.w_in[base + t + i];
+            }
         }
-        const float *st = sc + (int64_t)((t - t_lo) / kStreamTile) * rows * kStreamTile + t % kStreamTile;
-        f32x4        sum = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int r = 0; r < rows; ++r) { // (scores past the end are -infinity)
-            const f32x4 s = *reinterpret_cast<const f32x4 *>(st + r * kStreamTile);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) sum[i] = fmaf(__builtin_amdgcn_exp2f(s[i] - m[r]), inv[r], sum[i]);
-        }
+        for (int u = 0; u < U; ++u) {
+            const int t = t0 + u * 4 * NT;
+            if (t >= t_hi) break;
+            const float *st = sc + (int64_t)((t - t_lo) / kStreamTile) * rows * kStreamTile + t % kStreamTile;
+            f32x4        sum = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int r = 0; r < rows; ++r) { // (scores past the end are -infinity)
+                const f32x4 s = *reinterpret_cast<const f32x4 *>(st + r * kStreamTile);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w.x[i] += sum[i];
-        if (t + 4 <= t_hi) *reinterpret_cast<Four *>(a.w_out + base + t) = w;
-        else {
+                for (int i = 0; i < 4; ++i) sum[i] = fmaf(__builtin_amdgcn_exp2f(s[i] - m[r]), inv[r], sum[i]);
+            }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (t + i < t_hi) a.w_out[base + t + i] = w.x[i];
+            for (int i = 0; i < 4; ++i) w[u].x[i] += sum[i];
+            if (t + 4 <= t_hi) *reinterpret_cast<Four *>(a.w_out + base + t) = w[u];
+            else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (t + i < t_hi) a.w_out[base + t + i] = w[u].x[i];
+            }
         }
     }
 }
 
-// DEPTH steps' rows are on their way at once.  Dynamic LDS: the waves' V stages, then
-// with SCORES the chunk's scores.
-template <int D, bool PAGED, bool SCORES, int NW, int DEPTH>
-__global__ __launch_bounds__(NW * 64, D <= 128 && DEPTH == 1 ? 2 : 1) void attn_stream_kernel(StreamArgs a) {
+// Dynamic LDS: the waves' V stages, then with SCORES the chunk's scores.
+template <int D, bool PAGED, bool SCORES, int NW>
+__global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(StreamArgs a) {
     constexpr int TK = D <= 128 ? 64 : 32; // tokens of a wave's step
     constexpr int SUB = kStreamTile / TK;  // steps per tile
     constexpr int TT = TK / 16;
@@ -201,7 +211,8 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && DEPTH == 1 ? 2 : 1) void attn_
     const int steps = max(0, (tile_hi - tile_lo - wave + NW - 1) / NW) * SUB;
     auto start = [&](int x) { return (tile_lo + x / SUB * NW + wave) * kStreamTile + x % SUB * TK; };
     // Block ids of a step's quarters of 16 tokens, lane k that of quarter k (paged
-    // views): loaded a step before the rows they address, which so wait for nothing.
+    // views).  Loads complete in the order of their issue, so ids are asked for before
+    // the rows that are on their way when they are needed: two steps ahead.
     auto blocks = [&](int x) -> int {
         if constexpr (PAGED) return lane < TT ? bt[min(start(x) + 16 * lane, last) >> a.kv.log2_blk] : 0;
         else return 0;
@@ -215,9 +226,9 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && DEPTH == 1 ? 2 : 1) void attn_
             return (int64_t)__builtin_amdgcn_readlane(ids, k) * blk_bytes + (int64_t)(tq & mask) * tokb;
         else return (int64_t)row * blk_bytes + (int64_t)tq * tokb;
     };
-    f16x8 kf[DEPTH][TT][KS];
-    u32x4 vr[DEPTH][NV];
-    auto load_k = [&](int x, int ids, f16x8(&k)[TT][KS]) __attribute__((always_inline)) {
+    f16x8 kf[TT][KS];
+    u32x4 vr[NV];
+    auto load_k = [&](int x, int ids) __attribute__((always_inline)) {
         const int t0 = __builtin_amdgcn_readfirstlane(start(x));
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
@@ -225,10 +236,10 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && DEPTH == 1 ? 2 : 1) void attn_
             const char    *p = kb + quarter(t0, tt, ids, more);
             const uint32_t off = (uint32_t)min(c, more) * (uint32_t)tokb + 16 * qg;
 #pragma unroll
-            for (int s = 0; s < KS; ++s) k[tt][s] = *reinterpret_cast<const f16x8 *>(p + off + 64 * s);
+            for (int s = 0; s < KS; ++s) kf[tt][s] = *reinterpret_cast<const f16x8 *>(p + off + 64 * s);
         }
     };
-    auto load_v = [&](int x, int ids, u32x4(&v)[NV]) __attribute__((always_inline)) {
+    auto load_v = [&](int x, int ids) __attribute__((always_inline)) {
         const int t0 = __builtin_amdgcn_readfirstlane(start(x));
 #pragma unroll
         for (int u = 0; u < NV; ++u) {
@@ -237,7 +248,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && DEPTH == 1 ? 2 : 1) void attn_
             const char    *p = vb + quarter(t0, u * RPI / 16, ids, more);
             const uint32_t off = (uint32_t)min(r, more) * (uint32_t)tokb + 16 * (lane % KP);
             // (whole lines, read once; K's lines are read in halves, which the hint made slower)
-            v[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + off));
+            vr[u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(p + off));
         }
     };
     uint16_t *vst = smem + wave * STAGE;
@@ -245,21 +256,24 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && DEPTH == 1 ? 2 : 1) void attn_
     const int vrow = 4 * qg + (c >> 2);
     const int vlane = vrow * KP * 8 + 4 * (c & 1), vxor = ((c & 3) >> 1) ^ swz(vrow);
 
-    // One step: its rows are in k and v; those of step x + DEPTH take their place.
-    int  ids_next = 0;
-    auto step = [&](int x, f16x8(&k)[TT][KS], u32x4(&v)[NV]) __attribute__((always_inline)) {
+    int ids = blocks(0), next = PAGED && steps > 1 ? blocks(1) : 0;
+    if (steps > 0) {
+        load_k(0, ids);
+        load_v(0, ids);
+    }
+    for (int x = 0; x < steps; ++x) {
         const int  t0 = start(x);
-        const bool more = x + DEPTH < steps;
-        const int  ids = ids_next;
-        if (PAGED && x + DEPTH + 1 < steps) ids_next = blocks(x + DEPTH + 1);
+        const bool more = x + 1 < steps;
+        ids = next;
+        if (PAGED && x + 2 < steps) next = blocks(x + 2);
         f32x4 s[TT];
 #pragma unroll
         for (int tt = 0; tt < TT; ++tt) {
             s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < KS; ++i) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[tt][i], qb[i], s[tt], 0, 0, 0);
+            for (int i = 0; i < KS; ++i) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tt][i], qb[i], s[tt], 0, 0, 0);
         }
-        if (more) load_k(x + DEPTH, ids, k);
+        if (more) load_k(x + 1, ids);
         const int tb = t0 + 4 * qg;
         float     mloc = -INFINITY;
 #pragma unroll
@@ -301,7 +315,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && DEPTH == 1 ? 2 : 1) void attn_
 #pragma unroll
             for (int u = 0; u < NQ; ++u) {
                 const int r = u * RPI + lane / KP;
-                *reinterpret_cast<u32x4 *>(&vst[(r * KP + ((lane % KP) ^ swz(r))) * 8]) = v[q * NQ + u];
+                *reinterpret_cast<u32x4 *>(&vst[(r * KP + ((lane % KP) ^ swz(r))) * 8]) = vr[q * NQ + u];
             }
             wave_sync_lds();
 #pragma unroll
@@ -311,20 +325,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && DEPTH == 1 ? 2 : 1) void attn_
             }
             wave_sync_lds();
         }
-        if (more) load_v(x + DEPTH, ids, v);
-    };
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d)
-        if (d < steps) {
-            const int ids = blocks(d);
-            load_k(d, ids, kf[d]);
-            load_v(d, ids, vr[d]);
-        }
-    if (PAGED && DEPTH < steps) ids_next = blocks(DEPTH);
-    for (int x = 0; x < steps; x += DEPTH) {
-#pragma unroll
-        for (int d = 0; d < DEPTH; ++d)
-            if (x + d < steps) step(x + d, kf[d], vr[d]);
+        if (more) load_v(x + 1, ids);
     }
 
     // The waves' (m, l, o) through LDS.
@@ -431,9 +432,9 @@ __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArg
     }
 }
 
-template <int D, bool PAGED, bool SCORES, int NW, int DEPTH>
+template <int D, bool PAGED, bool SCORES, int NW>
 void launch_one(const StreamArgs &a, int items, int lds, hipStream_t stream) {
-    auto                 *fn = attn_stream_kernel<D, PAGED, SCORES, NW, DEPTH>;
+    auto                 *fn = attn_stream_kernel<D, PAGED, SCORES, NW>;
     static std::once_flag once;
     std::call_once(once, [&] {
         HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -443,19 +444,15 @@ void launch_one(const StreamArgs &a, int items, int lds, hipStream_t stream) {
 }
 template <int D, bool SCORES> void launch_ds(const StreamArgs &a, int items, bool paged, const StreamPlan &plan, hipStream_t stream) {
     const int lds = plan.waves * stream_stage_bytes(D, SCORES) + (SCORES ? plan.most * kStreamTile * a.rows * 4 : 0);
-#define TL_STREAM(NW, DEPTH)                                                                                           \
-    do {                                                                                                               \
-        if (paged) launch_one<D, true, SCORES, NW, DEPTH>(a, items, lds, stream);                                      \
-        else launch_one<D, false, SCORES, NW, DEPTH>(a, items, lds, stream);                                           \
-        return;                                                                                                        \
-    } while (0)
     if constexpr (D <= 128) {
-        if (plan.waves == 8) TL_STREAM(8, 1);
-        if constexpr (SCORES)
-            if (plan.depth == 2) TL_STREAM(4, 2);
+        if (plan.waves == 8) {
+            if (paged) launch_one<D, true, SCORES, 8>(a, items, lds, stream);
+            else launch_one<D, false, SCORES, 8>(a, items, lds, stream);
+            return;
+        }
     }
-    TL_STREAM(4, 1);
-#undef TL_STREAM
+    if (paged) launch_one<D, true, SCORES, 4>(a, items, lds, stream);
+    else launch_one<D, false, SCORES, 4>(a, items, lds, stream);
 }
 template <int D> void launch_d(const StreamArgs &a, int items, bool paged, const StreamPlan &plan, hipStream_t stream) {
     if (a.w_out) launch_ds<D, true>(a, items, paged, plan, stream);

@@ -7,15 +7,13 @@ namespace tiny_llm {
 namespace detail {
 
 void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
-    std::stable_sort(plan.entries.begin(), plan.entries.end(),
-                     [](const StreamEntry &x, const StreamEntry &y) { return x.S > y.S; });
-    int64_t total = 0, some = 0;
+    int64_t total = 0, some = 0, longest = 0;
     for (const auto &e : plan.entries) {
         total += stream_tiles(e.S);
         some += e.S > 0;
+        longest = std::max<int64_t>(longest, stream_tiles(e.S));
     }
     total *= Hkv;
-    const int64_t longest = plan.entries.empty() ? 0 : stream_tiles(plan.entries.front().S);
     const int64_t n = std::max(1, cus);
     int64_t       chunk;
     // An entry in one chunk is finished by its own workgroup: no partial results, no
@@ -28,7 +26,7 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
     } else {
         plan.waves = 4;
         const int64_t share = (total + 2 * n - 1) / (2 * n);
-        chunk = longest <= std::max<int64_t>(kStreamWhole, 2 * share + share / 2) ? longest : std::max<int64_t>(8, (share + 1) / 2);
+        chunk = longest <= std::max<int64_t>(kStreamWhole, 2 * share + share / 2) ? longest : std::max<int64_t>(8, share);
     }
     if (account_rows > 0) {
         const int64_t fits = stream_most_tiles(D, plan.waves, account_rows);
@@ -41,10 +39,13 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
         const int t = stream_tiles(e.S), k = stream_items(e.S, plan.chunk);
         if (k) plan.most = std::max(plan.most, (t + k - 1) / k);
     }
-    // Where the scores leave room for one workgroup per CU, its four waves have twice
-    // the registers, for twice the rows on their way.
-    const int64_t lds = plan.waves * stream_stage_bytes(D, true) + (int64_t)plan.most * kStreamTile * account_rows * 4;
-    plan.depth = account_rows > 0 && D <= 128 && plan.waves == 4 && lds > kStreamLds / 2 ? 2 : 1;
+    // Longest work items first.
+    auto item_tiles = [&](const StreamEntry &e) {
+        const int k = stream_items(e.S, plan.chunk);
+        return k ? (stream_tiles(e.S) + k - 1) / k : 0;
+    };
+    std::stable_sort(plan.entries.begin(), plan.entries.end(),
+                     [&](const StreamEntry &x, const StreamEntry &y) { return item_tiles(x) > item_tiles(y); });
     plan.launches.clear();
     for (size_t i = 0; i < plan.entries.size();) {
         StreamLaunch l{(int)i, 0, 0, 0, false, 0};
@@ -101,9 +102,9 @@ bool plan_cross(CrossPlan &plan, int D, int G, int Hkv, int cus) {
     const int tile = cross_rows(D, plan.waves);
     int64_t   tiles = 0;
     for (const auto &e : plan.entries) tiles += ((int64_t)e.nq * G + tile - 1) / tile;
-    // Row tiles that do not fill the chip twice have their keys split, into chunks of
-    // at least four tiles.
-    const int64_t want = (wide ? 2 : 4) * (int64_t)std::max(1, cus);
+    // Row tiles that do not fill the chip (twice where a CU holds one workgroup) have
+    // their keys split, into chunks of at least four tiles.
+    const int64_t want = 2 * (int64_t)std::max(1, cus);
     const int64_t split = std::max<int64_t>(1, want / std::max<int64_t>(1, tiles * Hkv));
     for (auto &e : plan.entries)
         e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(split, stream_tiles(e.S) / 4));

@@ -34,7 +34,6 @@ struct StreamPlan {
     int                       chunk = 1; // tiles
     int                       most = 0;  // tiles of the longest work item
     int                       waves = 4; // per workgroup
-    int                       depth = 1; // steps whose rows are on their way at once
     void                      clear() { entries.clear(), launches.clear(); }
 };
 
