@@ -93,31 +93,49 @@ static void account_random() {
     std::mt19937_64 rng(2);
     for (int it = 0; it < 500; ++it) {
         AccountPlan p;
-        const int   n = (int)(rng() % 250), most = 1 << (rng() % 14), G = 1 << (rng() % 4);
+        const int   n = (int)(rng() % 150), most = 1 << (rng() % 14), G = 1 << (rng() % 4);
         for (int i = 0; i < n; ++i) {
-            const int nt = 1 + (int)(rng() % most), w = rng() % 2 ? nt : 1 + (int)(rng() % nt);
-            p.entries.push_back({i, (int32_t)(rng() % most), nt, w, 0, -1, -1, -1, -1});
+            const int    nt = 1 + (int)(rng() % most), w = rng() % 2 ? nt : 1 + (int)(rng() % nt);
+            AccountEntry e{};
+            e.row = i, e.p0 = (int32_t)(rng() % most), e.n = nt, e.w = w;
+            p.entries.push_back(e);
         }
         CHECK(plan_account(p, G, 1 << (rng() % 6), 1 + (int)(rng() % 300)));
         size_t next = 0;
         for (const auto &l : p.launches) {
             CHECK((size_t)l.first == next && l.n > 0 && l.n <= kAccountBatch);
-            int64_t items = 0, sums = 0, stats = 0;
+            int64_t items = 0, sums = 0, stats = 0, lse = 0, parts = 0;
+            bool    keys_split = false, rows_split = false;
             for (int i = l.first; i < l.first + l.n; ++i) {
                 const AccountEntry &e = p.entries[(size_t)i];
-                CHECK(e.item0 == items && e.sum0 == sums && e.stat0 == stats);
-                CHECK(e.nch >= 1 && e.nch <= std::max(1, stream_tiles(e.p0 + e.n)));
-                items += ((int64_t)e.w * G + kAccountRows - 1) / kAccountRows * e.nch;
-                sums += (e.p0 + e.n + kAccountKeys - 1) / kAccountKeys;
-                stats += (int64_t)e.w * G * e.nch;
+                const int           keys = e.p0 + e.n, rows = e.w * G;
+                CHECK(e.item0 == items && e.sum0 == sums && e.stat0 == stats && e.lse0 == lse && e.part0 == parts);
+                CHECK(e.nch >= 1 && e.nch <= std::max(1, stream_tiles(keys)));
+                // row chunks of whole steps, none empty, all rows
+                CHECK(e.rc > 0 && e.rc % kAccountStep == 0 && e.nrc >= 1);
+                CHECK((int64_t)e.rc * e.nrc >= rows && (int64_t)e.rc * (e.nrc - 1) < rows);
+                items += ((int64_t)rows + kAccountRows - 1) / kAccountRows * e.nch;
+                sums += (int64_t)account_blocks(keys) * e.nrc;
+                lse += rows;
+                if (e.nch > 1) stats += (int64_t)rows * e.nch;
+                CHECK(e.nch == 1 || rows <= l.most_rows);
+                if (e.nrc > 1) parts += (int64_t)account_blocks(keys) * kAccountKeys * e.nrc;
+                CHECK(e.nrc == 1 || keys <= l.most_keys);
+                keys_split |= e.nch > 1;
+                rows_split |= e.nrc > 1;
             }
-            CHECK(l.items == items && l.sums == sums && l.stats == stats);
+            CHECK(l.items == items && l.sums == sums && l.stats == stats && l.lse == lse && l.parts == parts);
+            CHECK(l.split_keys == keys_split && l.split_rows == rows_split);
             next += (size_t)l.n;
         }
         CHECK(next == p.entries.size());
     }
-    AccountPlan big; // statistics that do not fit 31 bits
-    for (int i = 0; i < 5; ++i) big.entries.push_back({i, 0, 1 << 26, 1 << 26, 0, 0, 0, 0, 0});
+    AccountPlan big; // rows that do not fit 31 bits
+    for (int i = 0; i < 5; ++i) {
+        AccountEntry e{};
+        e.row = i, e.n = e.w = 1 << 26;
+        big.entries.push_back(e);
+    }
     CHECK(!plan_account(big, 8, 8, 256));
     std::puts("ok account_random");
 }

@@ -219,8 +219,9 @@ def test_decode_weights_refusals(tl):
 
 
 # ------------------------------------------------------------------- prompts
-def prompt_step(tl, c, pre, new, G, window, given=True, in_place=False, layer=0):
+def prompt_step(tl, c, pre, new, G, window, given=True, in_place=False, layer=0, scale=None):
     n, hq, d = len(new), c.hkv * G, c.d
+    scale = d ** -0.5 if scale is None else scale
     t = sum(new)
     q = c.rng.standard_normal((t, hq, d)).astype(np.float16)
     nk, nv = c.rows(t), c.rows(t)
@@ -234,14 +235,14 @@ def prompt_step(tl, c, pre, new, G, window, given=True, in_place=False, layer=0)
     if in_place:
         w_out = w_in
     start, before = w_in.cpu().numpy(), w_out.cpu().numpy()
-    p.weights(layer, dq.data_ptr(), d ** -0.5, window, w_in.data_ptr() if given else None, w_out.data_ptr(), s)
+    p.weights(layer, dq.data_ptr(), scale, window, w_in.data_ptr() if given else None, w_out.data_ptr(), s)
     torch.cuda.synchronize()
     acc, at = w_out.cpu().numpy(), 0
     for i in range(n):
         S, w_n = pre[i] + new[i], min(new[i], window or new[i])
         k = np.concatenate([c.k[layer][i], nk[at:at + new[i]]])
         last = pre[i] + np.arange(new[i] - w_n, new[i])
-        _, _, w, err = attend(q[at + new[i] - w_n:at + new[i]], k, k, d ** -0.5, last)
+        _, _, w, err = attend(q[at + new[i] - w_n:at + new[i]], k, k, scale, last)
         want = w.reshape(c.hkv, G * w_n, S).sum(axis=1)
         base = start[c.slot[i], :, :S].astype(np.float64) * (np.arange(S) < pre[i]) if given else np.zeros((c.hkv, S))
         check_account(acc[c.slot[i], :, :S], want + base, w, err, G * w_n, S, base)
@@ -271,6 +272,22 @@ def test_prompt_weights(tl, d, hkv, G, block, pre, new, window):
 def test_prompt_weights_forms(tl, given, in_place):
     c = Cache(tl, [20, 0], 2, 64, room=200, layers=2, seed=3, hq=4)
     prompt_step(tl, c, [20, 0], [100, 150], 2, 0, given, in_place, layer=1)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1.5])
+def test_prompt_weights_scales_of_either_sign(tl, scale):
+    c = Cache(tl, [70, 0], 2, 64, room=400, seed=13, hq=4)
+    prompt_step(tl, c, [70, 0], [300, 65], 2, 0, scale=scale)
+
+
+@pytest.mark.parametrize("d,hkv,G,pre,new,window", [
+    (128, 8, 4, [0, 900], [1100, 700], 0),   # rows and keys over several workgroups, the diagonal between them
+    (64, 1, 1, [0], [2500], 0),
+    (128, 1, 8, [3000], [1500], 1000),
+])
+def test_prompt_weights_long(tl, d, hkv, G, pre, new, window):
+    c = Cache(tl, pre, hkv, d, room=max(a + b for a, b in zip(pre, new)), seed=14, hq=hkv * G)
+    prompt_step(tl, c, pre, new, G, window)
 
 
 def test_prompt_weights_more_entries_than_a_launch_takes(tl):

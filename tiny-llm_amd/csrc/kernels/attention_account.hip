@@ -9,14 +9,21 @@
 // exponential rates for many rows, by K's bytes for few.  Scores, sums and
 // weights are fp32 throughout.
 //
-// account_stats_kernel: (m, l) of every row.  A workgroup has 128 rows, 32 per wave
-// in registers, and a chunk of the keys, whose tiles of 64 pass through LDS (DMA,
-// two buffers).  S^T = K Q^T on v_mfma_f32_16x16x32_f16 as in the prefill kernel: a
-// lane has 16 keys of its row column per tile.
-// account_sum_kernel: a workgroup has 256 keys, 64 per wave in registers, and
-// passes all rows that see them through LDS, 64 at a time; a lane adds its row
-// column's weights to 16 keys' sums, and the 16 columns are added at the end.
-// No atomics: every sum has one order.
+// account_stats_kernel: log2 of every row's sum, lse = m + log2 l, so that a weight is
+// one multiply-add and one exponential, 2^(s * scale * log2(e) - lse).  A workgroup
+// has 128 rows, 32 per wave in registers, and a chunk of the keys, whose tiles of 64
+// pass through LDS (DMA, two buffers).  S^T = K Q^T on v_mfma_f32_16x16x32_f16 as in
+// the prefill kernel: a lane has 16 keys of its row column per tile, and its own
+// reference point, which moves on jumps above 2^8 only.
+// account_sum_kernel: a workgroup has 256 keys, 64 per wave in registers, and passes
+// a chunk of the rows that see them through LDS, 64 at a time (DMA, two buffers); a
+// lane adds its row column's weights to 16 keys' sums, and the 16 columns are added
+// at the end.
+// Both are bound by the exponentials (a quarter of the VALU's rate), not by the
+// matrix unit: 96 against 64 cycles for 256 scores at head_dim 128.
+// account_merge_kernel joins the rows' chunks of keys where rows are few,
+// account_join_kernel adds the keys' chunks of rows.  No atomics: every sum has one
+// order.
 #include "account.h"
 
 #include "tiny_llm/hip_utils.h"
@@ -38,13 +45,15 @@ typedef float    f32x4 __attribute__((ext_vector_type(4)));
 constexpr int   kThreads = 256;
 constexpr int   kVmcnt0 = 0x0F70; // s_waitcnt vmcnt(0)
 constexpr int   kTile = kStreamTile;
-constexpr int   kQRows = 64;      // rows that account_sum_kernel stages
+constexpr float kLazyMax = 8.0f;
 
 struct AccountArgs {
     const __half *q;
     const float  *w_in;
     float        *w_out;
-    float        *stats; // [(stat0 * Hkv + (chunk * Hkv + g) * rows + r)][2]
+    float        *lse;   // [lse0 * Hkv + g * rows + r]
+    float        *stats; // (m, l) [stat0 * Hkv + (chunk * Hkv + g) * rows + r]
+    float        *parts; // [part0 * Hkv + (chunk * Hkv + g) * blocks * 256 + t]
     KvView        kv;
     int64_t       room;
     float         scale_log2;
@@ -81,6 +90,8 @@ template <int KP> __device__ __forceinline__ int swz(int r) {
     return f & (KP - 1);
 }
 
+__device__ __forceinline__ int account_blocks_dev(int keys) { return (keys + kAccountKeys - 1) / kAccountKeys; }
+
 __device__ __forceinline__ void lds_dma(const void *src, uint16_t *dst) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
                                      (__attribute__((address_space(3))) void *)dst, 16, 0, 0);
@@ -97,8 +108,9 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
     int       ei;
     ACCOUNT_ENTRY_OF(a, item0, item, ei);
     const int row = a.e[ei].row, p0 = a.e[ei].p0, n = a.e[ei].n, w = a.e[ei].w, nch = a.e[ei].nch;
-    const int rel = item - a.e[ei].item0, ch = rel % nch, rt = rel / nch;
+    const int rel = item - a.e[ei].item0, ch = rel % nch;
     const int rows = w * a.G;
+    const int rt = (rows - 1) / kAccountRows - rel / nch; // the tiles with the most keys first
     const int r_lo = rt * kAccountRows, r_hi = min(rows, r_lo + kAccountRows);
     const int first = p0 + n - w;                          // position of query row 0's token
     const int kend = first + (r_hi - 1) / a.G + 1;         // keys that some row of the tile sees
@@ -115,8 +127,13 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
         const __half *qp = a.q + ((int64_t)(a.e[ei].tok0 + n - w + r / a.G) * a.Hq + g * a.G + r % a.G) * D;
         pos[j] = first + r / a.G;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) qb[j][s] = *reinterpret_cast<const f16x8 *>(qp + 32 * s + 8 * qg);
+        for (int s = 0; s < KS; ++s) {
+            // (a negative scale's sign goes into q: the maximum over s is then that over s * scale)
+            const f16x8 v = *reinterpret_cast<const f16x8 *>(qp + 32 * s + 8 * qg);
+            qb[j][s] = a.scale_log2 < 0.0f ? -v : v;
+        }
     }
+    const float scale = fabsf(a.scale_log2);
     const char *kb = reinterpret_cast<const char *>(a.kv.k_base) + (int64_t)g * a.kv.head_stride * 2;
     auto issue = [&](int kt, uint16_t *dst) {
 #pragma unroll
@@ -128,7 +145,8 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
         }
     };
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    auto  step = [&](int kt, const uint16_t *kd, uint16_t *kn) __attribute__((always_inline)) {
+    const int low = first + (r_lo + wave * 32) / a.G; // the first position among the wave's rows
+    auto      step = [&](int kt, const uint16_t *kd, uint16_t *kn) __attribute__((always_inline)) {
         if (kt + 1 < t_hi) issue(kt + 1, kn);
         f32x4 s[2][4];
 #pragma unroll
@@ -144,28 +162,34 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
 #pragma unroll
                 for (int j = 0; j < 2; ++j) s[j][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qb[j][k], s[j][tt], 0, 0, 0);
             }
-        const int tb = kt * kTile + 4 * qg;
+        const int  tb = kt * kTile + 4 * qg;
+        const bool diagonal = kt * kTile + kTile - 1 > low;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            float mloc = -INFINITY;
-#pragma unroll
-            for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[j][tt][i] = tb + 16 * tt + i <= pos[j] ? s[j][tt][i] * a.scale_log2 : -INFINITY;
-                    mloc = fmaxf(mloc, s[j][tt][i]);
-                }
-            // (each lane its own reference point: its keys are its own until the end)
-            const float m_new = fmaxf(m[j], mloc);
-            float       sum = m[j] == -INFINITY ? 0.0f : l[j] * __builtin_amdgcn_exp2f(m[j] - m_new);
-            if (m_new != -INFINITY) {
+            if (diagonal) {
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f(s[j][tt][i] - m_new);
+                    for (int i = 0; i < 4; ++i)
+                        if (tb + 16 * tt + i > pos[j]) s[j][tt][i] = -INFINITY;
             }
-            l[j] = sum;
-            m[j] = m_new;
+            float mloc = s[j][0][0];
+#pragma unroll
+            for (int x = 1; x < 16; ++x) mloc = fmaxf(mloc, s[j][x / 4][x % 4]);
+            mloc *= scale;
+            if (__any(mloc > m[j] + kLazyMax)) {
+                const float m_new = fmaxf(m[j], mloc);
+                l[j] = m[j] == -INFINITY ? 0.0f : l[j] * __builtin_amdgcn_exp2f(m[j] - m_new);
+                m[j] = m_new;
+            }
+            // (a lane that has seen no key yet: its reference point is 0, its weights are)
+            const float ref = m[j] == -INFINITY ? 0.0f : m[j];
+            float       sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][tt][i], scale, -ref));
+            l[j] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         }
         __builtin_amdgcn_s_waitcnt(kVmcnt0);
         __syncthreads();
@@ -187,30 +211,76 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
         lr += __shfl_xor(lr, 16);
         lr += __shfl_xor(lr, 32);
         const int r = r_lo + wave * 32 + j * 16 + c;
-        if (qg == 0 && r < r_hi) {
+        if (qg > 0 || r >= r_hi) continue;
+        if (nch == 1) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = mr + __builtin_amdgcn_logf(lr);
+        else {
             const int64_t at = (int64_t)a.e[ei].stat0 * a.Hkv + ((int64_t)ch * a.Hkv + g) * rows + r;
             *reinterpret_cast<float2 *>(a.stats + 2 * at) = make_float2(mr, lr);
         }
     }
 }
 
+// lse of the rows of entries with several chunks of keys: a wave per row.
+__global__ __launch_bounds__(kThreads) void account_merge_kernel(AccountArgs a) {
+    const int ei = blockIdx.z, g = blockIdx.y;
+    const int nch = a.e[ei].nch, rows = a.e[ei].w * a.G;
+    const int r = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (nch == 1 || r >= rows) return;
+    const float *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows + r);
+    float        m = -INFINITY, l = 0.0f;
+    for (int ch = lane; ch < nch; ch += 64) {
+        const float2 ml = *reinterpret_cast<const float2 *>(st + 2 * (int64_t)ch * a.Hkv * rows);
+        const float  mn = fmaxf(m, ml.x);
+        if (mn == -INFINITY) continue; // no key of the chunk is seen
+        l = l * __builtin_amdgcn_exp2f(m - mn) + ml.y * __builtin_amdgcn_exp2f(ml.x - mn);
+        m = mn;
+    }
+    float mx = m;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    l = m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - mx);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+    if (lane == 0) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = mx + __builtin_amdgcn_logf(l);
+}
+
 template <int D, bool PAGED>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel(AccountArgs a) {
     constexpr int KS = D / 32, KP = D / 8;
-    constexpr int NQI = kQRows * KP / kThreads; // Q pieces per thread
-    __shared__ __align__(16) uint16_t qs[kQRows * D];
-    __shared__ float s_m[kQRows], s_inv[kQRows];
+    constexpr int NQI = kAccountStep * KP / kThreads; // Q pieces per thread
+    constexpr int NRG = kAccountStep / 16;
+    __shared__ __align__(16) uint16_t qs0[kAccountStep * D], qs1[kAccountStep * D];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int item = blockIdx.x / a.Hkv, g = blockIdx.x - item * a.Hkv;
     int       ei;
     ACCOUNT_ENTRY_OF(a, sum0, item, ei);
-    const int row = a.e[ei].row, p0 = a.e[ei].p0, n = a.e[ei].n, w = a.e[ei].w, nch = a.e[ei].nch;
-    const int k_lo = (item - a.e[ei].sum0) * kAccountKeys, keys = p0 + n;
+    const int row = a.e[ei].row, p0 = a.e[ei].p0, n = a.e[ei].n, w = a.e[ei].w, nrc = a.e[ei].nrc;
+    const int rel = item - a.e[ei].sum0, kblk = rel / nrc, rchunk = rel - kblk * nrc;
+    const int k_lo = kblk * kAccountKeys, keys = p0 + n;
     const int rows = w * a.G, first = keys - w;
+    // The chunk's rows, from the first step whose tokens see the block's first key.
+    const int sees = max(0, k_lo - first) * a.G / kAccountStep * kAccountStep;
+    const int r_lo = max(rchunk * a.e[ei].rc, sees), r_hi = (int)min((int64_t)rows, (int64_t)(rchunk + 1) * a.e[ei].rc);
+    if (r_lo >= r_hi && nrc > 1) return; // (account_join_kernel does not read it)
     const int c = lane & 15, qg = lane >> 4;
     const int wk = k_lo + wave * 64; // the wave's first key
 
+    const float  *lse = a.lse + (int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows;
+    const __half *qbase = a.q + ((int64_t)(a.e[ei].tok0 + n - w) * a.Hq + g * a.G) * D;
+    auto issue = [&](int r0, uint16_t *dst) {
+#pragma unroll
+        for (int u = 0; u < NQI; ++u) {
+            const int sl = u * kThreads + (int)threadIdx.x, r = sl / KP, x = (sl % KP) ^ swz<KP>(r);
+            const int qr = min(r0 + r, rows - 1);
+            lds_dma(qbase + ((int64_t)(qr / a.G) * a.Hq + qr % a.G) * D + 8 * x, dst + (u * kThreads + wave * 64) * 8);
+        }
+    };
+    auto load_lse = [&](int r0, float(&x)[NRG]) {
+#pragma unroll
+        for (int rg = 0; rg < NRG; ++rg) x[rg] = r0 + 16 * rg + c < r_hi ? lse[r0 + 16 * rg + c] : INFINITY; // weights of 0
+    };
+    if (r_lo < r_hi) issue(r_lo, qs0);
     const char *kb = reinterpret_cast<const char *>(a.kv.k_base) + (int64_t)g * a.kv.head_stride * 2;
     f16x8       kf[4][KS];
 #pragma unroll
@@ -222,86 +292,118 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     f32x4 acc[4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) acc[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    // Rows from the first whose token sees the workgroup's first key.
-    const int r_from = max(0, k_lo - first) * a.G / kQRows * kQRows;
-    for (int r0 = r_from; r0 < rows; r0 += kQRows) {
-        __syncthreads();
-#pragma unroll
-        for (int u = 0; u < NQI; ++u) {
-            const int sl = u * kThreads + (int)threadIdx.x, r = sl / KP, x = sl % KP;
-            const int qr = min(r0 + r, rows - 1);
-            const __half *qp = a.q + ((int64_t)(a.e[ei].tok0 + n - w + qr / a.G) * a.Hq + g * a.G + qr % a.G) * D;
-            *reinterpret_cast<uint4 *>(&qs[(r * KP + (x ^ swz<KP>(r))) * 8]) = *reinterpret_cast<const uint4 *>(qp + 8 * x);
+    float x[NRG];
+    load_lse(r_lo, x);
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    __syncthreads();
+    auto step = [&](int r0, const uint16_t *qd, uint16_t *qn) __attribute__((always_inline)) {
+        float y[NRG];
+        if (r0 + kAccountStep < r_hi) {
+            issue(r0 + kAccountStep, qn);
+            load_lse(r0 + kAccountStep, y);
         }
-        if ((int)threadIdx.x < kQRows) { // the row's maximum and sum over its chunks
-            const int r = r0 + (int)threadIdx.x;
-            float     m = INFINITY, l = 1.0f; // a row past the end: weights of 0
-            if (r < rows) {
-                const float  *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows + r);
-                const int64_t step = 2 * (int64_t)a.Hkv * rows;
-                m = -INFINITY;
-                for (int ch = 0; ch < nch; ++ch) m = fmaxf(m, st[ch * step]);
-                l = 0.0f;
-                for (int ch = 0; ch < nch; ++ch) l = fmaf(st[ch * step + 1], __builtin_amdgcn_exp2f(st[ch * step] - m), l);
-            }
-            s_m[threadIdx.x] = m;
-            s_inv[threadIdx.x] = 1.0f / l;
-        }
-        __syncthreads();
+        const bool diagonal = wk + 63 > first + r0 / a.G; // some row does not see every key of the wave
 #pragma unroll
-        for (int rg = 0; rg < kQRows / 16; ++rg) {
-            const int   rr = 16 * rg + c;
-            const float m = s_m[rr], inv = s_inv[rr];
-            const int   pos = first + min(r0 + rr, rows - 1) / a.G;
-            f32x4       s[4];
+        for (int rg = 0; rg < NRG; ++rg) {
+            const int rr = 16 * rg + c;
+            f32x4     s[4];
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt) s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int k = 0; k < KS; ++k) {
-                const f16x8 qf = *reinterpret_cast<const f16x8 *>(&qs[(rr * KP + ((4 * k + qg) ^ swz<KP>(rr))) * 8]);
+                const f16x8 qf = *reinterpret_cast<const f16x8 *>(&qd[(rr * KP + ((4 * k + qg) ^ swz<KP>(rr))) * 8]);
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tt][k], qf, s[tt], 0, 0, 0);
             }
+            if (diagonal) {
+                const int pos = first + min(r0 + rr, rows - 1) / a.G;
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt)
+                for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(s[tt][i] * a.scale_log2 - m) * inv;
-                    acc[tt][i] += wk + 16 * tt + 4 * qg + i <= pos ? p : 0.0f;
-                }
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, -x[rg]));
+                        acc[tt][i] += wk + 16 * tt + 4 * qg + i <= pos ? p : 0.0f;
+                    }
+            } else {
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[tt][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, -x[rg]));
+            }
         }
+#pragma unroll
+        for (int rg = 0; rg < NRG; ++rg) x[rg] = y[rg];
+        __builtin_amdgcn_s_waitcnt(kVmcnt0);
+        __syncthreads();
+    };
+    for (int r0 = r_lo; r0 < r_hi; r0 += 2 * kAccountStep) {
+        step(r0, qs0, qs1);
+        if (r0 + kAccountStep < r_hi) step(r0 + kAccountStep, qs1, qs0);
     }
     const int64_t base = ((int64_t)row * a.Hkv + g) * a.room;
+    float        *part = a.parts + (int64_t)a.e[ei].part0 * a.Hkv +
+                  ((int64_t)rchunk * a.Hkv + g) * ((int64_t)account_blocks_dev(keys) * kAccountKeys);
 #pragma unroll
-    for (int tt = 0; tt < 4; ++tt)
+    for (int tt = 0; tt < 4; ++tt) {
+        f32x4 v = acc[tt];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v = acc[tt][i];
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int o = 1; o < 16; o <<= 1) v += __shfl_xor(v, o);
-            const int t = wk + 16 * tt + 4 * qg + i;
-            if (c == 0 && t < keys) a.w_out[base + t] = (a.w_in && t < p0 ? a.w_in[base + t] : 0.0f) + v;
+            for (int o = 1; o < 16; o <<= 1) v[i] += __shfl_xor(v[i], o);
+        const int t = wk + 16 * tt + 4 * qg;
+        if (c > 0) continue;
+        if (nrc > 1) {
+            *reinterpret_cast<f32x4 *>(part + t) = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (t + i < keys) a.w_out[base + t + i] = (a.w_in && t + i < p0 ? a.w_in[base + t + i] : 0.0f) + v[i];
         }
+    }
+}
+
+// The accounts of entries with several chunks of rows, from the chunks that see the
+// token's block.
+__global__ __launch_bounds__(kThreads) void account_join_kernel(AccountArgs a) {
+    const int ei = blockIdx.z, g = blockIdx.y, t = blockIdx.x * kThreads + threadIdx.x;
+    const int p0 = a.e[ei].p0, keys = p0 + a.e[ei].n, nrc = a.e[ei].nrc, rc = a.e[ei].rc;
+    if (nrc == 1 || t >= keys) return;
+    const int     first = keys - a.e[ei].w, k_lo = t / kAccountKeys * kAccountKeys;
+    const int     sees = max(0, k_lo - first) * a.G / kAccountStep * kAccountStep;
+    const int64_t base = ((int64_t)a.e[ei].row * a.Hkv + g) * a.room, len = (int64_t)account_blocks_dev(keys) * kAccountKeys;
+    const float  *part = a.parts + (int64_t)a.e[ei].part0 * a.Hkv + (int64_t)g * len + t;
+    float         sum = a.w_in && t < p0 ? a.w_in[base + t] : 0.0f;
+    for (int k = sees / rc; k < nrc; ++k) sum += part[(int64_t)k * a.Hkv * len];
+    a.w_out[base + t] = sum;
 }
 
 template <int D> void launch_d(const AccountArgs &a, const AccountLaunch &l, bool paged, hipStream_t stream) {
     const dim3 stats((unsigned)l.items * (unsigned)a.Hkv), sums((unsigned)l.sums * (unsigned)a.Hkv), block(kThreads);
-    if (paged) {
-        hipLaunchKernelGGL((account_stats_kernel<D, true>), stats, block, 0, stream, a);
-        hipLaunchKernelGGL((account_sum_kernel<D, true>), sums, block, 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((account_stats_kernel<D, false>), stats, block, 0, stream, a);
-        hipLaunchKernelGGL((account_sum_kernel<D, false>), sums, block, 0, stream, a);
-    }
+    if (paged) hipLaunchKernelGGL((account_stats_kernel<D, true>), stats, block, 0, stream, a);
+    else hipLaunchKernelGGL((account_stats_kernel<D, false>), stats, block, 0, stream, a);
     HIP_CHECK(hipGetLastError());
+    if (l.split_keys) {
+        const dim3 grid((unsigned)((l.most_rows + kThreads / 64 - 1) / (kThreads / 64)), (unsigned)a.Hkv, (unsigned)l.n);
+        hipLaunchKernelGGL(account_merge_kernel, grid, block, 0, stream, a);
+        HIP_CHECK(hipGetLastError());
+    }
+    if (paged) hipLaunchKernelGGL((account_sum_kernel<D, true>), sums, block, 0, stream, a);
+    else hipLaunchKernelGGL((account_sum_kernel<D, false>), sums, block, 0, stream, a);
+    HIP_CHECK(hipGetLastError());
+    if (l.split_rows) {
+        const dim3 grid((unsigned)((l.most_keys + kThreads - 1) / kThreads), (unsigned)a.Hkv, (unsigned)l.n);
+        hipLaunchKernelGGL(account_join_kernel, grid, block, 0, stream, a);
+        HIP_CHECK(hipGetLastError());
+    }
 }
 
 } // namespace
 
 size_t account_workspace_floats(const AccountPlan &plan, int Hkv) {
     int64_t most = 0;
-    for (const auto &l : plan.launches) most = std::max(most, l.stats);
-    return 2 * (size_t)most * (size_t)Hkv;
+    for (const auto &l : plan.launches) most = std::max(most, l.lse + 2 * l.stats + l.parts);
+    return (size_t)most * (size_t)Hkv;
 }
 
 void launch_account(const AccountCall &c, const KvView &kv, const AccountPlan &plan, float *workspace,
@@ -310,19 +412,20 @@ void launch_account(const AccountCall &c, const KvView &kv, const AccountPlan &p
     a.q = c.q;
     a.w_in = c.w_in;
     a.w_out = c.w_out;
-    a.stats = workspace;
     a.kv = kv;
     a.room = c.room;
-    a.scale_log2 = c.scale * 1.4426950408889634f;
+    // (0: so small that every score is 0 beside a masked one's -infinity)
+    a.scale_log2 = c.scale == 0.0f ? 1e-37f : c.scale * 1.4426950408889634f;
     a.Hq = c.Hq;
     a.Hkv = c.Hkv;
     a.G = c.Hq / c.Hkv;
     const bool paged = kv.block_table != nullptr;
     for (const auto &l : plan.launches) {
         if (l.n == 0 || l.items == 0) continue;
-        if ((int64_t)std::max(l.items, l.sums) * c.Hkv > INT32_MAX)
-            throw std::invalid_argument("attention account: too many work items");
         a.n = l.n;
+        a.parts = workspace; // (multiples of 256 first: their stores are of 16 bytes)
+        a.stats = a.parts + l.parts * c.Hkv;
+        a.lse = a.stats + 2 * l.stats * c.Hkv;
         std::memcpy(a.e, plan.entries.data() + l.first, sizeof(AccountEntry) * (size_t)l.n);
         profile_begin(KernelId::AttnAccount, stream);
         switch (c.D) {

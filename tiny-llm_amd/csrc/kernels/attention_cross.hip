@@ -47,7 +47,7 @@ struct CrossArgs {
     float        *part_o;  // [item][Hkv][rows of a workgroup][D]
     float        *part_ml; // [item][Hkv][rows][2]
     KvView        kv;
-    float         scale_log2; // not negative
+    float         scale_log2; // positive
     int           negate;
     int           Hq, Hkv, G, n;
     CrossEntry    e[kCrossBatch];
@@ -226,16 +226,6 @@ attn_cross_kernel(CrossArgs a) {
                     pf[j][tt >> 1][4 * (tt & 1) + i] =
                         (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[j][tt][i], a.scale_log2, -m_new));
         }
-        if (a.scale_log2 == 0.0f && (kt + 1) * kTile > S) { // -inf * 0: those keys' weights again
-            const int tb = kt * kTile + 4 * qg;
-#pragma unroll
-            for (int j = 0; j < NQG; ++j)
-#pragma unroll
-                for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (tb + 16 * tt + i >= S) pf[j][tt >> 1][4 * (tt & 1) + i] = (_Float16)0.0f;
-        }
 #pragma unroll
         for (int tp = 0; tp < 2; ++tp) {
 #pragma unroll
@@ -388,7 +378,8 @@ void launch_attn_cross(const CrossCall &c, const KvView &kv, const CrossPlan &pl
     a.q = c.q;
     a.out = c.out;
     a.kv = kv;
-    a.scale_log2 = std::fabs(c.scale) * 1.4426950408889634f;
+    // (0: so small that every score is 0 beside a masked one's -infinity)
+    a.scale_log2 = c.scale == 0.0f ? 1e-37f : std::fabs(c.scale) * 1.4426950408889634f;
     a.negate = c.scale < 0.0f;
     a.Hq = c.Hq;
     a.Hkv = c.Hkv;

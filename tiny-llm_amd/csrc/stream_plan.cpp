@@ -64,29 +64,51 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
 }
 
 bool plan_account(AccountPlan &plan, int G, int Hkv, int cus) {
-    // Row tiles of all entries fill the chip by themselves, or their keys are
-    // split, into chunks of at least four tiles.
-    int64_t tiles = 0;
-    for (const auto &e : plan.entries) tiles += ((int64_t)e.w * G + kAccountRows - 1) / kAccountRows;
-    const int64_t want = 4 * (int64_t)std::max(1, cus);
-    const int64_t split = std::max<int64_t>(1, want / std::max<int64_t>(1, tiles * Hkv));
+    // Row tiles of all entries fill the chip (two workgroups a CU), or their keys are
+    // split, into chunks of at least four tiles; likewise key blocks, or their rows
+    // are, into chunks of at least two steps.  (Half of a whole prompt's blocks are
+    // above the diagonal and empty, hence more of them.)
+    const int64_t n = std::max(1, cus);
+    int64_t       tiles = 0, blocks = 0;
+    for (const auto &e : plan.entries) {
+        tiles += ((int64_t)e.w * G + kAccountRows - 1) / kAccountRows;
+        blocks += account_blocks(e.p0 + e.n);
+    }
+    const int64_t split = std::max<int64_t>(1, 2 * n / std::max<int64_t>(1, tiles * Hkv));
+    const int64_t row_split = std::max<int64_t>(1, 8 * n / std::max<int64_t>(1, blocks * Hkv));
     plan.launches.clear();
     for (size_t i = 0; i < plan.entries.size();) {
-        AccountLaunch l{(int)i, 0, 0, 0, 0};
+        AccountLaunch l{};
+        l.first = (int)i;
+        int64_t items = 0, sums = 0;
         for (; i < plan.entries.size() && l.n < kAccountBatch; ++i, ++l.n) {
             AccountEntry &e = plan.entries[i];
-            const int     keys = e.p0 + e.n;
+            const int     keys = e.p0 + e.n, kb = account_blocks(keys);
             const int64_t rows = (int64_t)e.w * G, rt = (rows + kAccountRows - 1) / kAccountRows;
+            if (rows > INT32_MAX) return false;
             e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(split, stream_tiles(keys) / 4));
+            const int64_t steps = (rows + kAccountStep - 1) / kAccountStep;
+            const int64_t each = std::max<int64_t>(2, (steps + row_split - 1) / row_split);
+            e.rc = (int)std::min<int64_t>(each * kAccountStep, 1 << 30);
+            e.nrc = (int)((rows + e.rc - 1) / e.rc);
+            e.item0 = (int32_t)items;
+            e.sum0 = (int32_t)sums;
+            e.lse0 = (int32_t)l.lse;
             e.stat0 = (int32_t)l.stats;
-            e.item0 = l.items;
-            e.sum0 = l.sums;
-            l.stats += rows * e.nch;
-            const int64_t items = l.items + rt * e.nch;
-            if (l.stats > INT32_MAX || items > INT32_MAX) return false;
-            l.items = (int)items;
-            l.sums += keys / kAccountKeys + (keys % kAccountKeys != 0);
+            e.part0 = (int32_t)l.parts;
+            items += rt * e.nch;
+            sums += (int64_t)kb * e.nrc;
+            l.lse += rows;
+            if (e.nch > 1) l.stats += rows * e.nch;
+            if (e.nrc > 1) l.parts += (int64_t)kb * kAccountKeys * e.nrc;
+            if (std::max({items * Hkv, sums * Hkv, l.lse, l.stats, l.parts}) > INT32_MAX) return false;
+            l.split_keys |= e.nch > 1;
+            l.split_rows |= e.nrc > 1;
+            if (e.nch > 1) l.most_rows = std::max(l.most_rows, (int)rows);
+            if (e.nrc > 1) l.most_keys = std::max(l.most_keys, keys);
         }
+        l.items = (int)items;
+        l.sums = (int)sums;
         plan.launches.push_back(l);
     }
     return true;

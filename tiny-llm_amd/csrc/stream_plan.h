@@ -57,18 +57,24 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus);
 
 constexpr int kAccountRows = 128;  // query rows of a workgroup of account_stats_kernel
 constexpr int kAccountKeys = 256;  // keys of a workgroup of account_sum_kernel
-constexpr int kAccountBatch = 96;  // entries per launch
+constexpr int kAccountStep = 64;   // rows that it stages at a time
+constexpr int kAccountBatch = 72;  // entries per launch
 
 // The last w of the n new tokens of cache row `row` (positions p0 .. p0 + n - 1; tok0:
-// the first one's index in the call's tokens) attend causally.  nch: chunks of
-// its keys in account_stats_kernel, stat0: its first row of partial statistics
-// (per kv head), item0 / sum0: work items of the entries before it in its launch.
+// the first one's index in the call's tokens) attend causally: w * G query rows per
+// kv head.  account_stats_kernel cuts them into tiles and their keys into nch chunks
+// (item0: its work items of the entries before); lse0, stat0: the entries' rows of
+// results and of partial results before.  account_sum_kernel cuts the keys into
+// blocks and the rows into nrc chunks of `rc` (sum0: work items before; part0: tokens
+// of partial sums before).
 struct AccountEntry {
-    int32_t row, p0, n, w, tok0, nch, stat0, item0, sum0;
+    int32_t row, p0, n, w, tok0, nch, item0, lse0, stat0, nrc, rc, sum0, part0;
 };
 struct AccountLaunch {
-    int first, n, items, sums;
-    int64_t stats; // rows of partial statistics, per kv head
+    int     first, n, items, sums;
+    bool    split_keys, split_rows;   // some nch, nrc is above 1
+    int     most_rows, most_keys;     // of an entry
+    int64_t lse, stats, parts;        // per kv head
 };
 struct AccountPlan {
     std::vector<AccountEntry>  entries;
@@ -77,8 +83,10 @@ struct AccountPlan {
     void                       clear() { entries.clear(), launches.clear(), window = -1; }
 };
 
-// Sets nch, stat0, item0 and sum0 of plan.entries, and the launches.  False when
-// a launch's statistics do not fit 31 bits.
+inline int account_blocks(int keys) { return keys / kAccountKeys + (keys % kAccountKeys != 0); }
+
+// Sets the rest of plan.entries, and the launches.  False when a launch's rows or
+// items do not fit 31 bits.
 bool plan_account(AccountPlan &plan, int G, int Hkv, int cus);
 
 // Query tokens tok0 .. tok0 + nq - 1 attend to the first S >= 1 tokens of cache row
