@@ -13,8 +13,8 @@
 // one multiply-add and one exponential, 2^(s * scale * log2(e) - lse).  A workgroup
 // has 128 rows, 32 per wave in registers, and a chunk of the keys, whose tiles of 64
 // pass through LDS (DMA, two buffers).  S^T = K Q^T on v_mfma_f32_16x16x32_f16 as in
-// the prefill kernel: a lane has 16 keys of its row column per tile, and its own
-// reference point, which moves on jumps above 2^8 only.
+// the prefill kernel: a lane has 16 keys of its row column per tile, and a running
+// maximum of its own.
 // account_sum_kernel: a workgroup has 256 keys, 64 per wave in registers, and passes
 // a chunk of the rows that see them through LDS, 64 at a time (DMA, two buffers); a
 // lane adds its row column's weights to 16 keys' sums, and the 16 columns are added
@@ -33,6 +33,7 @@
 #include <algorithm>
 #include <cstring>
 #include <stdexcept>
+#include <type_traits>
 
 namespace tiny_llm {
 namespace detail {
@@ -45,7 +46,7 @@ typedef float    f32x4 __attribute__((ext_vector_type(4)));
 constexpr int   kThreads = 256;
 constexpr int   kVmcnt0 = 0x0F70; // s_waitcnt vmcnt(0)
 constexpr int   kTile = kStreamTile;
-constexpr float kLazyMax = 8.0f;
+constexpr float kNone = -1e30f;  // a maximum over no score
 
 struct AccountArgs {
     const __half *q;
@@ -57,7 +58,7 @@ struct AccountArgs {
     KvView        kv;
     int64_t       room;
     float         scale_log2;
-    int           Hq, Hkv, G, n;
+    int           Hq, Hkv, lg, n; // lg: log2 of the query heads per kv head
     AccountEntry  e[kAccountBatch];
 };
 static_assert(sizeof(AccountArgs) <= 4096, "kernel arguments");
@@ -109,11 +110,11 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
     ACCOUNT_ENTRY_OF(a, item0, item, ei);
     const int row = a.e[ei].row, p0 = a.e[ei].p0, n = a.e[ei].n, w = a.e[ei].w, nch = a.e[ei].nch;
     const int rel = item - a.e[ei].item0, ch = rel % nch;
-    const int rows = w * a.G;
+    const int rows = w << a.lg;
     const int rt = (rows - 1) / kAccountRows - rel / nch; // the tiles with the most keys first
     const int r_lo = rt * kAccountRows, r_hi = min(rows, r_lo + kAccountRows);
     const int first = p0 + n - w;                          // position of query row 0's token
-    const int kend = first + (r_hi - 1) / a.G + 1;         // keys that some row of the tile sees
+    const int kend = first + ((r_hi - 1) >> a.lg) + 1;         // keys that some row of the tile sees
     const int tiles = (p0 + n + kTile - 1) / kTile;        // of the whole, so that chunks agree
     const int t_lo = (int)((int64_t)ch * tiles / nch);
     const int t_hi = min((int)((int64_t)(ch + 1) * tiles / nch), (kend + kTile - 1) / kTile);
@@ -124,8 +125,8 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         const int     r = min(r_lo + wave * 32 + j * 16 + c, rows - 1);
-        const __half *qp = a.q + ((int64_t)(a.e[ei].tok0 + n - w + r / a.G) * a.Hq + g * a.G + r % a.G) * D;
-        pos[j] = first + r / a.G;
+        const __half *qp = a.q + ((int64_t)(a.e[ei].tok0 + n - w + (r >> a.lg)) * a.Hq + (g << a.lg) + (r & ((1 << a.lg) - 1))) * D;
+        pos[j] = first + (r >> a.lg);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             // (a negative scale's sign goes into q: the maximum over s is then that over s * scale)
@@ -135,19 +136,51 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
     }
     const float scale = fabsf(a.scale_log2);
     const char *kb = reinterpret_cast<const char *>(a.kv.k_base) + (int64_t)g * a.kv.head_stride * 2;
-    auto issue = [&](int kt, uint16_t *dst) {
+    // A wave's 64 pieces of a load lie in one quarter of 16 tokens, whose offset is
+    // uniform: ids has the quarters' blocks in its first lanes (paged views), asked
+    // for a tile ahead.
+    const uint32_t tokb = (uint32_t)(a.kv.tok_stride * 2);
+    const int32_t *bt = PAGED ? a.kv.block_table + (int64_t)row * a.kv.bt_stride : nullptr;
+    auto blocks = [&](int kt) -> int {
+        if constexpr (PAGED) return lane < 4 ? bt[min(kt * kTile + 16 * lane, kend - 1) >> a.kv.log2_blk] : 0;
+        else return 0;
+    };
+    uint32_t lane_off[NKI]; // in the quarter
+#pragma unroll
+    for (int u = 0; u < NKI; ++u) {
+        const int sl = u * kThreads + (int)threadIdx.x, r = sl / KP;
+        lane_off[u] = (uint32_t)(r % 16) * tokb + 16u * ((sl % KP) ^ swz<KP>(r));
+    }
+    auto issue = [&](int kt, int ids, uint16_t *dst) __attribute__((always_inline)) {
+        const bool whole = kt * kTile + kTile <= kend;
 #pragma unroll
         for (int u = 0; u < NKI; ++u) {
-            const int sl = u * kThreads + (int)threadIdx.x;
-            const int r = sl / KP, x = (sl % KP) ^ swz<KP>(r);
-            const int t = min(kt * kTile + r, kend - 1);
-            lds_dma(kb + key_off<PAGED>(a.kv, row, t) + 16 * x, dst + (u * kThreads + wave * 64) * 8);
+            const int q = (u * kThreads + wave * 64) / KP / 16; // the quarter
+            const int tq = min(kt * kTile + 16 * q, kend - 1);
+            int64_t   off;
+            if constexpr (PAGED)
+                off = ((int64_t)__builtin_amdgcn_readlane(ids, q) * a.kv.blk_stride +
+                       (int64_t)(tq & ((1 << a.kv.log2_blk) - 1)) * a.kv.tok_stride) * 2;
+            else off = ((int64_t)row * a.kv.blk_stride + (int64_t)tq * a.kv.tok_stride) * 2;
+            uint32_t lo = lane_off[u];
+            if (!whole) { // rows past the end: the last one
+                const int r = (u * kThreads + (int)threadIdx.x) / KP % 16, more = kend - 1 - tq;
+                lo -= (uint32_t)max(0, r - more) * tokb;
+            }
+            lds_dma(kb + off + lo, dst + (u * kThreads + wave * 64) * 8);
         }
     };
-    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    const int low = first + (r_lo + wave * 32) / a.G; // the first position among the wave's rows
-    auto      step = [&](int kt, const uint16_t *kd, uint16_t *kn) __attribute__((always_inline)) {
-        if (kt + 1 < t_hi) issue(kt + 1, kn);
+    float m[2] = {kNone, kNone}, l[2] = {0.0f, 0.0f};
+    const int low = first + ((r_lo + wave * 32) >> a.lg); // the first position among the wave's rows
+    // Straight-line code, so that one row group's matrix operations run under the
+    // other's exponentials; tiles at the diagonal have code of their own.
+    int  ids = 0;
+    auto step = [&](auto diagonal, int kt, const uint16_t *kd, uint16_t *kn) __attribute__((always_inline)) {
+        if (kt + 1 < t_hi) {
+            const int now = ids;
+            if (PAGED && kt + 2 < t_hi) ids = blocks(kt + 2);
+            issue(kt + 1, now, kn);
+        }
         f32x4 s[2][4];
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
@@ -162,11 +195,10 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
 #pragma unroll
                 for (int j = 0; j < 2; ++j) s[j][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qb[j][k], s[j][tt], 0, 0, 0);
             }
-        const int  tb = kt * kTile + 4 * qg;
-        const bool diagonal = kt * kTile + kTile - 1 > low;
+        const int tb = kt * kTile + 4 * qg;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-            if (diagonal) {
+            if constexpr (diagonal) {
 #pragma unroll
                 for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
@@ -176,38 +208,37 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
             float mloc = s[j][0][0];
 #pragma unroll
             for (int x = 1; x < 16; ++x) mloc = fmaxf(mloc, s[j][x / 4][x % 4]);
-            mloc *= scale;
-            if (__any(mloc > m[j] + kLazyMax)) {
-                const float m_new = fmaxf(m[j], mloc);
-                l[j] = m[j] == -INFINITY ? 0.0f : l[j] * __builtin_amdgcn_exp2f(m[j] - m_new);
-                m[j] = m_new;
-            }
-            // (a lane that has seen no key yet: its reference point is 0, its weights are)
-            const float ref = m[j] == -INFINITY ? 0.0f : m[j];
-            float       sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            const float m_new = fmaxf(m[j], mloc * scale);
+            float       sum[4] = {l[j] * __builtin_amdgcn_exp2f(m[j] - m_new), 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][tt][i], scale, -ref));
-            l[j] += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                for (int i = 0; i < 4; ++i) sum[i] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[j][tt][i], scale, -m_new));
+            l[j] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            m[j] = m_new;
         }
         __builtin_amdgcn_s_waitcnt(kVmcnt0);
         __syncthreads();
     };
+    auto any_step = [&](int kt, const uint16_t *kd, uint16_t *kn) __attribute__((always_inline)) {
+        if (kt * kTile + kTile - 1 > low) step(std::true_type(), kt, kd, kn);
+        else step(std::false_type(), kt, kd, kn);
+    };
     if (t_lo < t_hi) {
-        issue(t_lo, ks0);
+        issue(t_lo, blocks(t_lo), ks0);
+        if (PAGED && t_lo + 1 < t_hi) ids = blocks(t_lo + 1);
         __builtin_amdgcn_s_waitcnt(kVmcnt0);
         __syncthreads();
         for (int kt = t_lo; kt < t_hi; kt += 2) {
-            step(kt, ks0, ks1);
-            if (kt + 1 < t_hi) step(kt + 1, ks1, ks0);
+            any_step(kt, ks0, ks1);
+            if (kt + 1 < t_hi) any_step(kt + 1, ks1, ks0);
         }
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
         float mr = fmaxf(m[j], __shfl_xor(m[j], 16));
         mr = fmaxf(mr, __shfl_xor(mr, 32));
-        float lr = m[j] == -INFINITY ? 0.0f : l[j] * __builtin_amdgcn_exp2f(m[j] - mr);
+        float lr = l[j] * __builtin_amdgcn_exp2f(m[j] - mr);
         lr += __shfl_xor(lr, 16);
         lr += __shfl_xor(lr, 32);
         const int r = r_lo + wave * 32 + j * 16 + c;
@@ -223,22 +254,21 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
 // lse of the rows of entries with several chunks of keys: a wave per row.
 __global__ __launch_bounds__(kThreads) void account_merge_kernel(AccountArgs a) {
     const int ei = blockIdx.z, g = blockIdx.y;
-    const int nch = a.e[ei].nch, rows = a.e[ei].w * a.G;
+    const int nch = a.e[ei].nch, rows = a.e[ei].w << a.lg;
     const int r = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (nch == 1 || r >= rows) return;
     const float *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows + r);
-    float        m = -INFINITY, l = 0.0f;
+    float        m = kNone, l = 0.0f;
     for (int ch = lane; ch < nch; ch += 64) {
         const float2 ml = *reinterpret_cast<const float2 *>(st + 2 * (int64_t)ch * a.Hkv * rows);
         const float  mn = fmaxf(m, ml.x);
-        if (mn == -INFINITY) continue; // no key of the chunk is seen
         l = l * __builtin_amdgcn_exp2f(m - mn) + ml.y * __builtin_amdgcn_exp2f(ml.x - mn);
         m = mn;
     }
     float mx = m;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-    l = m == -INFINITY ? 0.0f : l * __builtin_amdgcn_exp2f(m - mx);
+    l *= __builtin_amdgcn_exp2f(m - mx);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
     if (lane == 0) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = mx + __builtin_amdgcn_logf(l);
@@ -258,27 +288,47 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     const int row = a.e[ei].row, p0 = a.e[ei].p0, n = a.e[ei].n, w = a.e[ei].w, nrc = a.e[ei].nrc;
     const int rel = item - a.e[ei].sum0, kblk = rel / nrc, rchunk = rel - kblk * nrc;
     const int k_lo = kblk * kAccountKeys, keys = p0 + n;
-    const int rows = w * a.G, first = keys - w;
+    const int rows = w << a.lg, first = keys - w;
     // The chunk's rows, from the first step whose tokens see the block's first key.
-    const int sees = max(0, k_lo - first) * a.G / kAccountStep * kAccountStep;
+    const int sees = (max(0, k_lo - first) << a.lg) / kAccountStep * kAccountStep;
     const int r_lo = max(rchunk * a.e[ei].rc, sees), r_hi = (int)min((int64_t)rows, (int64_t)(rchunk + 1) * a.e[ei].rc);
     if (r_lo >= r_hi && nrc > 1) return; // (account_join_kernel does not read it)
     const int c = lane & 15, qg = lane >> 4;
     const int wk = k_lo + wave * 64; // the wave's first key
 
     const float  *lse = a.lse + (int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows;
-    const __half *qbase = a.q + ((int64_t)(a.e[ei].tok0 + n - w) * a.Hq + g * a.G) * D;
-    auto issue = [&](int r0, uint16_t *dst) {
+    const __half *qbase = a.q + ((int64_t)(a.e[ei].tok0 + n - w) * a.Hq + (g << a.lg)) * D;
+    // (a step's rows begin at a whole token: 64 rows hold 64 >> lg tokens)
+    uint32_t lane_off[NQI];
 #pragma unroll
-        for (int u = 0; u < NQI; ++u) {
-            const int sl = u * kThreads + (int)threadIdx.x, r = sl / KP, x = (sl % KP) ^ swz<KP>(r);
-            const int qr = min(r0 + r, rows - 1);
-            lds_dma(qbase + ((int64_t)(qr / a.G) * a.Hq + qr % a.G) * D + 8 * x, dst + (u * kThreads + wave * 64) * 8);
+    for (int u = 0; u < NQI; ++u) {
+        const int sl = u * kThreads + (int)threadIdx.x, r = sl / KP;
+        lane_off[u] = ((uint32_t)(r >> a.lg) * (uint32_t)a.Hq + (uint32_t)(r & ((1 << a.lg) - 1))) * D + 8 * ((sl % KP) ^ swz<KP>(r));
+    }
+    auto issue = [&](int r0, uint16_t *dst) __attribute__((always_inline)) {
+        const __half *base = qbase + (int64_t)(r0 >> a.lg) * a.Hq * D;
+        if (r0 + kAccountStep <= rows) {
+#pragma unroll
+            for (int u = 0; u < NQI; ++u) lds_dma(base + lane_off[u], dst + (u * kThreads + wave * 64) * 8);
+        } else { // rows past the end: the last one
+#pragma unroll
+            for (int u = 0; u < NQI; ++u) {
+                const int sl = u * kThreads + (int)threadIdx.x, r = sl / KP, x = (sl % KP) ^ swz<KP>(r);
+                const int qr = min(r, rows - 1 - r0);
+                lds_dma(base + ((int64_t)(qr >> a.lg) * a.Hq + (qr & ((1 << a.lg) - 1))) * D + 8 * x,
+                        dst + (u * kThreads + wave * 64) * 8);
+            }
         }
     };
-    auto load_lse = [&](int r0, float(&x)[NRG]) {
+    auto load_lse = [&](int r0, float(&x)[NRG]) __attribute__((always_inline)) {
+        const float *p = lse + r0;
+        if (r0 + kAccountStep <= r_hi) {
 #pragma unroll
-        for (int rg = 0; rg < NRG; ++rg) x[rg] = r0 + 16 * rg + c < r_hi ? lse[r0 + 16 * rg + c] : INFINITY; // weights of 0
+            for (int rg = 0; rg < NRG; ++rg) x[rg] = p[16 * rg + c];
+        } else {
+#pragma unroll
+            for (int rg = 0; rg < NRG; ++rg) x[rg] = r0 + 16 * rg + c < r_hi ? p[16 * rg + c] : INFINITY; // weights of 0
+        }
     };
     if (r_lo < r_hi) issue(r_lo, qs0);
     const char *kb = reinterpret_cast<const char *>(a.kv.k_base) + (int64_t)g * a.kv.head_stride * 2;
@@ -296,50 +346,51 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     load_lse(r_lo, x);
     __builtin_amdgcn_s_waitcnt(kVmcnt0);
     __syncthreads();
-    auto step = [&](int r0, const uint16_t *qd, uint16_t *qn) __attribute__((always_inline)) {
+    auto compute = [&](auto diagonal, int r0, const uint16_t *qd) __attribute__((always_inline)) {
+        // One group's scores are computed under the exponentials of the one before.
+        f32x4 s[2][4];
+        auto  scores = [&](int rg, f32x4(&t)[4]) __attribute__((always_inline)) {
+            const int rr = 16 * rg + c;
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt) t[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int k = 0; k < KS; ++k) {
+                const f16x8 qf = *reinterpret_cast<const f16x8 *>(&qd[(rr * KP + ((4 * k + qg) ^ swz<KP>(rr))) * 8]);
+#pragma unroll
+                for (int tt = 0; tt < 4; ++tt) t[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tt][k], qf, t[tt], 0, 0, 0);
+            }
+        };
+        scores(0, s[0]);
+#pragma unroll
+        for (int rg = 0; rg < NRG; ++rg) {
+            if (rg + 1 < NRG) scores(rg + 1, s[(rg + 1) & 1]);
+            const int pos = first + (min(r0 + 16 * rg + c, rows - 1) >> a.lg);
+#pragma unroll
+            for (int tt = 0; tt < 4; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rg & 1][tt][i], a.scale_log2, -x[rg]));
+                    if constexpr (diagonal) acc[tt][i] += wk + 16 * tt + 4 * qg + i <= pos ? p : 0.0f;
+                    else acc[tt][i] += p;
+                }
+        }
+    };
+    auto any_step = [&](int r0, const uint16_t *qd, uint16_t *qn) __attribute__((always_inline)) {
         float y[NRG];
         if (r0 + kAccountStep < r_hi) {
             issue(r0 + kAccountStep, qn);
             load_lse(r0 + kAccountStep, y);
         }
-        const bool diagonal = wk + 63 > first + r0 / a.G; // some row does not see every key of the wave
-#pragma unroll
-        for (int rg = 0; rg < NRG; ++rg) {
-            const int rr = 16 * rg + c;
-            f32x4     s[4];
-#pragma unroll
-            for (int tt = 0; tt < 4; ++tt) s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int k = 0; k < KS; ++k) {
-                const f16x8 qf = *reinterpret_cast<const f16x8 *>(&qd[(rr * KP + ((4 * k + qg) ^ swz<KP>(rr))) * 8]);
-#pragma unroll
-                for (int tt = 0; tt < 4; ++tt) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[tt][k], qf, s[tt], 0, 0, 0);
-            }
-            if (diagonal) {
-                const int pos = first + min(r0 + rr, rows - 1) / a.G;
-#pragma unroll
-                for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, -x[rg]));
-                        acc[tt][i] += wk + 16 * tt + 4 * qg + i <= pos ? p : 0.0f;
-                    }
-            } else {
-#pragma unroll
-                for (int tt = 0; tt < 4; ++tt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[tt][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[tt][i], a.scale_log2, -x[rg]));
-            }
-        }
+        if (wk + 63 <= first + (r0 >> a.lg)) compute(std::false_type(), r0, qd); // every row sees every key
+        else if (wk <= first + ((r0 + kAccountStep - 1) >> a.lg)) compute(std::true_type(), r0, qd);
 #pragma unroll
         for (int rg = 0; rg < NRG; ++rg) x[rg] = y[rg];
         __builtin_amdgcn_s_waitcnt(kVmcnt0);
         __syncthreads();
     };
     for (int r0 = r_lo; r0 < r_hi; r0 += 2 * kAccountStep) {
-        step(r0, qs0, qs1);
-        if (r0 + kAccountStep < r_hi) step(r0 + kAccountStep, qs1, qs0);
+        any_step(r0, qs0, qs1);
+        if (r0 + kAccountStep < r_hi) any_step(r0 + kAccountStep, qs1, qs0);
     }
     const int64_t base = ((int64_t)row * a.Hkv + g) * a.room;
     float        *part = a.parts + (int64_t)a.e[ei].part0 * a.Hkv +
@@ -370,7 +421,7 @@ __global__ __launch_bounds__(kThreads) void account_join_kernel(AccountArgs a) {
     const int p0 = a.e[ei].p0, keys = p0 + a.e[ei].n, nrc = a.e[ei].nrc, rc = a.e[ei].rc;
     if (nrc == 1 || t >= keys) return;
     const int     first = keys - a.e[ei].w, k_lo = t / kAccountKeys * kAccountKeys;
-    const int     sees = max(0, k_lo - first) * a.G / kAccountStep * kAccountStep;
+    const int     sees = (max(0, k_lo - first) << a.lg) / kAccountStep * kAccountStep;
     const int64_t base = ((int64_t)a.e[ei].row * a.Hkv + g) * a.room, len = (int64_t)account_blocks_dev(keys) * kAccountKeys;
     const float  *part = a.parts + (int64_t)a.e[ei].part0 * a.Hkv + (int64_t)g * len + t;
     float         sum = a.w_in && t < p0 ? a.w_in[base + t] : 0.0f;
@@ -418,7 +469,7 @@ void launch_account(const AccountCall &c, const KvView &kv, const AccountPlan &p
     a.scale_log2 = c.scale == 0.0f ? 1e-37f : c.scale * 1.4426950408889634f;
     a.Hq = c.Hq;
     a.Hkv = c.Hkv;
-    a.G = c.Hq / c.Hkv;
+    a.lg = __builtin_ctz((unsigned)(c.Hq / c.Hkv));
     const bool paged = kv.block_table != nullptr;
     for (const auto &l : plan.launches) {
         if (l.n == 0 || l.items == 0) continue;

@@ -49,7 +49,7 @@ struct CrossArgs {
     KvView        kv;
     float         scale_log2; // positive
     int           negate;
-    int           Hq, Hkv, G, n;
+    int           Hq, Hkv, lg, n; // lg: log2 of the query heads per kv head
     CrossEntry    e[kCrossBatch];
 };
 static_assert(sizeof(CrossArgs) <= 4096, "kernel arguments");
@@ -107,7 +107,7 @@ attn_cross_kernel(CrossArgs a) {
     int       ei;
     CROSS_ENTRY_OF(a, item, ei);
     const int row = a.e[ei].row, S = a.e[ei].S, tok0 = a.e[ei].tok0, nch = a.e[ei].nch;
-    const int rows = a.e[ei].nq * a.G;
+    const int rows = a.e[ei].nq << a.lg;
     const int rel = item - a.e[ei].item0, rt = rel / nch, ch = rel - rt * nch;
     const int tiles = (S + kTile - 1) / kTile;
     const int t_lo = (int)((int64_t)ch * tiles / nch), t_hi = (int)((int64_t)(ch + 1) * tiles / nch);
@@ -119,7 +119,7 @@ attn_cross_kernel(CrossArgs a) {
         return __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr(&vd[vlane + ((2 * dt) ^ vxor) * 8 + r0 * KP * 8]));
     };
     auto row_of = [&](int r) -> int64_t { // element offset of query row r in q and out
-        return ((int64_t)(tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D;
+        return ((int64_t)(tok0 + (r >> a.lg)) * a.Hq + (g << a.lg) + (r & ((1 << a.lg) - 1))) * D;
     };
     f16x8 qb[NQG][KS];
 #pragma unroll
@@ -138,22 +138,31 @@ attn_cross_kernel(CrossArgs a) {
     const char    *vb = reinterpret_cast<const char *>(a.kv.v_base) + head;
     const int64_t  blk_bytes = a.kv.blk_stride * 2, tokb = a.kv.tok_stride * 2;
     const int32_t *bt = PAGED ? a.kv.block_table + (int64_t)row * a.kv.bt_stride : nullptr;
-    auto token_off = [&](int t) -> int64_t {
-        if constexpr (PAGED)
-            return (int64_t)bt[t >> a.kv.log2_blk] * blk_bytes + (int64_t)(t & ((1 << a.kv.log2_blk) - 1)) * tokb;
-        else return (int64_t)row * blk_bytes + (int64_t)t * tokb;
+    // A wave's 64 pieces of a load lie in one quarter of 16 tokens, whose offset is
+    // uniform: ids has the quarters' blocks in its first lanes (paged views), asked
+    // for a tile ahead.
+    auto blocks = [&](int kt) -> int {
+        if constexpr (PAGED) return lane < 4 ? bt[min(kt * kTile + 16 * lane, S - 1) >> a.kv.log2_blk] : 0;
+        else return 0;
     };
-    auto issue_tile = [&](int kt, uint16_t *kdst, uint16_t *vdst) {
+    int  ids = 0;
+    auto issue_tile = [&](int kt, int now, uint16_t *kdst, uint16_t *vdst) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < NKI; ++u) {
             const int sl = u * NT + tid;
             if (NKI * NT > PIECES && sl >= PIECES) break; // whole waves (PIECES % 64 == 0)
-            const int     r = sl / KP, x = (sl % KP) ^ swz(r);
-            const int64_t off = token_off(min(kt * kTile + r, S - 1)) + 16 * x;
-            const int     lbase = (u * NT + wave * 64) * 8; // halves, wave-uniform
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(kb + off),
+            const int r = sl / KP, x = (sl % KP) ^ swz(r);
+            const int q = __builtin_amdgcn_readfirstlane((u * NT + wave * 64) / KP / 16); // the quarter
+            const int tq = min(kt * kTile + 16 * q, S - 1), more = S - 1 - tq;
+            int64_t   off;
+            if constexpr (PAGED)
+                off = (int64_t)__builtin_amdgcn_readlane(now, q) * blk_bytes + (int64_t)(tq & ((1 << a.kv.log2_blk) - 1)) * tokb;
+            else off = (int64_t)row * blk_bytes + (int64_t)tq * tokb;
+            const uint32_t lane_off = (uint32_t)min(r % 16, more) * (uint32_t)tokb + 16u * x;
+            const int      lbase = (u * NT + wave * 64) * 8; // halves, wave-uniform
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(kb + off + lane_off),
                                              (__attribute__((address_space(3))) void *)(&kdst[lbase]), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(vb + off),
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(vb + off + lane_off),
                                              (__attribute__((address_space(3))) void *)(&vdst[lbase]), 16, 0, 0);
         }
     };
@@ -171,7 +180,11 @@ attn_cross_kernel(CrossArgs a) {
 
     auto tile_step = [&](int kt, const uint16_t *kd, const uint16_t *vd, uint16_t *kn, uint16_t *vn)
                          __attribute__((always_inline)) {
-        if (kt + 1 < t_hi) issue_tile(kt + 1, kn, vn);
+        if (kt + 1 < t_hi) {
+            const int now = ids;
+            if (PAGED && kt + 2 < t_hi) ids = blocks(kt + 2);
+            issue_tile(kt + 1, now, kn, vn);
+        }
         f32x4 s[NQG][4];
 #pragma unroll
         for (int tt = 0; tt < 4; ++tt)
@@ -242,7 +255,8 @@ attn_cross_kernel(CrossArgs a) {
         __builtin_amdgcn_s_waitcnt(kVmcnt0); // this wave's part of the next tile has landed
         __syncthreads();                      // ... every wave's, and this tile's buffer is free
     };
-    issue_tile(t_lo, ks0, vt0);
+    issue_tile(t_lo, blocks(t_lo), ks0, vt0);
+    if (PAGED && t_lo + 1 < t_hi) ids = blocks(t_lo + 1);
     __builtin_amdgcn_s_waitcnt(kVmcnt0);
     __syncthreads();
     for (int kt = t_lo; kt < t_hi; kt += 2) {
@@ -306,7 +320,7 @@ template <int ROWS> __global__ __launch_bounds__(kMergeThreads) void cross_merge
     __shared__ f32x4 s_o[kMergeThreads];
     __shared__ float s_ml[kMergeThreads][2];
     const int ei = blockIdx.z, g = blockIdx.y;
-    const int nch = a.e[ei].nch, rows = a.e[ei].nq * a.G;
+    const int nch = a.e[ei].nch, rows = a.e[ei].nq << a.lg;
     const int per = D / 4, tid = threadIdx.x;
     const int grp = tid / per % groups, d = 4 * (tid % per);
     const int r = blockIdx.x * (kMergeThreads / (per * groups)) + tid / (per * groups);
@@ -345,7 +359,7 @@ template <int ROWS> __global__ __launch_bounds__(kMergeThreads) void cross_merge
     uint2         w;
     w.x = __builtin_bit_cast(uint32_t, lo);
     w.y = __builtin_bit_cast(uint32_t, hi);
-    *reinterpret_cast<uint2 *>(a.out + ((int64_t)(a.e[ei].tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D + d) = w;
+    *reinterpret_cast<uint2 *>(a.out + ((int64_t)(a.e[ei].tok0 + (r >> a.lg)) * a.Hq + (g << a.lg) + (r & ((1 << a.lg) - 1))) * D + d) = w;
 }
 
 template <int D, int NW> void launch_dw(const CrossArgs &a, int items, bool paged, hipStream_t stream) {
@@ -383,7 +397,7 @@ void launch_attn_cross(const CrossCall &c, const KvView &kv, const CrossPlan &pl
     a.negate = c.scale < 0.0f;
     a.Hq = c.Hq;
     a.Hkv = c.Hkv;
-    a.G = c.Hq / c.Hkv;
+    a.lg = __builtin_ctz((unsigned)(c.Hq / c.Hkv));
     const bool paged = kv.block_table != nullptr;
     const int  tile = cross_rows(c.D, plan.waves);
     for (const auto &l : plan.launches) {
@@ -407,7 +421,7 @@ void launch_attn_cross(const CrossCall &c, const KvView &kv, const CrossPlan &pl
             for (int i = l.first; i < l.first + l.n; ++i) {
                 const CrossEntry &e = plan.entries[(size_t)i];
                 chunks = std::max(chunks, (int)e.nch);
-                if (e.nch > 1) rows = std::max(rows, (int64_t)e.nq * a.G);
+                if (e.nch > 1) rows = std::max(rows, (int64_t)e.nq << a.lg);
             }
             while (2 * groups <= chunks && 2 * groups * (c.D / 4) <= kMergeThreads) groups *= 2;
             const int  per_block = kMergeThreads / (groups * (c.D / 4)); // rows
