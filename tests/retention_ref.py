@@ -138,3 +138,26 @@ def evict(w, pos, keep, newest):
     for t in range(keep):
         src.append(t if t in stay else next(m))
     return src
+
+
+def even_tail(tl, n, d, block=0):
+    """A cache whose every 64th token has a weight 2^25 times the others', which have
+    values of 1000 and it of 0, the query that sees it so (at a scale of 1) and what
+    attention gives: most of the output is from weights that one fp16 cannot hold
+    beside a largest one of 1."""
+    c = Cache(tl, [0], 1, d, room=n, block=block)
+    k, v = np.zeros((n, 1, d), np.float16), np.full((n, 1, d), 1000.0, np.float16)
+    k[::64, 0, 0], v[::64] = 4.34375, 0.0
+    parts = iter([k, v])
+    c.rows = lambda m, std=1.0: next(parts)
+    c.append([n])
+    q = np.zeros(d, np.float16)
+    q[0] = 4.0
+    heavy = len(k[::64])
+    light = (n - heavy) * np.exp(-4.0 * 4.34375)
+    want = 1000.0 * light / (heavy + light)
+    # A weight's rounding to fp16, where the largest is 2^7 at least: half a step of
+    # 2^-24 / 2^7, (n - heavy) / heavy of them per largest one, times 1000; the
+    # output's rounding; scores of 17.4 with d + 4 roundings, and sums of n terms.
+    tol = 1000.0 * (n - heavy) / heavy * 2.0 ** -32 + want * (2.0 ** -11 + (17.4 * (d + 4) + n) * 2.0 ** -23) + 2.0 ** -25
+    return c, q, want, tol

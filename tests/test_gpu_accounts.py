@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from retention_ref import Cache, attend, check_account, check_out, dev
+from retention_ref import Cache, attend, check_account, check_out, dev, even_tail
 
 pytestmark = pytest.mark.gpu
 
@@ -121,6 +121,18 @@ def test_decode_weights_values_at_the_ends_of_their_range(tl):
     top = int(w[0, 0].argmax())
     assert w[0, 0, top] > 0.999 and got[0, top] >= 0.999
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("d,block", [(64, 0), (128, 16), (256, 0)])
+def test_decode_weights_far_below_the_largest(tl, d, block):
+    c, q, want, tol = even_tail(tl, 4096, d, block)
+    b = tl.DecodeBatch(c.mgr, 1, 1)
+    b.prepare_lengths(c.ids, [4096])
+    dq, w = dev(q[None, None]), c.account()
+    out = torch.empty_like(dq)
+    b.decode_weights(0, dq.data_ptr(), None, None, out.data_ptr(), 1.0, None, w.data_ptr())
+    torch.cuda.synchronize()
+    assert np.abs(out.cpu().numpy().astype(np.float64) - want).max() <= tol
 
 
 def test_decode_weights_offsets_beyond_32_bits(tl):

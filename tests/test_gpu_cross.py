@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from retention_ref import Cache, attend, check_out, dev
+from retention_ref import Cache, attend, check_out, dev, even_tail
 
 pytestmark = pytest.mark.gpu
 
@@ -98,6 +98,18 @@ def test_cross_scale_of_zero(tl, nq):
     mean = c.v[0][0][:, 0].astype(np.float64).mean(axis=0)
     # the output's rounding, values below 1
     assert np.abs(out.cpu().numpy().astype(np.float64) - mean).max() <= 2.0 ** -11
+
+
+@pytest.mark.parametrize("nq,d", [(1, 64), (16, 128), (200, 128), (300, 64), (40, 256)])
+def test_cross_weights_far_below_the_largest(tl, nq, d):
+    c, q, want, tol = even_tail(tl, 4096, d)
+    dq = dev(np.tile(q, (nq, 1, 1)))
+    out = torch.empty_like(dq)
+    b = tl.CrossBatch(c.mgr, 1, 1)
+    b.prepare(c.ids, [nq])
+    b.attention(0, dq.data_ptr(), out.data_ptr(), 1.0)
+    torch.cuda.synchronize()
+    assert np.abs(out.cpu().numpy().astype(np.float64) - want).max() <= tol
 
 
 def test_cross_neighbours_over_the_same_states(tl):

@@ -65,7 +65,7 @@ Result<void> CrossBatch::prepare(const int *seq_ids, const int *num_queries, con
         lens[static_cast<size_t>(i)] = a;
         total += num_queries[i];
     }
-    if (total > INT32_MAX / 2) return Result<void>::err("CrossBatch: too many query tokens in one step");
+    if (total * group > INT32_MAX / 2) return Result<void>::err("CrossBatch: too many query rows in one step");
     mgr_.syncTable(stream);
     // Neighbours over the same states are one entry of the plans: their rows share
     // every key.  Up to 16 rows (and entries over nothing) take attn_stream_kernel,

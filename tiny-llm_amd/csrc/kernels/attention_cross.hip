@@ -8,8 +8,8 @@
 // (head_dim 256: 16) query rows each in registers; key tiles of 64 tokens through
 // double-buffered LDS by the LDS DMA load, in XOR-swizzled 16-byte slots;
 //   S^T = K Q^T      v_mfma_f32_16x16x32_f16: A = K rows, B = Q
-//   online softmax   per query column, its reference point moving on jumps above 2^8
-//                    only; p rounded to fp16 for the product, the normaliser sums
+//   online softmax   per query column, over a reference point 2^7 below the maximum,
+//                    which moves on jumps above 2^15 only; p rounded to fp16 for the product, the normaliser sums
 //                    the rounded ones (on the matrix unit, a row of ones)
 //   O^T += V^T P^T   V^T by the transposing ds_read_b64_tr_b16, P^T as the S^T
 //                    fragments stand
@@ -37,7 +37,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float    f32x4 __attribute__((ext_vector_type(4)));
 typedef short    s16x4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLazyMax = 8.0f;
+constexpr float kBelow = 7.0f, kLazyMax = 15.0f; // of the softmax reference, as in attn_stream_kernel
 constexpr int   kVmcnt0 = 0x0F70; // s_waitcnt vmcnt(0)
 constexpr int   kTile = kStreamTile;
 
@@ -224,7 +224,7 @@ attn_cross_kernel(CrossArgs a) {
                 for (int i = 0; i < 4; ++i) mloc = fmaxf(mloc, s[j][tt][i]);
             if (__any(mloc * a.scale_log2 > m_run[j] + kLazyMax)) {
                 const float m_tile = xor_lane_max<32>(xor_lane_max<16>(mloc)) * a.scale_log2;
-                const float m_new = fmaxf(m_run[j], m_tile);
+                const float m_new = fmaxf(m_run[j], m_tile - kBelow);
                 const float alpha = m_run[j] == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run[j] - m_new);
 #pragma unroll
                 for (int dt = 0; dt < DT; ++dt) acc[j][dt] *= alpha;

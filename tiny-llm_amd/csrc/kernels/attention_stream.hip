@@ -20,10 +20,9 @@
 //   S^T = K Q^T      v_mfma_f32_16x16x32_f16: A = K rows (token l%16, dims
 //                    8(l/16)..+7) straight from memory, B = Q (row l%16),
 //                    D = S^T (tokens 4(l/16)+i, row l%16)
-//   softmax          per row column in the log2 domain; the reference point
-//                    moves on jumps above 2^8 only, p is at most 2^8 (fp16 for the
-//                    product, a relative rounding of 2^-11 per weight; its sum
-//                    stays fp32)
+//   softmax          per row column in the log2 domain, over a reference point near
+//                    the maximum (kBelow); p is fp16 for the product, a relative
+//                    rounding of 2^-11 per weight, its sum stays fp32
 //   O^T += V^T P^T   over 32 tokens; V^T from the wave's row-major LDS stage by
 //                    the transposing ds_read_b64_tr_b16
 // stream_finish_kernel: merges the outputs of entries with several chunks and turns
@@ -50,7 +49,11 @@ typedef float    f32x4 __attribute__((ext_vector_type(4)));
 typedef short    s16x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr float kLazyMax = 8.0f;
+// Weights are 2^(s - ref).  The reference is 2^7 below the maximum when it moves, and
+// moves on scores 2^15 above it only: weights stay below 2^15 in fp16, and those 2^-31
+// of the largest are still above its smallest step.  (A reference at the maximum lost
+// all weights 2^-25 below it, which a long cache of even ones feels.)
+constexpr float kBelow = 7.0f, kLazyMax = 15.0f;
 
 struct StreamArgs {
     const __half *q;
@@ -293,7 +296,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
         if (__any(mloc > m_run + kLazyMax)) {
             mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
             mloc = fmaxf(mloc, __shfl_xor(mloc, 32));
-            const float m_new = fmaxf(m_run, mloc);
+            const float m_new = fmaxf(m_run, mloc - kBelow);
             const float alpha = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
@@ -379,19 +382,19 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
 }
 
 constexpr int kFinishThreads = 256;
-constexpr int kFinishTokens = 1024; // tokens of a workgroup
+constexpr int kFinishTokens = 1024; // tokens of a block
+constexpr int kMostBlocks = 32768;  // grid.y
 
-// Entries of several chunks (or none: zero rows).  Workgroup (entry, kv head, block
+// Entries of several chunks (or none: zero rows).  Workgroup (entry, kv head, blocks
 // of tokens): the rows' maxima and sums over the chunks, the account of the
-// block's tokens, and in block 0 the outputs.
+// blocks' tokens, and with block 0 the outputs.
 __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArgs a, int D) {
     __shared__ float s_m[kStreamRows], s_l[kStreamRows], s_inv[kStreamRows];
     const int ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv;
     const int S = a.e[ei].S, tok0 = a.e[ei].tok0, rows = a.e[ei].nq * a.G;
     const int tiles = (S + kStreamTile - 1) / kStreamTile;
     const int nch = (tiles + a.chunk - 1) / a.chunk;
-    const int t_lo = blockIdx.y * kFinishTokens, t_hi = min(S, t_lo + kFinishTokens);
-    if (nch == 1 || (blockIdx.y > 0 && t_lo >= t_hi)) return;
+    if (nch == 1 || (blockIdx.y > 0 && (int)blockIdx.y * kFinishTokens >= S)) return;
     const int64_t p0 = ((int64_t)a.e[ei].item0 * a.Hkv + g) * a.rows; // row 0 of chunk 0
     const int64_t pc = (int64_t)a.Hkv * a.rows;                      // from chunk to chunk
     const int     lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -415,8 +418,11 @@ __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArg
     }
     __syncthreads();
     if (a.w_out) { // (a launch with accounts has entries of one query: rows = a.rows)
-        const float *sc = a.scores + ((int64_t)a.e[ei].tile0 * a.Hkv + (int64_t)g * tiles + t_lo / kStreamTile) * a.rows * kStreamTile;
-        account_tokens<kFinishThreads>(a, ei, g, rows, t_lo, t_hi, sc, s_m, s_inv);
+        for (int64_t t = (int64_t)blockIdx.y * kFinishTokens; t < S; t += (int64_t)gridDim.y * kFinishTokens) {
+            const int    t_lo = (int)t, t_hi = (int)min((int64_t)S, t + kFinishTokens);
+            const float *sc = a.scores + ((int64_t)a.e[ei].tile0 * a.Hkv + (int64_t)g * tiles + t_lo / kStreamTile) * a.rows * kStreamTile;
+            account_tokens<kFinishThreads>(a, ei, g, rows, t_lo, t_hi, sc, s_m, s_inv);
+        }
     }
     if (blockIdx.y > 0) return;
     for (int idx = threadIdx.x; idx < rows * D; idx += kFinishThreads) {
@@ -518,7 +524,7 @@ void launch_attn_stream(const StreamCall &c, const KvView &kv, const StreamPlan 
             HIP_CHECK(hipGetLastError());
         }
         if (l.finish) {
-            const unsigned blocks = c.w_out ? (unsigned)std::max(1, (l.max_len + kFinishTokens - 1) / kFinishTokens) : 1u;
+            const unsigned blocks = c.w_out ? (unsigned)std::clamp(l.max_len / kFinishTokens + 1, 1, kMostBlocks) : 1u;
             hipLaunchKernelGGL(stream_finish_kernel, dim3((unsigned)(l.n * c.Hkv), blocks), dim3(kFinishThreads), 0, stream,
                                a, c.D);
             HIP_CHECK(hipGetLastError());

@@ -85,7 +85,7 @@ bool plan_account(AccountPlan &plan, int G, int Hkv, int cus) {
             AccountEntry &e = plan.entries[i];
             const int     keys = e.p0 + e.n, kb = account_blocks(keys);
             const int64_t rows = (int64_t)e.w * G, rt = (rows + kAccountRows - 1) / kAccountRows;
-            if (rows > INT32_MAX) return false;
+            if (rows > INT32_MAX / 2) return false;
             e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(split, stream_tiles(keys) / 4));
             const int64_t steps = (rows + kAccountStep - 1) / kAccountStep;
             const int64_t each = std::max<int64_t>(2, (steps + row_split - 1) / row_split);
