@@ -251,6 +251,85 @@ def test_evict_refusals(tl):
     torch.cuda.synchronize()
 
 
+def test_an_eviction_that_has_begun_is_committed_first(tl):
+    """Its rows have moved: a second selection would read what the first overwrote."""
+    c = Cache(tl, [30, 40], 1, 32, layers=2, seed=14)
+    w, p = weights(c, "tail"), c.account(0, torch.int32)
+    w2, p2 = c.account(), c.account(0, torch.int32)
+    W, P, W2, P2 = (x.data_ptr() for x in (w, p, w2, p2))
+    first, second, third = (tl.EvictBatch(c.mgr, 2) for _ in range(3))
+    for ev in (first, second):
+        ev.prepare(c.ids, [10, 50], 2)
+    first.run(0, W, W2, P, P2)
+    want = w2.clone(), p2.clone()
+    with pytest.raises(tl.TinyLLMError, match="not committed"):
+        second.run(0, W, W2, P, P2)
+    with pytest.raises(tl.TinyLLMError, match="not committed"):
+        first.prepare(c.ids, [10, 50], 2)
+    assert first.info() == {"n": 2, "evicted": 20}
+    with pytest.raises(tl.TinyLLMError, match="not committed"):
+        third.prepare(c.ids[:1], [5], 2)
+    assert third.info()["n"] == 0
+    third.prepare(c.ids[1:], [5], 2)  # nothing of it was taken
+    second.close()
+    for layer in (0, 1):
+        first.run(layer, W, W2, P, P2)
+    first.commit()
+    torch.cuda.synchronize()
+    assert torch.equal(w2[0, :, :10], want[0][0, :, :10]) and torch.equal(p2[0, :, :10], want[1][0, :, :10])
+    assert [c.mgr.getSeqLen(s) for s in c.ids] == [10, 40]
+    third.close()
+    third = tl.EvictBatch(c.mgr, 2)
+    third.prepare(c.ids, [5, 5], 2)
+    third.run(0, W2, W2, P2, P2)
+    third.close()  # abandoned: the sequences are for release
+    with pytest.raises(tl.TinyLLMError, match="not committed"):
+        first.prepare(c.ids, [5, 5], 2)
+    for s in c.ids:
+        c.mgr.releaseSequence(s)
+    sid, _ = c.mgr.allocateSequence(30)
+    c.mgr.advanceSeqLen(sid, 6)
+    first.prepare([sid], [6], 2)
+    torch.cuda.synchronize()
+
+
+def test_evict_prepared_in_a_capture_does_not_grow_the_workspace(tl):
+    c = Cache(tl, [300], 1, 32, seed=15)
+    ev = tl.EvictBatch(c.mgr, 1)
+    x = torch.zeros(4, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        x.add_(1)  # a capture of something
+        with pytest.raises(tl.TinyLLMError, match="captured"):
+            ev.prepare(c.ids, [100], 0, torch.cuda.current_stream().cuda_stream)
+    assert ev.info()["n"] == 0
+
+
+def test_evict_millions_of_tokens(tl):
+    """More pairs than a grid has blocks for; all of the newest half stays."""
+    n = 4 * 2 ** 20 + 77
+    keep = n // 2
+    mgr = tl.KVCacheManager(num_layers=1, num_heads=1, head_dim=32, max_seq_len=n, max_batch_size=1)
+    sid, _ = mgr.allocateSequence(n)
+    k, v = (torch.randn((n, 1, 32), device="cuda", dtype=torch.float16) for _ in range(2))
+    assert mgr.appendKV(sid, 0, k.data_ptr(), v.data_ptr(), n) is None
+    mgr.advanceSeqLen(sid, n)
+    w = torch.arange(n, device="cuda", dtype=torch.float32)[None, None].contiguous()  # exact below 2^24
+    pos = torch.zeros((1, 1, n), dtype=torch.int32, device="cuda")
+    ev = tl.EvictBatch(mgr, 1)
+    ev.prepare([sid], [keep], 0)
+    ev.run(0, w.data_ptr(), w.data_ptr(), pos.data_ptr(), pos.data_ptr())
+    ev.commit()
+    out = [torch.empty((1, 1, keep, 32), dtype=torch.float16, device="cuda") for _ in range(2)]
+    b = tl.DecodeBatch(mgr, 1, 1)
+    b.prepare_lengths([sid], [keep])
+    b.gather(0, out[0].data_ptr(), out[1].data_ptr(), keep)
+    torch.cuda.synchronize()
+    src = torch.arange(n - keep, n, device="cuda")  # movers in order to all places
+    assert torch.equal(pos[0, 0, :keep].long(), src) and torch.equal(w[0, 0, :keep], src.float())
+    assert torch.equal(out[0][0, 0], k[src, 0]) and torch.equal(out[1][0, 0], v[src, 0])
+
+
 def test_a_slot_starts_anew(tl):
     c = Cache(tl, [30], 1, 32, room=64, seed=10)
     step(tl, c, [10], 2, [weights(c, "tail")], [c.account(0, torch.int32)], True, [(0, 0)])

@@ -37,7 +37,8 @@ namespace {
 
 constexpr int kBins = 2048;      // 11 bits of the key
 constexpr int kMoveThreads = 256;
-constexpr int kMovePairs = 32;   // pairs of a workgroup of evict_move_kernel
+constexpr int kMovePairs = 32;   // pairs that a workgroup of evict_move_kernel moves at once
+constexpr int kMostBlocks = 32768; // grid.y
 constexpr int kOneThreads = 256;
 constexpr int kList = 2048;      // candidates that the second digit finds in a list
 constexpr uint32_t kNewest = 0xFFFFFFFFu; // above every account's key
@@ -553,28 +554,29 @@ template <int D> __global__ __launch_bounds__(kMoveThreads) void evict_move_kern
     const int        ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv;
     const EvictEntry e = a.e[ei];
     const int        cap = min(e.len - e.keep, e.keep);
-    const int        first = blockIdx.y * kMovePairs;
-    if (first >= cap) return; // (before the count: none of the entry's workgroups behind its list reads it)
+    if ((int)blockIdx.y * kMovePairs >= cap) return; // (before the count: no workgroup behind the list reads it)
     const int   cnt = a.counts[(int64_t)ei * a.Hkv + g];
     const int2 *pairs = reinterpret_cast<const int2 *>(a.pairs) + (int64_t)e.list * a.Hkv + (int64_t)g * cap;
-    u32x4       v[N];
-    __half     *to[N];
+    for (int first = blockIdx.y * kMovePairs; first < cap; first += gridDim.y * kMovePairs) {
+        u32x4   v[N];
+        __half *to[N];
 #pragma unroll
-    for (int u = 0; u < N; ++u) { // every row on its way before the first is written
-        const int x = u * kMoveThreads + (int)threadIdx.x;
-        const int r = first + x / (2 * PIECES);
-        to[u] = nullptr;
-        const int2 p = pairs[min(r, cap - 1)]; // (on its way with the count)
-        if (r < cnt) {
-            __half    *b = const_cast<__half *>(x / PIECES & 1 ? a.kv.v_base : a.kv.k_base) + (int64_t)g * a.kv.head_stride +
-                        8 * (x % PIECES);
-            v[u] = *reinterpret_cast<const u32x4 *>(b + row_off(a.kv, e.row, p.x));
-            to[u] = b + row_off(a.kv, e.row, p.y);
+        for (int u = 0; u < N; ++u) { // every row on its way before the first is written
+            const int x = u * kMoveThreads + (int)threadIdx.x;
+            const int r = first + x / (2 * PIECES);
+            to[u] = nullptr;
+            const int2 p = pairs[min(r, cap - 1)]; // (on its way with the count)
+            if (r < cnt) {
+                __half    *b = const_cast<__half *>(x / PIECES & 1 ? a.kv.v_base : a.kv.k_base) + (int64_t)g * a.kv.head_stride +
+                            8 * (x % PIECES);
+                v[u] = *reinterpret_cast<const u32x4 *>(b + row_off(a.kv, e.row, p.x));
+                to[u] = b + row_off(a.kv, e.row, p.y);
+            }
         }
-    }
 #pragma unroll
-    for (int u = 0; u < N; ++u)
-        if (to[u]) *reinterpret_cast<u32x4 *>(to[u]) = v[u];
+        for (int u = 0; u < N; ++u)
+            if (to[u]) *reinterpret_cast<u32x4 *>(to[u]) = v[u];
+    }
 }
 
 template <int NT, int IT> void launch_select(const EvictArgs &a, dim3 grid, hipStream_t stream) {
@@ -637,7 +639,7 @@ void launch_evict(const KvView &kv, const std::vector<EvictEntry> &entries, cons
             else if (len <= 32768) launch_select<1024, 8>(a, heads, stream);
             else hipLaunchKernelGGL((evict_select_any_kernel<1024>), heads, dim3(1024), 0, stream, a);
             HIP_CHECK(hipGetLastError());
-            const dim3 grid(heads.x, (unsigned)((cap + kMovePairs - 1) / kMovePairs));
+            const dim3 grid(heads.x, (unsigned)std::min((cap + kMovePairs - 1) / kMovePairs, kMostBlocks));
             switch (D) {
             case 32: hipLaunchKernelGGL((evict_move_kernel<32>), grid, dim3(kMoveThreads), 0, stream, a); break;
             case 64: hipLaunchKernelGGL((evict_move_kernel<64>), grid, dim3(kMoveThreads), 0, stream, a); break;

@@ -336,6 +336,7 @@ void KVCacheManager::truncate(int slot, int keep) {
     Eviction      &ev = evictions_[static_cast<size_t>(slot)];
     ev.gone += sc.current_len - keep;
     ev.base = keep;
+    ev.by = nullptr;
     sc.current_len = keep;
     if (blocks_) blocks_->shrink(slot, (keep + block_tokens_ - 1) / block_tokens_);
 }

@@ -37,6 +37,10 @@ std::string check_accounts(const char *who, const KVCacheConfig &cfg, const floa
     return "";
 }
 
+std::string begun(int seq_id) {
+    return "EvictBatch: an eviction of sequence " + std::to_string(seq_id) + " has run and is not committed";
+}
+
 std::string check_device(const char *who, int device) {
     const int now = detail::current_device();
     return now == device ? std::string()
@@ -161,6 +165,9 @@ Result<std::unique_ptr<EvictBatch>> EvictBatch::create(KVCacheManager &mgr, int 
 }
 
 Result<void> EvictBatch::prepare(const int *seq_ids, const int *budgets, int n, int recent, hipStream_t stream) {
+    for (size_t i = 0; i < ids_.size(); ++i)
+        if (mgr_.sequence(ids_[i]) && mgr_.evictions_[static_cast<size_t>(entries_[i].row)].by == this)
+            return Result<void>::err(begun(ids_[i]));
     // A failing prepare leaves an empty batch.
     ids_.clear();
     entries_.clear();
@@ -189,6 +196,7 @@ Result<void> EvictBatch::prepare(const int *seq_ids, const int *budgets, int n, 
                                      std::to_string(seq_ids[i]) + " must be positive and hold the " +
                                      std::to_string(recent) + " newest tokens");
         const KVCacheManager::Eviction &ev = mgr_.evictions_[static_cast<size_t>(slot)];
+        if (ev.by) return Result<void>::err(begun(seq_ids[i]));
         if (ev.gone > INT32_MAX - cfg.max_seq_len)
             return Result<void>::err("EvictBatch: positions of sequence " + std::to_string(seq_ids[i]) +
                                      " exceed 31 bits");
@@ -199,6 +207,9 @@ Result<void> EvictBatch::prepare(const int *seq_ids, const int *budgets, int n, 
     }
     if (pairs > INT32_MAX) return Result<void>::err("EvictBatch: too many tokens in one step");
     const size_t words = detail::evict_workspace_words(entries, cfg.num_heads);
+    if (!work_->holds(words) && detail::stream_capturing(stream))
+        return Result<void>::err("EvictBatch: the workspace cannot grow while the stream is captured: prepare before "
+                                 "the capture");
     lists_ = reinterpret_cast<int32_t *>(work_->get(std::max<size_t>(words, 1)));
     mgr_.syncTable(stream);
     entries_ = std::move(entries);
@@ -240,6 +251,12 @@ Result<void> EvictBatch::run(int layer_idx, const float *weights_in, float *weig
         return Result<void>::err("EvictBatch: layer " + std::to_string(layer_idx) +
                                  " ran in place: commit before it runs again");
     if (std::string err = check_device("EvictBatch", mgr_.device()); !err.empty()) return Result<void>::err(err);
+    for (size_t i = 0; i < ids_.size(); ++i) {
+        const EvictBatch *by = mgr_.evictions_[static_cast<size_t>(entries_[i].row)].by;
+        if (by && by != this) return Result<void>::err(begun(ids_[i]));
+    }
+    for (const auto &e : entries_)
+        if (e.keep < e.len) mgr_.evictions_[static_cast<size_t>(e.row)].by = this;
     detail::EvictState st;
     st.w_in = weights_in;
     st.w_out = weights_out;

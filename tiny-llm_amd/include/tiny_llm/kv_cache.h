@@ -52,6 +52,8 @@ struct SequenceCache {
     bool active = false;
 };
 
+class EvictBatch;
+
 class KVCacheManager {
   public:
     static Result<std::unique_ptr<KVCacheManager>> create(const KVCacheConfig &config);
@@ -135,10 +137,12 @@ class KVCacheManager {
     int    findFreeSlot() const;
 
     // What evictions did to a slot's sequence: tokens gone, and its length right
-    // after the last one (the tokens from there on came since, in order).
+    // after the last one (the tokens from there on came since, in order); by: the
+    // batch that has moved its rows and not committed (compared, never followed).
     struct Eviction {
-        int gone = 0;
-        int base = 0;
+        int               gone = 0;
+        int               base = 0;
+        const EvictBatch *by = nullptr;
     };
     friend class EvictBatch;
     void truncate(int slot, int keep);
@@ -351,6 +355,12 @@ class PrefillBatch {
 // run() writes the first min(length, budget) of both, and may work in place; an
 // output that is not its input must not overlap it.  A layer that ran in place
 // is not run again before commit().
+//
+// A run moves rows, so an eviction that has begun is to be committed: until then
+// no prepare() takes its sequences, no other batch's run() does, and the cache is
+// not to be read at the layers that ran.  A captured run() counts as run.  run()
+// calls of one batch share its lists: one stream, or the caller orders them, also
+// the replays of graphs that captured them.
 class EvictBatch {
   public:
     static Result<std::unique_ptr<EvictBatch>> create(KVCacheManager &mgr, int max_seqs);
@@ -390,7 +400,9 @@ class EvictBatch {
 // beside the queries': every query of an entry attends to all of the states.
 // The states are a sequence of `mgr` like any other, appended once (appendKV or
 // PrefillBatch::append, then advanceSeqLen); several entries may name the same
-// one.  prepare() snapshots a step, attention() runs a layer of it.
+// one.  prepare() snapshots a step, attention() runs a layer of it.  The calls of one
+// batch share its workspace: one stream, or the caller orders them, also the
+// replays of graphs that captured them.
 class CrossBatch {
   public:
     static Result<std::unique_ptr<CrossBatch>> create(KVCacheManager &mgr, int max_entries, int num_q_heads);
