@@ -40,7 +40,7 @@ constexpr int kMoveThreads = 256;
 constexpr int kMovePairs = 32;   // pairs that a workgroup of evict_move_kernel moves at once
 constexpr int kMostBlocks = 32768; // grid.y
 constexpr int kOneThreads = 256;
-constexpr int kList = 2048;      // candidates that the second digit finds in a list
+constexpr int kList = 2048;      // candidates at least that the second digit finds in a list
 constexpr uint32_t kNewest = 0xFFFFFFFFu; // above every account's key
 
 struct EvictArgs {
@@ -183,9 +183,12 @@ template <int NT> __device__ __forceinline__ void pick_bin(const uint32_t *hist,
 template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
     constexpr int NW = NT / 64;
     static_assert(IT <= 8, "a bit per token");
-    // Histogram and list, then the free places (half of the tokens at most).
-    __shared__ uint32_t buf[kBins + kList > NT * IT * 2 ? kBins + kList : NT * IT * 2];
-    uint32_t *const hist = buf, *const list = buf + kBins, *const places = buf;
+    // Histogram and list, then the free places and behind them the movers, by index.
+    constexpr int kBuf = kBins + kList > NT * IT * 2 ? kBins + kList : NT * IT * 2, kListed = kBuf - kBins;
+    static_assert(NT * IT * 4 <= 1 << 16, "an index of 16 bits, two a word");
+    __shared__ __align__(4) uint32_t buf[kBuf];
+    uint32_t *const hist = buf, *const list = buf + kBins;
+    uint16_t *const order = reinterpret_cast<uint16_t *>(buf);
     __shared__ uint32_t lds[NW];
     __shared__ uint32_t pick[3];
     __shared__ uint32_t before[IT * NW]; // flags of step it's wave w, then of those before it
@@ -195,7 +198,13 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
     const EvictEntry &e = h.e;
     const int cap = min(e.len - e.keep, e.keep);
     int2     *pairs = reinterpret_cast<int2 *>(a.pairs) + (int64_t)e.list * a.Hkv + (int64_t)h.g * cap;
-    auto      token = [&](int it) { return (it * NT + tid) * 4; };
+    // (Computed anew at each use: kept for all steps from phase to phase, the tokens'
+    // addresses pushed keys out of the registers.)
+    auto token = [&](int it) __attribute__((always_inline)) {
+        int t = tid;
+        if (IT > 4) asm volatile("" : "+v"(t));
+        return (it * NT + t) * 4;
+    };
 
     // The keys stay in registers: 0 past the end, which is below or equal to every
     // other and last in order.
@@ -241,7 +250,7 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
         need = pick[1];
         equal = pick[2];
         shift = 21;
-        const bool     listed = equal <= (uint32_t)kList;
+        const bool     listed = equal <= (uint32_t)kListed;
         const uint32_t n = equal;
         if (listed && equal != need) {
 #pragma unroll
@@ -362,48 +371,46 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
     };
 #pragma unroll
     for (int it = 0; it < IT; ++it) {
+        uint32_t r = before[it * NW + wave] + scan[it];
+        for (uint32_t f = moving(it); f; f &= f - 1) order[r++] = (uint16_t)(token(it) + __builtin_ctz(f));
+    }
+#pragma unroll
+    for (int it = 0; it < IT; ++it) {
         if (IT > 4) __builtin_amdgcn_sched_barrier(0);
         const int      i = token(it);
         const uint32_t f = moving(it);
-        uint32_t       r = before[it * NW + wave] + scan[it];
         if (i >= e.keep) continue;
         Words p = {}, x = {};
         if (copy_w) x = accounts(it);
         if (copy_p && i < e.base) p = load4(h.p_in, i, e.base);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (i + u >= e.keep) continue;
-            if (f >> u & 1) {
-                places[r++] = (uint32_t)(i + u);
-            } else {
-                if (copy_w) h.w_out[i + u] = __uint_as_float(x.x[u]);
-                if (i + u >= e.base) h.p_out[i + u] = i + u + e.gone;
-                else if (copy_p) h.p_out[i + u] = (int32_t)p.x[u];
-            }
+            if (i + u >= e.keep || (f >> u & 1)) continue;
+            if (copy_w) h.w_out[i + u] = __uint_as_float(x.x[u]);
+            if (i + u >= e.base) h.p_out[i + u] = i + u + e.gone;
+            else if (copy_p) h.p_out[i + u] = (int32_t)p.x[u];
         }
     }
     if (tid == 0) a.counts[(int64_t)h.ei * a.Hkv + h.g] = (int32_t)moved;
     __syncthreads();
-#pragma unroll
-    for (int it = 0; it < IT; ++it) {
-        if (IT > 4) __builtin_amdgcn_sched_barrier(0);
-        const int      i = token(it);
-        const uint32_t f = moving(it);
-        uint32_t       r = before[it * NW + wave] + scan[it];
-        if (!f || i + 3 < e.keep) continue;
-        const Words x = accounts(it);
-        Words       p = {};
-        if (i < e.base) p = load4(h.p_in, i, e.base);
+    for (uint32_t r0 = tid; r0 < moved; r0 += 4 * NT) { // four on their way at once
+        int     from[4];
+        float   w[4];
+        int32_t p[4];
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            if (!(f >> u & 1)) continue;
-            if (i + u >= e.keep) {
-                const int to = (int)places[r - moved];
-                pairs[r - moved] = make_int2(i + u, to);
-                h.w_out[to] = __uint_as_float(x.x[u]);
-                h.p_out[to] = i + u < e.base ? (int32_t)p.x[u] : i + u + e.gone;
-            }
-            ++r;
+            from[u] = order[moved + min(r0 + u * NT, moved - 1)];
+            w[u] = h.w_in[from[u]];
+            p[u] = h.position(from[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const uint32_t r = r0 + u * NT;
+            if (r >= moved) break;
+            const int to = order[r];
+            pairs[r] = make_int2(from[u], to);
+            h.w_out[to] = w[u];
+            h.p_out[to] = p[u];
         }
     }
 }
