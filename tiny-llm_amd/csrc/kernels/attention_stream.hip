@@ -385,20 +385,22 @@ constexpr int kFinishThreads = 256;
 constexpr int kFinishTokens = 1024; // tokens of a block
 constexpr int kMostBlocks = 32768;  // grid.y
 
-// Entries of several chunks (or none: zero rows).  Workgroup (entry, kv head, blocks
-// of tokens): the rows' maxima and sums over the chunks, the account of the
-// blocks' tokens, and with block 0 the outputs.
+// Entries of several chunks (or none: zero rows).  Workgroup (entry, kv head, y):
+// the rows' maxima and sums over the chunks; every gridDim.y-th block of tokens'
+// account and row's output, whose chunks are spread over the threads.
 __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArgs a, int D) {
     __shared__ float s_m[kStreamRows], s_l[kStreamRows], s_inv[kStreamRows];
+    __shared__ f32x4 s_o[kFinishThreads];
     const int ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv;
     const int S = a.e[ei].S, tok0 = a.e[ei].tok0, rows = a.e[ei].nq * a.G;
     const int tiles = (S + kStreamTile - 1) / kStreamTile;
     const int nch = (tiles + a.chunk - 1) / a.chunk;
-    if (nch == 1 || (blockIdx.y > 0 && (int)blockIdx.y * kFinishTokens >= S)) return;
+    if (nch == 1 || ((int)blockIdx.y >= rows && (!a.w_out || (int)blockIdx.y * kFinishTokens >= S))) return;
     const int64_t p0 = ((int64_t)a.e[ei].item0 * a.Hkv + g) * a.rows; // row 0 of chunk 0
     const int64_t pc = (int64_t)a.Hkv * a.rows;                      // from chunk to chunk
     const int     lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int r = wave; r < rows; r += kFinishThreads / 64) {
+        if (!a.w_out && r % (int)gridDim.y != (int)blockIdx.y) continue; // (an account takes every row)
         float m = -INFINITY, l = 0.0f;
         for (int ch = lane; ch < nch; ch += 64) {
             const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (p0 + ch * pc + r) * 2);
@@ -417,6 +419,27 @@ __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArg
         }
     }
     __syncthreads();
+    const int per = D / 4, groups = kFinishThreads / per, grp = threadIdx.x / per, d = 4 * (threadIdx.x % per);
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+        f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+        for (int ch = grp; ch < nch; ch += groups) {
+            const int64_t pr = p0 + ch * pc + r;
+            o += __builtin_amdgcn_exp2f(a.part_ml[pr * 2] - s_m[r]) * *reinterpret_cast<const f32x4 *>(a.part_o + pr * D + d);
+        }
+        s_o[threadIdx.x] = o;
+        __syncthreads();
+        if (grp == 0) {
+            for (int k = 1; k < groups; ++k) o += s_o[threadIdx.x + k * per];
+            const float   inv = nch ? 1.0f / (s_l[r] + 1e-6f) : 0.0f;
+            const __half2 lo = __floats2half2_rn(o[0] * inv, o[1] * inv), hi = __floats2half2_rn(o[2] * inv, o[3] * inv);
+            uint2         w;
+            w.x = __builtin_bit_cast(uint32_t, lo);
+            w.y = __builtin_bit_cast(uint32_t, hi);
+            *reinterpret_cast<uint2 *>(a.out + ((int64_t)(tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D + d) = w;
+        }
+        __syncthreads();
+    }
     if (a.w_out) { // (a launch with accounts has entries of one query: rows = a.rows)
         for (int64_t t = (int64_t)blockIdx.y * kFinishTokens; t < S; t += (int64_t)gridDim.y * kFinishTokens) {
             const int    t_lo = (int)t, t_hi = (int)min((int64_t)S, t + kFinishTokens);
@@ -424,19 +447,10 @@ __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArg
             account_tokens<kFinishThreads>(a, ei, g, rows, t_lo, t_hi, sc, s_m, s_inv);
         }
     }
-    if (blockIdx.y > 0) return;
-    for (int idx = threadIdx.x; idx < rows * D; idx += kFinishThreads) {
-        const int r = idx / D, d = idx - r * D;
-        float     o = 0.0f;
-#pragma unroll 4
-        for (int ch = 0; ch < nch; ++ch) {
-            const int64_t pr = p0 + ch * pc + r;
-            o = fmaf(a.part_o[pr * D + d], __builtin_amdgcn_exp2f(a.part_ml[pr * 2] - s_m[r]), o);
-        }
-        a.out[((int64_t)(tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D + d] =
-            __float2half(nch ? o * (1.0f / (s_l[r] + 1e-6f)) : 0.0f);
-    }
 }
+
+// Floats of the partial maxima and sums, then the outputs at a multiple of 16 bytes.
+size_t part_ml_floats(size_t rows) { return (2 * rows + 3) / 4 * 4; }
 
 template <int D, bool PAGED, bool SCORES, int NW>
 void launch_one(const StreamArgs &a, int items, int lds, hipStream_t stream) {
@@ -477,7 +491,7 @@ size_t stream_workspace_floats(const StreamPlan &plan, int Hq, int Hkv, int D, b
     size_t most = 0;
     for (const auto &l : plan.launches) {
         const size_t rows = (size_t)plan_rows(plan, l.first, l.n, Hq / Hkv) * Hkv;
-        size_t       f = (size_t)l.items * rows * (size_t)(D + 2);
+        size_t       f = part_ml_floats((size_t)l.items * rows) + (size_t)l.items * rows * (size_t)D;
         if (account) f += (size_t)l.tiles * kStreamTile * rows;
         most = std::max(most, f);
     }
@@ -511,7 +525,7 @@ void launch_attn_stream(const StreamCall &c, const KvView &kv, const StreamPlan 
         std::memcpy(a.e, plan.entries.data() + l.first, sizeof(StreamEntry) * (size_t)l.n);
         a.scores = workspace;
         a.part_ml = workspace + (c.w_out ? (size_t)l.tiles * kStreamTile * a.rows * c.Hkv : 0);
-        a.part_o = a.part_ml + (size_t)l.items * c.Hkv * a.rows * 2;
+        a.part_o = a.part_ml + part_ml_floats((size_t)l.items * c.Hkv * a.rows);
         profile_begin(KernelId::AttnStream, stream);
         if (l.items > 0) {
             switch (c.D) {
@@ -524,7 +538,7 @@ void launch_attn_stream(const StreamCall &c, const KvView &kv, const StreamPlan 
             HIP_CHECK(hipGetLastError());
         }
         if (l.finish) {
-            const unsigned blocks = c.w_out ? (unsigned)std::clamp(l.max_len / kFinishTokens + 1, 1, kMostBlocks) : 1u;
+            const unsigned blocks = (unsigned)std::max(a.rows, c.w_out ? std::min(l.max_len / kFinishTokens + 1, kMostBlocks) : 1);
             hipLaunchKernelGGL(stream_finish_kernel, dim3((unsigned)(l.n * c.Hkv), blocks), dim3(kFinishThreads), 0, stream,
                                a, c.D);
             HIP_CHECK(hipGetLastError());

@@ -16,17 +16,31 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
     total *= Hkv;
     const int64_t n = std::max(1, cus);
     int64_t       chunk;
+    const int64_t share = (total + n - 1) / n, half = (total + 2 * n - 1) / (2 * n); // of a CU, of one of two workgroups
+    const bool    few = some * Hkv <= n;
     // An entry in one chunk is finished by its own workgroup: no partial results, no
-    // second launch, and its scores never leave the LDS.  That pays while no entry is
-    // much longer than a workgroup's share of all tiles; short ones are not worth
-    // splitting at all.
-    if (D <= 128 && some * Hkv <= n) { // few entries: eight waves each, one workgroup per CU
+    // second launch, and its scores never leave the LDS.  Short entries are left whole
+    // (16 x 300 states, 8 heads of 64: 7.4 us against 9.4 split), with eight waves
+    // where they have so many tiles.  Work that is little for the chip is spread over
+    // as many workgroups as it has pieces of four tiles (decode with accounts, 1 x
+    // 4096 tokens, 8 heads of 128: 16.4 us, in pieces of 8 on eight waves 18.5, of 32
+    // 29.7); where a CU has several tiles to itself, eight waves and fewer pieces are
+    // better (1 x 32768 tokens: 38.4 against 44.8 us; 1 x 8192: 22.8 against 24.4, without
+    // accounts 19.8 against 19.3), or whole entries while none is much longer than a
+    // CU's share (8 x 1024: 19.2 against 21.0).
+    if (few && longest <= (D <= 128 ? kStreamWhole : kStreamWhole / 4)) {
+        plan.waves = D <= 128 && longest > 4 ? 8 : 4;
+        chunk = longest;
+    } else if (few && total < (account_rows > 0 ? 4 : 8) * n) {
+        plan.waves = 4;
+        chunk = std::max<int64_t>(4, half);
+    } else if (few && D <= 128) {
         plan.waves = 8;
-        chunk = std::max<int64_t>(kStreamWhole, (total + n - 1) / n);
+        chunk = std::max<int64_t>(8, share);
+        if (2 * longest <= 5 * chunk) chunk = longest;
     } else {
         plan.waves = 4;
-        const int64_t share = (total + 2 * n - 1) / (2 * n);
-        chunk = longest <= std::max<int64_t>(kStreamWhole, 2 * share + share / 2) ? longest : std::max<int64_t>(8, share);
+        chunk = longest <= std::max<int64_t>(32, 2 * half + half / 2) ? longest : std::max<int64_t>(8, half);
     }
     if (account_rows > 0) {
         const int64_t fits = stream_most_tiles(D, plan.waves, account_rows);

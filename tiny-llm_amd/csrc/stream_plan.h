@@ -10,7 +10,7 @@ namespace tiny_llm {
 namespace detail {
 
 constexpr int kStreamTile = 64;    // keys
-constexpr int kStreamWhole = 32;   // tiles that one workgroup takes whatever else there is
+constexpr int kStreamWhole = 12;   // tiles that one workgroup takes whatever else there is (a quarter at head_dim 256)
 constexpr int kStreamRows = 16;    // query rows (tokens x heads of one kv head) of an entry at most
 constexpr int kStreamBatch = 144;  // entries per launch: they travel in the kernel arguments
 
