@@ -59,6 +59,7 @@ struct AccountArgs {
     int64_t       room;
     float         scale_log2;
     int           Hq, Hkv, lg, n; // lg: log2 of the query heads per kv head
+    int           fold;           // no account_merge_kernel ran
     AccountEntry  e[kAccountBatch];
 };
 static_assert(sizeof(AccountArgs) <= 4096, "kernel arguments");
@@ -251,27 +252,36 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
     }
 }
 
-// lse of the rows of entries with several chunks of keys: a wave per row.
-__global__ __launch_bounds__(kThreads) void account_merge_kernel(AccountArgs a) {
-    const int ei = blockIdx.z, g = blockIdx.y;
-    const int nch = a.e[ei].nch, rows = a.e[ei].w << a.lg;
-    const int r = blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (nch == 1 || r >= rows) return;
-    const float *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows + r);
-    float        m = kNone, l = 0.0f;
-    for (int ch = lane; ch < nch; ch += 64) {
-        const float2 ml = *reinterpret_cast<const float2 *>(st + 2 * (int64_t)ch * a.Hkv * rows);
+// lse of row r from its nch chunks' (m, l), st: those of chunk 0, `step` floats from
+// chunk to chunk.  Four lanes a row, 16 apart, take every fourth chunk, so that a
+// load is of 16 neighbouring rows.
+__device__ __forceinline__ float merged_lse(const float *st, int64_t step, int nch) {
+    float m = kNone, l = 0.0f;
+#pragma unroll 4
+    for (int ch = (threadIdx.x >> 4) & 3; ch < nch; ch += 4) {
+        const float2 ml = *reinterpret_cast<const float2 *>(st + ch * step);
         const float  mn = fmaxf(m, ml.x);
         l = l * __builtin_amdgcn_exp2f(m - mn) + ml.y * __builtin_amdgcn_exp2f(ml.x - mn);
         m = mn;
     }
-    float mx = m;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
+    float mx = fmaxf(m, __shfl_xor(m, 16));
+    mx = fmaxf(mx, __shfl_xor(mx, 32));
     l *= __builtin_amdgcn_exp2f(m - mx);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
-    if (lane == 0) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = mx + __builtin_amdgcn_logf(l);
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    return mx + __builtin_amdgcn_logf(l);
+}
+
+// lse of the rows of entries with several chunks of keys, where account_sum_kernel
+// does not merge them itself.
+__global__ __launch_bounds__(kThreads) void account_merge_kernel(AccountArgs a) {
+    const int ei = blockIdx.z, g = blockIdx.y;
+    const int nch = a.e[ei].nch, rows = a.e[ei].w << a.lg;
+    const int r = blockIdx.x * (kThreads / 4) + (threadIdx.x >> 6) * 16 + (threadIdx.x & 15);
+    if (nch == 1) return;
+    const float *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows + min(r, rows - 1));
+    const float  lse = merged_lse(st, 2 * (int64_t)a.Hkv * rows, nch);
+    if ((threadIdx.x & 63) < 16 && r < rows) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = lse;
 }
 
 template <int D, bool PAGED>
@@ -280,6 +290,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     constexpr int NQI = kAccountStep * KP / kThreads; // Q pieces per thread
     constexpr int NRG = kAccountStep / 16;
     __shared__ __align__(16) uint16_t qs0[kAccountStep * D], qs1[kAccountStep * D];
+    __shared__ float s_lse[kAccountFold];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int item = blockIdx.x / a.Hkv, g = blockIdx.x - item * a.Hkv;
@@ -320,7 +331,13 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
             }
         }
     };
+    const bool merges = a.fold && a.e[ei].nch > 1; // (the chunk has kAccountFold rows at most)
     auto load_lse = [&](int r0, float(&x)[NRG]) __attribute__((always_inline)) {
+        if (merges) {
+#pragma unroll
+            for (int rg = 0; rg < NRG; ++rg) x[rg] = r0 + 16 * rg + c < r_hi ? s_lse[min(r0 + 16 * rg + c - r_lo, kAccountFold - 1)] : INFINITY;
+            return;
+        }
         const float *p = lse + r0;
         if (r0 + kAccountStep <= r_hi) {
 #pragma unroll
@@ -342,6 +359,14 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     f32x4 acc[4];
 #pragma unroll
     for (int tt = 0; tt < 4; ++tt) acc[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (merges) { // while the first rows and the keys are on their way
+        const float *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows);
+        for (int r0 = r_lo + 16 * wave; r0 < r_hi; r0 += kThreads / 4) {
+            const float v = merged_lse(st + 2 * (int64_t)min(r0 + c, r_hi - 1), 2 * (int64_t)a.Hkv * rows, a.e[ei].nch);
+            if (qg == 0 && r0 + c < r_hi) s_lse[r0 + c - r_lo] = v;
+        }
+        __syncthreads();
+    }
     float x[NRG];
     load_lse(r_lo, x);
     __builtin_amdgcn_s_waitcnt(kVmcnt0);
@@ -425,6 +450,7 @@ __global__ __launch_bounds__(kThreads) void account_join_kernel(AccountArgs a) {
     const int64_t base = ((int64_t)a.e[ei].row * a.Hkv + g) * a.room, len = (int64_t)account_blocks_dev(keys) * kAccountKeys;
     const float  *part = a.parts + (int64_t)a.e[ei].part0 * a.Hkv + (int64_t)g * len + t;
     float         sum = a.w_in && t < p0 ? a.w_in[base + t] : 0.0f;
+#pragma unroll 8
     for (int k = sees / rc; k < nrc; ++k) sum += part[(int64_t)k * a.Hkv * len];
     a.w_out[base + t] = sum;
 }
@@ -434,8 +460,8 @@ template <int D> void launch_d(const AccountArgs &a, const AccountLaunch &l, boo
     if (paged) hipLaunchKernelGGL((account_stats_kernel<D, true>), stats, block, 0, stream, a);
     else hipLaunchKernelGGL((account_stats_kernel<D, false>), stats, block, 0, stream, a);
     HIP_CHECK(hipGetLastError());
-    if (l.split_keys) {
-        const dim3 grid((unsigned)((l.most_rows + kThreads / 64 - 1) / (kThreads / 64)), (unsigned)a.Hkv, (unsigned)l.n);
+    if (l.split_keys && !l.fold) {
+        const dim3 grid((unsigned)((l.most_rows + kThreads / 4 - 1) / (kThreads / 4)), (unsigned)a.Hkv, (unsigned)l.n);
         hipLaunchKernelGGL(account_merge_kernel, grid, block, 0, stream, a);
         HIP_CHECK(hipGetLastError());
     }
@@ -474,6 +500,7 @@ void launch_account(const AccountCall &c, const KvView &kv, const AccountPlan &p
     for (const auto &l : plan.launches) {
         if (l.n == 0 || l.items == 0) continue;
         a.n = l.n;
+        a.fold = l.fold;
         a.parts = workspace; // (multiples of 256 first: their stores are of 16 bytes)
         a.stats = a.parts + l.parts * c.Hkv;
         a.lse = a.stats + 2 * l.stats * c.Hkv;

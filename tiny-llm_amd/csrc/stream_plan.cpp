@@ -79,9 +79,12 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
 
 bool plan_account(AccountPlan &plan, int G, int Hkv, int cus) {
     // Row tiles of all entries fill the chip (two workgroups a CU), or their keys are
-    // split, into chunks of at least four tiles; likewise key blocks, or their rows
-    // are, into chunks of at least two steps.  (Half of a whole prompt's blocks are
-    // above the diagonal and empty, hence more of them.)
+    // split, into chunks of at least two tiles (1 x 4096 tokens, the last one's
+    // account: 15.4 us, of at least four 17.4).  Likewise key blocks, or their rows are:
+    // eight workgroups a CU, as half of a whole prompt's blocks are above the diagonal
+    // and empty (1 x 8192: 661 us, four 748), in chunks of at least four steps (1 x
+    // 1000: 38.5, of two 41.5) while those are as many as CUs, else two (1 x 300: 21.9
+    // against 24.7).
     const int64_t n = std::max(1, cus);
     int64_t       tiles = 0, blocks = 0;
     for (const auto &e : plan.entries) {
@@ -94,15 +97,17 @@ bool plan_account(AccountPlan &plan, int G, int Hkv, int cus) {
     for (size_t i = 0; i < plan.entries.size();) {
         AccountLaunch l{};
         l.first = (int)i;
+        l.fold = true;
         int64_t items = 0, sums = 0;
         for (; i < plan.entries.size() && l.n < kAccountBatch; ++i, ++l.n) {
             AccountEntry &e = plan.entries[i];
             const int     keys = e.p0 + e.n, kb = account_blocks(keys);
             const int64_t rows = (int64_t)e.w * G, rt = (rows + kAccountRows - 1) / kAccountRows;
             if (rows > INT32_MAX / 2) return false;
-            e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(split, stream_tiles(keys) / 4));
+            e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(split, stream_tiles(keys) / 2));
             const int64_t steps = (rows + kAccountStep - 1) / kAccountStep;
-            const int64_t each = std::max<int64_t>(2, (steps + row_split - 1) / row_split);
+            const int64_t least = blocks * Hkv * steps >= 4 * n ? 4 : 2;
+            const int64_t each = std::max(least, (steps + row_split - 1) / row_split);
             e.rc = (int)std::min<int64_t>(each * kAccountStep, 1 << 30);
             e.nrc = (int)((rows + e.rc - 1) / e.rc);
             e.item0 = (int32_t)items;
@@ -117,6 +122,8 @@ bool plan_account(AccountPlan &plan, int G, int Hkv, int cus) {
             if (e.nrc > 1) l.parts += (int64_t)kb * kAccountKeys * e.nrc;
             if (std::max({items * Hkv, sums * Hkv, l.lse, l.stats, l.parts}) > INT32_MAX) return false;
             l.split_keys |= e.nch > 1;
+            const int64_t chunk_rows = std::min<int64_t>(rows, e.rc);
+            if (e.nch > 1 && (chunk_rows > kAccountFold || chunk_rows * e.nch > kAccountFoldParts)) l.fold = false;
             l.split_rows |= e.nrc > 1;
             if (e.nch > 1) l.most_rows = std::max(l.most_rows, (int)rows);
             if (e.nrc > 1) l.most_keys = std::max(l.most_keys, keys);
@@ -138,12 +145,19 @@ bool plan_cross(CrossPlan &plan, int D, int G, int Hkv, int cus) {
     const int tile = cross_rows(D, plan.waves);
     int64_t   tiles = 0;
     for (const auto &e : plan.entries) tiles += ((int64_t)e.nq * G + tile - 1) / tile;
-    // Row tiles that do not fill the chip (twice where a CU holds one workgroup) have
-    // their keys split, into chunks of at least four tiles.
-    const int64_t want = 2 * (int64_t)std::max(1, cus);
-    const int64_t split = std::max<int64_t>(1, want / std::max<int64_t>(1, tiles * Hkv));
-    for (auto &e : plan.entries)
-        e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(split, stream_tiles(e.S) / 4));
+    // Row tiles that do not fill the chip have their keys split, into chunks of at least
+    // three tiles, once per CU (4 x 32 queries over 8192, 8 heads of 128, groups of 4:
+    // 44.6 us, twice per CU 47.9; 500 over 4096: 57 against 79): a chunk's partial outputs
+    // are written and read again.  Twice pays where half of a tile's rows are empty
+    // (16 x 32 over 1500, 8 heads of 64: 18.5 against 20.3) or chunks stay long (64 over
+    // 32768: 65.7 against 68.5).
+    const int64_t work = std::max<int64_t>(1, tiles * Hkv), n = std::max(1, cus);
+    const int64_t once = std::max<int64_t>(1, n / work), twice = std::max<int64_t>(1, 2 * n / work);
+    const bool    sparse = 2 * rows <= tiles * tile;
+    for (auto &e : plan.entries) {
+        const int64_t t = stream_tiles(e.S);
+        e.nch = (int)std::max<int64_t>({1, std::min<int64_t>(once, t / 3), sparse ? std::min<int64_t>(twice, t / 4) : t >= 16 * twice ? twice : 1});
+    }
     std::stable_sort(plan.entries.begin(), plan.entries.end(), [](const CrossEntry &x, const CrossEntry &y) {
         return (int64_t)x.S * y.nch > (int64_t)y.S * x.nch;
     });

@@ -59,6 +59,8 @@ constexpr int kAccountRows = 128;  // query rows of a workgroup of account_stats
 constexpr int kAccountKeys = 256;  // keys of a workgroup of account_sum_kernel
 constexpr int kAccountStep = 64;   // rows that it stages at a time
 constexpr int kAccountBatch = 72;  // entries per launch
+constexpr int kAccountFold = 256;  // rows of a chunk whose statistics account_sum_kernel merges,
+constexpr int kAccountFoldParts = 8192; // and their partial results at most
 
 // The last w of the n new tokens of cache row `row` (positions p0 .. p0 + n - 1; tok0:
 // the first one's index in the call's tokens) attend causally: w * G query rows per
@@ -73,6 +75,7 @@ struct AccountEntry {
 struct AccountLaunch {
     int     first, n, items, sums;
     bool    split_keys, split_rows;   // some nch, nrc is above 1
+    bool    fold;                     // account_sum_kernel merges the key chunks' statistics itself
     int     most_rows, most_keys;     // of an entry
     int64_t lse, stats, parts;        // per kv head
 };
