@@ -343,7 +343,9 @@ int  tl_kv_prefill_weights(tl_kv_prefill *p, int layer, const void *q, float sca
  *            them otherwise.  positions_in is read only below the length that
  *            the sequence's last eviction left (the tokens after that came in
  *            order), so it needs no initial value.  A layer that ran in place is
- *            not run again before commit;
+ *            not run again before commit.  A run moves rows of the cache (a captured
+ *            one counts as run): until its commit the layer is not to be read, no
+ *            prepare takes its sequences and no other batch runs over them;
  *   commit:  when every layer has run: the sequences are as long as what they
  *            kept, and a block pool gets the blocks behind it back.  Other
  *            batches must be prepared again.  Nothing changes when it fails.

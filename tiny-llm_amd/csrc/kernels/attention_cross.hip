@@ -17,6 +17,11 @@
 // (m, l, o) go through a workspace in fp32 to cross_merge_kernel.  Grid: kv head
 // fastest, so that with 8 kv heads an XCD's workgroups share one head's keys in
 // its L2.
+//
+// Measured: 2 x 2048 queries over 8192 states, 8 heads of 128, group 4: 492 us = 1.12
+// PFLOP/s (an 8192^3 fp16 matrix product 1.2-1.34), matrix unit busy 47% of the
+// cycles, VALU 21%; 16 x 64..448 over 300..1500, 16 heads of 64: 28 us; 8 over 32768, a
+// quarter of a tile's rows in use: 29 us for the 134 MB of states, + 7 for the merge.
 #include "cross.h"
 
 #include "tiny_llm/hip_utils.h"

@@ -8,25 +8,31 @@
 //   account_out[t] = account_in[t] + sum_r P_rt
 // Bound by HBM: K and V once, 4 D bytes a token and kv head.  The account needs the
 // rows' maxima and sums over all tokens before its first weight, but reading K a
-// second time for it would cost half of the whole; the scores cost 4 bytes a row and token
-// written and read (group 4, D 128: 32 against 512 bytes), so they go through the
-// workspace.  They and the sums are fp32: an account is compared with others of
-// like size.
+// second time for it would cost half of the whole, so the scores (fp32, as the sums: an
+// account is compared with others of like size) wait in LDS, 4 bytes a row and token.
 //
 // attn_stream_kernel: a workgroup of 4 or 8 waves per (entry, chunk of tiles, kv
 // head); wave w takes every 4th (8th) tile of 64 tokens (32 at head_dim 256) and keeps
 // its own running maximum, sum and output; the next tile's rows are on their way
-// while one is computed.  A workgroup that has a whole entry finishes it.
+// while one is computed.  A workgroup that has a whole entry finishes it; the others
+// write their chunk's scores at the end, in one go (a write among the reads costs far
+// more than its bytes: scores stored tile by tile took 77-95 of 474 us).
 //   S^T = K Q^T      v_mfma_f32_16x16x32_f16: A = K rows (token l%16, dims
 //                    8(l/16)..+7) straight from memory, B = Q (row l%16),
 //                    D = S^T (tokens 4(l/16)+i, row l%16)
 //   softmax          per row column in the log2 domain, over a reference point near
 //                    the maximum (kBelow); p is fp16 for the product, a relative
 //                    rounding of 2^-11 per weight, its sum stays fp32
-//   O^T += V^T P^T   over 32 tokens; V^T from the wave's row-major LDS stage by
+//   O^T += V^T P^T   over 16 tokens; V^T from the wave's row-major LDS stage by
 //                    the transposing ds_read_b64_tr_b16
 // stream_finish_kernel: merges the outputs of entries with several chunks and turns
 // their scores into the account.
+//
+// Measured, with accounts, 8 kv heads of 128: 64 x 8192 tokens, group 4, whole
+// entries: 360 us, 6.0 TB/s of K and V (without accounts the decode kernel takes 309 on
+// the same cache); 96 lognormal lengths to 16384 on blocks, group 8: 264 + 27 us for
+// the finish; 4 x 128..512 tokens, 8 heads of 64: 7.4 us, one launch's latency.  Two or
+// three steps of rows on their way in registers were level or slower (occupancy).
 #include "stream.h"
 
 #include "tiny_llm/hip_utils.h"

@@ -177,9 +177,10 @@ template <int NT> __device__ __forceinline__ void pick_bin(const uint32_t *hist,
 // * 4 .. + 3.  Where the first digit leaves up to kList candidates, the next ones are
 // found among a list of them.  Bound by the instructions of the one workgroup that
 // a (sequence, kv head) has, not by memory.  Four tokens a step, with one scan per
-// step, instead of one with its ballots, and no token looked at again after the
-// first digit: 8192 tokens 14.4 -> 11.1 us, 32768 39.8 -> 24.9.  Accounts in registers
-// beside or instead of the keys cost more instructions than they saved (34 us).
+// step, instead of one with its ballots, no token looked at again after the first
+// digit, and movers from an ordered list instead of from their steps: 8192 tokens
+// 14.4 -> 10.1 us, 32768 39.8 -> 20.8.  Accounts in registers beside or instead of the
+// keys cost more instructions than they saved (34 us).
 template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_kernel(EvictArgs a) {
     constexpr int NW = NT / 64;
     static_assert(IT <= 8, "a bit per token");

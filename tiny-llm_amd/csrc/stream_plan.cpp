@@ -136,11 +136,19 @@ bool plan_account(AccountPlan &plan, int G, int Hkv, int cus) {
 }
 
 bool plan_cross(CrossPlan &plan, int D, int G, int Hkv, int cus) {
-    // 8 waves share a key tile among 256 rows and have a CU to themselves; 4 waves waste
-    // fewer rows of a short entry, two workgroups to a CU.
-    int64_t rows = 0;
-    for (const auto &e : plan.entries) rows += (int64_t)e.nq * G;
-    const bool wide = D <= 128 && D != 64 && !plan.entries.empty() && rows >= 512 * (int64_t)plan.entries.size();
+    // 8 waves share a key tile among 256 rows and have a CU to themselves, 4 waves waste
+    // fewer rows of a short entry, two workgroups to a CU.  Measured, 8 heads of 128, groups of 4,
+    // 8 against 4 waves: 2 x 2048 queries over 8192 544 us, 584; 1 x 500 over 4096 55.6, 60.3;
+    // 16 x 64 over 2048 61, 67.  One full round of large workgroups and a part of
+    // another is worse: 4 x 512 over 2048 105, 77; 3 x 1024 over 4096 245, 229.  Level at 64.
+    const int64_t n = std::max(1, cus);
+    int64_t       rows = 0, large = 0;
+    for (const auto &e : plan.entries) {
+        rows += (int64_t)e.nq * G;
+        large += ((int64_t)e.nq * G + cross_rows(D, 8) - 1) / cross_rows(D, 8);
+    }
+    const bool wide = D <= 128 && D != 64 && !plan.entries.empty() && rows >= 256 * (int64_t)plan.entries.size() &&
+                      (large * Hkv < n || large * Hkv >= 2 * n);
     plan.waves = wide ? 8 : 4;
     const int tile = cross_rows(D, plan.waves);
     int64_t   tiles = 0;
@@ -151,7 +159,7 @@ bool plan_cross(CrossPlan &plan, int D, int G, int Hkv, int cus) {
     // are written and read again.  Twice pays where half of a tile's rows are empty
     // (16 x 32 over 1500, 8 heads of 64: 18.5 against 20.3) or chunks stay long (64 over
     // 32768: 65.7 against 68.5).
-    const int64_t work = std::max<int64_t>(1, tiles * Hkv), n = std::max(1, cus);
+    const int64_t work = std::max<int64_t>(1, tiles * Hkv);
     const int64_t once = std::max<int64_t>(1, n / work), twice = std::max<int64_t>(1, 2 * n / work);
     const bool    sparse = 2 * rows <= tiles * tile;
     for (auto &e : plan.entries) {
