@@ -10,9 +10,10 @@ from retention_ref import Cache, attend, check_account, check_out, dev, even_tai
 pytestmark = pytest.mark.gpu
 
 
-def decode_step(tl, c, lens, G, append=True, given=True, in_place=False, layer=0, stream=None, attended=None):
+def decode_step(tl, c, lens, G, append=True, given=True, in_place=False, layer=0, attended=None, scale=None):
     """One decode_weights call on the cache, checked."""
     n, hq, d = len(lens), c.hkv * G, c.d
+    scale = d ** -0.5 if scale is None else scale
     q = c.rng.standard_normal((n, hq, d)).astype(np.float16)
     nk, nv = c.rows(n), c.rows(n)
     b = tl.DecodeBatch(c.mgr, n, hq)
@@ -31,7 +32,7 @@ def decode_step(tl, c, lens, G, append=True, given=True, in_place=False, layer=0
     if attended is None and not append:
         b.append(0, 1, dk.data_ptr(), dv.data_ptr(), s)
     b.decode_weights(layer, dq.data_ptr(), dk.data_ptr() if append else None, dv.data_ptr() if append else None,
-                     out.data_ptr(), d ** -0.5, w_in.data_ptr() if given else None, w_out.data_ptr(), s)
+                     out.data_ptr(), scale, w_in.data_ptr() if given else None, w_out.data_ptr(), s)
     torch.cuda.synchronize()
     got, acc = out.cpu().numpy(), w_out.cpu().numpy()
     for i in range(n):
@@ -42,7 +43,7 @@ def decode_step(tl, c, lens, G, append=True, given=True, in_place=False, layer=0
         else:
             k, v, old = c.k[layer][i][:attended[i]], c.v[layer][i][:attended[i]], attended[i]
         S = len(k)
-        o, mass, w, err = attend(q[i:i + 1], k, v, d ** -0.5)
+        o, mass, w, err = attend(q[i:i + 1], k, v, scale)
         check_out(got[i:i + 1], o, mass, err, S)
         want = w.reshape(c.hkv, G, S).sum(axis=1)
         base = start[c.slot[i], :, :S].astype(np.float64) * (np.arange(S) < old) if given else np.zeros((c.hkv, S))
@@ -66,6 +67,30 @@ def decode_step(tl, c, lens, G, append=True, given=True, in_place=False, layer=0
 def test_decode_weights(tl, d, hkv, G, block, lens):
     c = Cache(tl, lens, hkv, d, block=block, seed=d + G, spare=1, hq=hkv * G)
     decode_step(tl, c, lens, G)
+
+
+@pytest.mark.parametrize("d,hkv,G,block,lens", [
+    (32, 8, 1, 0, [3000]),         # little work: pieces of four tiles
+    (64, 8, 4, 16, [2500, 40]),
+    (128, 8, 8, 16, [1500]),
+    (256, 4, 4, 0, [900, 300]),
+    (256, 2, 2, 16, [2600]),
+    (128, 8, 4, 0, [8300]),        # more: eight waves
+    (64, 8, 1, 0, [1024] * 8),     # whole entries on eight waves
+    (64, 2, 2, 0, [300, 767]),
+    (32, 8, 1, 16, [(i * 97) % 700 for i in range(40)]),   # many entries
+    (64, 8, 2, 0, [50] * 33 + [4000]),                     # ... and a long one among them
+])
+def test_decode_weights_in_pieces(tl, d, hkv, G, block, lens):
+    c = Cache(tl, lens, hkv, d, block=block, seed=d + G + 1, hq=hkv * G)
+    decode_step(tl, c, lens, G)
+
+
+@pytest.mark.parametrize("scale", [-0.3, 0.0, 1.5])
+def test_decode_weights_scales_of_either_sign(tl, scale):
+    lens = [70, 900]
+    c = Cache(tl, lens, 2, 64, seed=16, hq=4)
+    decode_step(tl, c, lens, 2, scale=scale)
 
 
 @pytest.mark.parametrize("block", [0, 16])
@@ -191,6 +216,50 @@ def test_decode_weights_captured(tl):
         assert torch.equal(out, want[0]) and torch.equal(w_out, want[1]), i
 
 
+def test_graphs_of_one_batch_share_its_workspace(tl):
+    """Decode and prompt accounts of two layers and windows, each captured into a graph
+    of its own, replayed in turn with eager calls between."""
+    lens, new = [3000, 40], [33, 150]
+    c = Cache(tl, lens, 2, 64, room=3300, layers=2, seed=17, hq=8)
+    d, p = tl.DecodeBatch(c.mgr, 2, 8), tl.PrefillBatch(c.mgr, 2, 8)
+    d.prepare(c.ids)
+    p.prepare(c.ids, new)
+    q = dev(c.rng.standard_normal((sum(new), 8, 64)).astype(np.float16))
+    k, v = dev(c.rows(sum(new))), dev(c.rows(sum(new)))
+    outs = [torch.zeros((2, 8, 64), dtype=torch.float16, device="cuda") for _ in range(2)]
+    accs = [c.account() for _ in range(4)]
+    for layer in range(2):
+        p.append(layer, k.data_ptr(), v.data_ptr())
+
+    def decode(layer):
+        d.decode_weights(layer, q.data_ptr(), k.data_ptr(), v.data_ptr(), outs[layer].data_ptr(), 0.125, None,
+                         accs[layer].data_ptr(), torch.cuda.current_stream().cuda_stream)
+
+    def prompt(i):  # (decode appends the rows that the prompt begins with)
+        p.weights(i, q.data_ptr(), 0.125, [0, 20][i], None, accs[2 + i].data_ptr(), torch.cuda.current_stream().cuda_stream)
+
+    calls = [lambda: decode(0), lambda: decode(1), lambda: prompt(0), lambda: prompt(1)]
+    # (the plan of a window is made anew after another one: its launches do not depend on that)
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
+    want = [x.clone() for x in outs + accs]
+    graphs = []
+    for call in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            call()
+    for order in ([0, 1, 2, 3], [3, 1, 0, 2], [2, 0, 3, 1]):
+        for x in outs + accs:
+            x.zero_()
+        for i in order:
+            graphs[i].replay()
+            calls[order[0]]()
+        torch.cuda.synchronize()
+        for x, y in zip(outs + accs, want):
+            assert torch.equal(x, y), order
+
+
 def test_a_capture_does_not_grow_the_workspace(tl):
     c = Cache(tl, [300], 1, 64, seed=12)
     b = tl.DecodeBatch(c.mgr, 1, 1)
@@ -296,6 +365,8 @@ def test_prompt_weights_scales_of_either_sign(tl, scale):
     (128, 8, 4, [0, 900], [1100, 700], 0),   # rows and keys over several workgroups, the diagonal between them
     (64, 1, 1, [0], [2500], 0),
     (128, 1, 8, [3000], [1500], 1000),
+    (128, 1, 8, [8968], [32], 0),            # few rows, many chunks of keys
+    (256, 2, 4, [4000], [40], 20),
 ])
 def test_prompt_weights_long(tl, d, hkv, G, pre, new, window):
     c = Cache(tl, pre, hkv, d, room=max(a + b for a, b in zip(pre, new)), seed=14, hq=hkv * G)

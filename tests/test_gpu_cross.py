@@ -49,6 +49,25 @@ def test_cross(tl, d, hkv, G, block, states, src, nq):
     cross(tl, c, G, src, nq)
 
 
+@pytest.mark.parametrize("d,hkv,G,block,states,nq", [
+    (64, 8, 1, 0, [1500, 900], [1, 3]),      # few rows, little work: pieces of four tiles
+    (32, 4, 2, 16, [3000], [2]),
+    (256, 4, 4, 0, [3000], [2]),
+    (128, 8, 4, 0, [16500], [1]),            # more: eight waves
+    (128, 1, 1, 0, [40, 700], [16, 1]),      # whole entries
+    (128, 8, 4, 16, [3000], [8]),            # tiles half empty
+    (64, 2, 4, 0, [3000], [30]),
+    (256, 2, 4, 16, [2500], [20]),
+    (32, 2, 8, 16, [3000], [40]),
+    (128, 2, 4, 0, [2000], [100]),           # large workgroups, keys split
+    (32, 8, 4, 0, [700, 300], [130, 257]),
+    (128, 8, 1, 0, [200] * 32, [300] * 32),  # ... one round and a part of another
+])
+def test_cross_in_pieces(tl, d, hkv, G, block, states, nq):
+    c = Cache(tl, states, hkv, d, block=block, seed=d + G + 1, hq=hkv * G)
+    cross(tl, c, G, list(range(len(states))), nq)
+
+
 @pytest.mark.parametrize("block", [0, 16])
 @pytest.mark.parametrize("nq", [[1, 2, 1, 3], [40, 150, 64, 1]])
 def test_cross_over_padded_states(tl, block, nq):
