@@ -104,18 +104,35 @@ static void account_random() {
         size_t next = 0;
         for (const auto &l : p.launches) {
             CHECK((size_t)l.first == next && l.n > 0 && l.n <= kAccountBatch);
+            CHECK((int)l.tile_pieces.size() <= kAccountPieces && (int)l.block_pieces.size() <= kAccountPieces);
             int64_t items = 0, sums = 0, stats = 0, lse = 0, parts = 0;
             bool    keys_split = false, rows_split = false;
-            for (int i = l.first; i < l.first + l.n; ++i) {
-                const AccountEntry &e = p.entries[(size_t)i];
+            for (int i = 0; i < l.n; ++i) {
+                const AccountEntry &e = p.entries[next + (size_t)i];
                 const int           keys = e.p0 + e.n, rows = e.w * G;
-                CHECK(e.item0 == items && e.sum0 == sums && e.stat0 == stats && e.lse0 == lse && e.part0 == parts);
-                CHECK(e.nch >= 1 && e.nch <= std::max(1, stream_tiles(keys)));
-                // row chunks of whole steps, none empty, all rows
-                CHECK(e.rc > 0 && e.rc % kAccountStep == 0 && e.nrc >= 1);
-                CHECK((int64_t)e.rc * e.nrc >= rows && (int64_t)e.rc * (e.nrc - 1) < rows);
-                items += ((int64_t)rows + kAccountRows - 1) / kAccountRows * e.nch;
-                sums += (int64_t)account_blocks(keys) * e.nrc;
+                CHECK(e.stat0 == stats && e.lse0 == lse && e.part0 == parts);
+                // every row tile and every key block in one piece
+                std::vector<int> tile(((size_t)rows + kAccountRows - 1) / kAccountRows), block((size_t)account_blocks(keys));
+                int              nch = 1, nrc = 1;
+                for (const auto &c : l.tile_pieces) {
+                    if (c.entry() != i) continue;
+                    CHECK(c.first >= 0 && c.first < c.last && c.last <= (int)tile.size());
+                    CHECK(c.chunks() >= 1 && c.chunks() <= account_seen(e, G, c.last - 1));
+                    for (int x = c.first; x < c.last; ++x) ++tile[(size_t)x];
+                    nch = std::max(nch, c.chunks());
+                }
+                for (const auto &c : l.block_pieces) {
+                    if (c.entry() != i) continue;
+                    CHECK(c.first >= 0 && c.first < c.last && c.last <= (int)block.size());
+                    const int steps = (rows + kAccountStep - 1) / kAccountStep - account_sees(e, G, c.first);
+                    CHECK(c.chunks() >= 1 && c.chunks() <= steps);
+                    CHECK(!l.fold || e.nch == 1 || (steps + c.chunks() - 1) / c.chunks() * kAccountStep <= kAccountFold);
+                    for (int x = c.first; x < c.last; ++x) ++block[(size_t)x];
+                    nrc = std::max(nrc, c.chunks());
+                }
+                for (int x : tile) CHECK(x == 1);
+                for (int x : block) CHECK(x == 1);
+                CHECK(e.nch == nch && e.nrc == nrc);
                 lse += rows;
                 if (e.nch > 1) stats += (int64_t)rows * e.nch;
                 CHECK(e.nch == 1 || rows <= l.most_rows);
@@ -123,6 +140,14 @@ static void account_random() {
                 CHECK(e.nrc == 1 || keys <= l.most_keys);
                 keys_split |= e.nch > 1;
                 rows_split |= e.nrc > 1;
+            }
+            for (const auto &c : l.tile_pieces) {
+                CHECK(c.item0 == items);
+                items += (int64_t)(c.last - c.first) * c.chunks();
+            }
+            for (const auto &c : l.block_pieces) {
+                CHECK(c.item0 == sums);
+                sums += (int64_t)(c.last - c.first) * c.chunks();
             }
             CHECK(l.items == items && l.sums == sums && l.stats == stats && l.lse == lse && l.parts == parts);
             CHECK(l.split_keys == keys_split && l.split_rows == rows_split);

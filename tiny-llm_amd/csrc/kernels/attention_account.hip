@@ -25,10 +25,10 @@
 // order.
 //
 // Measured, 8 kv heads of 128, group 4: 4 x 1700..2048 new tokens on prefixes to 600,
-// 139 us for the statistics (matrix unit busy 25% of the cycles, VALU 40%) and 134 for
-// the sums (26%, 24%), no bank conflicts: the phases of a step follow each other, and
-// the registers leave room for two or three waves a SIMD to fill the gaps.  The last 32
-// tokens of 8192: 9 + 13 us, two launches' latency and K's 17 MB each.
+// 124 us for the statistics (matrix unit busy 28% of the cycles, VALU 46%) and 114 for
+// the sums (31%, 28%), no bank conflicts: the phases of a step follow each other, and
+// the registers leave room for two to four waves a SIMD to fill the gaps.  The last 32
+// tokens of 8192: 9 + 14 us, two launches' latency and K's 17 MB each.
 #include "account.h"
 
 #include "tiny_llm/hip_utils.h"
@@ -65,20 +65,40 @@ struct AccountArgs {
     float         scale_log2;
     int           Hq, Hkv, lg, n; // lg: log2 of the query heads per kv head
     int           fold;           // no account_merge_kernel ran
+    int           nt, nb;         // pieces of row tiles, of key blocks
+    AccountPiece  tiles[kAccountPieces], blocks[kAccountPieces];
     AccountEntry  e[kAccountBatch];
 };
 static_assert(sizeof(AccountArgs) <= 4096, "kernel arguments");
 
-// The last entry whose first item is at most `item`.
-#define ACCOUNT_ENTRY_OF(a, field, item, out)                                                                          \
-    do {                                                                                                               \
-        int seen_ = 0;                                                                                                 \
-        for (int k_ = 0; k_ < (a).n; k_ += 64) {                                                                       \
-            const int i_ = k_ + (int)(threadIdx.x & 63);                                                               \
-            seen_ += __popcll(__ballot(i_ < (a).n && (a).e[min(i_, (a).n - 1)].field <= (item)));                      \
-        }                                                                                                              \
-        out = __builtin_amdgcn_readfirstlane(seen_ - 1);                                                               \
-    } while (0)
+// A launch's pieces, one per lane, so that a look-up is a ballot and lane reads
+// instead of a chain of loads (2 to 7 us a call of few rows).
+struct Pieces {
+    AccountPiece p;
+    int          n;
+    __device__ __forceinline__ Pieces(const AccountPiece *all, int count) : n(count) {
+        static_assert(kAccountPieces <= 64, "a lane per piece");
+        p = all[min((int)(threadIdx.x & 63), count - 1)];
+    }
+    // The piece of work item `item`: the last whose first item is at most that.
+    __device__ __forceinline__ AccountPiece of_item(int item) const {
+        return at(__popcll(__ballot((int)(threadIdx.x & 63) < n && p.item0 <= item)) - 1);
+    }
+    // Chunks of tile (block) x, the same for the whole wave, of entry ei.
+    __device__ __forceinline__ int chunks(int ei, int x) const {
+        const uint64_t hit = __ballot((int)(p.what & 255u) == ei && p.first <= x && x < p.last);
+        return (int)((uint32_t)__builtin_amdgcn_readlane((int)p.what, __ffsll((unsigned long long)hit) - 1) >> 8);
+    }
+    __device__ __forceinline__ AccountPiece at(int i) const {
+        i = __builtin_amdgcn_readfirstlane(i);
+        AccountPiece c;
+        c.item0 = __builtin_amdgcn_readlane(p.item0, i);
+        c.first = __builtin_amdgcn_readlane(p.first, i);
+        c.last = __builtin_amdgcn_readlane(p.last, i);
+        c.what = (uint32_t)__builtin_amdgcn_readlane((int)p.what, i);
+        return c;
+    }
+};
 
 // Byte offset of token t's row in a kv head's K.
 template <bool PAGED> __device__ __forceinline__ int64_t key_off(const KvView &v, int row, int t) {
@@ -112,18 +132,16 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int item = blockIdx.x / a.Hkv, g = blockIdx.x - item * a.Hkv;
-    int       ei;
-    ACCOUNT_ENTRY_OF(a, item0, item, ei);
-    const int row = a.e[ei].row, p0 = a.e[ei].p0, n = a.e[ei].n, w = a.e[ei].w, nch = a.e[ei].nch;
-    const int rel = item - a.e[ei].item0, ch = rel % nch;
+    const AccountPiece piece = Pieces(a.tiles, a.nt).of_item(item);
+    const int          ei = (int)(piece.what & 255u), nch = (int)(piece.what >> 8);
+    const int row = a.e[ei].row, p0 = a.e[ei].p0, n = a.e[ei].n, w = a.e[ei].w;
+    const int rel = item - piece.item0, ch = rel % nch, rt = piece.first + rel / nch;
     const int rows = w << a.lg;
-    const int rt = (rows - 1) / kAccountRows - rel / nch; // the tiles with the most keys first
     const int r_lo = rt * kAccountRows, r_hi = min(rows, r_lo + kAccountRows);
     const int first = p0 + n - w;                          // position of query row 0's token
-    const int kend = first + ((r_hi - 1) >> a.lg) + 1;         // keys that some row of the tile sees
-    const int tiles = (p0 + n + kTile - 1) / kTile;        // of the whole, so that chunks agree
-    const int t_lo = (int)((int64_t)ch * tiles / nch);
-    const int t_hi = min((int)((int64_t)(ch + 1) * tiles / nch), (kend + kTile - 1) / kTile);
+    const int kend = first + ((r_hi - 1) >> a.lg) + 1;     // keys that some row of the tile sees
+    const int tiles = (kend + kTile - 1) / kTile;
+    const int t_lo = (int)((int64_t)ch * tiles / nch), t_hi = (int)((int64_t)(ch + 1) * tiles / nch);
     const int c = lane & 15, qg = lane >> 4;
 
     f16x8 qb[2][KS];
@@ -249,7 +267,7 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
         lr += __shfl_xor(lr, 32);
         const int r = r_lo + wave * 32 + j * 16 + c;
         if (qg > 0 || r >= r_hi) continue;
-        if (nch == 1) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = mr + __builtin_amdgcn_logf(lr);
+        if (a.e[ei].nch == 1) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = mr + __builtin_amdgcn_logf(lr);
         else {
             const int64_t at = (int64_t)a.e[ei].stat0 * a.Hkv + ((int64_t)ch * a.Hkv + g) * rows + r;
             *reinterpret_cast<float2 *>(a.stats + 2 * at) = make_float2(mr, lr);
@@ -283,9 +301,10 @@ __global__ __launch_bounds__(kThreads) void account_merge_kernel(AccountArgs a) 
     const int ei = blockIdx.z, g = blockIdx.y;
     const int nch = a.e[ei].nch, rows = a.e[ei].w << a.lg;
     const int r = blockIdx.x * (kThreads / 4) + (threadIdx.x >> 6) * 16 + (threadIdx.x & 15);
-    if (nch == 1) return;
+    const int r0 = blockIdx.x * (kThreads / 4) + (threadIdx.x >> 6) * 16; // the wave's first row
+    if (nch == 1 || r0 >= rows) return;
     const float *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows + min(r, rows - 1));
-    const float  lse = merged_lse(st, 2 * (int64_t)a.Hkv * rows, nch);
+    const float  lse = merged_lse(st, 2 * (int64_t)a.Hkv * rows, Pieces(a.tiles, a.nt).chunks(ei, r0 / kAccountRows));
     if ((threadIdx.x & 63) < 16 && r < rows) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = lse;
 }
 
@@ -299,16 +318,18 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int item = blockIdx.x / a.Hkv, g = blockIdx.x - item * a.Hkv;
-    int       ei;
-    ACCOUNT_ENTRY_OF(a, sum0, item, ei);
-    const int row = a.e[ei].row, p0 = a.e[ei].p0, n = a.e[ei].n, w = a.e[ei].w, nrc = a.e[ei].nrc;
-    const int rel = item - a.e[ei].sum0, kblk = rel / nrc, rchunk = rel - kblk * nrc;
+    const Pieces       tile_pieces(a.tiles, a.nt);
+    const AccountPiece piece = Pieces(a.blocks, a.nb).of_item(item);
+    const int          ei = (int)(piece.what & 255u), nrc = (int)(piece.what >> 8);
+    const int row = a.e[ei].row, p0 = a.e[ei].p0, n = a.e[ei].n, w = a.e[ei].w;
+    const int rel = item - piece.item0, rchunk = rel % nrc, kblk = piece.first + rel / nrc;
     const int k_lo = kblk * kAccountKeys, keys = p0 + n;
     const int rows = w << a.lg, first = keys - w;
-    // The chunk's rows, from the first step whose tokens see the block's first key.
-    const int sees = (max(0, k_lo - first) << a.lg) / kAccountStep * kAccountStep;
-    const int r_lo = max(rchunk * a.e[ei].rc, sees), r_hi = (int)min((int64_t)rows, (int64_t)(rchunk + 1) * a.e[ei].rc);
-    if (r_lo >= r_hi && nrc > 1) return; // (account_join_kernel does not read it)
+    // The chunk's rows, of the steps from the first one whose tokens see the block's first key.
+    const int sees = (max(0, k_lo - first) << a.lg) / kAccountStep;
+    const int steps = (rows + kAccountStep - 1) / kAccountStep - sees;
+    const int r_lo = (sees + (int)((int64_t)rchunk * steps / nrc)) * kAccountStep;
+    const int r_hi = min(rows, (sees + (int)((int64_t)(rchunk + 1) * steps / nrc)) * kAccountStep);
     const int c = lane & 15, qg = lane >> 4;
     const int wk = k_lo + wave * 64; // the wave's first key
 
@@ -367,7 +388,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     if (merges) { // while the first rows and the keys are on their way
         const float *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows);
         for (int r0 = r_lo + 16 * wave; r0 < r_hi; r0 += kThreads / 4) {
-            const float v = merged_lse(st + 2 * (int64_t)min(r0 + c, r_hi - 1), 2 * (int64_t)a.Hkv * rows, a.e[ei].nch);
+            const int   nch = tile_pieces.chunks(ei, r0 / kAccountRows);
+            const float v = merged_lse(st + 2 * (int64_t)min(r0 + c, r_hi - 1), 2 * (int64_t)a.Hkv * rows, nch);
             if (qg == 0 && r0 + c < r_hi) s_lse[r0 + c - r_lo] = v;
         }
         __syncthreads();
@@ -434,7 +456,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
             for (int o = 1; o < 16; o <<= 1) v[i] += __shfl_xor(v[i], o);
         const int t = wk + 16 * tt + 4 * qg;
         if (c > 0) continue;
-        if (nrc > 1) {
+        if (a.e[ei].nrc > 1) {
             *reinterpret_cast<f32x4 *>(part + t) = v;
         } else {
 #pragma unroll
@@ -444,20 +466,19 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     }
 }
 
-// The accounts of entries with several chunks of rows, from the chunks that see the
-// token's block.
+// The accounts of entries with several chunks of rows.
 __global__ __launch_bounds__(kThreads) void account_join_kernel(AccountArgs a) {
+    static_assert(kThreads == kAccountKeys, "a workgroup per block");
     const int ei = blockIdx.z, g = blockIdx.y, t = blockIdx.x * kThreads + threadIdx.x;
-    const int p0 = a.e[ei].p0, keys = p0 + a.e[ei].n, nrc = a.e[ei].nrc, rc = a.e[ei].rc;
-    if (nrc == 1 || t >= keys) return;
-    const int     first = keys - a.e[ei].w, k_lo = t / kAccountKeys * kAccountKeys;
-    const int     sees = (max(0, k_lo - first) << a.lg) / kAccountStep * kAccountStep;
+    const int p0 = a.e[ei].p0, keys = p0 + a.e[ei].n;
+    if (a.e[ei].nrc == 1 || (int)blockIdx.x * kThreads >= keys) return;
+    const int     nrc = Pieces(a.blocks, a.nb).chunks(ei, blockIdx.x);
     const int64_t base = ((int64_t)a.e[ei].row * a.Hkv + g) * a.room, len = (int64_t)account_blocks_dev(keys) * kAccountKeys;
     const float  *part = a.parts + (int64_t)a.e[ei].part0 * a.Hkv + (int64_t)g * len + t;
     float         sum = a.w_in && t < p0 ? a.w_in[base + t] : 0.0f;
 #pragma unroll 8
-    for (int k = sees / rc; k < nrc; ++k) sum += part[(int64_t)k * a.Hkv * len];
-    a.w_out[base + t] = sum;
+    for (int k = 0; k < nrc; ++k) sum += part[(int64_t)k * a.Hkv * len];
+    if (t < keys) a.w_out[base + t] = sum;
 }
 
 template <int D> void launch_d(const AccountArgs &a, const AccountLaunch &l, bool paged, hipStream_t stream) {
@@ -510,6 +531,10 @@ void launch_account(const AccountCall &c, const KvView &kv, const AccountPlan &p
         a.stats = a.parts + l.parts * c.Hkv;
         a.lse = a.stats + 2 * l.stats * c.Hkv;
         std::memcpy(a.e, plan.entries.data() + l.first, sizeof(AccountEntry) * (size_t)l.n);
+        a.nt = (int)l.tile_pieces.size();
+        a.nb = (int)l.block_pieces.size();
+        std::memcpy(a.tiles, l.tile_pieces.data(), sizeof(AccountPiece) * l.tile_pieces.size());
+        std::memcpy(a.blocks, l.block_pieces.data(), sizeof(AccountPiece) * l.block_pieces.size());
         profile_begin(KernelId::AttnAccount, stream);
         switch (c.D) {
         case 32: launch_d<32>(a, l, paged, stream); break;

@@ -120,7 +120,7 @@ Result<void> PrefillBatch::weights(int layer_idx, const half *q, float scale, in
         for (int i = 0; i < n_; ++i) {
             const size_t k = static_cast<size_t>(i);
             const int    w = window ? std::min(window, counts_[k]) : counts_[k];
-            plan.entries.push_back({slots_[k], pos0_[k], counts_[k], w, tok, 0, 0, 0, 0, 0, 0, 0, 0});
+            plan.entries.push_back({slots_[k], pos0_[k], counts_[k], w, tok, 1, 0, 0, 1, 0});
             tok += counts_[k];
         }
         if (!detail::plan_account(plan, num_q_heads_ / cfg.num_heads, cfg.num_heads, detail::device_cus())) {

@@ -2,6 +2,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <utility>
 
 namespace tiny_llm {
 namespace detail {
@@ -78,59 +79,95 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
 }
 
 bool plan_account(AccountPlan &plan, int G, int Hkv, int cus) {
-    // Row tiles of all entries fill the chip (two workgroups a CU), or their keys are
-    // split, into chunks of at least two tiles (1 x 4096 tokens, the last one's
-    // account: 15.4 us, of at least four 17.4).  Likewise key blocks, or their rows are:
-    // eight workgroups a CU, as half of a whole prompt's blocks are above the diagonal
-    // and empty (1 x 8192: 661 us, four 748), in chunks of at least four steps (1 x
-    // 1000: 38.5, of two 41.5) while those are as many as CUs, else two (1 x 300: 21.9
-    // against 24.7).
+    // Work items take about a third of a CU's share of all key tiles (or row steps), in the
+    // order of their length: a whole prompt's row tiles see from one key tile to all of
+    // them, and its key blocks are seen by all rows to few (8 heads of 128, groups of 4: 4 x
+    // 1700..2048 on prefixes 214 us, whole tiles entry by entry 246; 1 x 2048 69 and 80).
+    // Row tiles that are fewer than CUs: half of a share (the last 32 of 4 x 8192: 46.9
+    // against 49.3).  Chunks have two key tiles at least (1 x 4096 tokens, the last
+    // one's account: 15.4 us, of four 17.4), and four row steps (1 x 1000: 38.5 us, of two
+    // 41.5) or, where those are fewer than CUs, two (1 x 300: 21.9 against 24.7).
     const int64_t n = std::max(1, cus);
-    int64_t       tiles = 0, blocks = 0;
+    int64_t       seen = 0, steps = 0, all = 0; // key tiles of all row tiles, row steps of all key blocks, row tiles
     for (const auto &e : plan.entries) {
-        tiles += ((int64_t)e.w * G + kAccountRows - 1) / kAccountRows;
-        blocks += account_blocks(e.p0 + e.n);
+        const int64_t rows = (int64_t)e.w * G;
+        if (rows > INT32_MAX / 2) return false;
+        const int64_t rt = (rows + kAccountRows - 1) / kAccountRows, kb = account_blocks(e.p0 + e.n);
+        const int64_t st = (rows + kAccountStep - 1) / kAccountStep;
+        all += rt;
+        seen += rt * (account_seen(e, G, 0) + account_seen(e, G, (int)rt - 1)) / 2;
+        steps += kb * st - std::min(kb, (e.w + kAccountKeys - 1) / (int64_t)kAccountKeys) * st / 2;
     }
-    const int64_t split = std::max<int64_t>(1, 2 * n / std::max<int64_t>(1, tiles * Hkv));
-    const int64_t row_split = std::max<int64_t>(1, 8 * n / std::max<int64_t>(1, blocks * Hkv));
+    auto          ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    const int64_t keys_each = std::max<int64_t>(2, ceil_div(seen * Hkv, (all * Hkv < n ? 2 : 3) * n));
+    const int64_t rows_each = std::max<int64_t>(steps * Hkv >= 4 * n ? 4 : 2, ceil_div(steps * Hkv, 3 * n));
+    // Pieces in the order of their items' lengths (cost), with their item0; the number of items.
+    auto order = [&](std::vector<std::pair<int64_t, AccountPiece>> &cost, std::vector<AccountPiece> &out) {
+        std::stable_sort(cost.begin(), cost.end(), [](const auto &x, const auto &y) { return x.first > y.first; });
+        int64_t items = 0;
+        for (auto &c : cost) {
+            c.second.item0 = (int32_t)std::min<int64_t>(items, INT32_MAX);
+            items += (int64_t)(c.second.last - c.second.first) * c.second.chunks();
+            out.push_back(c.second);
+        }
+        return items;
+    };
     plan.launches.clear();
+    std::vector<std::pair<int64_t, AccountPiece>> tiles, blocks;
     for (size_t i = 0; i < plan.entries.size();) {
         AccountLaunch l{};
         l.first = (int)i;
+        l.n = (int)std::min<size_t>(kAccountBatch, plan.entries.size() - i);
         l.fold = true;
-        int64_t items = 0, sums = 0;
-        for (; i < plan.entries.size() && l.n < kAccountBatch; ++i, ++l.n) {
+        tiles.clear(), blocks.clear();
+        const int pieces = kAccountPieces / l.n; // of an entry
+        int64_t   fold_rows = 0, fold_parts = 0;
+        for (int k = 0; k < l.n; ++k, ++i) {
             AccountEntry &e = plan.entries[i];
-            const int     keys = e.p0 + e.n, kb = account_blocks(keys);
-            const int64_t rows = (int64_t)e.w * G, rt = (rows + kAccountRows - 1) / kAccountRows;
-            if (rows > INT32_MAX / 2) return false;
-            e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(split, stream_tiles(keys) / 2));
-            const int64_t steps = (rows + kAccountStep - 1) / kAccountStep;
-            const int64_t least = blocks * Hkv * steps >= 4 * n ? 4 : 2;
-            const int64_t each = std::max(least, (steps + row_split - 1) / row_split);
-            e.rc = (int)std::min<int64_t>(each * kAccountStep, 1 << 30);
-            e.nrc = (int)((rows + e.rc - 1) / e.rc);
-            e.item0 = (int32_t)items;
-            e.sum0 = (int32_t)sums;
+            const int     keys = e.p0 + e.n, rows = e.w * G;
+            const int     rt = (rows + kAccountRows - 1) / kAccountRows, kb = account_blocks(keys);
+            const int     st = (rows + kAccountStep - 1) / kAccountStep;
+            e.nch = e.nrc = 1;
+            for (int x = 0, lo = 0; x < pieces; ++x) {
+                const int hi = (int)((int64_t)(x + 1) * rt / pieces);
+                if (hi == lo) continue;
+                const int64_t most = account_seen(e, G, hi - 1), c = ceil_div(most, keys_each);
+                tiles.push_back({ceil_div(most, c), {0, lo, hi, (uint32_t)k | (uint32_t)c << 8}});
+                e.nch = std::max(e.nch, (int)c);
+                lo = hi;
+            }
+            int64_t chunk_rows = 0;
+            for (int x = 0, lo = 0; x < pieces; ++x) {
+                const int hi = (int)((int64_t)(x + 1) * kb / pieces);
+                if (hi == lo) continue;
+                const int64_t most = st - account_sees(e, G, lo), c = ceil_div(most, rows_each);
+                blocks.push_back({ceil_div(most, c), {0, lo, hi, (uint32_t)k | (uint32_t)c << 8}});
+                e.nrc = std::max(e.nrc, (int)c);
+                chunk_rows = std::max(chunk_rows, ceil_div(most, c) * kAccountStep);
+                lo = hi;
+            }
             e.lse0 = (int32_t)l.lse;
             e.stat0 = (int32_t)l.stats;
             e.part0 = (int32_t)l.parts;
-            items += rt * e.nch;
-            sums += (int64_t)kb * e.nrc;
             l.lse += rows;
-            if (e.nch > 1) l.stats += rows * e.nch;
+            if (e.nch > 1) l.stats += (int64_t)rows * e.nch;
             if (e.nrc > 1) l.parts += (int64_t)kb * kAccountKeys * e.nrc;
-            if (std::max({items * Hkv, sums * Hkv, l.lse, l.stats, l.parts}) > INT32_MAX) return false;
+            if (std::max({l.lse, l.stats, l.parts}) > INT32_MAX) return false;
             l.split_keys |= e.nch > 1;
-            const int64_t chunk_rows = std::min<int64_t>(rows, e.rc);
-            if (e.nch > 1 && (chunk_rows > kAccountFold || chunk_rows * e.nch > kAccountFoldParts)) l.fold = false;
             l.split_rows |= e.nrc > 1;
-            if (e.nch > 1) l.most_rows = std::max(l.most_rows, (int)rows);
+            if (e.nch > 1) {
+                l.most_rows = std::max(l.most_rows, rows);
+                fold_rows = std::max(fold_rows, chunk_rows);
+                fold_parts = std::max(fold_parts, chunk_rows * e.nch);
+            }
             if (e.nrc > 1) l.most_keys = std::max(l.most_keys, keys);
         }
+        l.fold = fold_rows <= kAccountFold && fold_parts <= kAccountFoldParts;
+        const int64_t items = order(tiles, l.tile_pieces), sums = order(blocks, l.block_pieces);
+        if (std::max(items, sums) * Hkv > INT32_MAX) return false;
         l.items = (int)items;
         l.sums = (int)sums;
-        plan.launches.push_back(l);
+        plan.launches.push_back(std::move(l));
     }
     return true;
 }

@@ -58,26 +58,35 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus);
 constexpr int kAccountRows = 128;  // query rows of a workgroup of account_stats_kernel
 constexpr int kAccountKeys = 256;  // keys of a workgroup of account_sum_kernel
 constexpr int kAccountStep = 64;   // rows that it stages at a time
-constexpr int kAccountBatch = 72;  // entries per launch
+constexpr int kAccountBatch = 44;  // entries per launch
+constexpr int kAccountPieces = 64; // pieces per launch and kernel
 constexpr int kAccountFold = 256;  // rows of a chunk whose statistics account_sum_kernel merges,
 constexpr int kAccountFoldParts = 8192; // and their partial results at most
 
 // The last w of the n new tokens of cache row `row` (positions p0 .. p0 + n - 1; tok0:
 // the first one's index in the call's tokens) attend causally: w * G query rows per
-// kv head.  account_stats_kernel cuts them into tiles and their keys into nch chunks
-// (item0: its work items of the entries before); lse0, stat0: the entries' rows of
-// results and of partial results before.  account_sum_kernel cuts the keys into
-// blocks and the rows into nrc chunks of `rc` (sum0: work items before; part0: tokens
-// of partial sums before).
+// kv head.  account_stats_kernel cuts them into tiles and the keys that a tile sees into
+// nch chunks at most; account_sum_kernel cuts the keys into blocks and the rows that see
+// a block into nrc chunks at most.  lse0, stat0, part0: rows of results, rows of partial
+// results and tokens of partial sums of the entries before.
 struct AccountEntry {
-    int32_t row, p0, n, w, tok0, nch, item0, lse0, stat0, nrc, rc, sum0, part0;
+    int32_t row, p0, n, w, tok0, nch, lse0, stat0, nrc, part0;
+};
+// Tiles (blocks) first .. last - 1 of an entry, each in `chunks` equal chunks, some of
+// them empty where it has less: work items item0 .. of the launch.
+struct AccountPiece {
+    int32_t  item0, first, last;
+    uint32_t what; // entry of the launch | chunks << 8
+    int      entry() const { return (int)(what & 255u); }
+    int      chunks() const { return (int)(what >> 8); }
 };
 struct AccountLaunch {
     int     first, n, items, sums;
     bool    split_keys, split_rows;   // some nch, nrc is above 1
     bool    fold;                     // account_sum_kernel merges the key chunks' statistics itself
-    int     most_rows, most_keys;     // of an entry
+    int     most_rows, most_keys;     // of an entry that is split
     int64_t lse, stats, parts;        // per kv head
+    std::vector<AccountPiece> tile_pieces, block_pieces; // longest items first
 };
 struct AccountPlan {
     std::vector<AccountEntry>  entries;
@@ -87,6 +96,15 @@ struct AccountPlan {
 };
 
 inline int account_blocks(int keys) { return keys / kAccountKeys + (keys % kAccountKeys != 0); }
+// Key tiles that row tile rt sees, and the first of the row steps that see key block kb.
+inline int account_seen(const AccountEntry &e, int G, int rt) {
+    const int64_t rows = (int64_t)e.w * G, r_hi = rows < (int64_t)(rt + 1) * kAccountRows ? rows : (int64_t)(rt + 1) * kAccountRows;
+    return stream_tiles((int)(e.p0 + e.n - e.w + (r_hi - 1) / G + 1));
+}
+inline int account_sees(const AccountEntry &e, int G, int kb) {
+    const int64_t behind = (int64_t)kb * kAccountKeys - (e.p0 + e.n - e.w);
+    return behind > 0 ? (int)(behind * G / kAccountStep) : 0;
+}
 
 // Sets the rest of plan.entries, and the launches.  False when a launch's rows or
 // items do not fit 31 bits.
