@@ -30,11 +30,12 @@
 //
 // Measured, with accounts, 8 kv heads of 128: 64 x 8192 tokens, group 4, whole
 // entries: 360 us, 6.0 TB/s of K and V (without accounts the decode kernel takes 309 on
-// the same cache); 96 lognormal lengths to 16384 on blocks, group 8: 264 + 27 us for
-// the finish; 4 x 128..512 tokens, 8 heads of 64: 7.4 us, one launch's latency.  Two or
+// the same cache); 96 lognormal lengths to 16384 on blocks, group 8: 264 + 20 us for
+// the finish (27 with a row's scores on their way at a time, 30 with all eight); 4 x 128..512 tokens, 8 heads of 64: 7.4 us, one launch's latency.  Two or
 // three steps of rows on their way in registers were level or slower (occupancy).
 #include "stream.h"
 
+#include "../runtime.h"
 #include "tiny_llm/hip_utils.h"
 
 #include <hip/hip_runtime.h>
@@ -108,13 +109,14 @@ struct __attribute__((packed, aligned(4))) Four {
 
 // The account of tokens [t_lo, t_hi) of entry ei and kv head g, t_lo a multiple of a
 // tile, from their scores (sc: [tile][rows][64], in LDS or memory), the rows' final
-// maxima and the inverse of their sums (in LDS).
-template <int NT>
+// maxima and the inverse of their sums (in LDS).  U: accounts of so many fours on
+// their way at once; 1 with several rows' scores (from memory).
+template <int NT, int U>
 __device__ __forceinline__ void account_tokens(const StreamArgs &a, int ei, int g, int rows, int t_lo, int t_hi,
                                                const float *sc, const float *m, const float *inv) {
+    constexpr int ROWS = U == 1 && NT == 256 ? 4 : 1;
     const int     old = a.e[ei].S - a.fresh;
     const int64_t base = ((int64_t)a.e[ei].row * a.Hkv + g) * a.room;
-    constexpr int U = NT > 256 ? 1 : 8; // accounts of so many fours on their way at once (8 waves: short entries)
     for (int t0 = t_lo + 4 * (int)threadIdx.x; t0 < t_hi; t0 += 4 * NT * U) {
         Four w[U];
 #pragma unroll
@@ -134,6 +136,7 @@ __device__ __forceinline__ void account_tokens(const StreamArgs &a, int ei, int 
             if (t >= t_hi) break;
             const float *st = sc + (int64_t)((t - t_lo) / kStreamTile) * rows * kStreamTile + t % kStreamTile;
             f32x4        sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll ROWS
             for (int r = 0; r < rows; ++r) { // (scores past the end are -infinity)
                 const f32x4 s = *reinterpret_cast<const f32x4 *>(st + r * kStreamTile);
 #pragma unroll
@@ -378,7 +381,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
     }
     if constexpr (SCORES) {
         if (nch == 1) {
-            account_tokens<NW * 64>(a, ei, g, rows, 0, S, lsc, s_m, s_inv);
+            account_tokens<NW * 64, NW == 8 ? 1 : 8>(a, ei, g, rows, 0, S, lsc, s_m, s_inv);
         } else { // the chunk's scores in one go
             float *dst = a.scores + ((int64_t)a.e[ei].tile0 * a.Hkv + (int64_t)g * tiles + tile_lo) * a.rows * kStreamTile;
             for (int k = threadIdx.x; k < (tile_hi - tile_lo) * rows * (kStreamTile / 4); k += NW * 64)
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArg
         for (int64_t t = (int64_t)blockIdx.y * kFinishTokens; t < S; t += (int64_t)gridDim.y * kFinishTokens) {
             const int    t_lo = (int)t, t_hi = (int)min((int64_t)S, t + kFinishTokens);
             const float *sc = a.scores + ((int64_t)a.e[ei].tile0 * a.Hkv + (int64_t)g * tiles + t_lo / kStreamTile) * a.rows * kStreamTile;
-            account_tokens<kFinishThreads>(a, ei, g, rows, t_lo, t_hi, sc, s_m, s_inv);
+            account_tokens<kFinishThreads, 1>(a, ei, g, rows, t_lo, t_hi, sc, s_m, s_inv);
         }
     }
 }
@@ -461,8 +464,8 @@ size_t part_ml_floats(size_t rows) { return (2 * rows + 3) / 4 * 4; }
 template <int D, bool PAGED, bool SCORES, int NW>
 void launch_one(const StreamArgs &a, int items, int lds, hipStream_t stream) {
     auto                 *fn = attn_stream_kernel<D, PAGED, SCORES, NW>;
-    static std::once_flag once;
-    std::call_once(once, [&] {
+    static std::once_flag once[64]; // per device
+    std::call_once(once[current_device() & 63], [&] {
         HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
                                       kStreamLds));
     });
