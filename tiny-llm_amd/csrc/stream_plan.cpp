@@ -21,14 +21,14 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
     const bool    few = some * Hkv <= n;
     // An entry in one chunk is finished by its own workgroup: no partial results, no
     // second launch, and its scores never leave the LDS.  Short entries are left whole
-    // (16 x 300 states, 8 heads of 64: 7.4 us against 9.4 split), with eight waves
+    // (16 x 300 tokens with accounts, 8 heads of 64: 7.2 us, 11.6 split), with eight waves
     // where they have so many tiles.  Work that is little for the chip is spread over
-    // as many workgroups as it has pieces of four tiles (decode with accounts, 1 x
-    // 4096 tokens, 8 heads of 128: 16.4 us, in pieces of 8 on eight waves 18.5, of 32
-    // 29.7); where a CU has several tiles to itself, eight waves and fewer pieces are
-    // better (1 x 32768 tokens: 38.4 against 44.8 us; 1 x 8192: 22.8 against 24.4, without
-    // accounts 19.8 against 19.3), or whole entries while none is much longer than a
-    // CU's share (8 x 1024: 19.2 against 21.0).
+    // as many workgroups as it has pieces of four tiles (1 x 4096, 8 heads of 128: 14.0 us,
+    // 16.8 in pieces of 8 on eight waves, 30 of 32).  Where a CU has several tiles to itself,
+    // eight waves and fewer pieces are better (4 x 2048: 17.6 against 19.0 us; 1 x 32768:
+    // 33.0, 34.5), and whole entries are while they fill half of the chip and none is much
+    // longer than a CU's share (30 x 4096: 96 us, 112; 20 x 1500, 8 heads of 64: 17.5, 21;
+    // but 8 x 1024: 19.3, 16.9).
     if (few && longest <= (D <= 128 ? kStreamWhole : kStreamWhole / 4)) {
         plan.waves = D <= 128 && longest > 4 ? 8 : 4;
         chunk = longest;
@@ -38,7 +38,7 @@ void plan_stream(StreamPlan &plan, int Hkv, int D, int account_rows, int cus) {
     } else if (few && D <= 128) {
         plan.waves = 8;
         chunk = std::max<int64_t>(8, share);
-        if (2 * longest <= 5 * chunk) chunk = longest;
+        if (2 * some * Hkv >= n && 2 * longest <= 5 * chunk) chunk = longest;
     } else {
         plan.waves = 4;
         chunk = longest <= std::max<int64_t>(32, 2 * half + half / 2) ? longest : std::max<int64_t>(8, half);
