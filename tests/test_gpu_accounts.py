@@ -76,7 +76,8 @@ def test_decode_weights(tl, d, hkv, G, block, lens):
     (256, 4, 4, 0, [900, 300]),
     (256, 2, 2, 16, [2600]),
     (128, 8, 4, 0, [8300]),        # more: eight waves
-    (64, 8, 1, 0, [1024] * 8),     # whole entries on eight waves
+    (64, 8, 1, 0, [1024] * 8),
+    (64, 8, 1, 0, [1500] * 20),    # whole entries on eight waves
     (64, 2, 2, 0, [300, 767]),
     (32, 8, 1, 16, [(i * 97) % 700 for i in range(40)]),   # many entries
     (64, 8, 2, 0, [50] * 33 + [4000]),                     # ... and a long one among them
