@@ -144,10 +144,12 @@ struct Head {
         h.p_out = (a).st.pos_out + base_;                                                                              \
     } while (0)
 
-// The bin, of `bins` from the top, in which the need-th largest lies: pick = {bin, how
-// many of it, its count}.  lds: NT / 64 words.
-template <int NT> __device__ __forceinline__ void pick_bin(const uint32_t *hist, uint32_t need, uint32_t *lds, uint32_t *pick) {
+// The bin, of kBins from the top, in which the need-th largest lies: pick = {bin, how
+// many of it, its count}.  `hist` is complete (a barrier before the call); the waves'
+// sums have words of their own, which no wave may still be reading here.
+template <int NT> __device__ __forceinline__ void pick_bin(const uint32_t *hist, uint32_t need, uint32_t *pick) {
     constexpr int P = kBins / NT;
+    __shared__ uint32_t sums[NT / 64];
     const int     tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint32_t      c[P], own = 0;
 #pragma unroll
@@ -156,11 +158,11 @@ template <int NT> __device__ __forceinline__ void pick_bin(const uint32_t *hist,
         own += c[u];
     }
     const uint32_t inc = wave_scan(own);
-    if (lane == 63) lds[wave] = inc;
+    if (lane == 63) sums[wave] = inc;
     __syncthreads();
     uint32_t above = inc - own;
 #pragma unroll
-    for (int w = 0; w < NT / 64; ++w) above += w < wave ? lds[w] : 0u;
+    for (int w = 0; w < NT / 64; ++w) above += w < wave ? sums[w] : 0u;
 #pragma unroll
     for (int u = 0; u < P; ++u) {
         if (above < need && need <= above + c[u]) { // one bin
@@ -246,7 +248,7 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
     int      shift = 0;
     if (held < need) {
         need -= held;
-        pick_bin<NT>(hist, need, lds, pick);
+        pick_bin<NT>(hist, need, pick);
         thr = pick[0] << 21;
         need = pick[1];
         equal = pick[2];
@@ -281,7 +283,7 @@ template <int NT, int IT> __global__ __launch_bounds__(NT) void evict_select_ker
                     }
             }
             __syncthreads();
-            pick_bin<NT>(hist, need, lds, pick);
+            pick_bin<NT>(hist, need, pick);
             thr |= pick[0] << lo;
             need = pick[1];
             equal = pick[2];
@@ -445,7 +447,7 @@ template <int NT> __global__ __launch_bounds__(NT) void evict_select_any_kernel(
                     atomicAdd(&hist[(k >> lo) & ((1u << bits) - 1u)], 1u);
             }
             __syncthreads();
-            pick_bin<NT>(hist, need, lds, pick);
+            pick_bin<NT>(hist, need, pick);
             thr |= pick[0] << lo;
             need = pick[1];
             equal = pick[2];
