@@ -349,6 +349,9 @@ int  tl_kv_prefill_weights(tl_kv_prefill *p, int layer, const void *q, float sca
  *   commit:  when every layer has run: the sequences are as long as what they
  *            kept, and a block pool gets the blocks behind it back.  Other
  *            batches must be prepared again.  Nothing changes when it fails.
+ *            Sequences released since prepare are left out; it fails when no
+ *            other one loses tokens.  A sequence that grew after its rows moved
+ *            is to be released before the others can be committed.
  * head_dim in {32, 64, 128, 256}.  Everything a launch needs travels in its
  * arguments; the selection's lists are in a workspace of the batch, sized by
  * prepare, so one batch is used from one stream at a time. */

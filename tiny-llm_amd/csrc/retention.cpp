@@ -219,12 +219,34 @@ Result<void> EvictBatch::prepare(const int *seq_ids, const int *budgets, int n, 
     return Result<void>::ok();
 }
 
+// Sequences that were released since prepare() leave the step, and those that nothing is
+// taken from when another eviction changed them.  The id of a released one, or -1.
+int EvictBatch::leaveOut() {
+    int    released = -1;
+    size_t n = 0;
+    for (size_t i = 0; i < ids_.size(); ++i) {
+        const detail::EvictEntry e = entries_[i];
+        if (!mgr_.sequence(ids_[i])) {
+            released = ids_[i];
+            evicted_ -= e.len - e.keep;
+        } else if (e.keep < e.len || mgr_.evictions_[static_cast<size_t>(e.row)].gone == e.gone) {
+            ids_[n] = ids_[i];
+            entries_[n++] = e;
+        }
+    }
+    if (n < ids_.size()) {
+        ids_.resize(n);
+        entries_.resize(n);
+        detail::evict_workspace_words(entries_, mgr_.getConfig().num_heads); // (their lists, fewer than before)
+    }
+    return released;
+}
+
 std::string EvictBatch::changed() const {
     for (size_t i = 0; i < ids_.size(); ++i) {
-        const SequenceCache *sc = mgr_.sequence(ids_[i]);
-        if (!sc) return "EvictBatch: sequence not found: " + std::to_string(ids_[i]);
-        const KVCacheManager::Eviction &ev = mgr_.evictions_[static_cast<size_t>(entries_[i].row)];
-        if (sc->current_len != entries_[i].len || ev.gone != entries_[i].gone)
+        const detail::EvictEntry &e = entries_[i];
+        if (e.keep == e.len) continue; // stays as it is, also where it has grown
+        if (mgr_.sequence(ids_[i])->current_len != e.len || mgr_.evictions_[static_cast<size_t>(e.row)].gone != e.gone)
             return "EvictBatch: sequence " + std::to_string(ids_[i]) + " changed since prepare";
     }
     return "";
@@ -245,6 +267,8 @@ Result<void> EvictBatch::run(int layer_idx, const float *weights_in, float *weig
         overlap(wi, po, bytes) || overlap(wo, pi, bytes))
         return Result<void>::err("EvictBatch: an output overlaps an array that it is not");
     if (ids_.empty()) return Result<void>::ok();
+    if (const int id = leaveOut(); ids_.empty() && id >= 0)
+        return Result<void>::err("EvictBatch: sequence not found: " + std::to_string(id));
     if (const std::string err = changed(); !err.empty()) return Result<void>::err(err);
     char &ran = ran_[static_cast<size_t>(layer_idx)];
     if (ran == 2)
@@ -270,6 +294,8 @@ Result<void> EvictBatch::run(int layer_idx, const float *weights_in, float *weig
 }
 
 Result<void> EvictBatch::commit() {
+    if (const int id = leaveOut(); evicted_ == 0 && id >= 0) // nothing is left to take
+        return Result<void>::err("EvictBatch: sequence not found: " + std::to_string(id));
     if (const std::string err = changed(); !err.empty()) return Result<void>::err(err);
     if (evicted_ > 0) {
         for (size_t l = 0; l < ran_.size(); ++l)

@@ -358,7 +358,9 @@ class PrefillBatch {
 //
 // A run moves rows, so an eviction that has begun is to be committed: until then
 // no prepare() takes its sequences, no other batch's run() does, and the cache is
-// not to be read at the layers that ran.  A captured run() counts as run.  run()
+// not to be read at the layers that ran.  A captured run() counts as run.  A sequence
+// that is released leaves the step, the others are run and committed without it; one
+// that grew by advanceSeqLen after its rows moved is to be released first.  run()
 // calls of one batch share its lists: one stream, or the caller orders them, also
 // the replays of graphs that captured them.
 class EvictBatch {
@@ -381,7 +383,8 @@ class EvictBatch {
 
   private:
     EvictBatch(KVCacheManager &mgr, int max_seqs);
-    // "" while the sequences are as prepare() found them.
+    int         leaveOut();
+    // "" while the sequences that lose tokens are as prepare() found them.
     std::string changed() const;
 
     KVCacheManager  &mgr_;
