@@ -344,8 +344,10 @@ int  tl_kv_prefill_weights(tl_kv_prefill *p, int layer, const void *q, float sca
  *            the sequence's last eviction left (the tokens after that came in
  *            order), so it needs no initial value.  A layer that ran in place is
  *            not run again before commit.  A run moves rows of the cache (a captured
- *            one counts as run): until its commit the layer is not to be read, no
- *            prepare takes its sequences and no other batch runs over them;
+ *            one counts as run): until its commit tl_kv_append, every prepare
+ *            but tl_kv_batch_prepare_lengths, the commits of steps prepared
+ *            before and the runs of other evictions refuse its sequences, and the
+ *            layer is not to be read;
  *   commit:  when every layer has run: the sequences are as long as what they
  *            kept, and a block pool gets the blocks behind it back.  Other
  *            batches must be prepared again.  Nothing changes when it fails.

@@ -121,3 +121,52 @@ def test_a_sequence_that_grew_after_its_rows_moved(tl):
     c.mgr.releaseSequence(c.ids[0])
     r.ev.commit()
     r.check(1)
+
+
+@pytest.mark.parametrize("block", [0, 16])
+def test_an_eviction_under_way_refuses_other_steps(tl, block):
+    """Appends, steps that would append, attention to the states, and the commits of
+    steps that were prepared before; after the commit all of it goes on."""
+    c = Cache(tl, [50, 80, 10], 1, 32, room=112, block=block, layers=2, seed=35)
+    a, b, free = c.ids  # nothing is taken from the last one
+    k = dev(c.rows(4))
+    K = k.data_ptr()
+    dec, pf, cross = tl.DecodeBatch(c.mgr, 3, 1), tl.PrefillBatch(c.mgr, 3, 1), tl.CrossBatch(c.mgr, 2, 1)
+    dec.prepare(c.ids)
+    pf.prepare([b], [2])
+    r = Running(tl, c, [20, 20, 20])
+    r.run(0)
+    msg = "eviction of sequence {} has run and is not committed"
+    for call, who in ((lambda: tl.DecodeBatch(c.mgr, 1, 1).prepare([a]), a), (lambda: dec.commit(1), a), (lambda: pf.commit(), b),
+                      (lambda: tl.PrefillBatch(c.mgr, 2, 1).prepare([free, b], [1, 1]), b),
+                      (lambda: cross.prepare([free, b], [1, 1]), b)):
+        with pytest.raises(tl.TinyLLMError, match=msg.format(who)):
+            call()
+    assert msg.format(a) in c.mgr.appendKV(a, 0, K, K, 2)
+    assert [c.mgr.getSeqLen(s) for s in c.ids] == [50, 80, 10]  # no part of a step was committed
+    assert c.mgr.appendKV(free, 0, K, K, 2) is None
+    dec.prepare([free])
+    cross.prepare([free], [1])
+    held = tl.DecodeBatch(c.mgr, 1, 1)
+    held.prepare_lengths([a], [20])
+    r.run(1)
+    r.ev.commit()
+    for i in (0, 1):
+        r.check(i)
+    assert c.mgr.appendKV(a, 0, K, K, 2) is None
+    dec.prepare(c.ids)
+    dec.commit(1)
+    pf.prepare([b], [2])
+    cross.prepare([a, b], [1, 1])
+    assert [c.mgr.getSeqLen(s) for s in c.ids] == [21, 21, 11]
+    # a step whose sequence is gone says so, whatever its slot's next one does
+    c.mgr.releaseSequence(a)
+    new, _ = c.mgr.allocateSequence(30)
+    c.mgr.advanceSeqLen(new, 9)
+    r2 = tl.EvictBatch(c.mgr, 1)
+    r2.prepare([new], [5], 1)
+    w, p = r.w[0].data_ptr(), r.pos[0].data_ptr()
+    r2.run(0, w, w, p, p)
+    with pytest.raises(tl.TinyLLMError, match="not found"):
+        dec.commit(1)
+    torch.cuda.synchronize()

@@ -55,6 +55,8 @@ Result<void> CrossBatch::prepare(const int *seq_ids, const int *num_queries, con
     for (int i = 0; i < n; ++i) {
         const SequenceCache *sc = mgr_.sequence(seq_ids[i]);
         if (!sc) return Result<void>::err("CrossBatch: sequence not found: " + std::to_string(seq_ids[i]));
+        if (mgr_.evictionBegun(mgr_.slotOf(seq_ids[i])))
+            return Result<void>::err("CrossBatch: " + detail::eviction_begun(seq_ids[i]));
         if (num_queries[i] <= 0)
             return Result<void>::err("CrossBatch: num_queries must be positive: " + std::to_string(num_queries[i]));
         const int a = attended ? attended[i] : sc->current_len;

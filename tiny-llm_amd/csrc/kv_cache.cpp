@@ -246,6 +246,11 @@ Result<void> KVCacheManager::appendKV(int seq_id, int layer_idx, const half *new
     }
     const int slot_idx = it->second;
     auto     &slot = slots_[static_cast<size_t>(slot_idx)];
+    if (evictionBegun(slot_idx)) {
+        const std::string msg = "appendKV: " + detail::eviction_begun(seq_id);
+        TL_LOG_ERROR("%s", msg.c_str());
+        return Result<void>::err(msg);
+    }
     // All layers of a step see the same write position: the length is
     // advanced once after the last layer (kv_cache.cpp:204-208).
     const int write_pos = slot.current_len;
@@ -328,6 +333,10 @@ bool KVCacheManager::hasSequence(int seq_id) const noexcept {
 int KVCacheManager::getEvicted(int seq_id) const noexcept {
     const int s = slotOf(seq_id);
     return s < 0 ? 0 : evictions_[static_cast<size_t>(s)].gone;
+}
+
+bool KVCacheManager::evictionBegun(int slot) const noexcept {
+    return slot >= 0 && slot < config_.max_batch_size && evictions_[static_cast<size_t>(slot)].by != nullptr;
 }
 
 // The end of an eviction: the slot's sequence holds its first `keep` tokens.
@@ -546,6 +555,8 @@ Result<void> DecodeBatch::upload(const int *seq_ids, const int *attended, int n,
         const SequenceCache *sc = mgr_.sequence(id);
         if (!sc) return Result<void>::err("DecodeBatch: sequence not found: " + std::to_string(id));
         const int slot = mgr_.slotOf(id);
+        if (appendable && mgr_.evictionBegun(slot))
+            return Result<void>::err("DecodeBatch: " + detail::eviction_begun(id));
         if (taken[static_cast<size_t>(slot)])
             return Result<void>::err("DecodeBatch: duplicate sequence in batch: " + std::to_string(id));
         taken[static_cast<size_t>(slot)] = 1;
@@ -624,6 +635,9 @@ Result<void> DecodeBatch::prepare(const int *seq_ids, int n, hipStream_t stream)
 // The commit of InferenceEngine::decodeStep (inference_engine.cpp:291),
 // advanceSeqLen(seq, num_tokens), for every sequence of the last prepare.
 Result<void> DecodeBatch::commit(int num_tokens) {
+    for (size_t i = 0; i < ids_.size(); ++i)
+        if (mgr_.evictionBegun(slot_[i]) && mgr_.slotOf(ids_[i]) == slot_[i])
+            return Result<void>::err("DecodeBatch: " + detail::eviction_begun(ids_[i]));
     for (const int id : ids_) {
         auto r = mgr_.advanceSeqLen(id, num_tokens);
         if (r.isErr()) return r;
@@ -866,6 +880,7 @@ Result<void> PrefillBatch::prepare(const int *seq_ids, const int *num_tokens, in
         const SequenceCache *sc = mgr_.sequence(id);
         if (!sc) return Result<void>::err("PrefillBatch: sequence not found: " + std::to_string(id));
         const int slot = mgr_.slotOf(id);
+        if (mgr_.evictionBegun(slot)) return Result<void>::err("PrefillBatch: " + detail::eviction_begun(id));
         if (taken[static_cast<size_t>(slot)])
             return Result<void>::err("PrefillBatch: duplicate sequence in batch: " + std::to_string(id));
         taken[static_cast<size_t>(slot)] = 1;
@@ -990,6 +1005,9 @@ Result<void> PrefillBatch::launch(int layer_idx, const half *q, const half *new_
 // InferenceEngine::prefill's commit (inference_engine.cpp:272):
 // advanceSeqLen(seq, prompt tokens) once after all layers.
 Result<void> PrefillBatch::commit() {
+    for (size_t i = 0; i < ids_.size(); ++i)
+        if (mgr_.evictionBegun(slots_[i]) && mgr_.slotOf(ids_[i]) == slots_[i])
+            return Result<void>::err("PrefillBatch: " + detail::eviction_begun(ids_[i]));
     for (size_t i = 0; i < ids_.size(); ++i) {
         auto r = mgr_.advanceSeqLen(ids_[i], counts_[i]);
         if (r.isErr()) return r;

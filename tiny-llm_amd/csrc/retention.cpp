@@ -37,10 +37,6 @@ std::string check_accounts(const char *who, const KVCacheConfig &cfg, const floa
     return "";
 }
 
-std::string begun(int seq_id) {
-    return "EvictBatch: an eviction of sequence " + std::to_string(seq_id) + " has run and is not committed";
-}
-
 std::string check_device(const char *who, int device) {
     const int now = detail::current_device();
     return now == device ? std::string()
@@ -167,7 +163,7 @@ Result<std::unique_ptr<EvictBatch>> EvictBatch::create(KVCacheManager &mgr, int 
 Result<void> EvictBatch::prepare(const int *seq_ids, const int *budgets, int n, int recent, hipStream_t stream) {
     for (size_t i = 0; i < ids_.size(); ++i)
         if (mgr_.sequence(ids_[i]) && mgr_.evictions_[static_cast<size_t>(entries_[i].row)].by == this)
-            return Result<void>::err(begun(ids_[i]));
+            return Result<void>::err("EvictBatch: " + detail::eviction_begun(ids_[i]));
     // A failing prepare leaves an empty batch.
     ids_.clear();
     entries_.clear();
@@ -196,7 +192,7 @@ Result<void> EvictBatch::prepare(const int *seq_ids, const int *budgets, int n, 
                                      std::to_string(seq_ids[i]) + " must be positive and hold the " +
                                      std::to_string(recent) + " newest tokens");
         const KVCacheManager::Eviction &ev = mgr_.evictions_[static_cast<size_t>(slot)];
-        if (ev.by) return Result<void>::err(begun(seq_ids[i]));
+        if (ev.by) return Result<void>::err("EvictBatch: " + detail::eviction_begun(seq_ids[i]));
         if (ev.gone > INT32_MAX - cfg.max_seq_len)
             return Result<void>::err("EvictBatch: positions of sequence " + std::to_string(seq_ids[i]) +
                                      " exceed 31 bits");
@@ -277,7 +273,7 @@ Result<void> EvictBatch::run(int layer_idx, const float *weights_in, float *weig
     if (std::string err = check_device("EvictBatch", mgr_.device()); !err.empty()) return Result<void>::err(err);
     for (size_t i = 0; i < ids_.size(); ++i) {
         const EvictBatch *by = mgr_.evictions_[static_cast<size_t>(entries_[i].row)].by;
-        if (by && by != this) return Result<void>::err(begun(ids_[i]));
+        if (by && by != this) return Result<void>::err("EvictBatch: " + detail::eviction_begun(ids_[i]));
     }
     for (const auto &e : entries_)
         if (e.keep < e.len) mgr_.evictions_[static_cast<size_t>(e.row)].by = this;

@@ -7,6 +7,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <mutex>
+#include <string>
 #include <vector>
 
 namespace tiny_llm {
@@ -119,6 +120,11 @@ struct DeviceContext {
 };
 
 int current_device();
+
+// Why calls refuse a sequence whose eviction has moved rows and is not committed.
+inline std::string eviction_begun(int seq_id) {
+    return "an eviction of sequence " + std::to_string(seq_id) + " has run and is not committed";
+}
 
 // Event timing of the launchers (tl_profile_*); ids are KernelId values.
 void profile_set(bool on);

@@ -112,6 +112,8 @@ class KVCacheManager {
     // Tokens of the sequence that evictions took from the cache (EvictBatch): the
     // next token's position is getSeqLen + getEvicted.  0 for an unknown sequence.
     int getEvicted(int seq_id) const noexcept;
+    // Whether an eviction has moved rows of the slot's sequence and is not committed.
+    bool evictionBegun(int slot) const noexcept;
     // Elements from layer l's K base to layer l+1's.
     int64_t layerStride() const noexcept { return layer_stride_; }
 
@@ -356,13 +358,15 @@ class PrefillBatch {
 // output that is not its input must not overlap it.  A layer that ran in place
 // is not run again before commit().
 //
-// A run moves rows, so an eviction that has begun is to be committed: until then
-// no prepare() takes its sequences, no other batch's run() does, and the cache is
-// not to be read at the layers that ran.  A captured run() counts as run.  A sequence
-// that is released leaves the step, the others are run and committed without it; one
-// that grew by advanceSeqLen after its rows moved is to be released first.  run()
-// calls of one batch share its lists: one stream, or the caller orders them, also
-// the replays of graphs that captured them.
+// A run moves rows (a captured one counts), so an eviction that has begun is to be
+// committed: until then appendKV, the prepare() of every batch, the commit() of steps
+// prepared before and the run() of other evictions refuse its sequences, and the cache
+// is not to be read at the layers that ran, where rows are in two places.
+// prepareLengths and advanceSeqLen do not refuse.  A sequence that is released leaves
+// the step, the others are run and committed without it; one that grew by
+// advanceSeqLen after its rows moved is to be released first.  run() calls of one batch
+// share its lists: one stream, or the caller orders them, also the replays of graphs
+// that captured them.
 class EvictBatch {
   public:
     static Result<std::unique_ptr<EvictBatch>> create(KVCacheManager &mgr, int max_seqs);
