@@ -43,6 +43,7 @@ typedef float    f32x4 __attribute__((ext_vector_type(4)));
 typedef short    s16x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kBelow = 7.0f, kLazyMax = 15.0f; // of the softmax reference, as in attn_stream_kernel
+constexpr float kNone = -3e38f; // ... over no score, or over -infinite ones only
 constexpr int   kVmcnt0 = 0x0F70; // s_waitcnt vmcnt(0)
 constexpr int   kTile = kStreamTile;
 
@@ -179,7 +180,7 @@ attn_cross_kernel(CrossArgs a) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[j][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         l_run[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        m_run[j] = -INFINITY;
+        m_run[j] = kNone;
     }
     const f16x8 ones = __builtin_bit_cast(f16x8, make_uint4(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u));
 

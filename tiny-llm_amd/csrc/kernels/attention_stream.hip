@@ -61,6 +61,9 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // of the largest are still above its smallest step.  (A reference at the maximum lost
 // all weights 2^-25 below it, which a long cache of even ones feels.)
 constexpr float kBelow = 7.0f, kLazyMax = 15.0f;
+// The reference over no score, or over -infinite ones only: finite, so that a score of
+// -infinity has the weight 0 beside it, and below every finite score.
+constexpr float kNone = -3e38f;
 
 struct StreamArgs {
     const __half *q;
@@ -217,7 +220,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
     f32x4 acc[DT];
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    float m_run = -INFINITY, l_run = 0.0f;
+    float m_run = kNone, l_run = 0.0f;
 
     // The wave's steps: step x of the chunk's tiles, tile tile_lo + x / SUB * NW + wave.
     const int steps = max(0, (tile_hi - tile_lo - wave + NW - 1) / NW) * SUB;
@@ -317,7 +320,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
         for (int tt = 0; tt < TT; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float p = s[tt][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(s[tt][i] - m_run);
+                const float p = __builtin_amdgcn_exp2f(s[tt][i] - m_run);
                 l_run += p;
                 pf[tt][i] = (_Float16)p;
             }
@@ -359,7 +362,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
         for (int w = 1; w < NW; ++w) m = fmaxf(m, sm[w][r]);
 #pragma unroll
         for (int w = 0; w < NW; ++w) { // sm: the waves' weights
-            const float wgt = sm[w][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(sm[w][r] - m);
+            const float wgt = __builtin_amdgcn_exp2f(sm[w][r] - m);
             l = fmaf(wgt, sl[w][r], l);
             sm[w][r] = wgt;
         }
