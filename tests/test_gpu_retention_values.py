@@ -79,3 +79,19 @@ def test_queries_whose_scores_are_all_minus_infinity(tl, nq):
     for S in (40, 3000):
         q, k, v, _ = hidden_states(64, S, slice(0, S), 3)
         assert not cross(tl, cache_of(tl, k, v, 2), q[:nq], 0.125).any()
+
+
+@pytest.mark.parametrize("at", [0, 77, 199])
+@pytest.mark.parametrize("nq", [1, 30])
+def test_infinite_values(tl, nq, at):
+    """An attended value of infinity makes its dimension infinite and no other one NaN."""
+    rng = np.random.default_rng(5)
+    k, v = (rng.standard_normal((200, 1, 64)).astype(np.float16) for _ in range(2))
+    q = rng.standard_normal((nq, 2, 64)).astype(np.float16)
+    want, mass, _, err = attend(q, k, v, 0.125)
+    v[at, 0, 5], v[at, 0, 9] = np.inf, -np.inf
+    c = cache_of(tl, k, v, 2)
+    for got in [cross(tl, c, q, 0.125)] + ([decode(tl, c, q, 0.125)[0]] if nq == 1 else []):
+        assert (got[..., 5] == np.inf).all() and (got[..., 9] == -np.inf).all()
+        rest = [i for i in range(64) if i not in (5, 9)]
+        check_out(got[..., rest], want[..., rest], mass[..., rest], err, 200)

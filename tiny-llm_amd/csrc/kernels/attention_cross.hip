@@ -184,12 +184,17 @@ attn_cross_kernel(CrossArgs a) {
     }
     const f16x8 ones = __builtin_bit_cast(f16x8, make_uint4(0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u));
 
-    auto tile_step = [&](int kt, const uint16_t *kd, const uint16_t *vd, uint16_t *kn, uint16_t *vn)
+    auto tile_step = [&](int kt, const uint16_t *kd, uint16_t *vd, uint16_t *kn, uint16_t *vn)
                          __attribute__((always_inline)) {
         if (kt + 1 < t_hi) {
             const int now = ids;
             if (PAGED && kt + 2 < t_hi) ids = blocks(kt + 2);
             issue_tile(kt + 1, now, kn, vn);
+        }
+        if ((kt + 1) * kTile > S) { // rows past the end, read as the last one: 0 times its value would be NaN where that is infinite
+            for (int x = (S - kt * kTile) * KP + tid; x < kTile * KP; x += NT)
+                *reinterpret_cast<uint4 *>(&vd[8 * x]) = make_uint4(0u, 0u, 0u, 0u);
+            __syncthreads();
         }
         f32x4 s[NQG][4];
 #pragma unroll

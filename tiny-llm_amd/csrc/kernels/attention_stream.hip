@@ -324,6 +324,11 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
                 l_run += p;
                 pf[tt][i] = (_Float16)p;
             }
+        if (t0 + TK - 1 > last) { // rows past the end, read as the last one: 0 times its value would be NaN where that is infinite
+#pragma unroll
+            for (int u = 0; u < NV; ++u)
+                if (t0 + u * RPI + lane / KP > last) vr[u] = u32x4{0u, 0u, 0u, 0u};
+        }
         // 16 tokens at a time through the stage (a wave's LDS operations keep their order).
 #pragma unroll
         for (int q = 0; q < TT; ++q) {
