@@ -81,6 +81,39 @@ def test_queries_whose_scores_are_all_minus_infinity(tl, nq):
         assert not cross(tl, cache_of(tl, k, v, 2), q[:nq], 0.125).any()
 
 
+def half_step(S, d, seed=4):
+    """Half of the states have weights beside the others' that fp16 does not tell apart,
+    and values of the other sign: what is left of the sum is the difference, which is of
+    the size of a weight's rounding to fp16.  (q, k, v, out, tolerance at a scale of 1)"""
+    rng = np.random.default_rng(seed)
+    k, v = np.zeros((S, 1, d), np.float16), np.ones((S, 1, d), np.float16)
+    heavy = rng.permutation(S)[:S // 2]
+    k[heavy, 0, 0], v[heavy] = 1.5 * 2.0 ** -12, -1.0
+    q = np.zeros((40, 2, d), np.float16)
+    q[..., 0] = 1.0
+    s = 1.5 * 2.0 ** -12
+    n, m = S - S // 2, S // 2
+    out = (n - m * np.exp(s)) / (n + m * np.exp(s))
+    # Scores are one product (4 roundings of 2^-24 with the logarithm's, of s < 2^-11); exp2 and
+    # the division of 2 + 2; a weight in two parts 2^-22, half a step of the second one's 11 bits; sums of S
+    # terms of the same size, pairwise per lane (S / 16 long) and tile; the output's rounding, and the 1e-6 beside
+    # a sum of 2^7 S.
+    tol = 2.0 ** -22 + (4 * s + 4 + S / 16 + 16) * 2.0 ** -24 + 2.0 ** -11 * abs(out) + 2.0 ** -24
+    return q, k, v, out, tol
+
+
+@pytest.mark.parametrize("d,S,block", [(64, 2, 0), (32, 64, 16), (64, 200, 16), (128, 500, 0), (256, 330, 0), (128, 1200, 16)])
+def test_weights_between_two_fp16_numbers(tl, d, S, block):
+    q, k, v, out, tol = half_step(S, d)
+    c = cache_of(tl, k, v, 2, block)
+    assert tol < 2.0 ** -12 / 4  # of what a rounding of the weights to fp16 would be
+    got, acc = decode(tl, c, q[:1], 1.0)
+    assert np.abs(got.astype(np.float64) - out).max() <= tol
+    assert abs(acc.sum(dtype=np.float64) - 2) <= 2 * (S + 20) * 2.0 ** -23
+    for nq in (1, 5, 8):
+        assert np.abs(cross(tl, c, q[:nq], 1.0).astype(np.float64) - out).max() <= tol
+
+
 @pytest.mark.parametrize("at", [0, 77, 199])
 @pytest.mark.parametrize("nq", [1, 30])
 def test_infinite_values(tl, nq, at):

@@ -21,10 +21,12 @@
 //                    8(l/16)..+7) straight from memory, B = Q (row l%16),
 //                    D = S^T (tokens 4(l/16)+i, row l%16)
 //   softmax          per row column in the log2 domain, over a reference point near
-//                    the maximum (kBelow); p is fp16 for the product, a relative
-//                    rounding of 2^-11 per weight, its sum stays fp32
+//                    the maximum (kBelow), in fp32
 //   O^T += V^T P^T   over 16 tokens; V^T from the wave's row-major LDS stage by
-//                    the transposing ds_read_b64_tr_b16
+//                    the transposing ds_read_b64_tr_b16.  A weight takes part as two
+//                    fp16 numbers, its rounding and that of the rest, 2^-22 of it, side
+//                    by side in the instruction's 32 places beside V^T twice, so
+//                    the matrix unit has no more to do than for one of them
 // stream_finish_kernel: merges the outputs of entries with several chunks and turns
 // their scores into the account.
 //
@@ -315,15 +317,6 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
             l_run *= alpha;
             m_run = m_new;
         }
-        f16x4 pf[TT];
-#pragma unroll
-        for (int tt = 0; tt < TT; ++tt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(s[tt][i] - m_run);
-                l_run += p;
-                pf[tt][i] = (_Float16)p;
-            }
         if (t0 + TK - 1 > last) { // rows past the end, read as the last one: 0 times its value would be NaN where that is infinite
 #pragma unroll
             for (int u = 0; u < NV; ++u)
@@ -337,11 +330,24 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
                 const int r = u * RPI + lane / KP;
                 *reinterpret_cast<u32x4 *>(&vst[(r * KP + ((lane % KP) ^ swz(r))) * 8]) = vr[q * NQ + u];
             }
+            f16x8 pf; // p's rounding to fp16, then that of the rest
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(s[q][i] - m_run);
+                l_run += p;
+                pf[i] = (_Float16)p;
+                pf[4 + i] = (_Float16)(p - (float)pf[i]);
+            }
             wave_sync_lds();
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
-                const s16x4 vt = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr(&vst[vlane + ((2 * dt) ^ vxor) * 8]));
-                acc[dt] = __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, vt), pf[q], acc[dt], 0, 0, 0);
+                const f16x4 v = __builtin_bit_cast(
+                    f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_ptr(&vst[vlane + ((2 * dt) ^ vxor) * 8])));
+                // (an infinite value times a rest of 0, or of the other sign, would be NaN)
+                const f16x4 most = {65504.0f16, 65504.0f16, 65504.0f16, 65504.0f16};
+                const f16x4 fin = __builtin_elementwise_max(__builtin_elementwise_min(v, most), -most);
+                acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_shufflevector(v, fin, 0, 1, 2, 3, 4, 5, 6, 7), pf,
+                                                                 acc[dt], 0, 0, 0);
             }
             wave_sync_lds();
         }
