@@ -128,3 +128,39 @@ def test_infinite_values(tl, nq, at):
         assert (got[..., 5] == np.inf).all() and (got[..., 9] == -np.inf).all()
         rest = [i for i in range(64) if i not in (5, 9)]
         check_out(got[..., rest], want[..., rest], mass[..., rest], err, 200)
+
+
+@pytest.mark.parametrize("a,b", [(40.0, 4000.0), (-77.0, 2500.0), (300.0, -515.0), (0.5, 3.0)])
+@pytest.mark.parametrize("pre,new,window,G", [
+    (0, 200, 0, 1), (0, 700, 0, 4),
+    (3000, 3, 1, 2),       # few rows over many keys: their statistics are merged with the sums
+    (5000, 130, 0, 4),     # ... in a launch of their own
+])
+def test_prompt_accounts_of_scores_far_from_zero(tl, pre, new, window, G, a, b):
+    """Equal scores, exact in fp32: every weight is 1 / (keys that its row sees)."""
+    d = 64
+    c = Cache(tl, [0], 1, d, room=pre + new, hq=G)
+
+    def same(n, std=1.0):
+        k = np.zeros((n, 1, d), np.float16)
+        k[..., 7] = a
+        return k
+
+    c.rows = same
+    c.append([pre])
+    q = np.zeros((new, G, d), np.float16)
+    q[..., 7] = b
+    p = tl.PrefillBatch(c.mgr, 1, G)
+    p.prepare(c.ids, [new])
+    dq, dk, w = dev(q), dev(same(new)), c.account()
+    p.append(0, dk.data_ptr(), dk.data_ptr())
+    p.weights(0, dq.data_ptr(), 0.125, window, None, w.data_ptr())
+    torch.cuda.synchronize()
+    S = pre + new
+    weight = G / (1.0 + np.arange(S))
+    weight[:S - (window or new)] = 0  # rows that are not counted
+    want = np.cumsum(weight[::-1])[::-1]
+    got = w.cpu().numpy()[0, 0, :S].astype(np.float64)
+    # exp2 and the multiply-adds of both passes (12 roundings), and fp32 sums of S and of G * new terms; a score
+    # and its reference are one product, whose rounding both have
+    assert np.abs(got / want - 1).max() <= (12 + S + G * new) * 2.0 ** -24

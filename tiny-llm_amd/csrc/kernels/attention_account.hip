@@ -9,8 +9,9 @@
 // exponential rates for many rows, by K's bytes for few.  Scores, sums and
 // weights are fp32 throughout.
 //
-// account_stats_kernel: log2 of every row's sum, lse = m + log2 l, so that a weight is
-// one multiply-add and one exponential, 2^(s * scale * log2(e) - lse).  A workgroup
+// account_stats_kernel: every row's maximum m and the inverse of its sum l, so that a weight
+// is a multiply-add, an exponential and a multiply-add, 2^(s * scale * log2(e) - m) / l.  (In
+// one number, m + log2 l, its rounding would enter the weights, 2^-24 |m| of each.)  A workgroup
 // has 128 rows, 32 per wave in registers, and a chunk of the keys, whose tiles of 64
 // pass through LDS (DMA, two buffers).  S^T = K Q^T on v_mfma_f32_16x16x32_f16 as in
 // the prefill kernel: a lane has 16 keys of its row column per tile, and a running
@@ -57,7 +58,7 @@ struct AccountArgs {
     const __half *q;
     const float  *w_in;
     float        *w_out;
-    float        *lse;   // [lse0 * Hkv + g * rows + r]
+    float        *rows;  // (m, 1 / l) [lse0 * Hkv + g * rows + r]
     float        *stats; // (m, l) [stat0 * Hkv + (chunk * Hkv + g) * rows + r]
     float        *parts; // [part0 * Hkv + (chunk * Hkv + g) * blocks * 256 + t]
     KvView        kv;
@@ -267,18 +268,20 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
         lr += __shfl_xor(lr, 32);
         const int r = r_lo + wave * 32 + j * 16 + c;
         if (qg > 0 || r >= r_hi) continue;
-        if (a.e[ei].nch == 1) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = mr + __builtin_amdgcn_logf(lr);
-        else {
+        if (a.e[ei].nch == 1) {
+            const int64_t at = (int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r;
+            *reinterpret_cast<float2 *>(a.rows + 2 * at) = make_float2(mr, 1.0f / lr);
+        } else {
             const int64_t at = (int64_t)a.e[ei].stat0 * a.Hkv + ((int64_t)ch * a.Hkv + g) * rows + r;
             *reinterpret_cast<float2 *>(a.stats + 2 * at) = make_float2(mr, lr);
         }
     }
 }
 
-// lse of row r from its nch chunks' (m, l), st: those of chunk 0, `step` floats from
+// (m, 1 / l) of row r from its nch chunks' (m, l), st: those of chunk 0, `step` floats from
 // chunk to chunk.  Four lanes a row, 16 apart, take every fourth chunk, so that a
 // load is of 16 neighbouring rows.
-__device__ __forceinline__ float merged_lse(const float *st, int64_t step, int nch) {
+__device__ __forceinline__ float2 merged_row(const float *st, int64_t step, int nch) {
     float m = kNone, l = 0.0f;
 #pragma unroll 4
     for (int ch = (threadIdx.x >> 4) & 3; ch < nch; ch += 4) {
@@ -292,10 +295,10 @@ __device__ __forceinline__ float merged_lse(const float *st, int64_t step, int n
     l *= __builtin_amdgcn_exp2f(m - mx);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    return mx + __builtin_amdgcn_logf(l);
+    return make_float2(mx, 1.0f / l);
 }
 
-// lse of the rows of entries with several chunks of keys, where account_sum_kernel
+// The rows of entries with several chunks of keys, where account_sum_kernel
 // does not merge them itself.
 __global__ __launch_bounds__(kThreads) void account_merge_kernel(AccountArgs a) {
     const int ei = blockIdx.z, g = blockIdx.y;
@@ -304,8 +307,9 @@ __global__ __launch_bounds__(kThreads) void account_merge_kernel(AccountArgs a) 
     const int r0 = blockIdx.x * (kThreads / 4) + (threadIdx.x >> 6) * 16; // the wave's first row
     if (nch == 1 || r0 >= rows) return;
     const float *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows + min(r, rows - 1));
-    const float  lse = merged_lse(st, 2 * (int64_t)a.Hkv * rows, Pieces(a.tiles, a.nt).chunks(ei, r0 / kAccountRows));
-    if ((threadIdx.x & 63) < 16 && r < rows) a.lse[(int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r] = lse;
+    const float2 v = merged_row(st, 2 * (int64_t)a.Hkv * rows, Pieces(a.tiles, a.nt).chunks(ei, r0 / kAccountRows));
+    if ((threadIdx.x & 63) < 16 && r < rows)
+        *reinterpret_cast<float2 *>(a.rows + 2 * ((int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r)) = v;
 }
 
 template <int D, bool PAGED>
@@ -314,7 +318,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     constexpr int NQI = kAccountStep * KP / kThreads; // Q pieces per thread
     constexpr int NRG = kAccountStep / 16;
     __shared__ __align__(16) uint16_t qs0[kAccountStep * D], qs1[kAccountStep * D];
-    __shared__ float s_lse[kAccountFold];
+    __shared__ float2 s_rows[kAccountFold];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int item = blockIdx.x / a.Hkv, g = blockIdx.x - item * a.Hkv;
@@ -333,7 +337,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     const int c = lane & 15, qg = lane >> 4;
     const int wk = k_lo + wave * 64; // the wave's first key
 
-    const float  *lse = a.lse + (int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows;
+    const float2 *row_stats = reinterpret_cast<const float2 *>(a.rows) + (int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows;
     const __half *qbase = a.q + ((int64_t)(a.e[ei].tok0 + n - w) * a.Hq + (g << a.lg)) * D;
     // (a step's rows begin at a whole token: 64 rows hold 64 >> lg tokens)
     uint32_t lane_off[NQI];
@@ -358,19 +362,18 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
         }
     };
     const bool merges = a.fold && a.e[ei].nch > 1; // (the chunk has kAccountFold rows at most)
-    auto load_lse = [&](int r0, float(&x)[NRG]) __attribute__((always_inline)) {
-        if (merges) {
+    auto load_rows = [&](int r0, float2(&x)[NRG]) __attribute__((always_inline)) {
+        const float2 *p = row_stats + r0;
+        const bool    whole = r0 + kAccountStep <= r_hi;
 #pragma unroll
-            for (int rg = 0; rg < NRG; ++rg) x[rg] = r0 + 16 * rg + c < r_hi ? s_lse[min(r0 + 16 * rg + c - r_lo, kAccountFold - 1)] : INFINITY;
-            return;
-        }
-        const float *p = lse + r0;
-        if (r0 + kAccountStep <= r_hi) {
-#pragma unroll
-            for (int rg = 0; rg < NRG; ++rg) x[rg] = p[16 * rg + c];
-        } else {
-#pragma unroll
-            for (int rg = 0; rg < NRG; ++rg) x[rg] = r0 + 16 * rg + c < r_hi ? p[16 * rg + c] : INFINITY; // weights of 0
+        for (int rg = 0; rg < NRG; ++rg) {
+            const int r = 16 * rg + c;
+            if (!merges && whole) {
+                x[rg] = p[r];
+            } else { // rows past the end: weights of 0
+                x[rg] = make_float2(INFINITY, 0.0f);
+                if (r0 + r < r_hi) x[rg] = merges ? float2(s_rows[min(r0 + r - r_lo, kAccountFold - 1)]) : float2(p[r]);
+            }
         }
     };
     if (r_lo < r_hi) issue(r_lo, qs0);
@@ -388,14 +391,14 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
     if (merges) { // while the first rows and the keys are on their way
         const float *st = a.stats + 2 * ((int64_t)a.e[ei].stat0 * a.Hkv + (int64_t)g * rows);
         for (int r0 = r_lo + 16 * wave; r0 < r_hi; r0 += kThreads / 4) {
-            const int   nch = tile_pieces.chunks(ei, r0 / kAccountRows);
-            const float v = merged_lse(st + 2 * (int64_t)min(r0 + c, r_hi - 1), 2 * (int64_t)a.Hkv * rows, nch);
-            if (qg == 0 && r0 + c < r_hi) s_lse[r0 + c - r_lo] = v;
+            const int    nch = tile_pieces.chunks(ei, r0 / kAccountRows);
+            const float2 v = merged_row(st + 2 * (int64_t)min(r0 + c, r_hi - 1), 2 * (int64_t)a.Hkv * rows, nch);
+            if (qg == 0 && r0 + c < r_hi) s_rows[r0 + c - r_lo] = v;
         }
         __syncthreads();
     }
-    float x[NRG];
-    load_lse(r_lo, x);
+    float2 x[NRG];
+    load_rows(r_lo, x);
     __builtin_amdgcn_s_waitcnt(kVmcnt0);
     __syncthreads();
     auto compute = [&](auto diagonal, int r0, const uint16_t *qd) __attribute__((always_inline)) {
@@ -421,17 +424,17 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void account_sum_kernel
             for (int tt = 0; tt < 4; ++tt)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rg & 1][tt][i], a.scale_log2, -x[rg]));
-                    if constexpr (diagonal) acc[tt][i] += wk + 16 * tt + 4 * qg + i <= pos ? p : 0.0f;
-                    else acc[tt][i] += p;
+                    float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rg & 1][tt][i], a.scale_log2, -x[rg].x));
+                    if constexpr (diagonal) p = wk + 16 * tt + 4 * qg + i <= pos ? p : 0.0f;
+                    acc[tt][i] = __builtin_fmaf(p, x[rg].y, acc[tt][i]);
                 }
         }
     };
     auto any_step = [&](int r0, const uint16_t *qd, uint16_t *qn) __attribute__((always_inline)) {
-        float y[NRG];
+        float2 y[NRG];
         if (r0 + kAccountStep < r_hi) {
             issue(r0 + kAccountStep, qn);
-            load_lse(r0 + kAccountStep, y);
+            load_rows(r0 + kAccountStep, y);
         }
         if (wk + 63 <= first + (r0 >> a.lg)) compute(std::false_type(), r0, qd); // every row sees every key
         else if (wk <= first + ((r0 + kAccountStep - 1) >> a.lg)) compute(std::true_type(), r0, qd);
@@ -505,7 +508,7 @@ template <int D> void launch_d(const AccountArgs &a, const AccountLaunch &l, boo
 
 size_t account_workspace_floats(const AccountPlan &plan, int Hkv) {
     int64_t most = 0;
-    for (const auto &l : plan.launches) most = std::max(most, l.lse + 2 * l.stats + l.parts);
+    for (const auto &l : plan.launches) most = std::max(most, 2 * l.lse + 2 * l.stats + l.parts);
     return (size_t)most * (size_t)Hkv;
 }
 
@@ -529,7 +532,7 @@ void launch_account(const AccountCall &c, const KvView &kv, const AccountPlan &p
         a.fold = l.fold;
         a.parts = workspace; // (multiples of 256 first: their stores are of 16 bytes)
         a.stats = a.parts + l.parts * c.Hkv;
-        a.lse = a.stats + 2 * l.stats * c.Hkv;
+        a.rows = a.stats + 2 * l.stats * c.Hkv;
         std::memcpy(a.e, plan.entries.data() + l.first, sizeof(AccountEntry) * (size_t)l.n);
         a.nt = (int)l.tile_pieces.size();
         a.nb = (int)l.block_pieces.size();
