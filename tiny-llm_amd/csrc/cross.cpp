@@ -38,6 +38,7 @@ Result<void> CrossBatch::prepare(const int *seq_ids, const int *num_queries, con
     tokens_ = 0;
     ids_.clear();
     lens_.clear();
+    empty_.clear();
     stream_plan_->clear();
     cross_plan_->clear();
     if (n < 0 || n > max_entries_)
@@ -70,26 +71,29 @@ Result<void> CrossBatch::prepare(const int *seq_ids, const int *num_queries, con
     if (total * group > INT32_MAX / 2) return Result<void>::err("CrossBatch: too many query rows in one step");
     mgr_.syncTable(stream);
     // Neighbours over the same states are one entry of the plans: their rows share
-    // every key.  Up to 16 rows (and entries over nothing) take attn_stream_kernel,
-    // which reads the states once at the memory's rate; more take attn_cross_kernel.
+    // every key.  Up to 16 rows take attn_stream_kernel, which reads the states once at
+    // the memory's rate; more take attn_cross_kernel; queries over nothing get zeros.
     int64_t tok = 0;
     for (int i = 0; i < n;) {
         const int slot = mgr_.slotOf(seq_ids[i]);
         const int len = lens[static_cast<size_t>(i)];
+        const int first = static_cast<int>(tok);
         int       nq = 0;
         for (const int id = seq_ids[i]; i < n && seq_ids[i] == id && lens[static_cast<size_t>(i)] == len; ++i)
             nq += num_queries[i];
-        if (len > 0 && nq * static_cast<int64_t>(group) > detail::kStreamRows) {
-            cross_plan_->entries.push_back({slot, len, static_cast<int32_t>(tok), nq, 1, 0});
-        } else {
-            const int step = detail::kStreamRows / group;
-            for (int t = 0; t < nq; t += step)
-                stream_plan_->entries.push_back({slot, len, static_cast<int32_t>(tok + t), std::min(step, nq - t), 0, 0});
-        }
         tok += nq;
+        if (len > 0) {
+            if (nq * static_cast<int64_t>(group) > detail::kStreamRows) cross_plan_->entries.push_back({slot, len, first, nq, 1, 0});
+            else stream_plan_->entries.push_back({slot, len, first, nq, 0, 0});
+        } else if (!empty_.empty() && empty_.back().first + empty_.back().second == first) {
+            empty_.back().second += nq;
+        } else {
+            empty_.push_back({first, nq});
+        }
     }
     detail::plan_stream(*stream_plan_, cfg.num_heads, cfg.head_dim, 0, detail::device_cus());
     if (!detail::plan_cross(*cross_plan_, cfg.head_dim, group, cfg.num_heads, detail::device_cus())) {
+        empty_.clear();
         stream_plan_->clear();
         cross_plan_->clear();
         return Result<void>::err("CrossBatch: too many query rows in one step");
@@ -126,6 +130,7 @@ Result<void> CrossBatch::attention(int layer_idx, const half *q, half *out, floa
                                  "of this size before");
     float               *ws = work_->get(floats);
     const detail::KvView view = mgr_.layerView(layer_idx, nullptr);
+    detail::launch_cross_zeros(out, num_q_heads_ * cfg.head_dim, empty_, stream);
     if (!stream_plan_->entries.empty()) {
         detail::StreamCall c;
         c.q = q;

@@ -373,6 +373,22 @@ template <int ROWS> __global__ __launch_bounds__(kMergeThreads) void cross_merge
     *reinterpret_cast<uint2 *>(a.out + ((int64_t)(a.e[ei].tok0 + (r >> a.lg)) * a.Hq + (g << a.lg) + (r & ((1 << a.lg) - 1))) * D + d) = w;
 }
 
+constexpr int kZeroRanges = 256, kZeroThreads = 256;
+struct ZeroArgs {
+    __half *out;
+    int     row, n;
+    int2    range[kZeroRanges]; // first token, tokens
+};
+
+// Workgroups (x, range): 16 bytes a lane and step.
+__global__ __launch_bounds__(kZeroThreads) void cross_zero_kernel(ZeroArgs a) {
+    const int2    r = a.range[blockIdx.y];
+    const int64_t pieces = (int64_t)r.y * a.row / 8;
+    uint4        *out = reinterpret_cast<uint4 *>(a.out + (int64_t)r.x * a.row);
+    for (int64_t i = (int64_t)blockIdx.x * kZeroThreads + threadIdx.x; i < pieces; i += (int64_t)gridDim.x * kZeroThreads)
+        out[i] = make_uint4(0u, 0u, 0u, 0u);
+}
+
 template <int D, int NW> void launch_dw(const CrossArgs &a, int items, bool paged, hipStream_t stream) {
     const dim3 grid((unsigned)items * (unsigned)a.Hkv), block(NW * 64);
     if (paged) hipLaunchKernelGGL((attn_cross_kernel<D, true, NW>), grid, block, 0, stream, a);
@@ -444,6 +460,25 @@ void launch_attn_cross(const CrossCall &c, const KvView &kv, const CrossPlan &pl
             }
             HIP_CHECK(hipGetLastError());
         }
+        profile_end(KernelId::AttnCross, stream);
+    }
+}
+
+void launch_cross_zeros(__half *out, int row, const std::vector<std::pair<int32_t, int32_t>> &ranges, hipStream_t stream) {
+    ZeroArgs a;
+    a.out = out;
+    a.row = row;
+    for (size_t i = 0; i < ranges.size();) {
+        int32_t most = 0;
+        for (a.n = 0; i < ranges.size() && a.n < kZeroRanges; ++i, ++a.n) {
+            a.range[a.n] = make_int2(ranges[i].first, ranges[i].second);
+            most = std::max(most, ranges[i].second);
+        }
+        const int64_t blocks = ((int64_t)most * row / 8 + 4 * kZeroThreads - 1) / (4 * kZeroThreads);
+        profile_begin(KernelId::AttnCross, stream);
+        hipLaunchKernelGGL(cross_zero_kernel, dim3((unsigned)std::min<int64_t>(blocks, 4096), (unsigned)a.n), dim3(kZeroThreads),
+                           0, stream, a);
+        HIP_CHECK(hipGetLastError());
         profile_end(KernelId::AttnCross, stream);
     }
 }

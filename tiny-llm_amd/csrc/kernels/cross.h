@@ -6,6 +6,8 @@
 
 #include <cstddef>
 #include <cstdint>
+#include <utility>
+#include <vector>
 
 namespace tiny_llm {
 namespace detail {
@@ -22,6 +24,10 @@ size_t cross_workspace_floats(const CrossPlan &plan, int Hkv, int D);
 
 void launch_attn_cross(const CrossCall &c, const KvView &kv, const CrossPlan &plan, float *workspace,
                        hipStream_t stream);
+
+// Rows of zeros for queries over no states: tokens first .. first + second - 1 of `out`
+// ([token][row] halves, row a multiple of 8) for every range.
+void launch_cross_zeros(__half *out, int row, const std::vector<std::pair<int32_t, int32_t>> &ranges, hipStream_t stream);
 
 } // namespace detail
 } // namespace tiny_llm

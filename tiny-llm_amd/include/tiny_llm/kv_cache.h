@@ -437,7 +437,8 @@ class CrossBatch {
     int                  tokens_ = 0;
     std::vector<int>     ids_;
     std::vector<int32_t> lens_;
-    std::unique_ptr<detail::StreamPlan> stream_plan_; // entries of few rows, or over no states
+    std::vector<std::pair<int32_t, int32_t>> empty_;  // tokens (first, count) over no states
+    std::unique_ptr<detail::StreamPlan> stream_plan_; // entries of few rows
     std::unique_ptr<detail::CrossPlan>  cross_plan_;  // the others
     std::unique_ptr<detail::Workspace>  work_;
 };
