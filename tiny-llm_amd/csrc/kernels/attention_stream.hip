@@ -75,7 +75,7 @@ struct StreamArgs {
     float        *w_out;
     float        *part_o;  // [item][Hkv][16 rows at most][D]
     float        *part_ml; // [item][Hkv][rows][2]
-    float        *scores;  // [tile0 * Hkv + g * tiles + tile][rows][64]
+    float        *scores;  // [tile0 * Hkv + g * tiles + tile][rows][64], tile0 counted over entries of several chunks
     KvView        kv;
     int64_t       room;
     int           fresh;
@@ -508,6 +508,16 @@ int plan_rows(const StreamPlan &plan, int first, int n, int G) {
     return nq * G;
 }
 
+// Tiles whose scores go through memory: those of entries of several chunks.
+int64_t stored_tiles(const StreamPlan &plan, const StreamLaunch &l) {
+    int64_t tiles = 0;
+    for (int i = l.first; i < l.first + l.n; ++i) {
+        const StreamEntry &e = plan.entries[(size_t)i];
+        if (stream_items(e.S, plan.chunk) > 1) tiles += stream_tiles(e.S);
+    }
+    return tiles;
+}
+
 } // namespace
 
 size_t stream_workspace_floats(const StreamPlan &plan, int Hq, int Hkv, int D, bool account) {
@@ -515,7 +525,7 @@ size_t stream_workspace_floats(const StreamPlan &plan, int Hq, int Hkv, int D, b
     for (const auto &l : plan.launches) {
         const size_t rows = (size_t)plan_rows(plan, l.first, l.n, Hq / Hkv) * Hkv;
         size_t       f = part_ml_floats((size_t)l.items * rows) + (size_t)l.items * rows * (size_t)D;
-        if (account) f += (size_t)l.tiles * kStreamTile * rows;
+        if (account) f += (size_t)stored_tiles(plan, l) * kStreamTile * rows;
         most = std::max(most, f);
     }
     return most;
@@ -546,8 +556,14 @@ void launch_attn_stream(const StreamCall &c, const KvView &kv, const StreamPlan 
         if (a.rows > kStreamRows) throw std::invalid_argument("attention: too many query rows per entry");
         if ((int64_t)l.items * c.Hkv > INT32_MAX) throw std::invalid_argument("attention: too many work items");
         std::memcpy(a.e, plan.entries.data() + l.first, sizeof(StreamEntry) * (size_t)l.n);
+        int64_t tiles = 0; // (as stored_tiles)
+        for (int i = 0; c.w_out && i < l.n; ++i) {
+            if (stream_items(a.e[i].S, plan.chunk) <= 1) continue;
+            a.e[i].tile0 = (int32_t)tiles;
+            tiles += stream_tiles(a.e[i].S);
+        }
         a.scores = workspace;
-        a.part_ml = workspace + (c.w_out ? (size_t)l.tiles * kStreamTile * a.rows * c.Hkv : 0);
+        a.part_ml = workspace + (size_t)tiles * kStreamTile * a.rows * c.Hkv;
         a.part_o = a.part_ml + part_ml_floats((size_t)l.items * c.Hkv * a.rows);
         profile_begin(KernelId::AttnStream, stream);
         if (l.items > 0) {

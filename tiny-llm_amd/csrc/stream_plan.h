@@ -16,7 +16,7 @@ constexpr int kStreamBatch = 144;  // entries per launch: they travel in the ker
 
 // Query tokens tok0 .. tok0 + nq - 1 attend to the first S tokens of cache row
 // `row`.  item0, tile0: work items and tiles of the entries before it in its
-// launch.
+// launch (in the kernels' arguments tile0 counts entries of several chunks only).
 struct StreamEntry {
     int32_t row, S, tok0, nq, item0, tile0;
 };
