@@ -89,7 +89,7 @@ template <int S> __device__ __forceinline__ float xor_lane_max(float x) {
 template <int D, bool PAGED, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void
 attn_cross_kernel(CrossArgs a) {
-    static_assert(NW == 4 || (NW == 8 && D <= 128), "waves");
+    static_assert(NW == 4 || (NW == 8 && cross_wide(D)), "waves");
     constexpr int NQG = D <= 128 ? 2 : 1; // 16-row groups per wave
     constexpr int NT = NW * 64;
     constexpr int R = 16 * NQG;           // rows of a wave
@@ -395,7 +395,7 @@ template <int D, int NW> void launch_dw(const CrossArgs &a, int items, bool page
     else hipLaunchKernelGGL((attn_cross_kernel<D, false, NW>), grid, block, 0, stream, a);
 }
 template <int D> void launch_d(const CrossArgs &a, int items, bool paged, int waves, hipStream_t stream) {
-    if constexpr (D <= 128) {
+    if constexpr (cross_wide(D)) {
         if (waves == 8) {
             launch_dw<D, 8>(a, items, paged, stream);
             return;

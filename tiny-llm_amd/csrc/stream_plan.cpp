@@ -184,7 +184,7 @@ bool plan_cross(CrossPlan &plan, int D, int G, int Hkv, int cus) {
         rows += (int64_t)e.nq * G;
         large += ((int64_t)e.nq * G + cross_rows(D, 8) - 1) / cross_rows(D, 8);
     }
-    const bool wide = D <= 128 && D != 64 && !plan.entries.empty() && rows >= 256 * (int64_t)plan.entries.size() &&
+    const bool wide = cross_wide(D) && !plan.entries.empty() && rows >= 256 * (int64_t)plan.entries.size() &&
                       (large * Hkv < n || large * Hkv >= 2 * n);
     plan.waves = wide ? 8 : 4;
     const int tile = cross_rows(D, plan.waves);

@@ -128,6 +128,8 @@ struct CrossPlan {
     int                      waves = 4; // per workgroup
     void                     clear() { entries.clear(), launches.clear(); }
 };
+// Whether 8 waves are an option (64: level with 4).
+constexpr bool cross_wide(int D) { return D == 32 || D == 128; }
 // Rows of a workgroup: 32 per wave up to head_dim 128, 16 at 256.
 constexpr int cross_rows(int D, int waves) { return waves * (D <= 128 ? 32 : 16); }
 
