@@ -180,8 +180,10 @@ int tl_kv_batch_decode(tl_kv_batch *batch, int layer, const void *q, const void 
  * for every attended token t of the batch's sequences; the token that this step
  * appends (the last one after prepare) starts from zero, and all else of
  * weights_out stays as it is.  fp32 [max_batch_size][num_heads][max_seq_len], by
- * slot (tl_kv_slot_of) and cache index, the caller's, one per layer; weights_out
- * may be weights_in and must not overlap it otherwise.  q, out, new_k and new_v
+ * slot (tl_kv_slot_of) and cache index, the caller's, one per layer; a token that
+ * neither this nor tl_kv_prefill_weights counted when it came has no account, so
+ * memory that is given such tokens begins as zeros; weights_out may be weights_in
+ * and must not overlap it otherwise.  q, out, new_k and new_v
  * 16-byte aligned.  K and V are read once.  The outputs follow the same formula
  * as tl_kv_batch_decode, not its bits.  The scores pass through a workspace of the
  * batch, which the first call of a size allocates: one such call before a
@@ -339,8 +341,8 @@ int  tl_kv_prefill_weights(tl_kv_prefill *p, int layer, const void *q, float sca
  *            weights and positions: [max_batch_size][num_heads][max_seq_len]
  *            fp32 / int32, by slot (tl_kv_slot_of) and cache index, the caller's,
  *            one pair per layer.  Written are the first min(length, budget) of
- *            each kv head; outputs may be the inputs, and must not overlap
- *            them otherwise.  positions_in is read only below the length that
+ *            each kv head (in place, those that change); outputs may be the
+ *            inputs, and must not overlap them otherwise.  positions_in is read only below the length that
  *            the sequence's last eviction left (the tokens after that came in
  *            order), so it needs no initial value.  A layer that ran in place is
  *            not run again before commit.  A run moves rows of the cache (a captured
@@ -373,8 +375,9 @@ int tl_kv_evicted(const tl_kv_manager *mgr, int seq_id);
 /* ------------------------------------------------------------------------
  * Attention to cached states of another sequence (build addition: the reference
  * is decoder-only): query tokens over an encoder's states, or over a document that
- * several sequences share.  The states are a sequence of the manager like any
- * other, appended once (tl_kv_append or tl_kv_prefill_append, then
+ * several sequences share, and over those states alone: no sums of weights come out
+ * by which the outputs could be joined with a sequence's attention to its own cache.
+ * The states are a sequence of the manager like any other, appended once (tl_kv_append or tl_kv_prefill_append, then
  * tl_kv_advance).
  *   prepare:   entry i has num_queries[i] >= 1 query tokens, every one of which
  *              attends to the first attended[i] tokens of seq_ids[i] (0 <=

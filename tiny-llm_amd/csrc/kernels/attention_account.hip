@@ -26,10 +26,11 @@
 // order.
 //
 // Measured, 8 kv heads of 128, group 4: 4 x 1700..2048 new tokens on prefixes to 600,
-// 124 us for the statistics (matrix unit busy 28% of the cycles, VALU 46%) and 114 for
-// the sums (31%, 28%), no bank conflicts: the phases of a step follow each other, and
+// 125 us for the statistics (matrix unit busy 28% of the cycles, VALU 45%) and 119 for
+// the sums (30%, 26%), no bank conflicts: the phases of a step follow each other, and
 // the registers leave room for two to four waves a SIMD to fill the gaps.  The last 32
-// tokens of 8192: 9 + 14 us, two launches' latency and K's 17 MB each.
+// tokens of 8192: 9 + 14 us, two launches' latency and K's 17 MB each.  (A row in one
+// number: 217 and 22.0 us the two calls, in two 220 and 22.3.)
 #include "account.h"
 
 #include "tiny_llm/hip_utils.h"

@@ -9,10 +9,15 @@
 // double-buffered LDS by the LDS DMA load, in XOR-swizzled 16-byte slots;
 //   S^T = K Q^T      v_mfma_f32_16x16x32_f16: A = K rows, B = Q
 //   online softmax   per query column, over a reference point 2^7 below the maximum,
-//                    which moves on jumps above 2^15 only; p rounded to fp16 for the product, the normaliser sums
-//                    the rounded ones (on the matrix unit, a row of ones)
+//                    which moves on jumps above 2^15 only; p rounded to fp16 for the
+//                    product, the normaliser sums the rounded ones (on the matrix
+//                    unit, a row of ones)
 //   O^T += V^T P^T   V^T by the transposing ds_read_b64_tr_b16, P^T as the S^T
 //                    fragments stand
+// The rounding of p, 2^-11 of a weight, is of the size of the output's own (2.9e-4 from
+// 64 bits in the 2-norm, 2.1e-4 for fp32 weights).  As two fp16 numbers, as in
+// attn_stream_kernel, p costs a second product where the matrix unit is the bound: 2 x 2048
+// queries over 8192 670 us against 480, ragged prompts 39 against 30, so it has one.
 // Row tiles that do not fill the chip have their keys split into chunks, whose
 // (m, l, o) go through a workspace in fp32 to cross_merge_kernel.  Grid: kv head
 // fastest, so that with 8 kv heads an XCD's workgroups share one head's keys in
@@ -21,7 +26,7 @@
 // Measured: 2 x 2048 queries over 8192 states, 8 heads of 128, group 4: 492 us = 1.12
 // PFLOP/s (an 8192^3 fp16 matrix product 1.2-1.34), matrix unit busy 47% of the
 // cycles, VALU 21%; 16 x 64..448 over 300..1500, 16 heads of 64: 28 us; 8 over 32768, a
-// quarter of a tile's rows in use: 29 us for the 134 MB of states, + 7 for the merge.
+// quarter of a tile's rows in use: 30 us for the 134 MB of states, + 7 for the merge.
 #include "cross.h"
 
 #include "tiny_llm/hip_utils.h"

@@ -31,10 +31,12 @@
 // their scores into the account.
 //
 // Measured, with accounts, 8 kv heads of 128: 64 x 8192 tokens, group 4, whole
-// entries: 360 us, 6.0 TB/s of K and V (without accounts the decode kernel takes 309 on
-// the same cache); 96 lognormal lengths to 16384 on blocks, group 8: 264 + 20 us for
-// the finish (27 with a row's scores on their way at a time, 30 with all eight); 4 x 128..512 tokens, 8 heads of 64: 7.4 us, one launch's latency.  Two or
-// three steps of rows on their way in registers were level or slower (occupancy).
+// entries: 361 us, 6.0 TB/s of K and V (without accounts the decode kernel takes 309 on
+// the same cache); 96 lognormal lengths to 16384 on blocks, group 8: 272 + 20 us for
+// the finish (27 with a row's scores on their way at a time, 30 with all eight);
+// 4 x 128..512 tokens, 8 heads of 64: 7.7 us, one launch's latency (with the weights in one
+// part 7.4, the others level).  Two or three steps of rows on their way in registers
+// were level or slower (occupancy).
 #include "stream.h"
 
 #include "../runtime.h"

@@ -19,6 +19,9 @@
 // evict_move_kernel: the K and V rows of the pairs, 16 bytes a lane, every row on
 // its way before the first is written: 8 x 8192 tokens to 2048 (8 heads of 128,
 // 100 MB read and written) 17 us.
+// evict_select_any_kernel: more than 32768 tokens, the limit of the registers; a
+// (sequence, kv head)'s one workgroup reads its accounts anew in every pass, so it is slow:
+// 131072 tokens to 16384, 8 heads of 128, 393 us with the moves.
 // evict_one_kernel: sequences that lose one token, in one launch: 16 x 32 heads of
 // 1025 tokens 25.5 -> 6.4 us against the two launches above.
 #include "evict.h"

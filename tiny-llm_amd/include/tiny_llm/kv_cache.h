@@ -191,8 +191,9 @@ class DecodeBatch {
     // cached tokens' attention weights: weights_out[slot][kv head][t] = the running
     // sum weights_in[..][t] (null: zeros) + the step's softmax weights of token t,
     // summed over the query heads of the kv head, for the attended tokens; a token
-    // that this step appends starts from zero.  fp32 [max_batch_size][num_heads]
-    // [max_seq_len], weights_out may be weights_in.  What EvictBatch chooses by.
+    // that this step appends starts from zero (one that came without this call or
+    // PrefillBatch::weights: from what weights_in holds, so such memory begins as zeros).  fp32 [max_batch_size]
+    // [num_heads][max_seq_len], weights_out may be weights_in.  What EvictBatch chooses by.
     Result<void> decodeWeights(int layer_idx, const half *q, const half *new_k, const half *new_v, half *out,
                                float scale, const float *weights_in, float *weights_out, hipStream_t stream);
     Result<void> gather(int layer_idx, half *k_out, half *v_out, int s_max, hipStream_t stream);
@@ -354,7 +355,7 @@ class PrefillBatch {
 // [max_batch_size][num_heads][max_seq_len] by slot (slotOf) and cache index.  A
 // position is read only below the length that the sequence's last eviction left
 // (tokens after that came in order), so the memory needs no initial value.
-// run() writes the first min(length, budget) of both, and may work in place; an
+// run() writes the first min(length, budget) of both (in place: those that change); an
 // output that is not its input must not overlap it.  A layer that ran in place
 // is not run again before commit().
 //
@@ -404,7 +405,8 @@ class EvictBatch {
 
 // Attention of query tokens to cached states that are not their own sequence's --
 // an encoder's states, a document that several sequences share -- of any length
-// beside the queries': every query of an entry attends to all of the states.
+// beside the queries': every query of an entry attends to all of the states, and to
+// them alone (no sums come out by which to join it with attention to its own cache).
 // The states are a sequence of `mgr` like any other, appended once (appendKV or
 // PrefillBatch::append, then advanceSeqLen); several entries may name the same
 // one.  prepare() snapshots a step, attention() runs a layer of it.  The calls of one
