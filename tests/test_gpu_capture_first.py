@@ -1,5 +1,6 @@
 """GPU: a captured call whose kernels have not run before, where the workspace is large
 enough from other calls of the batch."""
+import numpy as np
 import pytest
 import torch
 

@@ -164,3 +164,27 @@ def test_prompt_accounts_of_scores_far_from_zero(tl, pre, new, window, G, a, b):
     # exp2 and the multiply-adds of both passes (12 roundings), and fp32 sums of S and of G * new terms; a score
     # and its reference are one product, whose rounding both have
     assert np.abs(got / want - 1).max() <= (12 + S + G * new) * 2.0 ** -24
+
+
+@pytest.mark.parametrize("pre,new,window,hidden", [(70, 300, 0, slice(64, 256)), (3000, 4, 0, slice(10, 2990)), (500, 200, 30, slice(1, 690))])
+def test_scores_of_minus_infinity_in_a_prompt_account(tl, pre, new, window, hidden):
+    q, k, v, seen = hidden_states(64, pre + new, hidden, 6)
+    q = np.random.default_rng(7).standard_normal((new, 2, 64)).astype(np.float16)
+    q[..., 3] = np.abs(q[..., 3]) + np.float16(0.1)
+    c = Cache(tl, [0], 1, 64, room=pre + new, hq=2)
+    parts = iter([k[:pre], v[:pre]])
+    c.rows = lambda n, std=1.0: next(parts)
+    c.append([pre])
+    p = tl.PrefillBatch(c.mgr, 1, 2)
+    p.prepare(c.ids, [new])
+    dq, dk, w = dev(q), dev(k[pre:]), c.account()
+    p.append(0, dk.data_ptr(), dk.data_ptr())
+    p.weights(0, dq.data_ptr(), 0.125, window, None, w.data_ptr())
+    torch.cuda.synchronize()
+    n = window or new
+    positions = np.arange(pre + new - n, pre + new)
+    last = np.searchsorted(seen, positions, side="right") - 1  # among the keys that have weights
+    _, _, weights, err = attend(q[new - n:], k[seen], k[seen], 0.125, last)
+    got = w.cpu().numpy()[0, :, :pre + new]
+    check_account(got[:, seen], weights.reshape(1, 2 * n, len(seen)).sum(axis=1), weights, err, 2 * n, len(seen))
+    assert not np.delete(got, seen, axis=1).any()
