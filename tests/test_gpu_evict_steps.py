@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from retention_ref import Cache, dev, evict
-from test_gpu_evict import step, weights
+from test_gpu_evict import weights
 
 pytestmark = pytest.mark.gpu
 

@@ -188,3 +188,33 @@ def test_scores_of_minus_infinity_in_a_prompt_account(tl, pre, new, window, hidd
     got = w.cpu().numpy()[0, :, :pre + new]
     check_account(got[:, seen], weights.reshape(1, 2 * n, len(seen)).sum(axis=1), weights, err, 2 * n, len(seen))
     assert not np.delete(got, seen, axis=1).any()
+
+
+@pytest.mark.parametrize("S", [40, 3000])
+def test_a_query_without_finite_scores_counts_nothing(tl, S):
+    """Zeros for an output, and the account as the other heads' queries leave it."""
+    rng = np.random.default_rng(8)
+    k, v = (rng.standard_normal((S, 1, 64)).astype(np.float16) for _ in range(2))
+    k[:, 0, 3] = -np.inf
+    q = rng.standard_normal((1, 2, 64)).astype(np.float16)
+    q[0, :, 3] = [1.0, 0.5]
+    c = cache_of(tl, k, v, 2)
+    got, acc = decode(tl, c, q, 0.125)
+    assert not got.any() and not acc.any()
+    # a prompt's first rows see hidden keys only, the others also the last ones
+    new = S // 2
+    k[new:, 0, 3] = 0.0
+    c = Cache(tl, [0], 1, 64, room=S, hq=2)
+    p = tl.PrefillBatch(c.mgr, 1, 2)
+    p.prepare(c.ids, [S])
+    qs = rng.standard_normal((S, 2, 64)).astype(np.float16)
+    qs[..., 3] = 1.0
+    dq, dk, w = dev(qs), dev(k), c.account()
+    p.append(0, dk.data_ptr(), dk.data_ptr())
+    p.weights(0, dq.data_ptr(), 0.125, 0, None, w.data_ptr())
+    torch.cuda.synchronize()
+    rows = np.arange(new, S)
+    _, _, weights, err = attend(qs[new:], k[new:], k[new:], 0.125, rows - new)
+    got = w.cpu().numpy()[0, :, :S]
+    check_account(got[:, new:], weights.reshape(1, 2 * len(rows), S - new).sum(axis=1), weights, err, 2 * len(rows), S - new)
+    assert not got[:, :new].any()

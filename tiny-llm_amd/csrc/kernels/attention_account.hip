@@ -119,6 +119,9 @@ template <int KP> __device__ __forceinline__ int swz(int r) {
     return f & (KP - 1);
 }
 
+// Of a row's sum of weights; a row without any (its scores are all -infinite) counts nothing.
+__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
 __device__ __forceinline__ int account_blocks_dev(int keys) { return (keys + kAccountKeys - 1) / kAccountKeys; }
 
 __device__ __forceinline__ void lds_dma(const void *src, uint16_t *dst) {
@@ -271,7 +274,7 @@ __global__ __launch_bounds__(kThreads, 2) void account_stats_kernel(AccountArgs 
         if (qg > 0 || r >= r_hi) continue;
         if (a.e[ei].nch == 1) {
             const int64_t at = (int64_t)a.e[ei].lse0 * a.Hkv + (int64_t)g * rows + r;
-            *reinterpret_cast<float2 *>(a.rows + 2 * at) = make_float2(mr, 1.0f / lr);
+            *reinterpret_cast<float2 *>(a.rows + 2 * at) = make_float2(mr, inverse(lr));
         } else {
             const int64_t at = (int64_t)a.e[ei].stat0 * a.Hkv + ((int64_t)ch * a.Hkv + g) * rows + r;
             *reinterpret_cast<float2 *>(a.stats + 2 * at) = make_float2(mr, lr);
@@ -296,7 +299,7 @@ __device__ __forceinline__ float2 merged_row(const float *st, int64_t step, int 
     l *= __builtin_amdgcn_exp2f(m - mx);
     l += __shfl_xor(l, 16);
     l += __shfl_xor(l, 32);
-    return make_float2(mx, 1.0f / l);
+    return make_float2(mx, inverse(l));
 }
 
 // The rows of entries with several chunks of keys, where account_sum_kernel

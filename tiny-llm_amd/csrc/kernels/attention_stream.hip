@@ -109,6 +109,9 @@ __device__ __forceinline__ void wave_sync_lds() {
         out = __builtin_amdgcn_readfirstlane(seen_ - 1);                                                               \
     } while (0)
 
+// Of a row's sum of weights; a row without any (its scores are all -infinite) counts nothing.
+__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
+
 // Four consecutive fp32 values; the rows of accounts begin at any multiple of 4 bytes.
 struct __attribute__((packed, aligned(4))) Four {
     float x[4];
@@ -381,7 +384,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_stream_kernel(
         }
         s_m[r] = m;
         s_l[r] = l;
-        s_inv[r] = 1.0f / l;
+        s_inv[r] = inverse(l);
         if (nch > 1)
             *reinterpret_cast<float2 *>(a.part_ml + (((int64_t)item * a.Hkv + g) * a.rows + r) * 2) = make_float2(m, l);
     }
@@ -440,7 +443,7 @@ __global__ __launch_bounds__(kFinishThreads) void stream_finish_kernel(StreamArg
         if (lane == 0) {
             s_m[r] = mx;
             s_l[r] = l;
-            s_inv[r] = 1.0f / l;
+            s_inv[r] = inverse(l);
         }
     }
     __syncthreads();
