@@ -429,8 +429,8 @@ def _held64(x, c):
     whole = x.shape[0] // _GROUP
     for h in range(c["hkv"] if whole else 0):
         body = x[:whole * _GROUP, h].reshape(whole, -1)
-        m, e = torch.frexp(body.abs().max(dim=1).values / 127)
-        step = torch.ldexp(torch.floor(m * 2048), e.to(torch.int32) - 11)
+        step = body.abs().max(dim=1).values / torch.tensor([127.0], dtype=torch.float64, device="cuda")
+        step = (step.view(torch.int64) >> 42 << 42).view(torch.float64)  # 11 significant bits
         near = torch.round(body / torch.where(step > 0, step, 1.0)[:, None]) * step[:, None]
         x[:whole * _GROUP, h] = near.view(-1, c["d"])
     return x
