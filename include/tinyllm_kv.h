@@ -115,6 +115,30 @@ int tl_kv_set_block_map(tl_kv_manager *mgr, int block_tokens, const int32_t *per
  * tl_kv_block_bytes.  tl_kv_get_cache fails (no contiguous region). */
 int tl_kv_create_paged(const tl_kv_config *cfg, int block_tokens, int num_blocks,
                        tl_kv_manager **out);
+/* Block pool in 8 bits (build addition: the reference's cache is fp16).  Groups of 32
+ * consecutive tokens of a kv head (from multiples of 32 on) have one scale for K and
+ * one for V:
+ *   scale = (largest magnitude / 127) cut down to 11 significant bits,
+ *   x is held as round_half_even(x / scale), -127 .. 127, and stands for that times scale;
+ * a group that has an infinity or a NaN stands for NaN.  A sequence's last, incomplete
+ * group stays in fp16 as given until the append of its 32nd token, so every value is
+ * rounded once, and the cached bytes do not depend on how the tokens came.
+ * block_tokens: a power of two >= 32; head_dim 32, 64, 128 or 256.  Memory per block is
+ * tl_kv_block_bytes (8-bit values and scales); beside the pool max_batch_size slots
+ * hold two open groups each.
+ *   tl_kv_append, tl_kv_batch_{append,attention,decode,gather} and
+ * tl_kv_prefill_{append,attention,run} take such a manager as any other, with 16-byte
+ * aligned buffers: they attend to, and read back, what the cache stands for after the
+ * append.  tl_kv_batch_prepare_lengths: at most the tokens held (appended ones
+ * included).  tl_kv_batch_project, accounts, tl_kv_evict_* and tl_kv_cross_* refuse it.
+ *   An append replaces what was appended behind the length before.  A batch's calls
+ * refuse when the length of one of its sequences changed since its prepare.  tl_kv_advance over
+ * less than was appended (drafted tokens that were rejected) may end at a multiple of
+ * 32, in the group in which the append began or in the one in which it ended; elsewhere it
+ * is refused, the rows of that group being gone.  The first call of a size allocates the
+ * workspace: make one before a captured one; one batch is used from one stream at a time. */
+int tl_kv_create_quantized(const tl_kv_config *cfg, int block_tokens, int num_blocks, tl_kv_manager **out);
+int tl_kv_is_quantized(const tl_kv_manager *mgr);
 /* Blocks in the pool / free now (0 for other pools). */
 int    tl_kv_num_blocks(const tl_kv_manager *mgr);
 int    tl_kv_free_blocks(const tl_kv_manager *mgr);
@@ -399,6 +423,33 @@ int  tl_kv_cross_prepare(tl_kv_cross *c, const int *seq_ids, const int *num_quer
 int  tl_kv_cross_info(const tl_kv_cross *c, int *n, int *tokens);
 int  tl_kv_cross_attention(tl_kv_cross *c, int layer, const void *q, void *out, float scale, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Norms of query and key heads and their rotation by position, in one pass (build
+ * addition: rope_theta and rms_norm_eps are ModelConfig's, include/tiny_llm/types.h; a
+ * cached key holds its rotary phase).  For every token t and head of q, and of k:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight   over head_dim; weight NULL: y = x
+ *   (a, b) -> (a cos - b sin, a sin + b cos)  for pair i of the first rotary_dim dims,
+ *             by the angle positions[axis_of[i]][t] * inv_freq[i]
+ * in fp32, rounded to fp16 once; angles are reduced in 64 bits.
+ *   create: head_dim in {32, 64, 128, 256}; rotary_dim a multiple of 16, at most
+ *           head_dim; pair i is dims (i, i + rotary_dim/2), or (2i, 2i+1) when
+ *           interleaved; inv_freq (host, rotary_dim/2 values) NULL: theta^(-2i/rotary_dim);
+ *           axis_of (host, rotary_dim/2 values of 0..7) NULL: all 0.  Images and video have
+ *           an axis each for time, height and width.  The handle holds no device memory.
+ *   apply:  q has rows of num_q_heads*head_dim fp16, q_stride elements from token to token
+ *           (a multiple of 8: rows of a fused projection), k likewise; q_out and k_out
+ *           [num_tokens][heads][head_dim]; positions int32 [axes][num_tokens] on the
+ *           device; weights fp16 [head_dim].  k and k_out NULL: queries alone.  An output may be
+ *           its own dense input and must not overlap inputs otherwise.  All but positions
+ *           16-byte aligned. */
+typedef struct tl_rotary tl_rotary;
+int  tl_rotary_create(int head_dim, int rotary_dim, double theta, int interleaved, const int *axis_of,
+                      const double *inv_freq, tl_rotary **out);
+void tl_rotary_destroy(tl_rotary *r);
+int  tl_rotary_apply(const tl_rotary *r, const void *q, int64_t q_stride, const void *k, int64_t k_stride, void *q_out,
+                     void *k_out, const int32_t *positions, int num_tokens, int num_q_heads, int num_kv_heads,
+                     const void *q_weight, const void *k_weight, float eps, void *stream);
+
 /* Waves per prefill-attention workgroup, process-wide: 0 = auto, 4 or 8
  * (8: one 256-row workgroup per CU; 4: two 128-row workgroups per CU, one's
  * start-up under the other's tiles).  Auto takes 4 at head_dim 64 (three
@@ -567,7 +618,8 @@ int tl_fill_normal_f16(uint64_t seed, uint64_t first, float stddev, void *out, s
  * named kernels is bracketed by hipEvents on its own stream.
  * Names: "attn_chunk", "attn_merge", "kv_append", "kv_gather", "w8a16"
  * (the W8A16 GEMM kernel), "w8a16_reduce" (its split-K reduction),
- * "attn_prefill", "kv_evict", "attn_stream", "attn_account", "attn_cross".
+ * "attn_prefill", "kv_evict", "attn_stream", "attn_account", "attn_cross",
+ * "attn_quant", "prefill_quant", "rotary".
  * ---------------------------------------------------------------------- */
 void tl_profile_enable(int on);
 void tl_profile_reset(void);

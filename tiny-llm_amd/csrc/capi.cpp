@@ -7,6 +7,7 @@
 #include "kernels/w8a16.h"
 #include "runtime.h"
 #include "tiny_llm/kernels/attention.h"
+#include "tiny_llm/kernels/rotary.h"
 #include "tiny_llm/kv_cache.h"
 #include "tl_log.h"
 
@@ -54,6 +55,9 @@ struct tl_kv_cross {
 };
 struct tl_kv_evict {
     std::unique_ptr<EvictBatch> b;
+};
+struct tl_rotary {
+    std::unique_ptr<tiny_llm::kernels::Rotary> r;
 };
 
 namespace {
@@ -204,6 +208,27 @@ int tl_kv_create_paged(const tl_kv_config *cfg, int block_tokens, int num_blocks
         return TL_OK;
     });
 }
+
+int tl_kv_create_quantized(const tl_kv_config *cfg, int block_tokens, int num_blocks, tl_kv_manager **out) {
+    if (!out) return fail(TL_ERR_INVALID, "tl_kv_create_quantized: out is null");
+    *out = nullptr;
+    if (!cfg) return fail(TL_ERR_INVALID, "tl_kv_create_quantized: cfg is null");
+    return guarded([&] {
+        tiny_llm::KVCacheConfig c;
+        c.num_layers = cfg->num_layers;
+        c.num_heads = cfg->num_heads;
+        c.head_dim = cfg->head_dim;
+        c.max_seq_len = cfg->max_seq_len;
+        c.max_batch_size = cfg->max_batch_size;
+        auto r = KVCacheManager::createQuantized(c, block_tokens, num_blocks);
+        if (r.isErr()) return fail(TL_ERR_INVALID, r.error());
+        *out = new tl_kv_manager{std::move(r.value())};
+        g_last_error.clear();
+        return TL_OK;
+    });
+}
+
+int tl_kv_is_quantized(const tl_kv_manager *mgr) { return mgr && mgr->m->isQuantized() ? 1 : 0; }
 
 int    tl_kv_num_blocks(const tl_kv_manager *mgr) { return mgr ? mgr->m->numBlocks() : 0; }
 int    tl_kv_free_blocks(const tl_kv_manager *mgr) { return mgr ? mgr->m->freeBlocks() : 0; }
@@ -390,6 +415,40 @@ int tl_w8a16_matmul_residual(const void *input, const int8_t *weight, const void
         if (!err.empty()) return fail(TL_ERR_INVALID, err);
         g_last_error.clear();
         return TL_OK;
+    });
+}
+
+int tl_rotary_create(int head_dim, int rotary_dim, double theta, int interleaved, const int *axis_of,
+                     const double *inv_freq, tl_rotary **out) {
+    if (!out) return fail(TL_ERR_INVALID, "tl_rotary_create: out is null");
+    *out = nullptr;
+    return guarded([&] {
+        tiny_llm::kernels::RotaryConfig c;
+        c.head_dim = head_dim;
+        c.rotary_dim = rotary_dim;
+        c.theta = theta;
+        c.interleaved = interleaved != 0;
+        const bool fits = rotary_dim > 0 && rotary_dim <= head_dim && head_dim <= 256; // else create refuses
+        if (axis_of && fits) c.axis_of.assign(axis_of, axis_of + rotary_dim / 2);
+        if (inv_freq && fits) c.inv_freq.assign(inv_freq, inv_freq + rotary_dim / 2);
+        auto r = tiny_llm::kernels::Rotary::create(c);
+        if (r.isErr()) return fail(TL_ERR_INVALID, r.error());
+        *out = new tl_rotary{std::move(r.value())};
+        g_last_error.clear();
+        return TL_OK;
+    });
+}
+
+void tl_rotary_destroy(tl_rotary *r) { delete r; }
+
+int tl_rotary_apply(const tl_rotary *r, const void *q, int64_t q_stride, const void *k, int64_t k_stride, void *q_out,
+                    void *k_out, const int32_t *positions, int num_tokens, int num_q_heads, int num_kv_heads,
+                    const void *q_weight, const void *k_weight, float eps, void *stream) {
+    if (!r) return fail(TL_ERR_INVALID, "tl_rotary_apply: null rotary");
+    return guarded([&] {
+        return status(r->r->apply(as_half(q), q_stride, as_half(k), k_stride, as_half(q_out), as_half(k_out), positions,
+                                  num_tokens, num_q_heads, num_kv_heads, as_half(q_weight), as_half(k_weight), eps,
+                                  as_stream(stream)));
     });
 }
 
@@ -757,7 +816,8 @@ void tl_profile_reset(void) { tiny_llm::detail::profile_reset(); }
 int tl_profile_query(const char *kernel, double *total_ms, long long *launches) {
     static const char *names[] = {"attn_chunk", "attn_merge",   "kv_append",   "kv_gather",
                                   "w8a16",      "w8a16_reduce", "attn_prefill", "kv_evict",
-                                  "attn_stream",  "attn_account", "attn_cross"};
+                                  "attn_stream",  "attn_account", "attn_cross", "attn_quant",
+                                  "prefill_quant", "rotary"};
     constexpr int      kNames = static_cast<int>(sizeof(names) / sizeof(names[0]));
     static_assert(kNames == static_cast<int>(tiny_llm::detail::KernelId::Count), "profile names");
     if (!kernel || !total_ms || !launches) return fail(TL_ERR_INVALID, "tl_profile_query: null argument");

@@ -21,6 +21,7 @@ CrossBatch::~CrossBatch() = default;
 Result<std::unique_ptr<CrossBatch>> CrossBatch::create(KVCacheManager &mgr, int max_entries, int num_q_heads) {
     using R = Result<std::unique_ptr<CrossBatch>>;
     const KVCacheConfig &cfg = mgr.getConfig();
+    if (mgr.isQuantized()) return R::err("CrossBatch: attends to fp16 caches only");
     if (max_entries <= 0) return R::err("CrossBatch: max_entries must be positive");
     if (num_q_heads <= 0 || num_q_heads % cfg.num_heads != 0)
         return R::err("CrossBatch: num_q_heads (" + std::to_string(num_q_heads) +

@@ -1,0 +1,426 @@
+// Attention of a few query rows over a cache in 8 bits (layout: quant.h), read once, for
+// gfx950: decode steps, and up to 16 rows (tokens x query heads of a kv head) of a prompt.
+//
+//   s_rt = (q_r . K_t) scale ks,   P_rt = exp(s_rt - max_t s_rt) / sum_t exp(...)
+//   o_r  = sum_groups vs sum_t P_rt V_t       (sum + 1e-6 in the denominator, as in decode)
+// K_t, V_t: the stored whole numbers, ks, vs: the scales of t's group.  Bound by HBM: 2 D
+// bytes a token and kv head.
+//
+// A workgroup of 4 or 8 waves per (entry, chunk of tiles of 64 tokens, kv head); wave w
+// takes every 4th (8th) tile (half a tile at a time at head_dim 256) and keeps its own running
+// maximum, sum and output; the next tile is on its way while one is computed.  Tiles lie in
+// memory as the operands that the matrix instructions take, so nothing passes through LDS:
+//   S^T = K Q^T      v_mfma_f32_16x16x32_f16: A = K (token l%16, dims 8(l/16)..+7),
+//                    B = Q (row l%16), D = S^T (tokens 4(l/16)+i, row l%16)
+//   O^T += vs V^T P^T  A = V^T (dim l%16, the group's tokens that the lane has weights of),
+//                    B = the weights as they came out; a group's product is scaled in fp32
+// Whole numbers up to 127 are exact in fp16, so the scales are all that rounds them.
+// The open group (fp16, at most 31 tokens) is a step of its own of one wave.
+#include "quant_device.h"
+
+#include "../runtime.h"
+#include "kv_kernels.h"
+#include "tiny_llm/hip_utils.h"
+
+#include <algorithm>
+#include <climits>
+#include <cstring>
+#include <mutex>
+
+namespace tiny_llm {
+namespace detail {
+
+namespace {
+
+using namespace quant;
+
+// Weights are 2^(s - ref): the reference is 2^7 below the maximum when it moves, and moves on
+// scores 2^15 above it only (below 2^15 in fp16, and 2^-31 of the largest still counts).
+constexpr float kBelow = 7.0f, kLazyMax = 15.0f;
+// The reference over no score, or over -infinite ones only: finite, and below every finite score.
+constexpr float kNone = -3e38f;
+
+struct QuantArgs {
+    const uint16_t *q;
+    uint16_t       *out;
+    const uint16_t *new_k, *new_v;
+    float          *part_o;  // [item][Hkv][rows][D]
+    float          *part_ml; // [item][Hkv][rows][2]
+    QuantView       v;
+    float           scale_log2;
+    int             Hq, Hkv, G, n, chunk, rows;
+    QuantEntry      e[kQuantBatch];
+};
+static_assert(sizeof(QuantArgs) <= 4096, "kernel arguments");
+
+template <int D, int NW>
+__global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(QuantArgs a) {
+    constexpr int NG = D <= 128 ? 2 : 1;  // groups of a step
+    constexpr int SUB = 2 / NG;           // steps per tile
+    constexpr int KS = D / 32, DT = D / 16;
+    constexpr int NT = NW * 64;
+    extern __shared__ __align__(16) float so[]; // the waves' outputs [NW][rows][D]
+    __shared__ float    sm[NW][16], sl[NW][16], s_l[16];
+    __shared__ uint32_t red[2 * NW];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int item = blockIdx.x / a.Hkv, g = blockIdx.x - item * a.Hkv;
+    int       ei;
+    QUANT_ENTRY_OF(a, item, ei);
+    const int row = a.e[ei].row, S = a.e[ei].S, tok0 = a.e[ei].tok0, nq = a.e[ei].nq, rows = nq * a.G;
+    const int tiles = (S + kQuantTile - 1) / kQuantTile;
+    const int nch = (tiles + a.chunk - 1) / a.chunk, ch = item - a.e[ei].item0;
+    const int tile_lo = (int)((int64_t)ch * tiles / nch), tile_hi = (int)((int64_t)(ch + 1) * tiles / nch);
+    int       open = a.e[ei].open;
+
+    if (a.new_k) {
+        if (ch == nch - 1) { // the new token, then read like any other
+            const int     t = S - 1;
+            const int64_t at = tile_of(a.v, a.Hkv, row, g, t / kGroup), src = ((int64_t)tok0 * a.Hkv + g) * D;
+            append_token<D, NT>(open_of<D>(a.v, a.Hkv, row, open, g), t % kGroup, a.new_k + src, a.new_v + src,
+                                a.v.tiles + at * (64 * D), a.v.scales + at, red);
+        }
+    }
+    if (S % kGroup == 0) open = -1; // the last token closed its group
+    const int closed = open < 0 ? S : S / kGroup * kGroup; // tokens in 8 bits
+    const int groups = (closed + kGroup - 1) / kGroup;
+
+    const int c = lane & 15, qg = lane >> 4;
+    f16x8     qb[KS]; // B operand: row c, dims 32s + 8qg .. +7
+    {
+        const int       r = min(c, rows - 1);
+        const uint16_t *qp = a.q + ((int64_t)(tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qb[s] = *reinterpret_cast<const f16x8 *>(qp + 32 * s + 8 * qg);
+    }
+    const int all = S - nq + 1;                         // tokens that every row sees
+    const int lim = min(S, all + min(c, rows - 1) / a.G); // that row c sees
+    f32x4     acc[DT];
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) acc[dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m_run = kNone, l_run = 0.0f;
+    auto  raise = [&](float mloc) __attribute__((always_inline)) { // the reference, where a score is far above it
+        if (__any(mloc > m_run + kLazyMax)) {
+            mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
+            mloc = fmaxf(mloc, __shfl_xor(mloc, 32));
+            const float m_new = fmaxf(m_run, mloc - kBelow);
+            const float alpha = m_run == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run - m_new);
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) acc[dt] *= alpha;
+            l_run *= alpha;
+            m_run = m_new;
+        }
+    };
+
+    // The wave's steps: step x is half (all) of tile tile_lo + x / SUB * NW + wave.
+    const int end = min(tile_hi, (groups + 1) / 2);
+    const int steps = max(0, (end - tile_lo - wave + NW - 1) / NW) * SUB;
+    auto      first_group = [&](int x) { return (tile_lo + x / SUB * NW + wave) * 2 + x % SUB * NG; };
+    const int32_t *bt = a.v.table + (int64_t)row * a.v.bt_stride;
+    // Blocks of a step's groups, lane k that of group k; asked for a step before the tiles.
+    auto blocks = [&](int x) -> int { return lane < NG ? bt[min(first_group(x) + lane, groups - 1) >> a.v.lg] : 0; };
+    auto tile_at = [&](int x, int k, int ids) __attribute__((always_inline)) -> int64_t {
+        const int i = min(first_group(x) + k, groups - 1) & ((1 << a.v.lg) - 1);
+        return (((int64_t)__builtin_amdgcn_readlane(ids, k) * a.Hkv + g) << a.v.lg) + i;
+    };
+    u32x4  kr[NG][KS], vr[NG][DT / 2];
+    float2 sc[NG], sc_next[NG];
+    auto   load_k = [&](int x, int ids) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            const int64_t at = tile_at(x, k, ids);
+            const u32x4  *p = reinterpret_cast<const u32x4 *>(a.v.tiles + at * (64 * D)) + lane;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) kr[k][s] = __builtin_nontemporal_load(p + 64 * s);
+            sc_next[k] = a.v.scales[at];
+        }
+    };
+    auto load_v = [&](int x, int ids) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            const u32x4 *p = reinterpret_cast<const u32x4 *>(a.v.tiles + tile_at(x, k, ids) * (64 * D) + 32 * D) + lane;
+#pragma unroll
+            for (int s = 0; s < DT / 2; ++s) vr[k][s] = __builtin_nontemporal_load(p + 64 * s);
+        }
+    };
+
+    int ids = steps > 0 ? blocks(0) : 0, next = steps > 1 ? blocks(1) : 0;
+    if (steps > 0) {
+        load_k(0, ids);
+        load_v(0, ids);
+    }
+    for (int x = 0; x < steps; ++x) {
+        const int  g0 = first_group(x), t0 = g0 * kGroup;
+        const bool more = x + 1 < steps;
+        ids = next;
+        if (x + 2 < steps) next = blocks(x + 2);
+#pragma unroll
+        for (int k = 0; k < NG; ++k) sc[k] = sc_next[k];
+        f32x4 s[NG][2];
+#pragma unroll
+        for (int k = 0; k < NG; ++k)
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt) {
+                s[k][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < KS; ++i)
+                    s[k][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(whole8(kr[k][i][2 * tt], kr[k][i][2 * tt + 1]), qb[i], s[k][tt], 0, 0, 0);
+            }
+        if (more) load_k(x + 1, ids);
+        float mloc = -INFINITY;
+        const bool masked = t0 + NG * kGroup > min(all, closed); // some score does not count
+        const int  bound = min(lim, closed);
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            const float f = sc[k].x * a.scale_log2;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float y = s[k][tt][i] * f;
+                    s[k][tt][i] = !masked || t0 + 32 * k + 16 * tt + 4 * qg + i < bound ? y : -INFINITY;
+                    mloc = fmaxf(mloc, s[k][tt][i]);
+                }
+        }
+        raise(mloc);
+#pragma unroll
+        for (int k = 0; k < NG; ++k) {
+            f16x8 pf;
+#pragma unroll
+            for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = __builtin_amdgcn_exp2f(s[k][tt][i] - m_run);
+                    l_run += p;
+                    pf[4 * tt + i] = (_Float16)p;
+                }
+            // (a group whose scale is NaN is none of the rows' business that see none of it)
+            const float vs = t0 + 32 * k < bound ? sc[k].y : 0.0f;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+                const u32x4 w = vr[k][dt / 2];
+                const f32x4 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(whole8(w[2 * (dt & 1)], w[2 * (dt & 1) + 1]), pf,
+                                                                      f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[dt][i] = fmaf(vs, o[i], acc[dt][i]);
+            }
+        }
+        if (more) load_v(x + 1, ids);
+    }
+
+    // The open group, by the wave whose turn its tile is.
+    if (open >= 0 && ch == nch - 1 && wave == (tiles - 1 - tile_lo) % NW) {
+        const int       t0 = closed, cnt = S - t0;
+        const uint16_t *tile = open_of<D>(a.v, a.Hkv, row, open, g);
+        const f16x8    *kp = reinterpret_cast<const f16x8 *>(tile) + 2 * lane;
+        const f16x8    *vp = reinterpret_cast<const f16x8 *>(tile + 32 * D) + 2 * lane;
+        f32x4           s[2];
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt) {
+            s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kp[128 * i + tt], qb[i], s[tt], 0, 0, 0);
+        }
+        float mloc = -INFINITY;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float y = s[tt][i] * a.scale_log2;
+                s[tt][i] = t0 + 16 * tt + 4 * qg + i < lim ? y : -INFINITY;
+                mloc = fmaxf(mloc, s[tt][i]);
+            }
+        raise(mloc);
+        f16x8 pf;
+#pragma unroll
+        for (int tt = 0; tt < 2; ++tt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = __builtin_amdgcn_exp2f(s[tt][i] - m_run);
+                l_run += p;
+                pf[4 * tt + i] = (_Float16)p;
+            }
+        // Values of tokens behind the last are whatever the tile held: 0 times them could be
+        // NaN.  The same goes for infinite values that only some of the rows see.
+        bool odd = false;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            f16x8 v = vp[128 * (dt / 2) + (dt & 1)];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool there = 16 * (j >> 2) + 4 * qg + (j & 3) < cnt;
+                const bool finite = __builtin_fabsf16(v[j]) <= (_Float16)65504.0f;
+                odd |= there && !finite;
+                if (!there || !finite) v[j] = (_Float16)0.0f;
+            }
+            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf, acc[dt], 0, 0, 0);
+        }
+        if (__any(odd)) {
+            for (int r = 0; r < cnt; ++r)
+                if (t0 + r < lim)
+#pragma unroll
+                    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = (float)__builtin_bit_cast(_Float16, tile[32 * D + v_half(r, 16 * dt + 4 * qg + i)]);
+                            if (!(__builtin_fabsf(x) <= 65504.0f)) acc[dt][i] += x;
+                        }
+        }
+    }
+
+    // The waves' (m, l, o) through LDS.
+    l_run += __shfl_xor(l_run, 16);
+    l_run += __shfl_xor(l_run, 32);
+    if (c < rows)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4 *>(so + ((wave * a.rows + c) * D + 16 * dt + 4 * qg)) = acc[dt];
+    if (qg == 0) {
+        sm[wave][c] = m_run;
+        sl[wave][c] = l_run;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+        const int r = threadIdx.x;
+        float     m = sm[0][r], l = 0.0f;
+#pragma unroll
+        for (int w = 1; w < NW; ++w) m = fmaxf(m, sm[w][r]);
+#pragma unroll
+        for (int w = 0; w < NW; ++w) { // sm: the waves' weights
+            const float wgt = __builtin_amdgcn_exp2f(sm[w][r] - m);
+            l = fmaf(wgt, sl[w][r], l);
+            sm[w][r] = wgt;
+        }
+        s_l[r] = l;
+        if (nch > 1)
+            *reinterpret_cast<float2 *>(a.part_ml + (((int64_t)item * a.Hkv + g) * a.rows + r) * 2) = make_float2(m, l);
+    }
+    __syncthreads();
+    for (int idx = threadIdx.x; idx < rows * (D / 4); idx += NT) {
+        const int r = idx / (D / 4), d = 4 * (idx - r * (D / 4));
+        f32x4     o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(so + (w * a.rows + r) * D + d);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(sm[w][r], x[i], o[i]);
+        }
+        if (nch == 1) {
+            const float   inv = 1.0f / (s_l[r] + 1e-6f);
+            const __half2 lo = __floats2half2_rn(o[0] * inv, o[1] * inv), hi = __floats2half2_rn(o[2] * inv, o[3] * inv);
+            *reinterpret_cast<u32x2 *>(a.out + ((int64_t)(tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D + d) =
+                u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+        } else {
+            *reinterpret_cast<f32x4 *>(a.part_o + (((int64_t)item * a.Hkv + g) * a.rows + r) * D + d) = o;
+        }
+    }
+}
+
+constexpr int kFinishThreads = 256;
+
+// Entries of several chunks, or of no tokens (zeros).  Workgroup (entry, kv head; row): the
+// row's maximum and sum over the chunks, then its output, the chunks spread over the threads.
+__global__ __launch_bounds__(kFinishThreads) void quant_finish_kernel(QuantArgs a, int D) {
+    __shared__ f32x4 s_o[kFinishThreads];
+    const int ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv, r = blockIdx.y;
+    const int S = a.e[ei].S, tok0 = a.e[ei].tok0, rows = a.e[ei].nq * a.G;
+    const int tiles = (S + kQuantTile - 1) / kQuantTile, nch = (tiles + a.chunk - 1) / a.chunk;
+    if (nch == 1 || r >= rows) return;
+    const int64_t p0 = ((int64_t)a.e[ei].item0 * a.Hkv + g) * a.rows + r; // of chunk 0
+    const int64_t pc = (int64_t)a.Hkv * a.rows;                          // from chunk to chunk
+    // (every wave for itself)
+    float m = kNone, l = 0.0f;
+    for (int ch = threadIdx.x & 63; ch < nch; ch += 64) m = fmaxf(m, a.part_ml[(p0 + ch * pc) * 2]);
+    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
+    for (int ch = threadIdx.x & 63; ch < nch; ch += 64) {
+        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (p0 + ch * pc) * 2);
+        l = fmaf(__builtin_amdgcn_exp2f(ml.x - m), ml.y, l);
+    }
+    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
+    const int per = D / 4, groups = kFinishThreads / per, grp = threadIdx.x / per, d = 4 * (threadIdx.x % per);
+    f32x4     o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+    for (int ch = grp; ch < nch; ch += groups) {
+        const int64_t pr = p0 + ch * pc;
+        const float   wgt = __builtin_amdgcn_exp2f(a.part_ml[pr * 2] - m);
+        const f32x4   x = *reinterpret_cast<const f32x4 *>(a.part_o + pr * D + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(wgt, x[i], o[i]);
+    }
+    s_o[threadIdx.x] = o;
+    __syncthreads();
+    if (grp == 0) {
+        for (int k = 1; k < groups; ++k) o += s_o[threadIdx.x + k * per];
+        const float   inv = nch ? 1.0f / (l + 1e-6f) : 0.0f;
+        const __half2 lo = __floats2half2_rn(o[0] * inv, o[1] * inv), hi = __floats2half2_rn(o[2] * inv, o[3] * inv);
+        *reinterpret_cast<u32x2 *>(a.out + ((int64_t)(tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D + d) =
+            u32x2{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+    }
+}
+
+// Floats of the partial maxima and sums, then the outputs at a multiple of 16 bytes.
+size_t part_ml_floats(size_t rows) { return (2 * rows + 3) / 4 * 4; }
+
+template <int D, int NW> void launch_one(const QuantArgs &a, int items, hipStream_t stream) {
+    auto                 *fn = attn_quant_kernel<D, NW>;
+    static std::once_flag once[64]; // per device
+    std::call_once(once[current_device() & 63], [&] {
+        HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      NW * kQuantRows * D * 4));
+    });
+    hipLaunchKernelGGL(fn, dim3((unsigned)items * (unsigned)a.Hkv), dim3(NW * 64), (size_t)(NW * a.rows * D * 4), stream, a);
+}
+
+} // namespace
+
+size_t quant_workspace_floats(const QuantPlan &plan, int Hkv, int D) {
+    size_t most = 0;
+    for (const auto &l : plan.launches) {
+        const size_t rows = (size_t)l.items * (size_t)l.rows * (size_t)Hkv;
+        if (l.finish) most = std::max(most, part_ml_floats(rows) + rows * (size_t)D);
+    }
+    return most;
+}
+
+void launch_attn_quant(const QuantCall &c, const QuantView &v, const QuantPlan &plan, float *workspace, hipStream_t stream) {
+    QuantArgs a{};
+    a.q = reinterpret_cast<const uint16_t *>(c.q);
+    a.out = reinterpret_cast<uint16_t *>(c.out);
+    a.new_k = reinterpret_cast<const uint16_t *>(c.new_k);
+    a.new_v = reinterpret_cast<const uint16_t *>(c.new_v);
+    a.v = v;
+    a.scale_log2 = c.scale * 1.4426950408889634f;
+    a.Hq = c.Hq;
+    a.Hkv = c.Hkv;
+    a.G = c.Hq / c.Hkv;
+    a.chunk = plan.chunk;
+    for (const auto &l : plan.launches) {
+        if (l.n == 0) continue;
+        a.n = l.n;
+        a.rows = l.rows;
+        if (a.rows > kQuantRows) throw std::invalid_argument("attention: too many query rows per entry");
+        if ((int64_t)l.items * c.Hkv > kQuantMostItems) throw std::invalid_argument("attention: too many work items");
+        std::memcpy(a.e, plan.entries.data() + l.first, sizeof(QuantEntry) * (size_t)l.n);
+        a.part_ml = workspace;
+        a.part_o = l.finish ? workspace + part_ml_floats((size_t)l.items * c.Hkv * a.rows) : nullptr;
+        profile_begin(KernelId::AttnQuant, stream);
+        if (l.items > 0) {
+            for_head_dim(c.D, [&](auto d) {
+                constexpr int D = decltype(d)::value;
+                if constexpr (D <= 128) {
+                    if (plan.waves == 8) return launch_one<D, 8>(a, l.items, stream);
+                }
+                launch_one<D, 4>(a, l.items, stream);
+            });
+            HIP_CHECK(hipGetLastError());
+        }
+        if (l.finish) {
+            hipLaunchKernelGGL(quant_finish_kernel, dim3((unsigned)(l.n * c.Hkv), (unsigned)a.rows), dim3(kFinishThreads), 0,
+                               stream, a, c.D);
+            HIP_CHECK(hipGetLastError());
+        }
+        profile_end(KernelId::AttnQuant, stream);
+    }
+}
+
+} // namespace detail
+} // namespace tiny_llm

@@ -197,7 +197,10 @@ enum class KernelId {
     AttnStream = 8, // with its finish
     AttnAccount = 9, // statistics and sums of one launch
     AttnCross = 10, // with its merge
-    Count = 11
+    AttnQuant = 11, // with its finish
+    PrefillQuant = 12, // with its merge
+    Rotary = 13,
+    Count = 14
 };
 void profile_begin(KernelId id, hipStream_t stream);
 void profile_end(KernelId id, hipStream_t stream);

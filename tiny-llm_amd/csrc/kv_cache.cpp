@@ -11,8 +11,10 @@
 #include "block_allocator.h"
 #include "kernels/kv_kernels.h"
 #include "kernels/prefill.h"
+#include "kernels/quant.h"
 #include "kernels/stream.h"
 #include "kernels/w8a16.h"
+#include "quantized.h"
 #include "runtime.h"
 #include "tl_log.h"
 
@@ -31,7 +33,7 @@ KVCacheManager::KVCacheManager(const KVCacheConfig &config) : config_(config) {}
 
 // KVCacheManager::create (kv_cache.cpp:8-60).
 Result<std::unique_ptr<KVCacheManager>> KVCacheManager::create(const KVCacheConfig &config) {
-    return build(config, 0, 0);
+    return build(config, 0, 0, false);
 }
 
 Result<std::unique_ptr<KVCacheManager>> KVCacheManager::createPaged(const KVCacheConfig &config,
@@ -50,13 +52,14 @@ Result<std::unique_ptr<KVCacheManager>> KVCacheManager::createPaged(const KVCach
             static_cast<int64_t>(UINT32_MAX))
         return R::err("KVCacheManager: a block of " + std::to_string(block_tokens) +
                       " tokens exceeds 4 GiB per layer and K/V region");
-    return build(config, block_tokens, num_blocks);
+    return build(config, block_tokens, num_blocks, false);
 }
 
 // The checks and pool set-up of create (kv_cache.cpp:8-60); with
-// block_tokens > 0 the pool is the block pool of createPaged.
+// block_tokens > 0 the pool is the block pool of createPaged or createQuantized.
 Result<std::unique_ptr<KVCacheManager>> KVCacheManager::build(const KVCacheConfig &config,
-                                                              int block_tokens, int num_blocks) {
+                                                              int block_tokens, int num_blocks,
+                                                              bool quantized) {
     using R = Result<std::unique_ptr<KVCacheManager>>;
     if (config.num_layers <= 0 || config.num_heads <= 0 || config.head_dim <= 0 ||
         config.max_seq_len <= 0 || config.max_batch_size <= 0) {
@@ -82,6 +85,10 @@ Result<std::unique_ptr<KVCacheManager>> KVCacheManager::build(const KVCacheConfi
             return R::err("KVCacheManager: pool size overflow");
         manager->pool_size_ = per_kv * 2 * static_cast<size_t>(config.num_layers) * sizeof(half);
         manager->layer_stride_ = 2 * static_cast<int64_t>(per_kv);
+        if (quantized) { // a byte a value, K and V of a group side by side
+            manager->pool_size_ /= sizeof(half);
+            manager->quantized_ = true;
+        }
         manager->block_tokens_ = block_tokens;
         const int bpr = (config.max_seq_len + block_tokens - 1) / block_tokens;
         manager->blocks_.reset(new detail::BlockAllocator(config.max_batch_size, bpr, num_blocks));
@@ -100,6 +107,20 @@ Result<std::unique_ptr<KVCacheManager>> KVCacheManager::build(const KVCacheConfi
         (void)hipFree(manager->memory_pool_);
         manager->memory_pool_ = nullptr;
         return R::err(std::string("KVCacheManager: hipMemset failed: ") + hipGetErrorString(err));
+    }
+    if (quantized) {
+        const size_t layers = static_cast<size_t>(config.num_layers), heads = static_cast<size_t>(config.num_heads);
+        const size_t scales = layers * (static_cast<size_t>(num_blocks) + 1) * heads *
+                              static_cast<size_t>(block_tokens / detail::kGroup) * sizeof(float2);
+        const size_t tiles = layers * static_cast<size_t>(config.max_batch_size) * 2 * heads *
+                             (2 * detail::kGroup * static_cast<size_t>(config.head_dim)) * sizeof(half);
+        err = hipMalloc(reinterpret_cast<void **>(&manager->scales_), scales);
+        if (err == hipSuccess) err = hipMalloc(reinterpret_cast<void **>(&manager->open_tiles_), tiles);
+        if (err == hipSuccess) err = hipMemset(manager->scales_, 0, scales);
+        if (err == hipSuccess) err = hipMemset(manager->open_tiles_, 0, tiles);
+        if (err != hipSuccess)
+            return R::err(std::string("KVCacheManager: scales and open groups: ") + hipGetErrorString(err));
+        manager->open_.resize(static_cast<size_t>(config.max_batch_size));
     }
     if (manager->blocks_) {
         // Every entry starts at the spare block.
@@ -126,6 +147,8 @@ Result<std::unique_ptr<KVCacheManager>> KVCacheManager::build(const KVCacheConfi
 // ~KVCacheManager (kv_cache.cpp:62-67).
 KVCacheManager::~KVCacheManager() {
     if (block_map_dev_) (void)hipFree(block_map_dev_);
+    if (scales_) (void)hipFree(scales_);
+    if (open_tiles_) (void)hipFree(open_tiles_);
     if (memory_pool_) {
         (void)hipFree(memory_pool_);
         memory_pool_ = nullptr;
@@ -168,6 +191,7 @@ Result<int> KVCacheManager::allocateSequence(int max_len) {
     slot.max_len = max_len;
     slot.active = true;
     evictions_[static_cast<size_t>(slot_idx)] = Eviction();
+    if (quantized_) open_[static_cast<size_t>(slot_idx)] = detail::OpenGroup();
     seq_to_slot_[seq_id] = slot_idx;
     return Result<int>::ok(seq_id);
 }
@@ -261,6 +285,12 @@ Result<void> KVCacheManager::appendKV(int seq_id, int layer_idx, const half *new
                                  ", appending: " + std::to_string(num_tokens) +
                                  ", max: " + std::to_string(slot.max_len));
     }
+    if (quantized_) {
+        if (std::string err = detail::check_quant_call("appendKV", *this, {new_k, new_v}); !err.empty()) {
+            TL_LOG_ERROR("%s", err.c_str());
+            return Result<void>::err(err);
+        }
+    }
     const int row = config_.num_heads * config_.head_dim;
     if (blocks_) {
         const int need = (write_pos + num_tokens + block_tokens_ - 1) / block_tokens_;
@@ -271,7 +301,12 @@ Result<void> KVCacheManager::appendKV(int seq_id, int layer_idx, const half *new
         }
         syncTable(stream);
     }
-    if (!isPaged()) {
+    if (quantized_) {
+        const auto [first, last] = openGroup(slot_idx).tiles(write_pos, num_tokens);
+        std::vector<detail::QuantAppend> one{{slot_idx, write_pos, num_tokens, 0, first | last << 1, 0}};
+        detail::launch_quant_append(quantView(layer_idx), one, config_.num_heads, config_.head_dim, new_k, new_v, stream);
+        noteAppend(slot_idx, num_tokens);
+    } else if (!isPaged()) {
         half        *k_cache = memory_pool_ + calculateOffset(slot_idx, layer_idx, false);
         half        *v_cache = memory_pool_ + calculateOffset(slot_idx, layer_idx, true);
         const size_t pos_offset = static_cast<size_t>(write_pos) * row;
@@ -305,7 +340,7 @@ Result<void> KVCacheManager::advanceSeqLen(int seq_id, int num_tokens) {
     }
     auto     &slot = slots_[static_cast<size_t>(it->second)];
     const int old_len = slot.current_len;
-    const int new_len = std::min(slot.current_len + num_tokens, slot.max_len);
+    const int new_len = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(slot.current_len) + num_tokens, slot.max_len));
     if (blocks_) {
         // Positions made visible without an append still get blocks, so
         // that every visible token of a block pool is backed.
@@ -314,6 +349,18 @@ Result<void> KVCacheManager::advanceSeqLen(int seq_id, int num_tokens) {
             auto r = exhausted(need - blocks_->mapped(it->second));
             TL_LOG_ERROR("advanceSeqLen: %s", r.error().c_str());
             return r;
+        }
+    }
+    if (quantized_) {
+        detail::OpenGroup &open = open_[static_cast<size_t>(it->second)];
+        if (!open.advance(old_len, new_len)) {
+            const std::string msg = "advanceSeqLen: length " + std::to_string(new_len) + " of sequence " +
+                                    std::to_string(seq_id) + " lies inside the tokens up to " + std::to_string(open.end) +
+                                    " that were appended at once: an 8-bit cache can be cut there at a multiple of " +
+                                    std::to_string(detail::kGroup) +
+                                    ", in the group in which they begin or in the one in which they end";
+            TL_LOG_ERROR("%s", msg.c_str());
+            return Result<void>::err(msg);
         }
     }
     slot.current_len = new_len;
@@ -377,6 +424,9 @@ const SequenceCache *KVCacheManager::sequence(int seq_id) const noexcept {
 int KVCacheManager::numBlocks() const noexcept { return blocks_ ? blocks_->numBlocks() : 0; }
 int KVCacheManager::freeBlocks() const noexcept { return blocks_ ? blocks_->freeBlocks() : 0; }
 size_t KVCacheManager::blockBytes() const noexcept {
+    if (quantized_) // with the scales
+        return static_cast<size_t>(block_tokens_ / detail::kGroup) * config_.num_heads * config_.num_layers *
+               (2 * detail::kGroup * static_cast<size_t>(config_.head_dim) + sizeof(float2));
     return blocks_ ? static_cast<size_t>(block_tokens_) * config_.num_heads * config_.head_dim *
                          config_.num_layers * 2 * sizeof(half)
                    : 0;
@@ -504,7 +554,7 @@ DecodeBatch::DecodeBatch(KVCacheManager &mgr, int max_seqs, int num_q_heads)
       work_(new detail::Workspace()), gemm_work_(new detail::Workspace()),
       plan_(new detail::WorkList()),
       inl_(new detail::InlineMeta()), account_plan_(new detail::StreamPlan()),
-      account_work_(new detail::Workspace()) {}
+      account_work_(new detail::Workspace()), quant_(mgr.isQuantized() ? new detail::QuantStep() : nullptr) {}
 
 DecodeBatch::~DecodeBatch() = default;
 
@@ -544,6 +594,7 @@ Result<void> DecodeBatch::upload(const int *seq_ids, const int *attended, int n,
     appendable_ = false;
     d_rows_ = d_gather_ = nullptr;
     account_plan_->clear();
+    if (quant_) quant_->clear();
     ids_.clear();
     const KVCacheConfig &cfg = mgr_.getConfig();
     std::vector<char>    taken(static_cast<size_t>(cfg.max_batch_size), 0);
@@ -575,6 +626,11 @@ Result<void> DecodeBatch::upload(const int *seq_ids, const int *attended, int n,
                 return Result<void>::err("DecodeBatch: attended length " + std::to_string(a) +
                                          " of sequence " + std::to_string(id) + " outside [0, " +
                                          std::to_string(sc->max_len) + "]");
+            if (quant_ && a > detail::held_tokens(mgr_, id, slot))
+                return Result<void>::err("DecodeBatch: attended length " + std::to_string(a) + " of sequence " +
+                                         std::to_string(id) + " is more than the " +
+                                         std::to_string(detail::held_tokens(mgr_, id, slot)) +
+                                         " tokens that its 8-bit cache holds");
             lens_[static_cast<size_t>(i)] = a;
         }
     }
@@ -586,6 +642,15 @@ Result<void> DecodeBatch::upload(const int *seq_ids, const int *attended, int n,
             if (r.isErr()) return r;
         }
         mgr_.syncTable(stream);
+    }
+    if (quant_) {
+        n_ = n;
+        appendable_ = appendable;
+        ids_.assign(seq_ids, seq_ids + n);
+        quant_->prepareDecode(mgr_, ids_, slot_, lens_, appendable, num_q_heads_);
+        chunk_ = quant_->stream.chunk * detail::kQuantTile;
+        n_work_ = quant_->items();
+        return Result<void>::ok();
     }
     // Split-K plan: work items (entry, chunk), longest first.
     detail::WorkList &wl = *plan_;
@@ -663,6 +728,7 @@ Result<void> DecodeBatch::append(int layer_begin, int num_layers, const half *ne
                                  std::to_string(layer_begin + num_layers) + ") outside [0, " +
                                  std::to_string(cfg.num_layers) + ")");
     if (n_ == 0) return Result<void>::ok();
+    if (quant_) return quant_->appendOne(mgr_, layer_begin, num_layers, new_k, new_v, stream);
     upload_device(stream);
     const KvView v = mgr_.layerView(layer_begin, d_slot_);
     detail::launch_kv_append(v, mgr_.layerStride(), d_wpos_, 0, n_, num_layers,
@@ -683,6 +749,7 @@ Result<void> DecodeBatch::run_attention(int layer_idx, const half *q, const half
     if (layer_idx < 0 || layer_idx >= cfg.num_layers)
         return Result<void>::err("DecodeBatch: Invalid layer_idx: " + std::to_string(layer_idx));
     if (n_ == 0) return Result<void>::ok();
+    if (quant_) return quant_->attention("DecodeBatch", mgr_, layer_idx, q, new_k, new_v, out, scale, num_q_heads_, stream);
     if (!inline_ok_) upload_device(stream);
     detail::AttnPlan plan;
     plan.seq_lens = d_lens_;
@@ -726,6 +793,7 @@ Result<void> DecodeBatch::gather(int layer_idx, half *k_out, half *v_out, int s_
         return Result<void>::err("DecodeBatch: Invalid layer_idx: " + std::to_string(layer_idx));
     if (s_max < 0) return Result<void>::err("DecodeBatch: s_max must be >= 0");
     if (n_ == 0 || s_max == 0) return Result<void>::ok();
+    if (quant_) return quant_->gather(mgr_, layer_idx, k_out, v_out, s_max, stream);
     detail::GatherMeta meta;
     const bool inl = detail::gather_inline(n_);
     const bool captured = inl && detail::stream_capturing(stream); // (as in project)
@@ -755,6 +823,8 @@ Result<void> DecodeBatch::project(int layer_idx, const half *x, int hidden, int 
                                   const half *sv, const int8_t *wq, const half *sq, half *q_out,
                                   hipStream_t stream, bool packed) {
     const KVCacheConfig &cfg = mgr_.getConfig();
+    if (quant_)
+        return Result<void>::err("DecodeBatch: an 8-bit cache takes projections by w8a16_matmul and decode() or append()");
     if (!appendable_)
         return Result<void>::err("DecodeBatch: project needs a batch made by prepare()");
     if (layer_idx < 0 || layer_idx >= cfg.num_layers)
@@ -827,7 +897,8 @@ PrefillBatch::PrefillBatch(KVCacheManager &mgr, int max_seqs, int num_q_heads)
     : mgr_(mgr), max_seqs_(max_seqs), num_q_heads_(num_q_heads), meta_(new detail::MetaRing(4)),
       inl_(new detail::PrefillInline),
       records_(new detail::DeviceRing(sizeof(int32_t) * detail::kPrefillItemWords * detail::kPrefillInlineWords)),
-      account_plan_(new detail::AccountPlan()), account_work_(new detail::Workspace()) {}
+      account_plan_(new detail::AccountPlan()), account_work_(new detail::Workspace()),
+      quant_(mgr.isQuantized() ? new detail::QuantStep() : nullptr) {}
 
 PrefillBatch::~PrefillBatch() = default;
 
@@ -859,6 +930,7 @@ Result<void> PrefillBatch::prepare(const int *seq_ids, const int *num_tokens, in
     inline_ok_ = false;
     launched_ = false;
     account_plan_->clear();
+    if (quant_) quant_->clear();
     ids_.clear();
     counts_.clear();
     slots_.clear();
@@ -887,7 +959,7 @@ Result<void> PrefillBatch::prepare(const int *seq_ids, const int *num_tokens, in
         const int nt = num_tokens[i];
         if (nt <= 0)
             return Result<void>::err("appendKV: num_tokens must be positive: " + std::to_string(nt));
-        if (sc->current_len + nt > sc->max_len)
+        if (static_cast<int64_t>(sc->current_len) + nt > sc->max_len)
             return Result<void>::err("appendKV: cache overflow. Current: " +
                                      std::to_string(sc->current_len) + ", appending: " +
                                      std::to_string(nt) + ", max: " + std::to_string(sc->max_len));
@@ -904,6 +976,21 @@ Result<void> PrefillBatch::prepare(const int *seq_ids, const int *num_tokens, in
         auto r = mgr_.reserveSlots(slots.data(), ends.data(), n);
         if (r.isErr()) return r;
         mgr_.syncTable(stream);
+    }
+    if (quant_) {
+        ids_.assign(seq_ids, seq_ids + n);
+        counts_.assign(num_tokens, num_tokens + n);
+        slots_ = std::move(slots);
+        if (!quant_->preparePrefill(mgr_, ids_, slots_, counts_, num_q_heads_)) {
+            quant_->clear();
+            ids_.clear();
+            counts_.clear();
+            slots_.clear();
+            return Result<void>::err("PrefillBatch: too many query rows in one step");
+        }
+        n_ = n;
+        tokens_ = static_cast<int>(total);
+        return Result<void>::ok();
     }
     waves_ = detail::prefill_waves(entries.data(), n, cfg.head_dim, num_q_heads_ / cfg.num_heads,
                                    cfg.num_heads, detail::device_cus());
@@ -934,6 +1021,7 @@ Result<void> PrefillBatch::append(int layer_idx, const half *new_k, const half *
     if (layer_idx < 0 || layer_idx >= cfg.num_layers)
         return Result<void>::err("PrefillBatch: Invalid layer_idx: " + std::to_string(layer_idx));
     if (tokens_ == 0) return Result<void>::ok();
+    if (quant_) return quant_->append("PrefillBatch", mgr_, layer_idx, new_k, new_v, stream);
     // Ranges (slot, write position, tokens) travel in kernel arguments.
     detail::launch_kv_append_ranges(mgr_.layerView(layer_idx, nullptr), slots_.data(), pos0_.data(),
                                     counts_.data(), n_, cfg.num_heads * cfg.head_dim, new_k, new_v,
@@ -971,6 +1059,14 @@ Result<void> PrefillBatch::launch(int layer_idx, const half *q, const half *new_
     if ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(out) |
          reinterpret_cast<uintptr_t>(new_k) | reinterpret_cast<uintptr_t>(new_v)) & 15u)
         return Result<void>::err("PrefillBatch: q, out, new_k and new_v must be 16-byte aligned");
+    if (quant_) {
+        if (tokens_ == 0) return Result<void>::ok();
+        if (new_k) {
+            auto r = quant_->append("PrefillBatch", mgr_, layer_idx, new_k, new_v, stream);
+            if (r.isErr()) return r;
+        }
+        return quant_->attention("PrefillBatch", mgr_, layer_idx, q, nullptr, nullptr, out, scale, num_q_heads_, stream);
+    }
     if (n_items_ == 0) return Result<void>::ok();
     detail::PrefillLaunch p;
     if (!inline_ok_) {

@@ -1,0 +1,70 @@
+#include "quant_plan.h"
+
+#include <algorithm>
+
+namespace tiny_llm {
+namespace detail {
+
+void plan_quant(QuantPlan &plan, int G, int Hkv, int, int cus) {
+    int64_t total = 0, longest = 0;
+    for (const auto &e : plan.entries) {
+        total += quant_tiles(e.S);
+        longest = std::max<int64_t>(longest, quant_tiles(e.S));
+    }
+    total *= Hkv;
+    const int64_t n = std::max(1, cus);
+    plan.waves = 4;
+    const int64_t half = (total + 2 * n - 1) / (2 * n); // of one of two workgroups of a CU
+    int64_t       chunk = longest <= std::max<int64_t>(16, 2 * half + half / 2) ? longest : std::max<int64_t>(8, half);
+    plan.chunk = (int)std::max<int64_t>(1, std::min<int64_t>(chunk, 1 << 24));
+    auto item_tiles = [&](const QuantEntry &e) {
+        const int k = quant_items(e.S, plan.chunk);
+        return k ? (quant_tiles(e.S) + k - 1) / k : 0;
+    };
+    std::stable_sort(plan.entries.begin(), plan.entries.end(),
+                     [&](const QuantEntry &x, const QuantEntry &y) { return item_tiles(x) > item_tiles(y); });
+    plan.launches.clear();
+    for (size_t i = 0; i < plan.entries.size();) {
+        QuantLaunch l{(int)i, 0, 0, 1, false};
+        for (; i < plan.entries.size() && l.n < kQuantBatch; ++i, ++l.n) {
+            QuantEntry &e = plan.entries[i];
+            const int   items = quant_items(e.S, plan.chunk);
+            e.item0 = l.items;
+            l.items += items;
+            l.rows = std::max(l.rows, e.nq * G);
+            l.finish |= items != 1;
+        }
+        plan.launches.push_back(l);
+    }
+}
+
+bool plan_quant_prefill(QuantPrefillPlan &plan, int D, int G, int Hkv, int cus) {
+    const int64_t n = std::max(1, cus);
+    plan.waves = D <= 128 ? 8 : 4;
+    const int tile = quant_prefill_rows(D, plan.waves);
+    int64_t   tiles = 0;
+    for (const auto &e : plan.entries) tiles += ((int64_t)e.nq * G + tile - 1) / tile;
+    const int64_t work = std::max<int64_t>(1, tiles * Hkv), once = std::max<int64_t>(1, n / work);
+    for (auto &e : plan.entries) e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(once, quant_tiles(e.S) / 3));
+    std::stable_sort(plan.entries.begin(), plan.entries.end(), [](const QuantPrefillEntry &x, const QuantPrefillEntry &y) {
+        return (int64_t)x.S * y.nch > (int64_t)y.S * x.nch;
+    });
+    plan.launches.clear();
+    for (size_t i = 0; i < plan.entries.size();) {
+        QuantPrefillLaunch l{(int)i, 0, 0, false};
+        int64_t            items = 0;
+        for (; i < plan.entries.size() && l.n < kQuantPrefillBatch; ++i, ++l.n) {
+            QuantPrefillEntry &e = plan.entries[i];
+            e.item0 = (int32_t)items;
+            items += ((int64_t)e.nq * G + tile - 1) / tile * e.nch;
+            l.split |= e.nch > 1;
+            if (items * Hkv > kQuantMostItems) return false;
+        }
+        l.items = (int)items;
+        plan.launches.push_back(l);
+    }
+    return true;
+}
+
+} // namespace detail
+} // namespace tiny_llm

@@ -1,0 +1,203 @@
+// The cache in 8 bits: KVCacheManager::createQuantized and the steps of batches over it.
+#include "quantized.h"
+
+#include "block_allocator.h"
+#include "tl_log.h"
+
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <string>
+#include <vector>
+
+namespace tiny_llm {
+
+using detail::kGroup;
+
+Result<std::unique_ptr<KVCacheManager>> KVCacheManager::createQuantized(const KVCacheConfig &config, int block_tokens,
+                                                                        int num_blocks) {
+    using R = Result<std::unique_ptr<KVCacheManager>>;
+    if (block_tokens < kGroup || (block_tokens & (block_tokens - 1)) != 0)
+        return R::err("KVCacheManager: block_tokens of an 8-bit cache must be a power of two >= 32 (got " +
+                      std::to_string(block_tokens) + ")");
+    if (num_blocks <= 0 || num_blocks == INT32_MAX)
+        return R::err("KVCacheManager: num_blocks must be in [1, 2^31 - 2] (got " + std::to_string(num_blocks) + ")");
+    const int d = config.head_dim;
+    if (d > 0 && d != 32 && d != 64 && d != 128 && d != 256)
+        return R::err("KVCacheManager: unsupported head_dim " + std::to_string(d) + " of an 8-bit cache (32, 64, 128 or 256)");
+    return build(config, block_tokens, num_blocks, true);
+}
+
+detail::QuantView KVCacheManager::quantView(int layer_idx) const {
+    const int64_t     heads = config_.num_heads, tile = 2 * kGroup * static_cast<int64_t>(config_.head_dim);
+    const int64_t     layer = (static_cast<int64_t>(blocks_->numBlocks()) + 1) * heads * (block_tokens_ / kGroup); // groups
+    detail::QuantView v;
+    v.tiles = reinterpret_cast<uint8_t *>(memory_pool_) + layer_idx * layer * tile;
+    v.scales = scales_ + layer_idx * layer;
+    v.open = open_tiles_ + layer_idx * (static_cast<int64_t>(config_.max_batch_size) * 2 * heads * tile);
+    v.table = block_map_dev_;
+    v.bt_stride = blocks_->blocksPerRow();
+    while ((kGroup << v.lg) < block_tokens_) ++v.lg;
+    return v;
+}
+
+const detail::OpenGroup &KVCacheManager::openGroup(int slot) const noexcept { return open_[static_cast<size_t>(slot)]; }
+
+void KVCacheManager::noteAppend(int slot, int n) noexcept {
+    open_[static_cast<size_t>(slot)].append(slots_[static_cast<size_t>(slot)].current_len, n);
+}
+
+namespace detail {
+
+std::string check_quant_call(const char *who, const KVCacheManager &mgr, std::initializer_list<const void *> buffers) {
+    if (const int now = current_device(); now != mgr.device())
+        return std::string(who) + ": the cache is on device " + std::to_string(mgr.device()) + ", the current one is " +
+               std::to_string(now);
+    for (const void *p : buffers)
+        if (reinterpret_cast<uintptr_t>(p) & 15u) return std::string(who) + ": buffers must be 16-byte aligned";
+    return std::string();
+}
+
+int held_tokens(const KVCacheManager &mgr, int seq_id, int slot) {
+    return mgr.openGroup(slot).held(mgr.sequence(seq_id)->current_len).first;
+}
+
+void QuantStep::clear() {
+    entries.clear();
+    appends.clear();
+    stream.clear();
+    prefill.clear();
+    seen_.clear();
+}
+
+int QuantStep::items() const {
+    int n = 0;
+    for (const auto &l : stream.launches) n += l.items;
+    for (const auto &l : prefill.launches) n += l.items;
+    return n;
+}
+
+void QuantStep::see(const KVCacheManager &mgr, int32_t id, int32_t slot, bool reads_only) {
+    seen_.push_back({id, slot, mgr.sequence(id)->current_len, reads_only ? held_tokens(mgr, id, slot) : -1});
+}
+
+std::string QuantStep::check(const char *who, const KVCacheManager &mgr, std::initializer_list<const void *> buffers) const {
+    for (const Seen &s : seen_) {
+        const SequenceCache *sc = mgr.sequence(s.id);
+        if (!sc || mgr.slotOf(s.id) != s.slot || sc->current_len != s.len || (s.held >= 0 && held_tokens(mgr, s.id, s.slot) != s.held))
+            return std::string(who) + ": sequence " + std::to_string(s.id) + " has changed since prepare";
+    }
+    return check_quant_call(who, mgr, buffers);
+}
+
+void QuantStep::noteAppends(KVCacheManager &mgr) const {
+    for (const QuantAppend &a : appends) mgr.noteAppend(a.row, a.n);
+}
+
+void QuantStep::prepareDecode(const KVCacheManager &mgr, const std::vector<int32_t> &ids, const std::vector<int32_t> &slots,
+                              const std::vector<int32_t> &lens, bool appendable, int num_q_heads) {
+    const KVCacheConfig &cfg = mgr.getConfig();
+    for (size_t i = 0; i < ids.size(); ++i) {
+        see(mgr, ids[i], slots[i], !appendable);
+        const int S = lens[i], tok = static_cast<int>(i);
+        if (appendable) {
+            const int tile = mgr.openGroup(slots[i]).cur;
+            appends.push_back({slots[i], S - 1, 1, tok, tile | tile << 1, 0});
+            entries.push_back({slots[i], S, tok, 1, tile, 0});
+        } else {
+            // A last group that is complete in the cache is read there; what a sequence has
+            // advanced over stands as it did then, whatever was appended behind it.
+            const int len = mgr.sequence(ids[i])->current_len;
+            auto [held, tile] = mgr.openGroup(slots[i]).held(len);
+            if (S <= len) {
+                held = len;
+                tile = mgr.openGroup(slots[i]).cur;
+            }
+            entries.push_back({slots[i], S, tok, 1, S > held / kGroup * kGroup ? tile : -1, 0});
+        }
+    }
+    stream.entries = entries;
+    plan_quant(stream, num_q_heads / cfg.num_heads, cfg.num_heads, cfg.head_dim, device_cus());
+}
+
+bool QuantStep::preparePrefill(const KVCacheManager &mgr, const std::vector<int32_t> &ids, const std::vector<int32_t> &slots,
+                               const std::vector<int32_t> &counts, int num_q_heads) {
+    const KVCacheConfig &cfg = mgr.getConfig();
+    const int            group = num_q_heads / cfg.num_heads;
+    int                  tok = 0;
+    for (size_t i = 0; i < ids.size(); ++i) {
+        see(mgr, ids[i], slots[i], false);
+        const int n = counts[i], p0 = mgr.sequence(ids[i])->current_len, S = p0 + n;
+        const auto [first, last] = mgr.openGroup(slots[i]).tiles(p0, n);
+        const int open = S % kGroup != 0 ? last : -1;
+        appends.push_back({slots[i], p0, n, tok, first | last << 1, 0});
+        entries.push_back({slots[i], S, tok, n, open, 0});
+        if (static_cast<int64_t>(n) * group <= kQuantRows) stream.entries.push_back(entries.back());
+        else if (static_cast<int64_t>(n) * group > INT32_MAX / 2) return false;
+        else prefill.entries.push_back({slots[i], S, tok, n, open, 1, 0});
+        tok += n;
+    }
+    plan_quant(stream, group, cfg.num_heads, cfg.head_dim, device_cus());
+    return plan_quant_prefill(prefill, cfg.head_dim, group, cfg.num_heads, device_cus());
+}
+
+Result<void> QuantStep::appendOne(KVCacheManager &mgr, int layer_begin, int num_layers, const half *new_k,
+                                  const half *new_v, hipStream_t stream) {
+    if (std::string err = check("DecodeBatch", mgr, {new_k, new_v}); !err.empty()) return Result<void>::err(err);
+    const KVCacheConfig &cfg = mgr.getConfig();
+    const QuantView      v = mgr.quantView(layer_begin);
+    QuantLayerSteps      steps;
+    if (num_layers > 1) {
+        const QuantView w = mgr.quantView(layer_begin + 1);
+        steps = {w.tiles - v.tiles, w.scales - v.scales, w.open - v.open};
+    }
+    launch_quant_append_one(v, steps, appends, num_layers, cfg.num_heads, cfg.head_dim, new_k, new_v, stream);
+    noteAppends(mgr);
+    return Result<void>::ok();
+}
+
+Result<void> QuantStep::append(const char *who, KVCacheManager &mgr, int layer_idx, const half *new_k, const half *new_v,
+                               hipStream_t stream) {
+    if (std::string err = check(who, mgr, {new_k, new_v}); !err.empty()) return Result<void>::err(err);
+    const KVCacheConfig &cfg = mgr.getConfig();
+    launch_quant_append(mgr.quantView(layer_idx), appends, cfg.num_heads, cfg.head_dim, new_k, new_v, stream);
+    noteAppends(mgr);
+    return Result<void>::ok();
+}
+
+Result<void> QuantStep::attention(const char *who, KVCacheManager &mgr, int layer_idx, const half *q, const half *new_k,
+                                  const half *new_v, half *out, float scale, int num_q_heads, hipStream_t stream) {
+    if (std::string err = check(who, mgr, {q, new_k, new_v, out}); !err.empty()) return Result<void>::err(err);
+    const KVCacheConfig &cfg = mgr.getConfig();
+    const size_t floats = std::max(quant_workspace_floats(this->stream, cfg.num_heads, cfg.head_dim),
+                                   quant_prefill_workspace_floats(prefill, cfg.num_heads, cfg.head_dim));
+    if (!work.holds(floats) && stream_capturing(stream))
+        return Result<void>::err(std::string(who) + ": the workspace cannot grow while the stream is captured: make one "
+                                                    "call of this size before");
+    float    *ws = work.get(floats);
+    QuantCall c;
+    c.q = q;
+    c.out = out;
+    c.new_k = new_k;
+    c.new_v = new_v;
+    c.scale = scale;
+    c.Hq = num_q_heads;
+    c.Hkv = cfg.num_heads;
+    c.D = cfg.head_dim;
+    const QuantView v = mgr.quantView(layer_idx);
+    if (!this->stream.entries.empty()) launch_attn_quant(c, v, this->stream, ws, stream);
+    if (!prefill.entries.empty()) launch_quant_prefill(c, v, prefill, ws, stream);
+    if (new_k) noteAppends(mgr);
+    return Result<void>::ok();
+}
+
+Result<void> QuantStep::gather(KVCacheManager &mgr, int layer_idx, half *k_out, half *v_out, int s_max,
+                               hipStream_t stream) {
+    if (std::string err = check("DecodeBatch", mgr, {k_out, v_out}); !err.empty()) return Result<void>::err(err);
+    const KVCacheConfig &cfg = mgr.getConfig();
+    launch_quant_gather(mgr.quantView(layer_idx), entries, cfg.num_heads, cfg.head_dim, s_max, k_out, v_out, stream);
+    return Result<void>::ok();
+}
+
+} // namespace detail
+} // namespace tiny_llm

@@ -1,0 +1,58 @@
+// Prepared steps of batches over a cache in 8 bits (KVCacheManager::createQuantized).
+#pragma once
+
+#include "kernels/kv_kernels.h"
+#include "kernels/quant.h"
+#include "runtime.h"
+#include "tiny_llm/kv_cache.h"
+
+#include <initializer_list>
+#include <string>
+#include <vector>
+
+namespace tiny_llm {
+namespace detail {
+
+// "" when a call may run on the manager's device with these (possibly null) buffers.
+std::string check_quant_call(const char *who, const KVCacheManager &mgr, std::initializer_list<const void *> buffers);
+
+// Tokens that a sequence's cache holds, appended ones that it did not advance over included.
+int held_tokens(const KVCacheManager &mgr, int seq_id, int slot);
+
+struct QuantStep {
+    std::vector<QuantEntry>  entries; // in the batch's order
+    std::vector<QuantAppend> appends;
+    QuantPlan                stream;  // entries of up to kQuantRows query rows,
+    QuantPrefillPlan         prefill; // and those of more
+    Workspace                work;
+
+    void clear();
+    int  items() const;
+    void prepareDecode(const KVCacheManager &mgr, const std::vector<int32_t> &ids, const std::vector<int32_t> &slots,
+                       const std::vector<int32_t> &lens, bool appendable, int num_q_heads);
+    // False: too many query rows for one step.
+    bool preparePrefill(const KVCacheManager &mgr, const std::vector<int32_t> &ids, const std::vector<int32_t> &slots,
+                        const std::vector<int32_t> &counts, int num_q_heads);
+
+    Result<void> appendOne(KVCacheManager &mgr, int layer_begin, int num_layers, const half *new_k, const half *new_v,
+                           hipStream_t stream);
+    Result<void> append(const char *who, KVCacheManager &mgr, int layer_idx, const half *new_k, const half *new_v,
+                        hipStream_t stream);
+    Result<void> attention(const char *who, KVCacheManager &mgr, int layer_idx, const half *q, const half *new_k,
+                           const half *new_v, half *out, float scale, int num_q_heads, hipStream_t stream);
+    Result<void> gather(KVCacheManager &mgr, int layer_idx, half *k_out, half *v_out, int s_max, hipStream_t stream);
+
+  private:
+    // The sequences as prepare found them: their lengths and, for a step that only reads,
+    // what they held.
+    struct Seen {
+        int32_t id, slot, len, held;
+    };
+    std::vector<Seen> seen_;
+    void              see(const KVCacheManager &mgr, int32_t id, int32_t slot, bool reads_only);
+    std::string       check(const char *who, const KVCacheManager &mgr, std::initializer_list<const void *> buffers) const;
+    void              noteAppends(KVCacheManager &mgr) const;
+};
+
+} // namespace detail
+} // namespace tiny_llm

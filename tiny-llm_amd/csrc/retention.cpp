@@ -54,6 +54,7 @@ Result<void> DecodeBatch::decodeWeights(int layer_idx, const half *q, const half
                                         float scale, const float *weights_in, float *weights_out,
                                         hipStream_t stream) {
     const KVCacheConfig &cfg = mgr_.getConfig();
+    if (mgr_.isQuantized()) return Result<void>::err("DecodeBatch: accounts are kept over fp16 caches only");
     if (q == nullptr || out == nullptr) return Result<void>::err("DecodeBatch: q/out is null");
     if ((new_k == nullptr) != (new_v == nullptr))
         return Result<void>::err(new_k ? "new_v is null" : "new_k is null");
@@ -100,6 +101,7 @@ Result<void> DecodeBatch::decodeWeights(int layer_idx, const half *q, const half
 Result<void> PrefillBatch::weights(int layer_idx, const half *q, float scale, int window, const float *weights_in,
                                    float *weights_out, hipStream_t stream) {
     const KVCacheConfig &cfg = mgr_.getConfig();
+    if (mgr_.isQuantized()) return Result<void>::err("PrefillBatch: accounts are kept over fp16 caches only");
     if (layer_idx < 0 || layer_idx >= cfg.num_layers)
         return Result<void>::err("PrefillBatch: Invalid layer_idx: " + std::to_string(layer_idx));
     if (q == nullptr) return Result<void>::err("PrefillBatch: q is null");
@@ -154,6 +156,7 @@ EvictBatch::~EvictBatch() = default;
 Result<std::unique_ptr<EvictBatch>> EvictBatch::create(KVCacheManager &mgr, int max_seqs) {
     using R = Result<std::unique_ptr<EvictBatch>>;
     const int d = mgr.getConfig().head_dim;
+    if (mgr.isQuantized()) return R::err("EvictBatch: tokens are evicted from fp16 caches only");
     if (max_seqs <= 0) return R::err("EvictBatch: max_seqs must be positive");
     if (d != 32 && d != 64 && d != 128 && d != 256)
         return R::err("EvictBatch: unsupported head_dim " + std::to_string(d) + " (32, 64, 128 or 256)");

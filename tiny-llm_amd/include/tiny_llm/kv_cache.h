@@ -9,7 +9,8 @@
 // A block-granular pool (createPaged) instead holds num_blocks blocks of
 // block_tokens tokens plus one spare block:
 //   [layer][K|V][num_blocks + 1][block_tokens][num_heads][head_dim]  fp16
-// and a sequence is handed blocks as it grows (see BlockAllocator).
+// and a sequence is handed blocks as it grows (see BlockAllocator).  A pool in 8 bits
+// (createQuantized) is a block pool of groups of 32 tokens (layout: csrc/kernels/quant.h).
 #pragma once
 
 #include "tiny_llm/hip_utils.h"
@@ -39,6 +40,9 @@ struct EvictEntry;
 struct StreamPlan;
 struct AccountPlan;
 struct CrossPlan;
+struct QuantView;
+struct QuantStep;
+struct OpenGroup;
 class MetaRing;
 class DeviceRing;
 class Workspace;
@@ -97,6 +101,27 @@ class KVCacheManager {
     static Result<std::unique_ptr<KVCacheManager>> createPaged(const KVCacheConfig &config,
                                                                int block_tokens, int num_blocks);
     bool   isBlockPool() const noexcept { return blocks_ != nullptr; }
+    // A block pool that holds K and V in 8 bits, block_tokens a power of two >= 32,
+    // head_dim 32, 64, 128 or 256.  32 consecutive tokens of a kv head (a group) share a scale, one
+    // for K and one for V: the group's largest magnitude / 127, cut down to 11 significant
+    // bits; a value x is the whole number round_half_even(x / scale), so at most half a
+    // scale off.  Groups begin at multiples of 32 tokens; a sequence's last, incomplete one
+    // stays in fp16 as it was given, and is rounded once, by the append of its last token:
+    // the cached bytes do not depend on how the tokens came.  A group with an infinity or a NaN
+    // reads back as NaN.
+    //   The calls are those of every manager: appendKV, DecodeBatch::append / attention /
+    // decode / gather and PrefillBatch::append / attention / prefill write, read and
+    // attend to what the cache stands for after the append; q, out, new_k and new_v are 16-byte
+    // aligned.  Accounts, projections, eviction and CrossBatch are refused.
+    //   An append replaces what was appended at its position before and not advanced over.
+    // Between prepare and commit of a batch its sequences' lengths must not change (its calls
+    // refuse).  A sequence may advance over less than was appended (drafted tokens that were
+    // rejected), to a multiple of 32, within the group in which the append began or the one
+    // in which it ended; elsewhere the rows that the open group needs are gone, and
+    // advanceSeqLen refuses.
+    static Result<std::unique_ptr<KVCacheManager>> createQuantized(const KVCacheConfig &config,
+                                                                   int block_tokens, int num_blocks);
+    bool   isQuantized() const noexcept { return quantized_; }
     int    numBlocks() const noexcept;
     int    freeBlocks() const noexcept;
     size_t blockBytes() const noexcept;
@@ -128,11 +153,16 @@ class KVCacheManager {
     int                  device() const noexcept { return device_; }
     // Layer view for batch kernels; seq_row_dev holds the slot of each entry.
     detail::KvView layerView(int layer_idx, const int32_t *seq_row_dev) const;
+    // The same of a pool in 8 bits.
+    detail::QuantView quantView(int layer_idx) const;
+    // The open group of a slot of such a pool, and that an append of n tokens to it was queued.
+    const detail::OpenGroup &openGroup(int slot) const noexcept;
+    void                     noteAppend(int slot, int n) noexcept;
 
   private:
     explicit KVCacheManager(const KVCacheConfig &config);
-    static Result<std::unique_ptr<KVCacheManager>> build(const KVCacheConfig &config,
-                                                         int block_tokens, int num_blocks);
+    static Result<std::unique_ptr<KVCacheManager>> build(const KVCacheConfig &config, int block_tokens,
+                                                         int num_blocks, bool quantized);
     Result<void> exhausted(int64_t need) const;
 
     size_t calculateOffset(int slot_idx, int layer_idx, bool is_value) const;
@@ -164,6 +194,11 @@ class KVCacheManager {
     std::vector<int32_t> block_map_host_;
     int64_t  layer_stride_ = 0;          // elements between consecutive layers' K bases
     std::unique_ptr<detail::BlockAllocator> blocks_;  // block pool only
+
+    bool    quantized_ = false;
+    float2 *scales_ = nullptr;     // [layer][block][kv head][group] (K, V)
+    half   *open_tiles_ = nullptr; // [layer][slot][2][kv head][64 D]
+    std::vector<detail::OpenGroup> open_;
 };
 
 // A decode step over n sequences of one manager.  prepare() snapshots the
@@ -257,6 +292,7 @@ class DecodeBatch {
     // decodeWeights: its plan, made by the first call of a prepared step, and workspace.
     std::unique_ptr<detail::StreamPlan> account_plan_;
     std::unique_ptr<detail::Workspace>  account_work_;
+    std::unique_ptr<detail::QuantStep>  quant_; // a pool in 8 bits: the prepared step
 };
 
 // A prefill step over n sequences of one manager: sequence i brings
@@ -335,6 +371,7 @@ class PrefillBatch {
     // weights: its plan, made by the first call of a prepared step and window, and workspace.
     std::unique_ptr<detail::AccountPlan> account_plan_;
     std::unique_ptr<detail::Workspace>   account_work_;
+    std::unique_ptr<detail::QuantStep>   quant_; // a pool in 8 bits: the prepared step
 };
 
 // Eviction from the caches of n sequences of one manager by accumulated

@@ -121,6 +121,8 @@ def _declare(L: C.CDLL) -> None:
         "tl_kv_slot_of": (i, [vp, i]),
         "tl_kv_set_block_map": (i, [vp, i, vp, sz]),
         "tl_kv_create_paged": (i, [C.POINTER(KVConfig), i, i, C.POINTER(vp)]),
+        "tl_kv_create_quantized": (i, [C.POINTER(KVConfig), i, i, C.POINTER(vp)]),
+        "tl_kv_is_quantized": (i, [vp]),
         "tl_kv_num_blocks": (i, [vp]),
         "tl_kv_free_blocks": (i, [vp]),
         "tl_kv_block_bytes": (sz, [vp]),
@@ -170,6 +172,9 @@ def _declare(L: C.CDLL) -> None:
         "tl_kv_cross_prepare": (i, [vp, vp, vp, vp, i, vp]),
         "tl_kv_cross_info": (i, [vp, ip, ip]),
         "tl_kv_cross_attention": (i, [vp, i, vp, vp, f, vp]),
+        "tl_rotary_create": (i, [i, i, C.c_double, i, vp, vp, C.POINTER(vp)]),
+        "tl_rotary_destroy": (None, [vp]),
+        "tl_rotary_apply": (i, [vp, vp, C.c_int64, vp, C.c_int64, vp, vp, vp, i, i, i, vp, vp, f, vp]),
         "tl_prefill_set_waves": (i, [i]),
         "tl_prefill_get_waves": (i, []),
         "tl_prefill_plan_waves": (i, [vp, vp, i, i, i, i, i, ip]),
@@ -222,16 +227,19 @@ class KVCacheManager:
     """tiny_llm::KVCacheManager over HIP (same method names as the reference)."""
 
     def __init__(self, num_layers=32, num_heads=32, head_dim=128, max_seq_len=2048,
-                 max_batch_size=1, block_tokens=0, num_blocks=0):
+                 max_batch_size=1, block_tokens=0, num_blocks=0, quantized=False):
         """block_tokens > 0: a block-granular pool of num_blocks blocks
-        (tl_kv_create_paged); otherwise the reference's slot pool."""
+        (tl_kv_create_paged; quantized: in 8 bits, tl_kv_create_quantized);
+        otherwise the reference's slot pool."""
         L = load()
         # the destructor's handle: module globals may already be None when a
         # manager is collected at interpreter shutdown
         self._destroy = L.tl_kv_destroy
         self.config = KVConfig(num_layers, num_heads, head_dim, max_seq_len, max_batch_size)
         self._h = C.c_void_p()
-        if block_tokens:
+        if quantized:
+            _check(L.tl_kv_create_quantized(C.byref(self.config), block_tokens, num_blocks, C.byref(self._h)))
+        elif block_tokens:
             _check(L.tl_kv_create_paged(C.byref(self.config), block_tokens, num_blocks,
                                         C.byref(self._h)))
         else:
@@ -271,6 +279,9 @@ class KVCacheManager:
     def getCache(self, seq_id, layer_idx):
         r, _ = self.getCacheChecked(seq_id, layer_idx)
         return r if r is not None else (0, 0)
+
+    def isQuantized(self):
+        return bool(load().tl_kv_is_quantized(self._h))
 
     def numBlocks(self):
         return load().tl_kv_num_blocks(self._h)
@@ -531,6 +542,43 @@ class CrossBatch:
 
     def attention(self, layer, q, out, scale, stream=0):
         _check(load().tl_kv_cross_attention(self._h, layer, q, out, scale, stream))
+
+
+class Rotary:
+    """tiny_llm::kernels::Rotary: RMS norm of query and key heads and their rotation
+    by position, in one pass (tl_rotary_*)."""
+
+    def __init__(self, head_dim, rotary_dim=None, theta=10000.0, interleaved=False, axis_of=None, inv_freq=None):
+        """rotary_dim None: all of head_dim; axis_of: the axis of each of the
+        rotary_dim / 2 pairs (None: one axis); inv_freq: the pairs' inverse
+        frequencies in place of theta's."""
+        self._h = C.c_void_p()
+        self._destroy = load().tl_rotary_destroy  # usable at interpreter shutdown
+        rd = head_dim if rotary_dim is None else rotary_dim
+        for name, x in (("axes", axis_of), ("inverse frequencies", inv_freq)):
+            if x is not None and len(x) != rd // 2:
+                raise ValueError(f"{len(x)} {name} for {rd // 2} pairs")
+        axes = (C.c_int * max(1, rd // 2))(*axis_of) if axis_of is not None else None
+        freq = (C.c_double * max(1, rd // 2))(*inv_freq) if inv_freq is not None else None
+        _check(load().tl_rotary_create(head_dim, rd, theta, int(interleaved), axes, freq, C.byref(self._h)))
+        self.head_dim = head_dim
+
+    def close(self):
+        if getattr(self, "_h", None):
+            self._destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        self.close()
+
+    def apply(self, q, k, q_out, k_out, positions, num_tokens, num_q_heads, num_kv_heads, q_weight=None, k_weight=None,
+              eps=1e-5, q_stride=0, k_stride=0, stream=0):
+        """Device addresses; strides in elements from token to token, 0: dense; k and
+        k_out None: queries alone; a weight None: that one is not normed."""
+        _check(load().tl_rotary_apply(self._h, q, q_stride or num_q_heads * self.head_dim, k or None,
+                                      k_stride or num_kv_heads * self.head_dim, q_out, k_out or None, positions,
+                                      num_tokens, num_q_heads, num_kv_heads, q_weight or None, k_weight or None, eps,
+                                      stream))
 
 
 def attention_prefill(q, k, v, out, scale, batch, num_heads, seq_len, head_dim, stream=0):
