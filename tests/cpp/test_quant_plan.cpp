@@ -77,7 +77,7 @@ static void prefill_random() {
             p.entries.push_back({i, S, i, nq, S % kGroup ? 1 : -1, 1, 0});
         }
         CHECK(plan_quant_prefill(p, D, G, Hkv, cus));
-        const int        rows = quant_prefill_rows(D, p.waves);
+        const int        rows = quant_prefill_rows(D);
         std::vector<int> seen((size_t)n, 0);
         int              next = 0;
         for (const auto &l : p.launches) {

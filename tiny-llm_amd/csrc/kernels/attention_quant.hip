@@ -48,7 +48,8 @@ struct QuantArgs {
     float          *part_ml; // [item][Hkv][rows][2]
     QuantView       v;
     float           scale_log2;
-    int             Hq, Hkv, G, n, chunk, rows;
+    int             Hq, Hkv, G, n, items, chunk, rows;
+    int             each; // work items of every entry, 0: they differ
     QuantEntry      e[kQuantBatch];
 };
 static_assert(sizeof(QuantArgs) <= 4096, "kernel arguments");
@@ -61,29 +62,26 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
     constexpr int NT = NW * 64;
     extern __shared__ __align__(16) float so[]; // the waves' outputs [NW][rows][D]
     __shared__ float    sm[NW][16], sl[NW][16], s_l[16];
-    __shared__ uint32_t red[2 * NW];
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int item = blockIdx.x / a.Hkv, g = blockIdx.x - item * a.Hkv;
-    int       ei;
-    QUANT_ENTRY_OF(a, item, ei);
+    int       item, g;
+    quant_place(blockIdx.x, a.Hkv, item, g);
+    if (item >= a.items) return;
+    int ei = a.each ? item / a.each : 0;
+    if (!a.each) QUANT_ENTRY_OF(a, item, ei);
     const int row = a.e[ei].row, S = a.e[ei].S, tok0 = a.e[ei].tok0, nq = a.e[ei].nq, rows = nq * a.G;
     const int tiles = (S + kQuantTile - 1) / kQuantTile;
     const int nch = (tiles + a.chunk - 1) / a.chunk, ch = item - a.e[ei].item0;
     const int tile_lo = (int)((int64_t)ch * tiles / nch), tile_hi = (int)((int64_t)(ch + 1) * tiles / nch);
-    int       open = a.e[ei].open;
-
-    if (a.new_k) {
-        if (ch == nch - 1) { // the new token, then read like any other
-            const int     t = S - 1;
-            const int64_t at = tile_of(a.v, a.Hkv, row, g, t / kGroup), src = ((int64_t)tok0 * a.Hkv + g) * D;
-            append_token<D, NT>(open_of<D>(a.v, a.Hkv, row, open, g), t % kGroup, a.new_k + src, a.new_v + src,
-                                a.v.tiles + at * (64 * D), a.v.scales + at, red);
-        }
-    }
-    if (S % kGroup == 0) open = -1; // the last token closed its group
-    const int closed = open < 0 ? S : S / kGroup * kGroup; // tokens in 8 bits
-    const int groups = (closed + kGroup - 1) / kGroup;
+    const int open = S % kGroup == 0 ? -1 : a.e[ei].open; // (-1: the last token closes its group)
+    const int last = (S - 1) / kGroup * kGroup;           // first token of the last group
+    // The last group is a step of its own where it is open, and where this launch appends to it, by
+    // the wave that has the fewest others.
+    const bool apart = a.new_k || open >= 0;
+    const int  closed = apart ? last : S;               // tokens of the other steps,
+    const int  groups = (closed + kGroup - 1) / kGroup; // all in 8 bits
+    const int  end = min(tile_hi, (groups + 1) / 2);
+    const bool ends = apart && ch == nch - 1 && wave == max(0, end - tile_lo) % NW;
 
     const int c = lane & 15, qg = lane >> 4;
     f16x8     qb[KS]; // B operand: row c, dims 32s + 8qg .. +7
@@ -113,18 +111,19 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
     };
 
     // The wave's steps: step x is half (all) of tile tile_lo + x / SUB * NW + wave.
-    const int end = min(tile_hi, (groups + 1) / 2);
     const int steps = max(0, (end - tile_lo - wave + NW - 1) / NW) * SUB;
     auto      first_group = [&](int x) { return (tile_lo + x / SUB * NW + wave) * 2 + x % SUB * NG; };
     const int32_t *bt = a.v.table + (int64_t)row * a.v.bt_stride;
-    // Blocks of a step's groups, lane k that of group k; asked for a step before the tiles.
-    auto blocks = [&](int x) -> int { return lane < NG ? bt[min(first_group(x) + lane, groups - 1) >> a.v.lg] : 0; };
+    // Blocks of a step's groups, lane k that of group k; asked for a step before the tiles.  (Neither
+    // these loads nor the tiles' are conditional: the compiler waits by counting the
+    // loads on their way, and behind a branch it waits for all of them.)
+    auto blocks = [&](int x) -> int { return bt[min(first_group(min(x, steps - 1)) + min(lane, NG - 1), groups - 1) >> a.v.lg]; };
     auto tile_at = [&](int x, int k, int ids) __attribute__((always_inline)) -> int64_t {
         const int i = min(first_group(x) + k, groups - 1) & ((1 << a.v.lg) - 1);
         return (((int64_t)__builtin_amdgcn_readlane(ids, k) * a.Hkv + g) << a.v.lg) + i;
     };
     u32x4  kr[NG][KS], vr[NG][DT / 2];
-    float2 sc[NG], sc_next[NG];
+    float2 sc[NG];
     auto   load_k = [&](int x, int ids) __attribute__((always_inline)) {
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
@@ -132,7 +131,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
             const u32x4  *p = reinterpret_cast<const u32x4 *>(a.v.tiles + at * (64 * D)) + lane;
 #pragma unroll
             for (int s = 0; s < KS; ++s) kr[k][s] = __builtin_nontemporal_load(p + 64 * s);
-            sc_next[k] = a.v.scales[at];
+            sc[k] = a.v.scales[at];
         }
     };
     auto load_v = [&](int x, int ids) __attribute__((always_inline)) {
@@ -144,18 +143,20 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
         }
     };
 
-    int ids = steps > 0 ? blocks(0) : 0, next = steps > 1 ? blocks(1) : 0;
-    if (steps > 0) {
-        load_k(0, ids);
-        load_v(0, ids);
-    }
-    for (int x = 0; x < steps; ++x) {
-        const int  g0 = first_group(x), t0 = g0 * kGroup;
-        const bool more = x + 1 < steps;
-        ids = next;
-        if (x + 2 < steps) next = blocks(x + 2);
+    int  ids = 0, next = 0;
+    auto step = [&](int x, auto more) __attribute__((always_inline)) {
+        const int g0 = first_group(x), t0 = g0 * kGroup;
+        if constexpr (more) {
+            ids = next;
+            next = blocks(x + 2);
+        }
+        // The scales in scalar registers, before the next ones' loads.
+        float ks[NG], vs[NG];
 #pragma unroll
-        for (int k = 0; k < NG; ++k) sc[k] = sc_next[k];
+        for (int k = 0; k < NG; ++k) {
+            ks[k] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sc[k].x)));
+            vs[k] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sc[k].y)));
+        }
         f32x4 s[NG][2];
 #pragma unroll
         for (int k = 0; k < NG; ++k)
@@ -166,13 +167,13 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
                 for (int i = 0; i < KS; ++i)
                     s[k][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(whole8(kr[k][i][2 * tt], kr[k][i][2 * tt + 1]), qb[i], s[k][tt], 0, 0, 0);
             }
-        if (more) load_k(x + 1, ids);
+        if constexpr (more) load_k(x + 1, ids);
         float mloc = -INFINITY;
         const bool masked = t0 + NG * kGroup > min(all, closed); // some score does not count
         const int  bound = min(lim, closed);
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
-            const float f = sc[k].x * a.scale_log2;
+            const float f = ks[k] * a.scale_log2;
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
@@ -195,39 +196,54 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
                     pf[4 * tt + i] = (_Float16)p;
                 }
             // (a group whose scale is NaN is none of the rows' business that see none of it)
-            const float vs = t0 + 32 * k < bound ? sc[k].y : 0.0f;
+            const float by = t0 + 32 * k < bound ? vs[k] : 0.0f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const u32x4 w = vr[k][dt / 2];
                 const f32x4 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(whole8(w[2 * (dt & 1)], w[2 * (dt & 1) + 1]), pf,
                                                                       f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc[dt][i] = fmaf(vs, o[i], acc[dt][i]);
+                for (int i = 0; i < 4; ++i) acc[dt][i] = fmaf(by, o[i], acc[dt][i]);
             }
         }
-        if (more) load_v(x + 1, ids);
+        if constexpr (more) load_v(x + 1, ids);
+    };
+    GroupRegs<D> group;
+    if (ends) {
+        const int64_t src = ((int64_t)tok0 * a.Hkv + g) * D;
+        if (a.new_k) group.fetch(S - 1 - last, a.new_k + src, a.new_v + src);
+        group.load(open_of<D>(a.v, a.Hkv, row, a.e[ei].open, g));
     }
-
-    // The open group, by the wave whose turn its tile is.
-    if (open >= 0 && ch == nch - 1 && wave == (tiles - 1 - tile_lo) % NW) {
-        const int       t0 = closed, cnt = S - t0;
-        const uint16_t *tile = open_of<D>(a.v, a.Hkv, row, open, g);
-        const f16x8    *kp = reinterpret_cast<const f16x8 *>(tile) + 2 * lane;
-        const f16x8    *vp = reinterpret_cast<const f16x8 *>(tile + 32 * D) + 2 * lane;
-        f32x4           s[2];
+    if (steps > 0) {
+        ids = blocks(0);
+        next = blocks(1);
+        load_k(0, ids);
+        load_v(0, ids);
+    }
+    if (ends) { // (while the first tile is on its way)
+        const int cnt = S - last;
+        if (a.new_k) {
+            group.append(open_of<D>(a.v, a.Hkv, row, a.e[ei].open, g), cnt - 1);
+            if (open < 0) {
+                const int64_t at = tile_of(a.v, a.Hkv, row, g, last / kGroup);
+                group.close(a.v.tiles + at * (64 * D), a.v.scales + at);
+            }
+        }
+        f32x4 s[2];
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt) {
             s[tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int i = 0; i < KS; ++i) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kp[128 * i + tt], qb[i], s[tt], 0, 0, 0);
+            for (int i = 0; i < KS; ++i) s[tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(group.kf[tt][i], qb[i], s[tt], 0, 0, 0);
         }
-        float mloc = -INFINITY;
+        float       mloc = -INFINITY;
+        const float f = group.ks * a.scale_log2;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float y = s[tt][i] * a.scale_log2;
-                s[tt][i] = t0 + 16 * tt + 4 * qg + i < lim ? y : -INFINITY;
+                const float y = s[tt][i] * f;
+                s[tt][i] = last + 16 * tt + 4 * qg + i < lim ? y : -INFINITY;
                 mloc = fmaxf(mloc, s[tt][i]);
             }
         raise(mloc);
@@ -245,7 +261,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
         bool odd = false;
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
-            f16x8 v = vp[128 * (dt / 2) + (dt & 1)];
+            f16x8 v = group.vf[dt];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const bool there = 16 * (j >> 2) + 4 * qg + (j & 3) < cnt;
@@ -253,19 +269,29 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
                 odd |= there && !finite;
                 if (!there || !finite) v[j] = (_Float16)0.0f;
             }
-            acc[dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf, acc[dt], 0, 0, 0);
+            const f32x4 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[dt][i] = fmaf(group.vs, o[i], acc[dt][i]);
         }
-        if (__any(odd)) {
+        if (__any(odd)) { // (of an open group: stored numbers are finite)
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            const uint16_t *tile = open_of<D>(a.v, a.Hkv, row, a.e[ei].open, g) + 32 * D;
             for (int r = 0; r < cnt; ++r)
-                if (t0 + r < lim)
+                if (last + r < lim)
 #pragma unroll
                     for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const float x = (float)__builtin_bit_cast(_Float16, tile[32 * D + v_half(r, 16 * dt + 4 * qg + i)]);
+                            const float x = (float)__builtin_bit_cast(_Float16, tile[v_half(r, 16 * dt + 4 * qg + i)]);
                             if (!(__builtin_fabsf(x) <= 65504.0f)) acc[dt][i] += x;
                         }
         }
+    }
+    if (steps > 0) {
+        for (int x = 0; x < steps - 1; ++x) step(x, std::true_type());
+        step(steps - 1, std::false_type());
     }
 
     // The waves' (m, l, o) through LDS.
@@ -317,39 +343,50 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
 
 constexpr int kFinishThreads = 256;
 
-// Entries of several chunks, or of no tokens (zeros).  Workgroup (entry, kv head; row): the
-// row's maximum and sum over the chunks, then its output, the chunks spread over the threads.
+// Entries of several chunks, or of no tokens (zeros).  Workgroup (entry, kv head; row): every
+// thread joins a few chunks' maxima, sums and outputs of four dims, all on their way at once,
+// then the threads of equal dims meet in LDS.
 __global__ __launch_bounds__(kFinishThreads) void quant_finish_kernel(QuantArgs a, int D) {
-    __shared__ f32x4 s_o[kFinishThreads];
+    __shared__ f32x4  s_o[kFinishThreads];
+    __shared__ float2 s_ml[kFinishThreads];
     const int ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv, r = blockIdx.y;
     const int S = a.e[ei].S, tok0 = a.e[ei].tok0, rows = a.e[ei].nq * a.G;
     const int tiles = (S + kQuantTile - 1) / kQuantTile, nch = (tiles + a.chunk - 1) / a.chunk;
     if (nch == 1 || r >= rows) return;
     const int64_t p0 = ((int64_t)a.e[ei].item0 * a.Hkv + g) * a.rows + r; // of chunk 0
     const int64_t pc = (int64_t)a.Hkv * a.rows;                          // from chunk to chunk
-    // (every wave for itself)
-    float m = kNone, l = 0.0f;
-    for (int ch = threadIdx.x & 63; ch < nch; ch += 64) m = fmaxf(m, a.part_ml[(p0 + ch * pc) * 2]);
-    for (int o = 1; o < 64; o <<= 1) m = fmaxf(m, __shfl_xor(m, o));
-    for (int ch = threadIdx.x & 63; ch < nch; ch += 64) {
-        const float2 ml = *reinterpret_cast<const float2 *>(a.part_ml + (p0 + ch * pc) * 2);
-        l = fmaf(__builtin_amdgcn_exp2f(ml.x - m), ml.y, l);
-    }
-    for (int o = 1; o < 64; o <<= 1) l += __shfl_xor(l, o);
-    const int per = D / 4, groups = kFinishThreads / per, grp = threadIdx.x / per, d = 4 * (threadIdx.x % per);
-    f32x4     o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int ch = grp; ch < nch; ch += groups) {
-        const int64_t pr = p0 + ch * pc;
-        const float   wgt = __builtin_amdgcn_exp2f(a.part_ml[pr * 2] - m);
-        const f32x4   x = *reinterpret_cast<const f32x4 *>(a.part_o + pr * D + d);
+    const int     per = D / 4, groups = kFinishThreads / per, grp = threadIdx.x / per, d = 4 * (threadIdx.x % per);
+    constexpr int U = 4;
+    float         m = kNone, l = 0.0f;
+    f32x4         o = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto          join = [&](float m2, float l2, f32x4 o2) {
+        const float mn = fmaxf(m, m2), x = __builtin_amdgcn_exp2f(m - mn), y = __builtin_amdgcn_exp2f(m2 - mn);
+        l = l * x + l2 * y;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = fmaf(wgt, x[i], o[i]);
+        for (int i = 0; i < 4; ++i) o[i] = o[i] * x + o2[i] * y;
+        m = mn;
+    };
+    for (int c0 = grp; c0 < nch; c0 += groups * U) {
+        float2 ml[U];
+        f32x4  po[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int64_t pr = p0 + min(c0 + u * groups, nch - 1) * pc;
+            ml[u] = *reinterpret_cast<const float2 *>(a.part_ml + pr * 2);
+            po[u] = *reinterpret_cast<const f32x4 *>(a.part_o + pr * D + d);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (c0 + u * groups < nch) join(ml[u].x, ml[u].y, po[u]);
     }
     s_o[threadIdx.x] = o;
+    s_ml[threadIdx.x] = make_float2(m, l);
     __syncthreads();
     if (grp == 0) {
-        for (int k = 1; k < groups; ++k) o += s_o[threadIdx.x + k * per];
+        for (int k = 1; k < groups; ++k) {
+            const float2 ml = s_ml[threadIdx.x + k * per];
+            join(ml.x, ml.y, s_o[threadIdx.x + k * per]);
+        }
         const float   inv = nch ? 1.0f / (l + 1e-6f) : 0.0f;
         const __half2 lo = __floats2half2_rn(o[0] * inv, o[1] * inv), hi = __floats2half2_rn(o[2] * inv, o[3] * inv);
         *reinterpret_cast<u32x2 *>(a.out + ((int64_t)(tok0 + r / a.G) * a.Hq + g * a.G + r % a.G) * D + d) =
@@ -367,7 +404,7 @@ template <int D, int NW> void launch_one(const QuantArgs &a, int items, hipStrea
         HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
                                       NW * kQuantRows * D * 4));
     });
-    hipLaunchKernelGGL(fn, dim3((unsigned)items * (unsigned)a.Hkv), dim3(NW * 64), (size_t)(NW * a.rows * D * 4), stream, a);
+    hipLaunchKernelGGL(fn, dim3((unsigned)quant_grid(items, a.Hkv)), dim3(NW * 64), (size_t)(NW * a.rows * D * 4), stream, a);
 }
 
 } // namespace
@@ -396,10 +433,14 @@ void launch_attn_quant(const QuantCall &c, const QuantView &v, const QuantPlan &
     for (const auto &l : plan.launches) {
         if (l.n == 0) continue;
         a.n = l.n;
+        a.items = l.items;
         a.rows = l.rows;
         if (a.rows > kQuantRows) throw std::invalid_argument("attention: too many query rows per entry");
         if ((int64_t)l.items * c.Hkv > kQuantMostItems) throw std::invalid_argument("attention: too many work items");
         std::memcpy(a.e, plan.entries.data() + l.first, sizeof(QuantEntry) * (size_t)l.n);
+        a.each = quant_items(a.e[0].S, plan.chunk);
+        for (int i = 1; i < l.n; ++i)
+            if (quant_items(a.e[i].S, plan.chunk) != a.each) a.each = 0;
         a.part_ml = workspace;
         a.part_o = l.finish ? workspace + part_ml_floats((size_t)l.items * c.Hkv * a.rows) : nullptr;
         profile_begin(KernelId::AttnQuant, stream);

@@ -65,35 +65,39 @@ template <int S> __device__ __forceinline__ float xor_lane_max(float x) {
 // fp16 number, which holds its 11 bits; a smaller scale by way of its 2^17-fold (the result
 // is then rounded again where it is subnormal).
 struct ValueScale {
-    f16x2 by, then;
+    f16x2 by;
     bool  twice;
     __device__ explicit ValueScale(float s) {
         twice = s < 6.103515625e-05f;
-        const _Float16 a = (_Float16)(twice ? s * 131072.0f : s), b = (_Float16)(1.0f / 131072.0f);
+        const _Float16 a = (_Float16)(twice ? s * 131072.0f : s);
         by = f16x2{a, a};
-        then = f16x2{b, b};
     }
-    __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
-        f16x2 y = __builtin_bit_cast(f16x2, x) * by;
-        if (twice) y = y * then;
-        return __builtin_bit_cast(uint32_t, y);
+    __device__ __forceinline__ void operator()(u32x4 &x) const {
+        f16x2 y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = __builtin_bit_cast(f16x2, (uint32_t)x[j]) * by;
+        if (__builtin_expect(twice, 0)) {
+            const _Float16 then = (_Float16)(1.0f / 131072.0f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] *= f16x2{then, then};
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(uint32_t, y[j]);
     }
 };
 
-template <int D, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void
+template <int D>
+__global__ __launch_bounds__(quant_prefill_waves(D) * 64) __attribute__((amdgpu_waves_per_eu(2))) void
 quant_prefill_kernel(PrefillArgs a) {
-    constexpr int NQG = D <= 128 ? 2 : 1; // 16-row parts of a wave
-    constexpr int NT = NW * 64;
-    constexpr int R = 16 * NQG;
-    constexpr int ROWS = NW * R;
-    static_assert(ROWS == quant_prefill_rows(D, NW), "the planner's row tile");
+    constexpr int NW = quant_prefill_waves(D), ROWS = quant_prefill_rows(D);
+    constexpr int R = ROWS / NW, NQG = R / 16;                      // rows of a wave, in parts of 16
+    constexpr int TILE = quant_prefill_tile(D), NG = TILE / kGroup; // tokens and groups of a tile
     constexpr int KS = D / 32, DT = D / 16;
-    constexpr int PAIRS = 4 * D;                      // pairs of pieces of a group, K and V
-    constexpr int NU = (2 * PAIRS + NT - 1) / NT;     // of a tile, per thread
-    __shared__ __align__(16) uint16_t ks0[kQuantTile * D], ks1[kQuantTile * D];
-    __shared__ __align__(16) uint16_t vs0[kQuantTile * D], vs1[kQuantTile * D];
-    __shared__ int                    s_odd; // the open group has values that are not finite
+    constexpr int UNITS = 2 * NG * KS;                  // of a tile: 64 pairs of pieces, K's first, then V's
+    constexpr int NU = (UNITS + NW - 1) / NW;           // of a wave: units wave, NW + wave, ...
+    __shared__ __align__(16) uint16_t s_k[2][TILE * D], s_v[2][TILE * D];
+    __shared__ float                  s_scale[2][NG]; // K's of the tiles' groups, 1 of an open one, NaN where V's is
+    __shared__ int                    s_odd;          // the open group has values that are not finite
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int item = blockIdx.x / a.Hkv, g = blockIdx.x - item * a.Hkv;
@@ -102,9 +106,9 @@ quant_prefill_kernel(PrefillArgs a) {
     const int row = a.e[ei].row, S = a.e[ei].S, tok0 = a.e[ei].tok0, nq = a.e[ei].nq, open = a.e[ei].open, nch = a.e[ei].nch;
     const int rows = nq << a.lgG;
     const int rel = item - a.e[ei].item0, ch = rel % nch, rt = (rows + ROWS - 1) / ROWS - 1 - rel / nch;
-    const int seen = S - nq + 1 + ((min(rows, (rt + 1) * ROWS) - 1) >> a.lgG); // tokens that the tile sees
-    const int tiles = (seen + kQuantTile - 1) / kQuantTile;
-    const int t_lo = (int)((int64_t)ch * tiles / nch), t_hi = (int)((int64_t)(ch + 1) * tiles / nch);
+    const int seen = S - nq + 1 + ((min(rows, (rt + 1) * ROWS) - 1) >> a.lgG); // tokens that the row tile sees
+    const int tiles = (seen + TILE - 1) / TILE;
+    const int t_lo = (int)((int64_t)ch * tiles / nch), t_n = (int)((int64_t)(ch + 1) * tiles / nch) - t_lo;
     const int closed = open < 0 ? S : S / kGroup * kGroup;
     const int groups = (closed + kGroup - 1) / kGroup;
     const int c = lane & 15, qg = lane >> 4;
@@ -127,87 +131,103 @@ quant_prefill_kernel(PrefillArgs a) {
             qb[j][s] = a.negate ? -v : v;
         }
     }
-    const int all = S - nq + 1 + (min(r_w, rows - 1) >> a.lgG);         // tokens that every row of the wave sees,
-    const int some = S - nq + 1 + (min(r_w + R - 1, rows - 1) >> a.lgG); // and that some row does
+    const int all = S - nq + 1 + (min(r_w, rows - 1) >> a.lgG); // tokens that every row of the wave sees,
+    const int some = r_w < rows ? S - nq + 1 + (min(r_w + R - 1, rows - 1) >> a.lgG) : 0; // and that some row does
 
-    // A wave's 64 pairs of a load lie in one group, K or V.
+    // Tile i of the chunk.  at: where the next one to load has its groups, lane k group k; made of
+    // blocks that were asked for a tile earlier.
     const int32_t *bt = a.v.table + (int64_t)row * a.v.bt_stride;
-    auto blocks = [&](int kt) -> int { return lane < 2 ? bt[max(0, min(2 * kt + lane, groups - 1)) >> a.v.lg] : 0; };
-    auto tile_at = [&](int kt, int k, int ids) __attribute__((always_inline)) -> int64_t {
-        const int i = min(2 * kt + k, groups - 1) & ((1 << a.v.lg) - 1);
-        return (((int64_t)__builtin_amdgcn_readlane(ids, k) * a.Hkv + g) << a.v.lg) + i;
-    };
-    u32x4  raw[NU];
-    float2 sc[2]; // scales of the loaded tile's groups
-    auto   load = [&](int kt, int ids) __attribute__((always_inline)) {
-        if (groups > 0) {
-            int64_t at[2];
+    const int      lane_g = min(lane, NG - 1);
+    u32x4          raw[NU];
+    float2         sc = {}; // scales of the loaded tile's groups, lane k those of group k.  (Loaded per lane: a
+                            // scalar load would be waited for with the LDS accesses, at every barrier.)
+    int            id = 0;
+    auto           group_of = [&](int i) { return max(0, min(NG * (t_lo + i) + lane_g, groups - 1)); };
+    auto           blocks = [&](int i) { id = bt[group_of(i) >> a.v.lg]; };
+    auto           load = [&](int i) __attribute__((always_inline)) {
+        if (groups == 0) return;
+        const int64_t  at = (((int64_t)id * a.Hkv + g) << a.v.lg) + (group_of(i) & ((1 << a.v.lg) - 1));
+        const uint8_t *tile = a.v.tiles + at * (64 * D);
+        sc = a.v.scales[at];
+        const __attribute__((address_space(1))) uint8_t *base[NG];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                at[k] = tile_at(kt, k, ids);
-                sc[k] = a.v.scales[at[k]];
-            }
-#pragma unroll
-            for (int u = 0; u < NU; ++u) {
-                const int p0 = u * NT + wave * 64; // wave-uniform
-                if (2 * PAIRS % NT != 0 && p0 >= 2 * PAIRS) break;
-                const int k = p0 / PAIRS;
-                raw[u] = reinterpret_cast<const u32x4 *>(a.v.tiles + (k ? at[1] : at[0]) * (64 * D))[p0 % PAIRS + lane];
-            }
+        for (int k = 0; k < NG; ++k) {
+            const uint64_t x = reinterpret_cast<uint64_t>(tile);
+            base[k] = reinterpret_cast<const __attribute__((address_space(1))) uint8_t *>((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, k) |
+                                                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(x >> 32), k) << 32);
         }
-    };
-    auto stage = [&](int kt, uint16_t *kd, uint16_t *vd) __attribute__((always_inline)) {
-        u32x4 *k16 = reinterpret_cast<u32x4 *>(kd), *v16 = reinterpret_cast<u32x4 *>(vd);
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
-            const int p0 = u * NT + wave * 64;
-            if (2 * PAIRS % NT != 0 && p0 >= 2 * PAIRS) break;
-            const int  k = p0 / PAIRS, s = p0 % (PAIRS / 2) / 64, group = 2 * kt + k;
-            const bool is_v = p0 % PAIRS >= PAIRS / 2;
+            const int q = u * NW + wave;
+            if (UNITS % NW != 0 && q >= UNITS) break;
+            const int x = q % (NG * KS);
+            raw[u] = *reinterpret_cast<const __attribute__((address_space(1))) u32x4 *>((NG == 2 && x >= KS ? base[NG - 1] : base[0]) +
+                                                      ((q >= NG * KS ? 2 * D : 0) + x % KS * 64 + lane) * 16);
+        }
+        blocks(i + 1);
+    };
+    auto stage = [&](int i) __attribute__((always_inline)) {
+        u32x4     *k16 = reinterpret_cast<u32x4 *>(s_k[i % 2]) + lane, *v16 = reinterpret_cast<u32x4 *>(s_v[i % 2]) + lane;
+        const int  group0 = NG * (t_lo + i);
+        if (wave == 0 && lane < NG) s_scale[i % 2][lane] = group0 + lane < groups ? (sc.y == sc.y ? sc.x : sc.y) : 1.0f;
+        auto unit = [&](int u, auto place) __attribute__((always_inline)) {
+            const int  q = u * NW + wave, k = q % (NG * KS) / KS, st = q % KS;
+            const bool is_v = q >= NG * KS;
             u32x4      x[2];
-            if (group < groups) {
-                const u32x4 w = raw[u];
+            place(x, is_v, k, st, u);
+            u32x4 *to = is_v ? v16 + (k * DT + 2 * st) * 64 : k16 + (2 * k * KS + st) * 64;
+            to[0] = x[0];
+            to[(is_v ? 1 : KS) * 64] = x[1];
+        };
+        auto stored = [&](u32x4 *x, bool is_v, int k, int, int u) __attribute__((always_inline)) {
+            const u32x4 w = raw[u];
 #pragma unroll
-                for (int h = 0; h < 2; ++h) x[h] = __builtin_bit_cast(u32x4, whole8(w[2 * h], w[2 * h + 1]));
-                if (is_v) {
-                    const float vs = k ? sc[1].y : sc[0].y;
-                    const ValueScale by(vs == vs ? vs : 0.0f); // (NaN: its rows get it below)
+            for (int h = 0; h < 2; ++h) x[h] = __builtin_bit_cast(u32x4, whole8(w[2 * h], w[2 * h + 1]));
+            if (is_v) {
+                const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.y), k));
+                const ValueScale by(vs == vs ? vs : 0.0f); // (NaN: its rows have it from their scores)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) x[h][i] = by(x[h][i]);
-                }
-            } else if (open >= 0 && group == groups) {
-                const u32x4 *src = reinterpret_cast<const u32x4 *>(open_of<D>(a.v, a.Hkv, row, open, g)) + 2 * (p0 % PAIRS + lane);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    x[h] = src[h];
-                    if (is_v) { // 0 times what is behind the last token, or not finite, could be NaN
-                        f16x8 v = __builtin_bit_cast(f16x8, x[h]);
-                        bool  odd = false;
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const bool there = group * kGroup + 16 * (j >> 2) + 4 * qg + (j & 3) < S;
-                            const bool finite = __builtin_fabsf16(v[j]) <= (_Float16)65504.0f;
-                            odd |= there && !finite;
-                            if (!there || !finite) v[j] = (_Float16)0.0f;
-                        }
-                        if (odd) s_odd = 1;
-                        x[h] = __builtin_bit_cast(u32x4, v);
-                    }
-                }
-            } else {
-                x[0] = x[1] = u32x4{0u, 0u, 0u, 0u};
+                for (int h = 0; h < 2; ++h) by(x[h]);
             }
+        };
+        auto any = [&](u32x4 *x, bool is_v, int k, int st, int u) __attribute__((always_inline)) {
+            const int group = group0 + k;
+            if (group < groups) return stored(x, is_v, k, st, u);
+            x[0] = x[1] = u32x4{0u, 0u, 0u, 0u};
+            if (open < 0 || group != groups) return;
+            const u32x4 *src = reinterpret_cast<const u32x4 *>(open_of<D>(a.v, a.Hkv, row, open, g)) +
+                               2 * ((is_v ? 2 * D : 0) + st * 64 + lane);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                if (!is_v) k16[((2 * k + h) * KS + s) * 64 + lane] = x[h];
-                else v16[(k * DT + 2 * s + h) * 64 + lane] = x[h];
+                x[h] = src[h];
+                if (is_v) { // 0 times what is behind the last token, or not finite, could be NaN
+                    f16x8 v = __builtin_bit_cast(f16x8, x[h]);
+                    bool  odd = false;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const bool there = group * kGroup + 16 * (j >> 2) + 4 * qg + (j & 3) < S;
+                        const bool finite = __builtin_fabsf16(v[j]) <= (_Float16)65504.0f;
+                        odd |= there && !finite;
+                        if (!there || !finite) v[j] = (_Float16)0.0f;
+                    }
+                    if (odd) s_odd = 1;
+                    x[h] = __builtin_bit_cast(u32x4, v);
+                }
             }
+        };
+        if (__builtin_expect(group0 + NG <= groups, 1)) {
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+                if (UNITS % NW == 0 || u * NW + wave < UNITS) unit(u, stored);
+        } else {
+#pragma unroll 1
+            for (int u = 0; u < NU; ++u)
+                if (UNITS % NW == 0 || u * NW + wave < UNITS) unit(u, any);
         }
     };
 
-    f32x4 acc[NQG][DT], l_run[NQG];
+    f32x4 acc[NQG][DT], l_run[NQG], s[NQG][2 * NG];
+    f16x8 pf[NQG][NG];
     float m_run[NQG];
 #pragma unroll
     for (int j = 0; j < NQG; ++j) {
@@ -218,57 +238,71 @@ quant_prefill_kernel(PrefillArgs a) {
     }
     const f16x8 ones = __builtin_bit_cast(f16x8, u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
 
-    auto compute = [&](int kt, float2 now0, float2 now1, const uint16_t *kd, const uint16_t *vd) __attribute__((always_inline)) {
-        const int t0 = kt * kQuantTile;
-        if (t0 >= some) return; // no row of the wave sees the tile
-        const f16x8 *k16 = reinterpret_cast<const f16x8 *>(kd) + lane, *v16 = reinterpret_cast<const f16x8 *>(vd) + lane;
-        float        f[2];
+    // Operands come from LDS in batches, the next one on its way while one is multiplied.  (The
+    // compiler would read two and wait for them: 512 -> @.)
+    constexpr int NB = NG * KS / 2; // batches of four, of scores and of values
+    f16x8         kf[4], vf[4];
+    auto scores_batch = [&](int i, int b, f16x8 *f) __attribute__((always_inline)) { // keys 16 tt .., dims 32 st ..
+        const f16x8 *k16 = reinterpret_cast<const f16x8 *>(s_k[i % 2]) + lane;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) f[k] = a.scale_log2 * (2 * kt + k < groups ? (k ? now1 : now0).x : 1.0f);
-        f32x4 s[NQG][4];
+        for (int u = 0; u < 4; ++u) f[u] = k16[(4 * b + u) * 64];
+    };
+    auto values_batch = [&](int i, int b, f16x8 *f) __attribute__((always_inline)) {
+        const f16x8 *v16 = reinterpret_cast<const f16x8 *>(s_v[i % 2]) + lane;
 #pragma unroll
-        for (int tt = 0; tt < 4; ++tt)
+        for (int u = 0; u < 4; ++u) f[u] = v16[(4 * b + u) * 64];
+    };
+    // (the first batch is in kf, vf)
+    auto scores = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int tt = 0; tt < 2 * NG; ++tt)
 #pragma unroll
             for (int j = 0; j < NQG; ++j) s[j][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int th = 0; th < 4; th += 2)
+        for (int b = 0; b < NB; ++b) {
+            f16x8 next[4];
+            if (b + 1 < NB) scores_batch(i, b + 1, next);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int st = 0; st < KS; ++st) {
-                f16x8 kf[2];
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int u = 0; u < 2; ++u) kf[u] = k16[((th + u) * KS + st) * 64];
+                for (int j = 0; j < NQG; ++j) {
+                    const int tt = (4 * b + u) / KS, st = (4 * b + u) % KS;
+                    s[j][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u], qb[j][st], s[j][tt], 0, 0, 0);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            if (b + 1 < NB)
 #pragma unroll
-                for (int u = 0; u < 2; ++u)
+                for (int u = 0; u < 4; ++u) kf[u] = next[u];
+        }
+    };
+    auto softmax = [&](int i) __attribute__((always_inline)) {
+        const int t0 = (t_lo + i) * TILE;
+        float     f[NG];
 #pragma unroll
-                    for (int j = 0; j < NQG; ++j)
-                        s[j][th + u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u], qb[j][st], s[j][th + u], 0, 0, 0);
-            }
-        if (t0 + kQuantTile > all) { // some score does not count
+        for (int k = 0; k < NG; ++k) f[k] = a.scale_log2 * s_scale[i % 2][k];
+        if (__builtin_expect(t0 + TILE > all, 0)) { // some score does not count
 #pragma unroll
             for (int j = 0; j < NQG; ++j)
 #pragma unroll
-                for (int tt = 0; tt < 4; ++tt)
+                for (int tt = 0; tt < 2 * NG; ++tt)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        s[j][tt][i] = t0 + 16 * tt + 4 * qg + i < seen_by(j) ? s[j][tt][i] * f[tt >> 1] : -INFINITY;
-            f[0] = f[1] = 1.0f;
+                    for (int x = 0; x < 4; ++x)
+                        s[j][tt][x] = t0 + 16 * tt + 4 * qg + x < seen_by(j) ? s[j][tt][x] * f[tt >> 1] : -INFINITY;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) f[k] = 1.0f;
         }
 #pragma unroll
-        for (int k = 0; k < 2; ++k) // a group whose scale is NaN: the rows that see some of it
-            if (const float vs = (k ? now1 : now0).y; 2 * kt + k < groups && !(vs == vs))
-#pragma unroll
-                for (int j = 0; j < NQG; ++j)
-                    if (t0 + kGroup * k < seen_by(j)) l_run[j] += vs;
-        f16x8 pf[NQG][2];
-#pragma unroll
         for (int j = 0; j < NQG; ++j) {
-            float mk[2] = {-INFINITY, -INFINITY};
+            float mloc = -INFINITY;
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt)
+            for (int k = 0; k < NG; ++k) {
+                float mk = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) mk[tt >> 1] = fmaxf(mk[tt >> 1], s[j][tt][i]);
-            const float mloc = fmaxf(mk[0] * f[0], mk[1] * f[1]);
-            if (__any(mloc > m_run[j] + kLazyMax)) {
+                for (int x = 0; x < 8; ++x) mk = __builtin_elementwise_maximum(mk, s[j][2 * k + (x >> 2)][x & 3]);
+                mloc = __builtin_elementwise_maximum(mloc, mk * f[k]); // (NaN: of a group that all rows see, or in scores)
+            }
+            if (__builtin_expect(__any(mloc > m_run[j] + kLazyMax), 0)) {
                 const float m_tile = xor_lane_max<32>(xor_lane_max<16>(mloc));
                 const float m_new = fmaxf(m_run[j], m_tile - kBelow);
                 const float alpha = m_run[j] == m_new ? 1.0f : __builtin_amdgcn_exp2f(m_run[j] - m_new);
@@ -279,60 +313,66 @@ quant_prefill_kernel(PrefillArgs a) {
             }
             const float m_new = m_run[j];
 #pragma unroll
-            for (int tt = 0; tt < 4; ++tt)
+            for (int tt = 0; tt < 2 * NG; ++tt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    pf[j][tt >> 1][4 * (tt & 1) + i] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[j][tt][i], f[tt >> 1], -m_new));
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-#pragma unroll
-            for (int j = 0; j < NQG; ++j) l_run[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[j][k], l_run[j], 0, 0, 0);
-#pragma unroll
-            for (int dt = 0; dt < DT; ++dt) {
-                const f16x8 vf = v16[(k * DT + dt) * 64];
-#pragma unroll
-                for (int j = 0; j < NQG; ++j) acc[j][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[j][k], acc[j][dt], 0, 0, 0);
-            }
-        }
-        if (open >= 0 && 2 * kt + 1 >= groups && s_odd) { // the open group's values that are not finite, token by token
-            const uint16_t *tile = open_of<D>(a.v, a.Hkv, row, open, g) + 32 * D;
-            const int first = groups * kGroup;
-            for (int r = 0; r < S - first; ++r)
-#pragma unroll
-                for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float x = (float)__builtin_bit_cast(_Float16, tile[v_half(r, 16 * dt + 4 * qg + i)]);
-#pragma unroll
-                        for (int j = 0; j < NQG; ++j)
-                            if (!(__builtin_fabsf(x) <= 65504.0f) && first + r < seen_by(j)) acc[j][dt][i] += x;
-                    }
+                for (int x = 0; x < 4; ++x)
+                    pf[j][tt >> 1][4 * (tt & 1) + x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[j][tt][x], f[tt >> 1], -m_new));
         }
     };
-
-    if (t_lo < t_hi) {
-        int    ids = blocks(t_lo), next = t_lo + 1 < t_hi ? blocks(t_lo + 1) : 0;
-        __syncthreads(); // s_odd
-        load(t_lo, ids);
-        stage(t_lo, ks0, vs0);
-        __syncthreads();
-        auto step = [&](int kt, uint16_t *kd, uint16_t *vd, uint16_t *kn, uint16_t *vn) __attribute__((always_inline)) {
-            const float2 now0 = sc[0], now1 = sc[1];
-            const bool   more = kt + 1 < t_hi;
-            if (more) {
-                ids = next;
-                if (kt + 2 < t_hi) next = blocks(kt + 2);
-                load(kt + 1, ids);
-            }
-            compute(kt, now0, now1, kd, vd);
-            if (more) stage(kt + 1, kn, vn);
-            __syncthreads();
-        };
-        for (int kt = t_lo; kt < t_hi; kt += 2) {
-            step(kt, ks0, vs0, ks1, vs1);
-            if (kt + 1 < t_hi) step(kt + 1, ks1, vs1, ks0, vs0);
+    auto values = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            f16x8 next[4];
+            if (b + 1 < NB) values_batch(i, b + 1, next);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int j = 0; j < NQG; ++j) {
+                    const int k = (4 * b + u) / DT, dt = (4 * b + u) % DT;
+                    if (dt == 0) l_run[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[j][k], l_run[j], 0, 0, 0);
+                    acc[j][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[u], pf[j][k], acc[j][dt], 0, 0, 0);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            if (b + 1 < NB)
+#pragma unroll
+                for (int u = 0; u < 4; ++u) vf[u] = next[u];
         }
+    };
+    if (t_n > 0) {
+        blocks(0);
+        load(0);
+        __syncthreads(); // s_odd
+        stage(0);
+        if (t_n > 1) load(1);
+        __syncthreads();
+        for (int i = 0; i < t_n; ++i) {
+            if ((t_lo + i) * TILE < some) { // some row of the wave sees the tile
+                scores_batch(i, 0, kf);
+                scores(i);
+                values_batch(i, 0, vf);
+                softmax(i);
+                values(i);
+            }
+            if (i + 1 < t_n) stage(i + 1);
+            if (i + 2 < t_n) load(i + 2);
+            __syncthreads();
+        }
+    }
+    // (behind every product: a value that is infinite decides)
+    if (open >= 0 && t_n > 0 && (t_lo + t_n) * NG > groups && s_odd) { // the open group's values that are not finite, token by token
+        const int       first = groups * kGroup;
+        const uint16_t *tile = open_of<D>(a.v, a.Hkv, row, open, g) + 32 * D;
+        for (int r = 0; r < S - first; ++r)
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const float y = (float)__builtin_bit_cast(_Float16, tile[v_half(r, 16 * dt + 4 * qg + x)]);
+#pragma unroll
+                    for (int j = 0; j < NQG; ++j)
+                        if (!(__builtin_fabsf(y) <= 65504.0f) && first + r < seen_by(j)) acc[j][dt][x] += y;
+                }
     }
 
     const int64_t p0 = ((int64_t)item * a.Hkv + g) * ROWS;
@@ -392,16 +432,12 @@ __global__ __launch_bounds__(kMergeThreads) void quant_prefill_merge_kernel(Pref
 
 size_t part_ml_floats(size_t rows) { return (2 * rows + 3) / 4 * 4; }
 
-template <int D, int NW> void launch_one(const PrefillArgs &a, int items, hipStream_t stream) {
-    hipLaunchKernelGGL((quant_prefill_kernel<D, NW>), dim3((unsigned)items * (unsigned)a.Hkv), dim3(NW * 64), 0, stream, a);
-}
-
 } // namespace
 
 size_t quant_prefill_workspace_floats(const QuantPrefillPlan &plan, int Hkv, int D) {
     size_t most = 0;
     for (const auto &l : plan.launches) {
-        const size_t rows = (size_t)l.items * (size_t)quant_prefill_rows(D, plan.waves) * (size_t)Hkv;
+        const size_t rows = (size_t)l.items * (size_t)quant_prefill_rows(D) * (size_t)Hkv;
         if (l.split) most = std::max(most, part_ml_floats(rows) + rows * (size_t)D);
     }
     return most;
@@ -418,7 +454,7 @@ void launch_quant_prefill(const QuantCall &c, const QuantView &v, const QuantPre
     a.Hq = c.Hq;
     a.Hkv = c.Hkv;
     while ((c.Hkv << a.lgG) < c.Hq) ++a.lgG;
-    const int ROWS = quant_prefill_rows(c.D, plan.waves);
+    const int ROWS = quant_prefill_rows(c.D);
     for (const auto &l : plan.launches) {
         if (l.n == 0 || l.items == 0) continue;
         if ((int64_t)l.items * c.Hkv > kQuantMostItems) throw std::invalid_argument("attention: too many work items");
@@ -429,10 +465,8 @@ void launch_quant_prefill(const QuantCall &c, const QuantView &v, const QuantPre
         profile_begin(KernelId::PrefillQuant, stream);
         for_head_dim(c.D, [&](auto d) {
             constexpr int D = decltype(d)::value;
-            if constexpr (D <= 128) {
-                if (plan.waves == 8) return launch_one<D, 8>(a, l.items, stream);
-            }
-            launch_one<D, 4>(a, l.items, stream);
+            hipLaunchKernelGGL(quant_prefill_kernel<D>, dim3((unsigned)l.items * (unsigned)a.Hkv),
+                               dim3(quant_prefill_waves(D) * 64), 0, stream, a);
         });
         HIP_CHECK(hipGetLastError());
         if (l.split) {

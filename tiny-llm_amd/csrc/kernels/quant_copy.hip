@@ -81,18 +81,20 @@ template <int D> __global__ __launch_bounds__(kThreads) void quant_append_kernel
     }
 }
 
-constexpr int kOneThreads = 128;
-
-template <int D> __global__ __launch_bounds__(kOneThreads) void quant_append_one_kernel(AppendArgs a) {
-    __shared__ uint32_t red[2 * kOneThreads / 64];
+// A wave per (entry, kv head) and layer.
+template <int D> __global__ __launch_bounds__(64) void quant_append_one_kernel(AppendArgs a) {
     const int     i = blockIdx.x / a.Hkv, g = blockIdx.x - i * a.Hkv, layer = blockIdx.y;
     const int     row = a.e[i].row, p = a.e[i].p0;
     const int64_t at = tile_of(a.v, a.Hkv, row, g, p / kGroup);
     // (rows of a launch's entries follow each other; item0: the entries of the call)
     const int64_t src = (((int64_t)layer * a.e[i].item0 + a.e[i].tok0) * a.Hkv + g) * D;
-    append_token<D, kOneThreads>(open_of<D>(a.v, a.Hkv, row, a.e[i].first_last & 1, g) + layer * a.steps.open, p % kGroup,
-                                 a.new_k + src, a.new_v + src, a.v.tiles + layer * a.steps.tiles + at * (64 * D),
-                                 a.v.scales + layer * a.steps.scales + at, red);
+    GroupRegs<D>  group;
+    uint16_t     *open = open_of<D>(a.v, a.Hkv, row, a.e[i].first_last & 1, g) + layer * a.steps.open;
+    const bool    closes = p % kGroup == kGroup - 1;
+    if (closes) group.load(open);
+    group.fetch(p % kGroup, a.new_k + src, a.new_v + src);
+    group.append(open, p % kGroup);
+    if (closes) group.close(a.v.tiles + layer * a.steps.tiles + at * (64 * D), a.v.scales + layer * a.steps.scales + at);
 }
 
 struct GatherArgs {
@@ -208,7 +210,7 @@ void launch_quant_append_one(const QuantView &v, const QuantLayerSteps &steps, c
         profile_begin(KernelId::KvAppend, stream);
         for_head_dim(D, [&](auto d) {
             hipLaunchKernelGGL(quant_append_one_kernel<decltype(d)::value>, dim3((unsigned)(a.n * Hkv), (unsigned)num_layers),
-                               dim3(kOneThreads), 0, stream, a);
+                               dim3(64), 0, stream, a);
         });
         HIP_CHECK(hipGetLastError());
         profile_end(KernelId::KvAppend, stream);

@@ -61,6 +61,16 @@ __device__ __forceinline__ float group_scale(uint32_t most) {
         out = __builtin_amdgcn_readfirstlane(seen_ - 1);                                                               \
     } while (0)
 
+// Workgroup b of a grid of quant_grid(items, Hkv): the heads of an item on one XCD (workgroups
+// go to the eight in turn), eight items at a time, so that an XCD's address translation serves
+// an eighth of the sequences' pages.
+__host__ __device__ inline int64_t quant_grid(int64_t items, int Hkv) { return (items + 7) / 8 * 8 * Hkv; }
+__device__ __forceinline__ void quant_place(int b, int Hkv, int &item, int &g) {
+    const int eights = b / (8 * Hkv), rest = b - eights * 8 * Hkv;
+    g = rest >> 3;
+    item = eights * 8 + (rest & 7);
+}
+
 // Index of a group's tile and scales.
 __device__ __forceinline__ int64_t tile_of(const QuantView &v, int Hkv, int row, int g, int group) {
     const int64_t block = v.table[(int64_t)row * v.bt_stride + (group >> v.lg)];
@@ -149,22 +159,80 @@ __device__ __forceinline__ void close_group(const uint16_t *open, uint8_t *tile,
     __syncthreads(); // (red is free again)
 }
 
-// Token r of the group goes into the open tile (64 D halves in memory), its rows of D
-// halves at k and v; the last one closes the group.  By the NT threads of a workgroup, whose
-// later reads see what was written.
-template <int D, int NT>
-__device__ __forceinline__ void append_token(uint16_t *open, int r, const uint16_t *k, const uint16_t *v, uint8_t *tile,
-                                             float2 *scale, uint32_t *red) {
-    for (int x = threadIdx.x; x < D / 8; x += NT)
-        reinterpret_cast<u32x4 *>(open)[k_piece(r, x)] = reinterpret_cast<const u32x4 *>(k)[x];
-    for (int d = threadIdx.x; d < D; d += NT) open[32 * D + v_half(r, d)] = v[d];
-    __threadfence_block();
-    __syncthreads();
-    if (r != kGroup - 1) return;
-    close_group<D, NT>(open, tile, scale, red);
-    __threadfence_block();
-    __syncthreads();
-}
+// A wave's registers hold a group as the operands of the products: kf[tt][s] the token 16 tt +
+// l % 16 (dims 32 s + 8 (l / 16) ..), vf[dt] the dim 16 dt + l % 16 (tokens 4 (l / 16) .. and 16 more).
+template <int D> struct GroupRegs {
+    static constexpr int KS = D / 32, DT = D / 16;
+    f16x8                kf[2][KS], vf[DT];
+    float                ks = 1.0f, vs = 1.0f;
+
+    __device__ __forceinline__ void load(const uint16_t *open) {
+        const f16x8 *k = reinterpret_cast<const f16x8 *>(open) + 2 * (threadIdx.x & 63), *v = k + 4 * D;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) kf[0][i] = k[128 * i], kf[1][i] = k[128 * i + 1];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) vf[dt] = v[128 * (dt / 2) + (dt & 1)];
+    }
+    // Token r of the group comes from rows of D halves: on their way to the lanes that take it ...
+    f16x8    xk[KS];
+    uint16_t xv[DT];
+    __device__ __forceinline__ void fetch(int r, const uint16_t *new_k, const uint16_t *new_v) {
+        const int c = threadIdx.x & 15, q = (threadIdx.x & 63) >> 4;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) xk[i] = *reinterpret_cast<const f16x8 *>(new_k + 32 * i + 8 * q);
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) xv[dt] = new_v[16 * dt + c];
+    }
+    // ... and into them and the open tile.
+    __device__ __forceinline__ void append(uint16_t *open, int r) {
+        const int  c = threadIdx.x & 15, q = (threadIdx.x & 63) >> 4, tr = r >> 4, slot = 4 * tr + (r & 3);
+        const bool mine_k = c == (r & 15), mine_v = q == (r & 15) >> 2;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            if (mine_k) *reinterpret_cast<f16x8 *>(open + 8 * k_piece(r, 4 * i + q)) = xk[i];
+            kf[0][i] = mine_k && !tr ? xk[i] : kf[0][i];
+            kf[1][i] = mine_k && tr ? xk[i] : kf[1][i];
+        }
+        uint32_t mask[4]; // of the half that is replaced
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mask[w] = mine_v && w == slot >> 1 ? (slot & 1 ? 0xFFFF0000u : 0x0000FFFFu) : 0u;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+            if (mine_v) open[32 * D + v_half(r, 16 * dt + c)] = xv[dt];
+            u32x4          v = __builtin_bit_cast(u32x4, vf[dt]);
+            const uint32_t x = xv[dt] | (uint32_t)xv[dt] << 16;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) v[w] = (v[w] & ~mask[w]) | (x & mask[w]);
+            vf[dt] = __builtin_bit_cast(f16x8, v);
+        }
+    }
+    // The group's whole numbers and scales, in the registers and in the cache.
+    __device__ __forceinline__ void close(uint8_t *tile, float2 *scale) {
+        uint32_t mk = 0, mv = 0;
+#pragma unroll
+        for (int i = 0; i < KS; ++i)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                mk = most_of(most_of(mk, __builtin_bit_cast(u32x4, kf[0][i])[x]), __builtin_bit_cast(u32x4, kf[1][i])[x]);
+                mv = most_of(most_of(mv, __builtin_bit_cast(u32x4, vf[2 * i])[x]), __builtin_bit_cast(u32x4, vf[2 * i + 1])[x]);
+            }
+        ks = group_scale(wave_max(mk));
+        vs = group_scale(wave_max(mv));
+        u32x4 *to = reinterpret_cast<u32x4 *>(tile) + (threadIdx.x & 63);
+        auto   put = [&](u32x4 *at, f16x8 &a, f16x8 &b, float s) __attribute__((always_inline)) {
+            const u32x4 w = stored16(__builtin_bit_cast(u32x4, a), __builtin_bit_cast(u32x4, b), s);
+            *at = w;
+            a = whole8(w[0], w[1]);
+            b = whole8(w[2], w[3]);
+        };
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            put(to + 64 * i, kf[0][i], kf[1][i], ks);
+            put(to + 2 * D + 64 * i, vf[2 * i], vf[2 * i + 1], vs);
+        }
+        if ((threadIdx.x & 63) == 0) *scale = make_float2(ks, vs);
+    }
+};
 
 template <typename F> void for_head_dim(int D, F &&f) {
     switch (D) {

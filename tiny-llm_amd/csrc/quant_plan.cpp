@@ -39,13 +39,19 @@ void plan_quant(QuantPlan &plan, int G, int Hkv, int, int cus) {
 }
 
 bool plan_quant_prefill(QuantPrefillPlan &plan, int D, int G, int Hkv, int cus) {
-    const int64_t n = std::max(1, cus);
-    plan.waves = D <= 128 ? 8 : 4;
-    const int tile = quant_prefill_rows(D, plan.waves);
-    int64_t   tiles = 0;
+    // Row tiles that leave workgroup slots empty have their keys split over them, in chunks of three tiles
+    // at least (8 heads of 128, groups of 4: 100 over 30000 106 us in 16 chunks, 122 in 8, 120 in 32; 8 x 16
+    // over 4000 .. 8000 58 in 8, 69 in 4, 72 in 16; 300 alone 22 whole, 25 in 2): a chunk's outputs are written
+    // and read again, so never beyond that (16 x 300: 58 whole, 138 in 2).
+    const int64_t slots = (int64_t)std::max(1, cus) * 8 / quant_prefill_waves(D);
+    const int     tile = quant_prefill_rows(D);
+    int64_t       tiles = 0;
     for (const auto &e : plan.entries) tiles += ((int64_t)e.nq * G + tile - 1) / tile;
-    const int64_t work = std::max<int64_t>(1, tiles * Hkv), once = std::max<int64_t>(1, n / work);
-    for (auto &e : plan.entries) e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(once, quant_tiles(e.S) / 3));
+    const int64_t each = slots / std::max<int64_t>(1, tiles * Hkv);
+    for (auto &e : plan.entries) {
+        const int64_t keys = ((int64_t)e.S + quant_prefill_tile(D) - 1) / quant_prefill_tile(D);
+        e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(each, keys / 3));
+    }
     std::stable_sort(plan.entries.begin(), plan.entries.end(), [](const QuantPrefillEntry &x, const QuantPrefillEntry &y) {
         return (int64_t)x.S * y.nch > (int64_t)y.S * x.nch;
     });

@@ -88,12 +88,16 @@ struct QuantPrefillLaunch {
 struct QuantPrefillPlan {
     std::vector<QuantPrefillEntry>  entries;
     std::vector<QuantPrefillLaunch> launches;
-    int                             waves = 4;
     void                            clear() { entries.clear(), launches.clear(); }
 };
-// Rows of a workgroup: 32 per wave up to head_dim 128, 16 at 256.
-constexpr int quant_prefill_rows(int D, int waves) { return waves * (D <= 128 ? 32 : 16); }
-// Sets the waves, nch and item0 of plan.entries and the launches (and orders the
+// Waves and rows of a workgroup, and the tokens of its key tiles.  Four waves and two
+// workgroups a CU at head_dim 128, eight waves and one elsewhere (1 x 8192, 4 x 500 over 3000 .. 6000; 8 heads,
+// groups of 4, eight waves against four: 128 611, 221 against 598, 190 us; 256 1288, 420 against 2704, 825;
+// 64 392, 138 against 396, 154; 32 313, 104 against 289, 114).
+constexpr int quant_prefill_waves(int D) { return D == 128 ? 4 : 8; }
+constexpr int quant_prefill_rows(int D) { return quant_prefill_waves(D) * (D <= 128 ? 32 : 16); }
+constexpr int quant_prefill_tile(int D) { return D <= 128 ? 64 : 32; }
+// Sets nch and item0 of plan.entries and the launches (and orders the
 // entries, longest items first).  False when a launch would have more than 2^32 threads.
 constexpr int64_t kQuantMostItems = (1 << 23) - 1;
 bool plan_quant_prefill(QuantPrefillPlan &plan, int D, int G, int Hkv, int cus);
