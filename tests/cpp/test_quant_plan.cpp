@@ -31,7 +31,7 @@ static void stream_random() {
             p.entries.push_back({i, S, i, 1 + upto(kQuantRows / G - 1), S % kGroup ? 0 : -1, 0});
         }
         plan_quant(p, G, Hkv, D, cus);
-        CHECK(p.chunk >= 1 && (p.waves == 4 || (p.waves == 8 && D <= 128)));
+        CHECK(p.chunk >= 1);
         std::vector<int> seen((size_t)n, 0);
         int              next = 0, longest = 1 << 30;
         for (const auto &l : p.launches) {

@@ -5,17 +5,25 @@
 namespace tiny_llm {
 namespace detail {
 
-void plan_quant(QuantPlan &plan, int G, int Hkv, int, int cus) {
-    int64_t total = 0, longest = 0;
+void plan_quant(QuantPlan &plan, int G, int Hkv, int D, int cus) {
+    int64_t total = 0, longest = 0, some = 0;
     for (const auto &e : plan.entries) {
         total += quant_tiles(e.S);
+        some += e.S > 0;
         longest = std::max<int64_t>(longest, quant_tiles(e.S));
     }
-    total *= Hkv;
-    const int64_t n = std::max(1, cus);
-    plan.waves = 4;
-    const int64_t half = (total + 2 * n - 1) / (2 * n); // of one of two workgroups of a CU
-    int64_t       chunk = longest <= std::max<int64_t>(16, 2 * half + half / 2) ? longest : std::max<int64_t>(8, half);
+    // A workgroup that has a whole entry finishes it; entries in chunks need a second launch, about 3 us
+    // more.  In hundredths of a us (head_dim 128): a tile takes a workgroup 28 alone and 70 where every CU has
+    // one, and takes the chip 60 of a CU's share.  So entries stay whole while the longest takes no more
+    // than that and the share; else they are cut into chunks of a CU's share, of a tile for every wave at least.
+    // Measured, 8 heads, groups of 4, whole and cut: 1 x 1000 tokens 10.4, 13.7 us, 1 x 2000 16.0, 12.9,
+    // 1 x 16000 80, 14.6; 16 x 4000 30.1, 33.5, 16 x 16000 98, 91; 64 x 8192 167, 177.
+    const int64_t n = std::max(1, cus), work = some * Hkv, waves = quant_waves(D);
+    const int64_t share = (total * Hkv + n - 1) / n;
+    const int64_t alone = D <= 128 ? 28 : 112, stream = std::max<int64_t>(1, 60 * D / 128);
+    const int64_t whole = longest * std::max(alone, stream * 7 / 6 * std::min(work, n) / n);
+    const int64_t cut = 300 + std::max(alone * waves, stream * share);
+    const int64_t chunk = whole <= cut ? longest : std::max(waves, share);
     plan.chunk = (int)std::max<int64_t>(1, std::min<int64_t>(chunk, 1 << 24));
     auto item_tiles = [&](const QuantEntry &e) {
         const int k = quant_items(e.S, plan.chunk);

@@ -66,13 +66,13 @@ struct QuantPlan {
     std::vector<QuantEntry>  entries;
     std::vector<QuantLaunch> launches;
     int                      chunk = 1; // tiles
-    int                      waves = 4; // per workgroup
     void                     clear() { entries.clear(), launches.clear(); }
 };
+// Waves of a workgroup.
+constexpr int quant_waves(int D) { return D <= 128 ? 8 : 4; }
 inline int quant_tiles(int S) { return S / kQuantTile + (S % kQuantTile != 0); }
 inline int quant_items(int S, int chunk) { return (quant_tiles(S) + chunk - 1) / chunk; }
-// Sets item0 of plan.entries (and orders them, longest first), the launches, the waves and
-// the chunk length.
+// Sets item0 of plan.entries (and orders them, longest first), the launches and the chunk length.
 void plan_quant(QuantPlan &plan, int G, int Hkv, int D, int cus);
 
 // The same for more query rows: rt row tiles (of tokens x heads of one kv head) x nch chunks
