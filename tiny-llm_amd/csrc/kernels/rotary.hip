@@ -4,10 +4,11 @@
 // Bound by HBM (a value is read and written once, 4 bytes) and, for a decode step, by the launch.
 //
 // D / 16 threads have a head's row, 8 + 8 values each: those of 8 pairs (dims that are not
-// rotated: 16 neighbours), so that a rotation needs no other thread.  A thread keeps its 8
-// angles over several heads of its token: an angle costs about as much as 8 values' loads and
-// stores (the turns, position * inv_freq / 2 pi, are reduced to half a turn in 64 bits, where a far
-// position times a high frequency still has its fraction; sine and cosine are then fp32).
+// rotated: 16 neighbours), so that a rotation needs no other thread.  A workgroup computes the angles
+// of its tokens once, into LDS, and a thread keeps its 8 over several heads of its token: an angle
+// costs about as much as 8 values' loads and stores (the turns, position * inv_freq / 2 pi, are
+// reduced to half a turn in 64 bits, where a far position times a high frequency still has its
+// fraction; sine and cosine are then fp32).
 #include "rotary.h"
 
 #include "kv_kernels.h"
@@ -34,9 +35,9 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryCall a, int lg_h
     constexpr int LPR = D / 16;
     const int     p = threadIdx.x % LPR, slot = threadIdx.x / LPR;
     const int     hs = 1 << lg_hs, h_first = (int)blockIdx.y * per * hs + (slot & (hs - 1));
-    const int64_t t = (int64_t)blockIdx.x * (kThreads / LPR >> lg_hs) + (slot >> lg_hs);
-    const int     H = a.Hq + a.Hkv;
-    if (t >= a.T) return; // (whole rows: the sums below stay among a row's threads)
+    const int     H = a.Hq + a.Hkv, tokens = kThreads / LPR >> lg_hs, pairs = a.rd / 2;
+    const int64_t t0 = (int64_t)blockIdx.x * tokens, t = t0 + (slot >> lg_hs);
+    __shared__ float2 s_angle[kThreads / LPR * D / 2]; // (cosine, sine) of the block's tokens
     const bool turned = 16 * p < a.rd;
     const int  d0 = turned && !a.interleaved ? 8 * p : 16 * p, d1 = turned && !a.interleaved ? a.rd / 2 + 8 * p : 16 * p + 8;
 
@@ -53,27 +54,41 @@ __global__ __launch_bounds__(kThreads) void rotary_kernel(RotaryCall a, int lg_h
             wk[1] = *reinterpret_cast<const f16x8 *>(a.k_weight + d1);
         }
     }
-    float cs[8], sn[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        cs[i] = 1.0f;
-        sn[i] = 0.0f;
-        if (turned) {
-            const double x = (double)a.positions[(int64_t)a.axis[8 * p + i] * a.T + t] * a.turns[8 * p + i];
-            sincospif(2.0f * (float)(x - __builtin_rint(x)), &sn[i], &cs[i]);
-        }
-    }
-    for (int n = 0; n < per; n += kHeads) {
-        f16x8 x[kHeads][2];
+    f16x8 x[kHeads][2];
+    auto  fetch = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < kHeads; ++u) {
             const int h = h_first + (n + u) * hs;
-            if (n + u < per && h < H) {
+            if (n + u < per && h < H && t < a.T) {
                 const __half *src = h < a.Hq ? a.q + t * a.q_stride + (int64_t)h * D : a.k + t * a.k_stride + (int64_t)(h - a.Hq) * D;
                 x[u][0] = *reinterpret_cast<const f16x8 *>(src + d0);
                 x[u][1] = *reinterpret_cast<const f16x8 *>(src + d1);
             }
         }
+    };
+    fetch(0);
+    // The block's angles, one a thread at a time, while its first rows are on their way.
+    for (int i = threadIdx.x; i < tokens * pairs; i += kThreads) {
+        const int     pair = i % pairs;
+        const int64_t at = t0 + i / pairs;
+        if (at < a.T) {
+            const double turn = (double)a.positions[(int64_t)a.axis[pair] * a.T + at] * a.turns[pair];
+            float        sn, cs;
+            sincospif(2.0f * (float)(turn - __builtin_rint(turn)), &sn, &cs);
+            s_angle[i] = make_float2(cs, sn);
+        }
+    }
+    __syncthreads();
+    if (t >= a.T) return; // (whole rows: the sums below stay among a row's threads)
+    float cs[8], sn[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float2 v = turned ? s_angle[(slot >> lg_hs) * pairs + 8 * p + i] : make_float2(1.0f, 0.0f);
+        cs[i] = v.x;
+        sn[i] = v.y;
+    }
+    for (int n = 0; n < per; n += kHeads) {
+        if (n) fetch(n);
 #pragma unroll
         for (int u = 0; u < kHeads; ++u) {
             const int h = h_first + (n + u) * hs;
