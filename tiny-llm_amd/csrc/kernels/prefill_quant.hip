@@ -11,8 +11,11 @@
 // into one of two LDS buffers as operands, 16 bytes a lane in lane order, so that every LDS access is
 // a whole row of the banks:
 //   K   whole numbers, exact in fp16; a group's scale meets the scores, in the softmax's fma
-//   V   times the group's scale, rounded to fp16 (a rounding 2^-11 beside the 2^-8 of the
-//       stored numbers): scaling the products instead would cost as much as the softmax
+//   V   times the scale's first 4 bits, exact in fp16 too (7 + 4 bits); what the scale is
+//       more than that, below 1.125 times, meets the weights in the softmax's exponent, and
+//       the row sums are freed of it.  So the weights' rounding to fp16 (2^-12, with errors
+//       of either sign) is all that there is.  Scaling the products instead would cost as
+//       much as the softmax
 //   S^T = K Q^T, O^T += V^T P^T by v_mfma_f32_16x16x32_f16 as in attention_quant.hip; the row
 //   sums of P by a product with ones
 // quant_prefill_merge_kernel: joins the chunks of entries whose keys were split.
@@ -26,6 +29,7 @@
 #include <climits>
 #include <cmath>
 #include <cstring>
+#include <type_traits>
 
 namespace tiny_llm {
 namespace detail {
@@ -61,30 +65,28 @@ template <int S> __device__ __forceinline__ float xor_lane_max(float x) {
     }
 }
 
-// A group's values in fp16 from its whole numbers: one rounding where the scale is a normal
-// fp16 number, which holds its 11 bits; a smaller scale by way of its 2^17-fold (the result
-// is then rounded again where it is subnormal).
-struct ValueScale {
-    f16x2 by;
-    bool  twice;
-    __device__ explicit ValueScale(float s) {
-        twice = s < 6.103515625e-05f;
-        const _Float16 a = (_Float16)(twice ? s * 131072.0f : s);
-        by = f16x2{a, a};
+// The first 4 significant bits of a scale.
+__device__ __forceinline__ float coarse(float s) { return __uint_as_float(__float_as_uint(s) & 0xFFF00000u); }
+
+// A group's values in fp16 from its whole numbers and a scale of 4 bits: exact where the scale
+// is a normal fp16 number; a smaller one by way of its 2^17-fold (the result is then rounded
+// where it is subnormal).
+constexpr uint32_t kLeastHalf = 0x38800000u, kInfinite = 0x7F800000u; // bits of 2^-14, and of infinity
+template <bool SMALL> __device__ __forceinline__ void scale_values(u32x4 &x, uint32_t scale_bits) {
+    const bool     twice = SMALL && scale_bits < kLeastHalf;
+    const float    s = coarse(__uint_as_float(scale_bits));
+    const _Float16 one = (_Float16)(SMALL && scale_bits > kInfinite ? 0.0f : twice ? s * 131072.0f : s); // (NaN: its rows have it from their scores)
+    f16x2          y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = __builtin_bit_cast(f16x2, (uint32_t)x[j]) * f16x2{one, one};
+    if (SMALL && twice) {
+        const _Float16 then = (_Float16)(1.0f / 131072.0f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] *= f16x2{then, then};
     }
-    __device__ __forceinline__ void operator()(u32x4 &x) const {
-        f16x2 y[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = __builtin_bit_cast(f16x2, (uint32_t)x[j]) * by;
-        if (__builtin_expect(twice, 0)) {
-            const _Float16 then = (_Float16)(1.0f / 131072.0f);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) y[j] *= f16x2{then, then};
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(uint32_t, y[j]);
-    }
-};
+    for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(uint32_t, y[j]);
+}
 
 template <int D>
 __global__ __launch_bounds__(quant_prefill_waves(D) * 64) __attribute__((amdgpu_waves_per_eu(2))) void
@@ -96,7 +98,8 @@ quant_prefill_kernel(PrefillArgs a) {
     constexpr int UNITS = 2 * NG * KS;                  // of a tile: 64 pairs of pieces, K's first, then V's
     constexpr int NU = (UNITS + NW - 1) / NW;           // of a wave: units wave, NW + wave, ...
     __shared__ __align__(16) uint16_t s_k[2][TILE * D], s_v[2][TILE * D];
-    __shared__ float                  s_scale[2][NG]; // K's of the tiles' groups, 1 of an open one, NaN where V's is
+    __shared__ float4                 s_scale[2][NG]; // the tiles' groups': x K's scale, 1 of an open one, NaN where
+                                                      // V's is; y log2 of V's over its first 4 bits, z 1 over it
     __shared__ int                    s_odd;          // the open group has values that are not finite
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -169,7 +172,14 @@ quant_prefill_kernel(PrefillArgs a) {
     auto stage = [&](int i) __attribute__((always_inline)) {
         u32x4     *k16 = reinterpret_cast<u32x4 *>(s_k[i % 2]) + lane, *v16 = reinterpret_cast<u32x4 *>(s_v[i % 2]) + lane;
         const int  group0 = NG * (t_lo + i);
-        if (wave == 0 && lane < NG) s_scale[i % 2][lane] = group0 + lane < groups ? (sc.y == sc.y ? sc.x : sc.y) : 1.0f;
+        if (wave == 0 && lane < NG) {
+            const bool  closed_one = group0 + lane < groups;
+            const float y = closed_one ? fmaxf(sc.y, 1e-37f) : 1.0f; // (not 0, not NaN)
+            const float less = coarse(y);
+            s_scale[i % 2][lane] = make_float4(closed_one ? (sc.y == sc.y ? sc.x : sc.y) : 1.0f,
+                                               __builtin_amdgcn_logf(y * __builtin_amdgcn_rcpf(less)),
+                                               less * __builtin_amdgcn_rcpf(y), 0.0f);
+        }
         auto unit = [&](int u, auto place) __attribute__((always_inline)) {
             const int  q = u * NW + wave, k = q % (NG * KS) / KS, st = q % KS;
             const bool is_v = q >= NG * KS;
@@ -179,20 +189,23 @@ quant_prefill_kernel(PrefillArgs a) {
             to[0] = x[0];
             to[(is_v ? 1 : KS) * 64] = x[1];
         };
-        auto stored = [&](u32x4 *x, bool is_v, int k, int, int u) __attribute__((always_inline)) {
+        const uint32_t vs0 = __builtin_amdgcn_readlane(__float_as_uint(sc.y), 0); // the groups' value scales' bits
+        const uint32_t vs1 = __builtin_amdgcn_readlane(__float_as_uint(sc.y), NG - 1);
+        const bool     plain = group0 + NG <= groups && vs0 - kLeastHalf < kInfinite - kLeastHalf && vs1 - kLeastHalf < kInfinite - kLeastHalf;
+        auto stored = [&](u32x4 *x, bool is_v, int k, int u, auto small) __attribute__((always_inline)) {
             const u32x4 w = raw[u];
 #pragma unroll
             for (int h = 0; h < 2; ++h) x[h] = __builtin_bit_cast(u32x4, whole8(w[2 * h], w[2 * h + 1]));
-            if (is_v) {
-                const float vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(sc.y), k));
-                const ValueScale by(vs == vs ? vs : 0.0f); // (NaN: its rows have it from their scores)
+            if (is_v)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) by(x[h]);
-            }
+                for (int h = 0; h < 2; ++h) scale_values<decltype(small)::value>(x[h], k == 0 ? vs0 : vs1);
+        };
+        auto normal = [&](u32x4 *x, bool is_v, int k, int, int u) __attribute__((always_inline)) {
+            stored(x, is_v, k, u, std::false_type{});
         };
         auto any = [&](u32x4 *x, bool is_v, int k, int st, int u) __attribute__((always_inline)) {
             const int group = group0 + k;
-            if (group < groups) return stored(x, is_v, k, st, u);
+            if (group < groups) return stored(x, is_v, k, u, std::true_type{});
             x[0] = x[1] = u32x4{0u, 0u, 0u, 0u};
             if (open < 0 || group != groups) return;
             const u32x4 *src = reinterpret_cast<const u32x4 *>(open_of<D>(a.v, a.Hkv, row, open, g)) +
@@ -215,25 +228,26 @@ quant_prefill_kernel(PrefillArgs a) {
                 }
             }
         };
-        if (__builtin_expect(group0 + NG <= groups, 1)) {
+        if (__builtin_expect(plain, 1)) {
 #pragma unroll
             for (int u = 0; u < NU; ++u)
-                if (UNITS % NW == 0 || u * NW + wave < UNITS) unit(u, stored);
+                if (UNITS % NW == 0 || u * NW + wave < UNITS) unit(u, normal);
         } else {
-#pragma unroll 1
+#pragma unroll
             for (int u = 0; u < NU; ++u)
                 if (UNITS % NW == 0 || u * NW + wave < UNITS) unit(u, any);
         }
     };
 
-    f32x4 acc[NQG][DT], l_run[NQG], s[NQG][2 * NG];
+    f32x4 acc[NQG][DT], s[NQG][2 * NG];
     f16x8 pf[NQG][NG];
-    float m_run[NQG];
+    float m_run[NQG], l_run[NQG];
+    float4 of[NG]; // s_scale of the tile
 #pragma unroll
     for (int j = 0; j < NQG; ++j) {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) acc[j][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        l_run[j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        l_run[j] = 0.0f;
         m_run[j] = kNone;
     }
     const f16x8 ones = __builtin_bit_cast(f16x8, u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
@@ -280,7 +294,7 @@ quant_prefill_kernel(PrefillArgs a) {
         const int t0 = (t_lo + i) * TILE;
         float     f[NG];
 #pragma unroll
-        for (int k = 0; k < NG; ++k) f[k] = a.scale_log2 * s_scale[i % 2][k];
+        for (int k = 0; k < NG; ++k) f[k] = a.scale_log2 * of[k].x;
         if (__builtin_expect(t0 + TILE > all, 0)) { // some score does not count
 #pragma unroll
             for (int j = 0; j < NQG; ++j)
@@ -311,15 +325,18 @@ quant_prefill_kernel(PrefillArgs a) {
                 l_run[j] *= alpha;
                 m_run[j] = m_new;
             }
-            const float m_new = m_run[j];
+            float less[NG];
+#pragma unroll
+            for (int k = 0; k < NG; ++k) less[k] = of[k].y - m_run[j];
 #pragma unroll
             for (int tt = 0; tt < 2 * NG; ++tt)
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    pf[j][tt >> 1][4 * (tt & 1) + x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[j][tt][x], f[tt >> 1], -m_new));
+                    pf[j][tt >> 1][4 * (tt & 1) + x] = (_Float16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[j][tt][x], f[tt >> 1], less[tt >> 1]));
         }
     };
     auto values = [&](int i) __attribute__((always_inline)) {
+        f32x4 sums[NQG][NG];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             f16x8 next[4];
@@ -330,7 +347,7 @@ quant_prefill_kernel(PrefillArgs a) {
 #pragma unroll
                 for (int j = 0; j < NQG; ++j) {
                     const int k = (4 * b + u) / DT, dt = (4 * b + u) % DT;
-                    if (dt == 0) l_run[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[j][k], l_run[j], 0, 0, 0);
+                    if (dt == 0) sums[j][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[j][k], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
                     acc[j][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[u], pf[j][k], acc[j][dt], 0, 0, 0);
                 }
             __builtin_amdgcn_sched_barrier(0);
@@ -338,6 +355,10 @@ quant_prefill_kernel(PrefillArgs a) {
 #pragma unroll
                 for (int u = 0; u < 4; ++u) vf[u] = next[u];
         }
+#pragma unroll
+        for (int j = 0; j < NQG; ++j)
+#pragma unroll
+            for (int k = 0; k < NG; ++k) l_run[j] = __builtin_fmaf(of[k].z, sums[j][k][0], l_run[j]);
     };
     if (t_n > 0) {
         blocks(0);
@@ -349,6 +370,8 @@ quant_prefill_kernel(PrefillArgs a) {
         for (int i = 0; i < t_n; ++i) {
             if ((t_lo + i) * TILE < some) { // some row of the wave sees the tile
                 scores_batch(i, 0, kf);
+#pragma unroll
+                for (int k = 0; k < NG; ++k) of[k] = s_scale[i % 2][k];
                 scores(i);
                 values_batch(i, 0, vf);
                 softmax(i);
@@ -384,10 +407,10 @@ quant_prefill_kernel(PrefillArgs a) {
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt)
                 *reinterpret_cast<f32x4 *>(a.part_o + (p0 + r) * D + 16 * dt + 4 * qg) = acc[j][dt];
-            if (qg == 0) *reinterpret_cast<float2 *>(a.part_ml + (p0 + r) * 2) = make_float2(m_run[j], l_run[j][0]);
+            if (qg == 0) *reinterpret_cast<float2 *>(a.part_ml + (p0 + r) * 2) = make_float2(m_run[j], l_run[j]);
             continue;
         }
-        const float inv = 1.0f / (l_run[j][0] + 1e-6f);
+        const float inv = 1.0f / (l_run[j] + 1e-6f);
         uint16_t   *op = a.out + row_of(rt * ROWS + r);
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
