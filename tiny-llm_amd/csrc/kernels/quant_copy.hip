@@ -56,29 +56,41 @@ template <int D> __global__ __launch_bounds__(kThreads) void quant_append_kernel
     const bool opens = t0 <= p0; // the group in which the append begins
     uint16_t  *tile0 = open_of<D>(a.v, a.Hkv, row, first, g);
 
+    constexpr int PER = (kGroup * KP + kThreads - 1) / kThreads; // pieces of a thread
+    const int     pieces = (r_hi - r_lo) * KP;
+    u32x4         k[PER], v[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        const int x = threadIdx.x + i * kThreads;
+        if (x >= pieces) break;
+        const int64_t src = ((int64_t)(tok0 + t0 + r_lo + x / KP - p0) * a.Hkv + g) * D + 8 * (x % KP);
+        k[i] = *reinterpret_cast<const u32x4 *>(a.new_k + src);
+        v[i] = *reinterpret_cast<const u32x4 *>(a.new_v + src);
+    }
+    auto put = [&](uint16_t *tile) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const int x = threadIdx.x + i * kThreads, r = r_lo + x / KP, o = x % KP;
+            if (x >= pieces) break;
+            reinterpret_cast<u32x4 *>(tile)[k_piece(r, o)] = k[i];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) tile[32 * D + v_half(r, 8 * o + j)] = (uint16_t)(v[i][j / 2] >> (16 * (j & 1)));
+        }
+    };
+    if (r_hi < kGroup) { // (behind its last row a tile holds anything)
+        put(opens ? tile0 : open_of<D>(a.v, a.Hkv, row, last, g));
+        return;
+    }
     u32x4 *s16 = reinterpret_cast<u32x4 *>(s_open);
-    if (r_lo > 0 || r_hi < kGroup) { // its earlier rows, or zeros behind the last
-        for (int p = threadIdx.x; p < 8 * D; p += kThreads)
-            s16[p] = r_lo > 0 ? reinterpret_cast<const u32x4 *>(tile0)[p] : u32x4{0u, 0u, 0u, 0u};
+    if (r_lo > 0) { // its earlier rows
+        for (int p = threadIdx.x; p < 8 * D; p += kThreads) s16[p] = reinterpret_cast<const u32x4 *>(tile0)[p];
         __syncthreads();
     }
-    for (int x = threadIdx.x; x < (r_hi - r_lo) * KP; x += kThreads) {
-        const int     r = r_lo + x / KP, o = x % KP;
-        const int64_t src = ((int64_t)(tok0 + t0 + r - p0) * a.Hkv + g) * D + 8 * o;
-        s16[k_piece(r, o)] = *reinterpret_cast<const u32x4 *>(a.new_k + src);
-        const u32x4 v = *reinterpret_cast<const u32x4 *>(a.new_v + src);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s_open[32 * D + v_half(r, 8 * o + i)] = (uint16_t)(v[i / 2] >> (16 * (i & 1)));
-    }
+    put(s_open);
+    if (opens) put(tile0);
     __syncthreads();
-    if (opens || r_hi < kGroup) {
-        u32x4 *dst = reinterpret_cast<u32x4 *>(opens ? tile0 : open_of<D>(a.v, a.Hkv, row, last, g));
-        for (int p = threadIdx.x; p < 8 * D; p += kThreads) dst[p] = s16[p];
-    }
-    if (r_hi == kGroup) {
-        const int64_t at = tile_of(a.v, a.Hkv, row, g, group);
-        close_group<D, kThreads>(s_open, a.v.tiles + at * (64 * D), a.v.scales + at, red);
-    }
+    const int64_t at = tile_of(a.v, a.Hkv, row, g, group);
+    close_group<D, kThreads>(s_open, a.v.tiles + at * (64 * D), a.v.scales + at, red);
 }
 
 // A wave per (entry, kv head) and layer.

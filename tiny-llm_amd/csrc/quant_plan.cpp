@@ -63,6 +63,17 @@ bool plan_quant_prefill(QuantPrefillPlan &plan, int D, int G, int Hkv, int cus) 
     std::stable_sort(plan.entries.begin(), plan.entries.end(), [](const QuantPrefillEntry &x, const QuantPrefillEntry &y) {
         return (int64_t)x.S * y.nch > (int64_t)y.S * x.nch;
     });
+    // Where every workgroup has a slot at once, those behind the first half share the CUs of the first in turn:
+    // the shortest with the longest (16 x 128 over 500 .. 9000: 267 us, longest first throughout 278, shortest
+    // first 299).
+    int64_t all = 0, before = 0;
+    for (const auto &e : plan.entries) all += ((int64_t)e.nq * G + tile - 1) / tile * e.nch * Hkv;
+    if (all <= slots) {
+        size_t i = 0;
+        for (; i < plan.entries.size() && before < slots / 2; ++i)
+            before += ((int64_t)plan.entries[i].nq * G + tile - 1) / tile * plan.entries[i].nch * Hkv;
+        std::reverse(plan.entries.begin() + (std::ptrdiff_t)i, plan.entries.end());
+    }
     plan.launches.clear();
     for (size_t i = 0; i < plan.entries.size();) {
         QuantPrefillLaunch l{(int)i, 0, 0, false};
