@@ -344,20 +344,22 @@ __global__ __launch_bounds__(quant_waves(D) * 64, D <= 128 ? 2 : 1) void attn_qu
 
 constexpr int kFinishThreads = 256;
 
-// Entries of several chunks, or of no tokens (zeros).  Workgroup (entry, kv head; row): every
-// thread joins a few chunks' maxima, sums and outputs of four dims, all on their way at once,
-// then the threads of equal dims meet in LDS.
-__global__ __launch_bounds__(kFinishThreads) void quant_finish_kernel(QuantArgs a, int D) {
+// Entries of several chunks, or of no tokens (zeros).  Workgroup (entry, kv head; a few rows):
+// every thread joins a few chunks' maxima, sums and outputs of four dims of a row, all on their
+// way at once, then the row's `split` threads of equal dims meet in LDS.
+constexpr int kFinishChunks = 4; // on their way at once
+__global__ __launch_bounds__(kFinishThreads) void quant_finish_kernel(QuantArgs a, int D, int split) {
     __shared__ f32x4  s_o[kFinishThreads];
     __shared__ float2 s_ml[kFinishThreads];
-    const int ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv, r = blockIdx.y;
+    const int ei = blockIdx.x / a.Hkv, g = blockIdx.x - ei * a.Hkv;
+    const int per = D / 4, grp = threadIdx.x / per, d = 4 * (threadIdx.x % per), part = grp % split;
+    const int r = blockIdx.y * (kFinishThreads / per / split) + grp / split;
     const int S = a.e[ei].S, tok0 = a.e[ei].tok0, rows = a.e[ei].nq * a.G;
     const int tiles = (S + kQuantTile - 1) / kQuantTile, nch = (tiles + a.chunk - 1) / a.chunk;
-    if (nch == 1 || r >= rows) return;
+    if (nch == 1) return;
     const int64_t p0 = ((int64_t)a.e[ei].item0 * a.Hkv + g) * a.rows + r; // of chunk 0
     const int64_t pc = (int64_t)a.Hkv * a.rows;                          // from chunk to chunk
-    const int     per = D / 4, groups = kFinishThreads / per, grp = threadIdx.x / per, d = 4 * (threadIdx.x % per);
-    constexpr int U = 4;
+    constexpr int U = kFinishChunks;
     float         m = kNone, l = 0.0f;
     f32x4         o = {0.0f, 0.0f, 0.0f, 0.0f};
     auto          join = [&](float m2, float l2, f32x4 o2) {
@@ -367,24 +369,24 @@ __global__ __launch_bounds__(kFinishThreads) void quant_finish_kernel(QuantArgs 
         for (int i = 0; i < 4; ++i) o[i] = o[i] * x + o2[i] * y;
         m = mn;
     };
-    for (int c0 = grp; c0 < nch; c0 += groups * U) {
+    for (int c0 = r < rows ? part : nch; c0 < nch; c0 += split * U) {
         float2 ml[U];
         f32x4  po[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t pr = p0 + min(c0 + u * groups, nch - 1) * pc;
+            const int64_t pr = p0 + min(c0 + u * split, nch - 1) * pc;
             ml[u] = *reinterpret_cast<const float2 *>(a.part_ml + pr * 2);
             po[u] = *reinterpret_cast<const f32x4 *>(a.part_o + pr * D + d);
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
-            if (c0 + u * groups < nch) join(ml[u].x, ml[u].y, po[u]);
+            if (c0 + u * split < nch) join(ml[u].x, ml[u].y, po[u]);
     }
     s_o[threadIdx.x] = o;
     s_ml[threadIdx.x] = make_float2(m, l);
     __syncthreads();
-    if (grp == 0) {
-        for (int k = 1; k < groups; ++k) {
+    if (part == 0 && r < rows) {
+        for (int k = 1; k < split; ++k) {
             const float2 ml = s_ml[threadIdx.x + k * per];
             join(ml.x, ml.y, s_o[threadIdx.x + k * per]);
         }
@@ -451,8 +453,13 @@ void launch_attn_quant(const QuantCall &c, const QuantView &v, const QuantPlan &
             HIP_CHECK(hipGetLastError());
         }
         if (l.finish) {
-            hipLaunchKernelGGL(quant_finish_kernel, dim3((unsigned)(l.n * c.Hkv), (unsigned)a.rows), dim3(kFinishThreads), 0,
-                               stream, a, c.D);
+            int       most = 1, split = 1;
+            const int groups = kFinishThreads / (c.D / 4);
+            for (int i = 0; i < l.n; ++i) most = std::max(most, quant_items(a.e[i].S, plan.chunk));
+            while (split < groups && split * kFinishChunks < most) split *= 2;
+            const int rows = groups / split;
+            hipLaunchKernelGGL(quant_finish_kernel, dim3((unsigned)(l.n * c.Hkv), (unsigned)((a.rows + rows - 1) / rows)),
+                               dim3(kFinishThreads), 0, stream, a, c.D, split);
             HIP_CHECK(hipGetLastError());
         }
         profile_end(KernelId::AttnQuant, stream);
