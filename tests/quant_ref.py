@@ -152,8 +152,8 @@ def attend(q, k, v, scale, last):
 
 def check_out(got, out, mass, err, terms, most):
     """Each weight is rounded to fp16 once (2^-11 of it; 2^-32 of the largest where it is
-    below fp16's normal numbers) and has the relative error of its score's (twice: the
-    maximum's too); a value may be rounded to fp16 (2^-11); sums of `terms` fp32 numbers
+    below fp16's normal numbers), in the products and in their sum, and has the relative error
+    of its score's (twice: the maximum's too); sums of `terms` fp32 numbers
     lose at most terms * 2^-24, the scaled sums of the groups as much again; the output is
     rounded to fp16 once.  most: the largest |value|."""
     rel = 2 * 2.0 ** -11 + 2 * err + (2 * terms + 8) * 2.0 ** -24

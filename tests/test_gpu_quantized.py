@@ -473,6 +473,60 @@ def test_a_capture_does_not_grow_the_workspace(tl):
             b.attention(0, q.data_ptr(), q.data_ptr(), 0.125, s.cuda_stream)
 
 
+def test_a_refused_prompt_appends_nothing(tl):
+    c = QuantCache(tl, [3000], 1, 64, seed=21, hq=8, block=256)
+    p = tl.PrefillBatch(c.mgr, 1, 8)
+    p.prepare(c.ids, [4])
+    x = torch.zeros((4, 8, 64), dtype=torch.float16, device="cuda")
+    s = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        x.zero_()
+        with pytest.raises(tl.TinyLLMError, match="captured"):
+            p.run(0, x.data_ptr(), x.data_ptr(), x.data_ptr(), x.data_ptr(), 0.125, s.cuda_stream)
+    with pytest.raises(tl.TinyLLMError, match="more than the 3000 tokens"):
+        tl.DecodeBatch(c.mgr, 1, 8).prepare_lengths(c.ids, [3001])
+    graph.replay()
+    torch.cuda.synchronize()
+    c.check()
+
+
+def test_beyond_4_gib(tl):
+    """A sequence whose last tokens lie behind 4 GiB of the pool and of a layer: the earlier
+    ones are one chunk over and over, whose scores are far below those of the last."""
+    hkv, d, chunk, times, n = 8, 128, 1 << 17, 17, 200
+    room = chunk * times + n + 40
+    mgr = tl.KVCacheManager(num_layers=1, num_heads=hkv, head_dim=d, max_seq_len=room, max_batch_size=1, block_tokens=256,
+                            num_blocks=-(-room // 256), quantized=True)
+    sid, err = mgr.allocateSequence(room)
+    assert err is None
+    rng = np.random.default_rng(22)
+    far = torch.full((chunk, hkv, d), -1.0, dtype=torch.float16, device="cuda")
+    for _ in range(times):
+        assert mgr.appendKV(sid, 0, far.data_ptr(), far.data_ptr(), chunk) is None
+        assert mgr.advanceSeqLen(sid, chunk) is None
+    assert chunk * times * hkv * d * 2 > 1 << 32
+    near = [(1 + rng.random((n, hkv, d)) / 4).astype(np.float16) for _ in range(2)]
+    near[1] = rng.standard_normal((n, hkv, d)).astype(np.float16)
+    for count, G in ((n - 70, 4), (66, 4), (3, 4), (1, 4)):  # by the prompt kernel, then by the step's
+        done = mgr.getSeqLen(sid) - chunk * times
+        k, v = (dev(x[done:done + count]) for x in near)
+        q = np.full((count, hkv * G, d), 0.5, dtype=np.float16)  # scores: -64 of the far tokens, 64 and more of the near ones
+        dq, out = dev(q), torch.empty((count, hkv * G, d), dtype=torch.float16, device="cuda")
+        b = tl.DecodeBatch(mgr, 1, hkv * G) if count == 1 else tl.PrefillBatch(mgr, 1, hkv * G)
+        if count == 1:
+            b.prepare([sid])
+            b.decode(0, dq.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 1.0, stream())
+        else:
+            b.prepare([sid], [count])
+            b.run(0, dq.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), 1.0, stream())
+        torch.cuda.synchronize()
+        b.commit(1) if count == 1 else b.commit()
+        kk, vv = (held(x[:done + count]) for x in near)
+        o, mass, err = attend(q, kk, vv, 1.0, done + np.arange(count))
+        check_out(out.cpu().numpy(), o, mass, err, done + count, np.abs(vv).max())
+
+
 def test_another_stream(tl):
     c = QuantCache(tl, [500, 64], 2, 64, seed=20, hq=8)
     s = torch.cuda.Stream()

@@ -120,6 +120,12 @@ def apply_args(**kw):
     (dict(q_out=0x100000), "overlap"),
     (dict(k_out=0x1000), "overlap"),
     (dict(k_out=0x200000), "overlap"),
+    (dict(q_stride=(1 << 30) + 8), "2\\^30"),
+    (dict(k_stride=1 << 62), "2\\^30"),
+    (dict(positions=0x200000 + 4 * 256 * 2 - 4), "q_out overlaps positions"),
+    (dict(positions=0x300000 - 12), "k_out overlaps positions"),
+    (dict(q_weight=0x200100), "q_out overlaps positions or weights"),
+    (dict(k_weight=0x300100), "k_out overlaps positions or weights"),
 ])
 def test_rotation_calls_that_are_refused(tlc, kw, word):
     """Before anything is launched: these addresses exist on no device."""

@@ -440,7 +440,7 @@ void launch_attn_quant(const QuantCall &c, const QuantView &v, const QuantPlan &
         a.items = l.items;
         a.rows = l.rows;
         if (a.rows > kQuantRows) throw std::invalid_argument("attention: too many query rows per entry");
-        if ((int64_t)l.items * c.Hkv > kQuantMostItems) throw std::invalid_argument("attention: too many work items");
+        if (quant_grid(l.items, c.Hkv) > kQuantMostItems) throw std::invalid_argument("attention: too many work items");
         std::memcpy(a.e, plan.entries.data() + l.first, sizeof(QuantEntry) * (size_t)l.n);
         a.each = quant_items(a.e[0].S, plan.chunk);
         for (int i = 1; i < l.n; ++i)

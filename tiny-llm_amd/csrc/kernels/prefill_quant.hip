@@ -13,7 +13,7 @@
 //   K   whole numbers, exact in fp16; a group's scale meets the scores, in the softmax's fma
 //   V   times the scale's first 4 bits, exact in fp16 too (7 + 4 bits); what the scale is
 //       more than that, below 1.125 times, meets the weights in the softmax's exponent, and
-//       the row sums are freed of it.  So the weights' rounding to fp16 (2^-12, with errors
+//       the row sums are freed of it.  So the weights' rounding to fp16 (2^-11, with errors
 //       of either sign) is all that there is.  Scaling the products instead would cost as
 //       much as the softmax
 //   S^T = K Q^T, O^T += V^T P^T by v_mfma_f32_16x16x32_f16 as in attention_quant.hip; the row

@@ -749,7 +749,7 @@ Result<void> DecodeBatch::run_attention(int layer_idx, const half *q, const half
     if (layer_idx < 0 || layer_idx >= cfg.num_layers)
         return Result<void>::err("DecodeBatch: Invalid layer_idx: " + std::to_string(layer_idx));
     if (n_ == 0) return Result<void>::ok();
-    if (quant_) return quant_->attention("DecodeBatch", mgr_, layer_idx, q, new_k, new_v, out, scale, num_q_heads_, stream);
+    if (quant_) return quant_->attention("DecodeBatch", mgr_, layer_idx, q, new_k, new_v, out, scale, num_q_heads_, false, stream);
     if (!inline_ok_) upload_device(stream);
     detail::AttnPlan plan;
     plan.seq_lens = d_lens_;
@@ -1061,11 +1061,7 @@ Result<void> PrefillBatch::launch(int layer_idx, const half *q, const half *new_
         return Result<void>::err("PrefillBatch: q, out, new_k and new_v must be 16-byte aligned");
     if (quant_) {
         if (tokens_ == 0) return Result<void>::ok();
-        if (new_k) {
-            auto r = quant_->append("PrefillBatch", mgr_, layer_idx, new_k, new_v, stream);
-            if (r.isErr()) return r;
-        }
-        return quant_->attention("PrefillBatch", mgr_, layer_idx, q, nullptr, nullptr, out, scale, num_q_heads_, stream);
+        return quant_->attention("PrefillBatch", mgr_, layer_idx, q, new_k, new_v, out, scale, num_q_heads_, true, stream);
     }
     if (n_items_ == 0) return Result<void>::ok();
     detail::PrefillLaunch p;

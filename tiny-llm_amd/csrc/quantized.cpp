@@ -166,7 +166,7 @@ Result<void> QuantStep::append(const char *who, KVCacheManager &mgr, int layer_i
 }
 
 Result<void> QuantStep::attention(const char *who, KVCacheManager &mgr, int layer_idx, const half *q, const half *new_k,
-                                  const half *new_v, half *out, float scale, int num_q_heads, hipStream_t stream) {
+                                  const half *new_v, half *out, float scale, int num_q_heads, bool apart, hipStream_t stream) {
     if (std::string err = check(who, mgr, {q, new_k, new_v, out}); !err.empty()) return Result<void>::err(err);
     const KVCacheConfig &cfg = mgr.getConfig();
     const size_t floats = std::max(quant_workspace_floats(this->stream, cfg.num_heads, cfg.head_dim),
@@ -174,17 +174,19 @@ Result<void> QuantStep::attention(const char *who, KVCacheManager &mgr, int laye
     if (!work.holds(floats) && stream_capturing(stream))
         return Result<void>::err(std::string(who) + ": the workspace cannot grow while the stream is captured: make one "
                                                     "call of this size before");
-    float    *ws = work.get(floats);
+    float            *ws = work.get(floats);
+    const QuantView   v = mgr.quantView(layer_idx);
+    // (behind the checks: a refused call has appended nothing)
+    if (new_k && apart) launch_quant_append(v, appends, cfg.num_heads, cfg.head_dim, new_k, new_v, stream);
     QuantCall c;
     c.q = q;
     c.out = out;
-    c.new_k = new_k;
-    c.new_v = new_v;
+    c.new_k = apart ? nullptr : new_k;
+    c.new_v = apart ? nullptr : new_v;
     c.scale = scale;
     c.Hq = num_q_heads;
     c.Hkv = cfg.num_heads;
     c.D = cfg.head_dim;
-    const QuantView v = mgr.quantView(layer_idx);
     if (!this->stream.entries.empty()) launch_attn_quant(c, v, this->stream, ws, stream);
     if (!prefill.entries.empty()) launch_quant_prefill(c, v, prefill, ws, stream);
     if (new_k) noteAppends(mgr);

@@ -38,8 +38,10 @@ struct QuantStep {
                            hipStream_t stream);
     Result<void> append(const char *who, KVCacheManager &mgr, int layer_idx, const half *new_k, const half *new_v,
                         hipStream_t stream);
+    // new_k, new_v (null: nothing new) are appended in front: by a launch of their own (apart), or as
+    // the entries' one token by the attention itself.
     Result<void> attention(const char *who, KVCacheManager &mgr, int layer_idx, const half *q, const half *new_k,
-                           const half *new_v, half *out, float scale, int num_q_heads, hipStream_t stream);
+                           const half *new_v, half *out, float scale, int num_q_heads, bool apart, hipStream_t stream);
     Result<void> gather(KVCacheManager &mgr, int layer_idx, half *k_out, half *v_out, int s_max, hipStream_t stream);
 
   private:

@@ -6,6 +6,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <iterator>
 #include <string>
 
 namespace tiny_llm {
@@ -45,7 +46,8 @@ struct Range {
     uintptr_t lo, hi;
     bool      meets(const Range &o) const { return lo < o.hi && o.lo < hi; }
 };
-Range range(const half *p, int64_t tokens, int64_t stride, int64_t row) {
+constexpr int64_t kMostStride = int64_t(1) << 30; // (2^31 tokens of it are still an offset in 64 bits)
+Range             range(const half *p, int64_t tokens, int64_t stride, int64_t row) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(p);
     return {a, a + static_cast<uintptr_t>(((tokens - 1) * stride + row) * static_cast<int64_t>(sizeof(half)))};
 }
@@ -67,6 +69,7 @@ Result<void> Rotary::apply(const half *q, int64_t q_stride, const half *k, int64
     const int64_t k_row = k ? static_cast<int64_t>(num_kv_heads) * config_.head_dim : 0;
     if (q_stride < q_row || q_stride % 8 != 0 || (k && (k_stride < k_row || k_stride % 8 != 0)))
         return err("strides must be multiples of 8, at least heads * head_dim");
+    if (q_stride > kMostStride || (k && k_stride > kMostStride)) return err("strides must be at most 2^30");
     for (const void *p : {static_cast<const void *>(q), static_cast<const void *>(k), static_cast<const void *>(q_out),
                           static_cast<const void *>(k_out), static_cast<const void *>(q_weight),
                           static_cast<const void *>(k_weight)})
@@ -74,12 +77,21 @@ Result<void> Rotary::apply(const half *q, int64_t q_stride, const half *k, int64
     if (reinterpret_cast<uintptr_t>(positions) & 3u) return err("positions must be 4-byte aligned");
     if (num_tokens == 0) return Result<void>::ok();
     const Range qi = range(q, num_tokens, q_stride, q_row), qo = range(q_out, num_tokens, q_row, q_row);
+    const uintptr_t pos = reinterpret_cast<uintptr_t>(positions);
+    const Range     given[] = {{pos, pos + static_cast<uintptr_t>(num_tokens) * axes_ * sizeof(int32_t)},
+                               range(q_weight, 1, 0, q_weight ? config_.head_dim : 0),
+                               range(k_weight, 1, 0, k_weight ? config_.head_dim : 0)};
+    auto            meets_given = [&](const Range &out) {
+        return std::any_of(std::begin(given), std::end(given), [&](const Range &x) { return out.meets(x); });
+    };
     const bool  q_in_place = q_out == q && (q_stride == q_row || num_tokens == 1);
     if (qo.meets(qi) && !q_in_place) return err("q_out overlaps q");
+    if (meets_given(qo)) return err("q_out overlaps positions or weights");
     if (k) {
         const Range ki = range(k, num_tokens, k_stride, k_row), ko = range(k_out, num_tokens, k_row, k_row);
         const bool  k_in_place = k_out == k && (k_stride == k_row || num_tokens == 1);
         if (ko.meets(ki) && !k_in_place) return err("k_out overlaps k");
+        if (meets_given(ko)) return err("k_out overlaps positions or weights");
         if (qo.meets(ki) || ko.meets(qi) || qo.meets(ko)) return err("q, k and their outputs overlap");
     }
     detail::RotaryCall c;
