@@ -5,9 +5,10 @@
 // 4 D operations a query row and token, and K and V pass through the CUs once per tile of
 // rows.
 //
-// quant_prefill_kernel: a workgroup of NW waves per (row tile, chunk of key tiles, kv head);
-// a wave has 32 rows (16 at head_dim 256: tokens x heads of the kv head).  A tile of 64 tokens is
-// loaded as stored while the one before is computed, made fp16 once per workgroup and put
+// quant_prefill_kernel: a workgroup of four waves at head_dim 128, two of them a CU, and of eight
+// elsewhere (figures: quant_prefill_waves), per (row tile, chunk of key tiles, kv head);
+// a wave has 32 rows (16 at head_dim 256: tokens x heads of the kv head).  A tile of 64 tokens (32 at
+// head_dim 256) is loaded as stored while the one before is computed, made fp16 once per workgroup and put
 // into one of two LDS buffers as operands, 16 bytes a lane in lane order, so that every LDS access is
 // a whole row of the banks:
 //   K   whole numbers, exact in fp16; a group's scale meets the scores, in the softmax's fma
@@ -15,9 +16,16 @@
 //       more than that, below 1.125 times, meets the weights in the softmax's exponent, and
 //       the row sums are freed of it.  So the weights' rounding to fp16 (2^-11, with errors
 //       of either sign) is all that there is.  Scaling the products instead would cost as
-//       much as the softmax
+//       much as the softmax.  (V times the whole scale, rounded: 564 us below in place of 570, and the
+//       error of outputs 3.6e-4 in place of 2.9e-4, of which the outputs' own rounding is 2.1e-4)
 //   S^T = K Q^T, O^T += V^T P^T by v_mfma_f32_16x16x32_f16 as in attention_quant.hip; the row
 //   sums of P by a product with ones
+// 8192 tokens, 32 heads over 8 of 128: 557 us, 0.99 PFLOP/s (0.91 on another card, where a large
+// fp16 product takes 1.10 in place of 1.15).  Of a SIMD's cycles MFMA takes 42%, VALU 40%; the LDS is read
+// 40% of the time, without bank conflicts.  What is left are the two waves of a SIMD waiting for each
+// other at barriers and for operands: a third needs 168 registers, and a wave has 226.
+// Tried and slower: eight waves of which four multiply while four do their softmax (636),
+// one group a step, priorities around the products.
 // quant_prefill_merge_kernel: joins the chunks of entries whose keys were split.
 #include "quant_device.h"
 
@@ -252,8 +260,8 @@ quant_prefill_kernel(PrefillArgs a) {
     }
     const f16x8 ones = __builtin_bit_cast(f16x8, u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
 
-    // Operands come from LDS in batches, the next one on its way while one is multiplied.  (The
-    // compiler would read two and wait for them: 512 -> @.)
+    // Operands come from LDS in batches, the next one on its way while one is multiplied.  (Left to itself the
+    // compiler reads two and waits for them: 607 us where this took 598.)
     constexpr int NB = NG * KS / 2; // batches of four, of scores and of values
     f16x8         kf[4], vf[4];
     auto scores_batch = [&](int i, int b, f16x8 *f) __attribute__((always_inline)) { // keys 16 tt .., dims 32 st ..

@@ -7,11 +7,16 @@
 // once).  Bound by HBM: 4 D bytes of new rows in and 2 D out per token and kv head, 2 D in and 4
 // D out to read back.
 //
-// quant_append_kernel: a workgroup per (entry, group, kv head).  The group's rows meet in LDS
-// as the pieces of a tile (V's tokens side by side: the transposition that its matrix operand
-// needs), then 16 pieces a lane go out in order.
-// quant_append_one_kernel: a decode step's token; 31 of 32 times only its row.
-// quant_gather_kernel: a workgroup per (entry, kv head, group), through LDS to rows.
+// quant_append_kernel: a workgroup per (entry, group, kv head).  Rows of a group that stays open go
+// straight into its open tile.  Those of one that closes meet in LDS as the pieces of a tile (V's
+// tokens side by side: the transposition that its matrix operand needs), then 16 bytes a lane
+// go out in order.  32768 tokens, 8 heads of 128, 201 MB: 38-46 us, 4.4-5.3 TB/s by how much of the
+// last call is still being written back (a copy by the library: 5.1).  Four tokens of 32 sequences: 5 us.
+// The V rows' 2-byte stores to LDS meet in its banks (40% of the cycles), which is hidden: four tokens
+// at a time, transposed in registers, swizzled, took as long.
+// quant_append_one_kernel: a decode step's token; 31 of 32 times only its row.  2.8 us, the launch.
+// quant_gather_kernel: a workgroup per (entry, kv head, group), through LDS to rows.  The same 201
+// MB: 31 us, 6.5 TB/s.
 #include "quant_device.h"
 
 #include "../runtime.h"

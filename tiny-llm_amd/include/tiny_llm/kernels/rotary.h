@@ -35,10 +35,10 @@ class Rotary {
     //   (a, b) -> (a cos - b sin, a sin + b cos)     for pair i, angle positions[axis_of[i]][t] * inv_freq[i]
     // in fp32, rounded to fp16 once; angles are reduced in 64 bits, so positions of any size keep
     // theirs.  q: rows of num_q_heads * head_dim, q_stride elements from token to token (a
-    // multiple of 8), k likewise; q_out, k_out: [num_tokens][heads][head_dim]; positions: int32
+    // multiple of 8 up to 2^30), k likewise; q_out, k_out: [num_tokens][heads][head_dim]; positions: int32
     // [axes][num_tokens]; weights [head_dim].  k, k_out null: queries alone.  An output may be its own
-    // input where that is dense, and must not overlap inputs otherwise.  Everything 16-byte
-    // aligned but positions.
+    // input where that is dense, and must not overlap inputs, positions or weights otherwise.
+    // Everything 16-byte aligned but positions.
     Result<void> apply(const half *q, int64_t q_stride, const half *k, int64_t k_stride, half *q_out, half *k_out,
                        const int32_t *positions, int num_tokens, int num_q_heads, int num_kv_heads, const half *q_weight,
                        const half *k_weight, float eps, hipStream_t stream) const;
