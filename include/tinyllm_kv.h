@@ -440,8 +440,8 @@ int  tl_kv_cross_attention(tl_kv_cross *c, int layer, const void *q, void *out, 
  *           (a multiple of 8: rows of a fused projection), k likewise; q_out and k_out
  *           [num_tokens][heads][head_dim]; positions int32 [axes][num_tokens] on the
  *           device; weights fp16 [head_dim].  k and k_out NULL: queries alone.  An output may be
- *           its own dense input and must not overlap inputs otherwise.  All but positions
- *           16-byte aligned. */
+ *           its own dense input and must not overlap inputs, positions or weights
+ *           otherwise; strides at most 2^30.  All but positions 16-byte aligned. */
 typedef struct tl_rotary tl_rotary;
 int  tl_rotary_create(int head_dim, int rotary_dim, double theta, int interleaved, const int *axis_of,
                       const double *inv_freq, tl_rotary **out);
