@@ -13,17 +13,40 @@ void plan_quant(QuantPlan &plan, int G, int Hkv, int D, int cus) {
         longest = std::max<int64_t>(longest, quant_tiles(e.S));
     }
     // A workgroup that has a whole entry finishes it; entries in chunks need a second launch, about 3 us
-    // more.  In hundredths of a us (head_dim 128): a tile takes a workgroup 28 alone and 70 where every CU has
-    // one, and takes the chip 60 of a CU's share.  So entries stay whole while the longest takes no more
-    // than that and the share; else they are cut into chunks of a CU's share, of a tile for every wave at least.
-    // Measured, 8 heads, groups of 4, whole and cut: 1 x 1000 tokens 10.4, 13.7 us, 1 x 2000 16.0, 12.9,
-    // 1 x 16000 80, 14.6; 16 x 4000 30.1, 33.5, 16 x 16000 98, 91; 64 x 8192 167, 177.
+    // more.  In hundredths of a us (head_dim 128): a tile takes a CU 28, whether one workgroup or two are on it,
+    // and the chip 60 of a CU's share, more where CUs have nothing.  Chunks are the shortest ones that give every CU
+    // one workgroup at most, or two: a few workgroups beyond that would leave their CUs alone with twice the
+    // work.  Beyond two the chip's share is all that counts.
+    // Measured, 8 heads, groups of 4, head_dim 128, whole and cut: 1 x 1000 tokens 10.4, 13.7 us, 1 x 2000 16.0, 12.9,
+    // 1 x 16000 80, 14.6; 16 x 4000 30.1, 33.5, 16 x 16000 98, 91; 64 x 8192 167, 177.  Chunks of a CU's share,
+    // however many, and these: 10 x 100 .. 30000 76, 64; head_dim 64 4 x 28000 .. 32000 34.4, 26.6; 256 16 x 500 ..
+    // 20000 133, 112.
     const int64_t n = std::max(1, cus), work = some * Hkv, waves = quant_waves(D);
     const int64_t share = (total * Hkv + n - 1) / n;
     const int64_t alone = D <= 128 ? 28 : 112, stream = std::max<int64_t>(1, 60 * D / 128);
-    const int64_t whole = longest * std::max(alone, stream * 7 / 6 * std::min(work, n) / n);
-    const int64_t cut = 300 + std::max(alone * waves, stream * share);
-    const int64_t chunk = whole <= cut ? longest : std::max(waves, share);
+    int64_t       chunk = longest;
+    int64_t       least = work <= n ? std::max(alone * longest, stream * total * Hkv / n * (4 * n - work) / (3 * n))
+                                    : longest * std::max(alone, stream * 7 / 6);
+    auto consider = [&](int64_t c, int64_t per_cu) {
+        const int64_t takes = (c < longest ? 300 : 0) + std::max(alone * per_cu * c, stream * share);
+        if (takes < least) {
+            least = takes;
+            chunk = c;
+        }
+    };
+    for (int64_t k = 1; k <= 2 && work > 0; ++k) {
+        if (work > k * n) continue;
+        int64_t lo = std::min(waves, longest), hi = longest; // the shortest chunks of which there are at most k n
+        while (lo < hi) {
+            const int64_t c = (lo + hi) / 2;
+            int64_t       items = 0;
+            for (const auto &e : plan.entries) items += quant_items(e.S, (int)std::min<int64_t>(c, 1 << 24));
+            if (items * Hkv <= k * n) hi = c;
+            else lo = c + 1;
+        }
+        consider(lo, k);
+    }
+    if (work > 2 * n) consider(std::max(waves, share), 1);
     plan.chunk = (int)std::max<int64_t>(1, std::min<int64_t>(chunk, 1 << 24));
     auto item_tiles = [&](const QuantEntry &e) {
         const int k = quant_items(e.S, plan.chunk);
