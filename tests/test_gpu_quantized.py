@@ -332,6 +332,10 @@ def prefill(tl, c, G, counts, layer=0, scale=None, fused=True, commit=False):
     (128, 1, 4, 64, [1000], [3]),
     (256, 4, 1, 64, [2000], [50]),
     (128, 1, 1, 32, [0], [1100]),
+    (128, 8, 4, 64, [4000, 100, 0], [20, 40, 17]),           # of some entries
+    (64, 2, 8, 32, [0, 5000], [3, 33]),
+    (128, 32, 1, 64, [3000] + [0] * 8, [300] + [200] * 8),   # of the longest, while the others fill the chip
+    (256, 16, 2, 64, [2500] + [10] * 9, [70] + [100] * 9),
 ])
 @pytest.mark.parametrize("fused", [True, False])
 def test_prefill(tl, d, hkv, G, block, lens, counts, fused):

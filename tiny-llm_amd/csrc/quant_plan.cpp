@@ -70,19 +70,38 @@ void plan_quant(QuantPlan &plan, int G, int Hkv, int D, int cus) {
 }
 
 bool plan_quant_prefill(QuantPrefillPlan &plan, int D, int G, int Hkv, int cus) {
-    // Row tiles that leave workgroup slots empty have their keys split over them, in chunks of three tiles
-    // at least (8 heads of 128, groups of 4: 100 over 30000 106 us in 16 chunks, 122 in 8, 120 in 32; 8 x 16
-    // over 4000 .. 8000 58 in 8, 69 in 4, 72 in 16; 300 alone 22 whole, 25 in 2): a chunk's outputs are written
-    // and read again, so never beyond that (16 x 300: 58 whole, 138 in 2).
+    // Row tiles that leave workgroup slots empty have their keys split over them, in chunks of one length, of
+    // three tiles at least, where the longest gets six shorter (8 heads of 128, groups of 4: 100 tokens over 30000
+    // 98 us in 16 chunks, 122 in 8, 120 in 32; 300 alone 22 whole, 25 in 2; entries cut by the length, and each into as
+    // many: 5 x 64 over 500 .. 20000 93, 114, 40 x 24 over 200 .. 3000 66, 91, head_dim 64 6 x 128 over 500 .. 20000
+    // 110, 236).  A chunk's outputs are written and read again, so where slots run out, only what would take
+    // half as long again as the chip's whole work is cut, to that length (longest entry 1.42 and 1.47 times that: 142
+    // and 169 us whole, 154 and 177 cut; 1.62 340, 303; 2.3 498, 333; 16 x 300 58 whole, 138 in 2).
     const int64_t slots = (int64_t)std::max(1, cus) * 8 / quant_prefill_waves(D);
     const int     tile = quant_prefill_rows(D);
-    int64_t       tiles = 0;
-    for (const auto &e : plan.entries) tiles += ((int64_t)e.nq * G + tile - 1) / tile;
-    const int64_t each = slots / std::max<int64_t>(1, tiles * Hkv);
-    for (auto &e : plan.entries) {
-        const int64_t keys = ((int64_t)e.S + quant_prefill_tile(D) - 1) / quant_prefill_tile(D);
-        e.nch = (int)std::max<int64_t>(1, std::min<int64_t>(each, keys / 3));
+    auto          keys = [&](const QuantPrefillEntry &e) { return ((int64_t)e.S + quant_prefill_tile(D) - 1) / quant_prefill_tile(D); };
+    auto          items = [&](int64_t c) { // of chunks of at most c tiles
+        int64_t k = 0;
+        for (const auto &e : plan.entries) k += ((int64_t)e.nq * G + tile - 1) / tile * ((keys(e) + c - 1) / c) * Hkv;
+        return k;
+    };
+    int64_t longest = 1;
+    for (const auto &e : plan.entries) longest = std::max(longest, keys(e));
+    int64_t    lo = std::min<int64_t>(3, longest), hi = longest;
+    const bool rounds = items(longest) > slots;
+    if (rounds) {
+        int64_t work = 0;
+        for (const auto &e : plan.entries) work += ((int64_t)e.nq * G + tile - 1) / tile * keys(e) * Hkv;
+        lo = std::clamp((work + slots - 1) / slots, lo, hi);
+    } else {
+        while (lo < hi) { // the shortest that all have a slot at once
+            const int64_t c = (lo + hi) / 2;
+            if (items(c) <= slots) hi = c;
+            else lo = c + 1;
+        }
     }
+    const int64_t chunk = longest - lo >= (rounds ? std::max<int64_t>(6, lo / 2) : 6) ? lo : longest;
+    for (auto &e : plan.entries) e.nch = (int)((keys(e) + chunk - 1) / chunk);
     std::stable_sort(plan.entries.begin(), plan.entries.end(), [](const QuantPrefillEntry &x, const QuantPrefillEntry &y) {
         return (int64_t)x.S * y.nch > (int64_t)y.S * x.nch;
     });
