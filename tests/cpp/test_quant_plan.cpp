@@ -84,15 +84,15 @@ static void prefill_random() {
             CHECK(l.first == next && l.n <= kQuantPrefillBatch);
             next += l.n;
             int64_t items = 0;
-            bool    split = false;
+            int64_t parts = 0;
             for (int i = l.first; i < l.first + l.n; ++i) {
                 const QuantPrefillEntry &e = p.entries[(size_t)i];
                 seen[(size_t)e.row]++;
                 CHECK(e.item0 == items && e.nch >= 1);
                 items += ((int64_t)e.nq * G + rows - 1) / rows * e.nch;
-                split |= e.nch > 1;
+                if (e.nch > 1) parts = items;
             }
-            CHECK(items == l.items && split == l.split);
+            CHECK(items == l.items && parts == l.parts);
         }
         CHECK(next == n);
         for (int s : seen) CHECK(s == 1);

@@ -468,8 +468,8 @@ size_t part_ml_floats(size_t rows) { return (2 * rows + 3) / 4 * 4; }
 size_t quant_prefill_workspace_floats(const QuantPrefillPlan &plan, int Hkv, int D) {
     size_t most = 0;
     for (const auto &l : plan.launches) {
-        const size_t rows = (size_t)l.items * (size_t)quant_prefill_rows(D) * (size_t)Hkv;
-        if (l.split) most = std::max(most, part_ml_floats(rows) + rows * (size_t)D);
+        const size_t rows = (size_t)l.parts * (size_t)quant_prefill_rows(D) * (size_t)Hkv;
+        if (l.parts) most = std::max(most, part_ml_floats(rows) + rows * (size_t)D);
     }
     return most;
 }
@@ -492,7 +492,7 @@ void launch_quant_prefill(const QuantCall &c, const QuantView &v, const QuantPre
         a.n = l.n;
         std::memcpy(a.e, plan.entries.data() + l.first, sizeof(QuantPrefillEntry) * (size_t)l.n);
         a.part_ml = workspace;
-        a.part_o = l.split ? workspace + part_ml_floats((size_t)l.items * (size_t)ROWS * (size_t)c.Hkv) : nullptr;
+        a.part_o = l.parts ? workspace + part_ml_floats((size_t)l.parts * (size_t)ROWS * (size_t)c.Hkv) : nullptr;
         profile_begin(KernelId::PrefillQuant, stream);
         for_head_dim(c.D, [&](auto d) {
             constexpr int D = decltype(d)::value;
@@ -500,9 +500,9 @@ void launch_quant_prefill(const QuantCall &c, const QuantView &v, const QuantPre
                                dim3(quant_prefill_waves(D) * 64), 0, stream, a);
         });
         HIP_CHECK(hipGetLastError());
-        if (l.split) {
+        if (l.parts) {
             const int rows = kMergeThreads / (c.D / 4);
-            hipLaunchKernelGGL(quant_prefill_merge_kernel, dim3((unsigned)(l.items * c.Hkv), (unsigned)((ROWS + rows - 1) / rows)),
+            hipLaunchKernelGGL(quant_prefill_merge_kernel, dim3((unsigned)(l.parts * c.Hkv), (unsigned)((ROWS + rows - 1) / rows)),
                                dim3(kMergeThreads), 0, stream, a, c.D, ROWS);
             HIP_CHECK(hipGetLastError());
         }

@@ -118,13 +118,13 @@ bool plan_quant_prefill(QuantPrefillPlan &plan, int D, int G, int Hkv, int cus) 
     }
     plan.launches.clear();
     for (size_t i = 0; i < plan.entries.size();) {
-        QuantPrefillLaunch l{(int)i, 0, 0, false};
+        QuantPrefillLaunch l{(int)i, 0, 0, 0};
         int64_t            items = 0;
         for (; i < plan.entries.size() && l.n < kQuantPrefillBatch; ++i, ++l.n) {
             QuantPrefillEntry &e = plan.entries[i];
             e.item0 = (int32_t)items;
             items += ((int64_t)e.nq * G + tile - 1) / tile * e.nch;
-            l.split |= e.nch > 1;
+            if (e.nch > 1) l.parts = (int)std::min<int64_t>(items, kQuantMostItems);
             if (items * Hkv > kQuantMostItems) return false;
         }
         l.items = (int)items;

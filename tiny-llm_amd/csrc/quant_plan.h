@@ -82,8 +82,8 @@ struct QuantPrefillEntry {
     int32_t row, S, tok0, nq, open, nch, item0;
 };
 struct QuantPrefillLaunch {
-    int  first, n, items;
-    bool split; // some entry has several chunks
+    int first, n, items;
+    int parts; // items up to the last of an entry of several chunks, 0: there is none
 };
 struct QuantPrefillPlan {
     std::vector<QuantPrefillEntry>  entries;
