@@ -429,7 +429,7 @@ quant_prefill_kernel(PrefillArgs a) {
     }
 }
 
-constexpr int kMergeThreads = 256;
+constexpr int kMergeThreads = 256, kMergeChunks = 4; // chunks on their way at once
 
 // Workgroup (item that is a row tile's first, kv head; a few rows): D / 4 threads a row.
 __global__ __launch_bounds__(kMergeThreads) void quant_prefill_merge_kernel(PrefillArgs a, int D, int ROWS) {
@@ -443,17 +443,31 @@ __global__ __launch_bounds__(kMergeThreads) void quant_prefill_merge_kernel(Pref
     if (r >= ROWS || qr >= rows) return;
     const int64_t p0 = ((int64_t)item * a.Hkv + g) * ROWS + r, pc = (int64_t)a.Hkv * ROWS;
     float         m = kNone, l = 0.0f;
-    for (int ch = 0; ch < nch; ++ch) m = fmaxf(m, a.part_ml[(p0 + ch * pc) * 2]);
-    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int ch = 0; ch < nch; ++ch) {
-        const int64_t pr = p0 + ch * pc;
-        const float2  ml = *reinterpret_cast<const float2 *>(a.part_ml + pr * 2);
-        const float   wgt = __builtin_amdgcn_exp2f(ml.x - m);
-        const f32x4   x = *reinterpret_cast<const f32x4 *>(a.part_o + pr * D + d);
-        l = fmaf(wgt, ml.y, l);
+    f32x4         o = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c0 = 0; c0 < nch; c0 += kMergeChunks) {
+        float2 ml[kMergeChunks];
+        f32x4  x[kMergeChunks];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = fmaf(wgt, x[i], o[i]);
+        for (int u = 0; u < kMergeChunks; ++u) {
+            const int64_t pr = p0 + min(c0 + u, nch - 1) * pc;
+            ml[u] = *reinterpret_cast<const float2 *>(a.part_ml + pr * 2);
+            x[u] = *reinterpret_cast<const f32x4 *>(a.part_o + pr * D + d);
+        }
+        float most = m;
+#pragma unroll
+        for (int u = 0; u < kMergeChunks; ++u) most = fmaxf(most, ml[u].x);
+        const float before = __builtin_amdgcn_exp2f(m - most);
+        l *= before;
+        o *= before;
+        m = most;
+#pragma unroll
+        for (int u = 0; u < kMergeChunks; ++u) {
+            if (c0 + u >= nch) break;
+            const float wgt = __builtin_amdgcn_exp2f(ml[u].x - m);
+            l = fmaf(wgt, ml[u].y, l);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[i] = fmaf(wgt, x[u][i], o[i]);
+        }
     }
     const float   inv = 1.0f / (l + 1e-6f);
     const __half2 lo = __floats2half2_rn(o[0] * inv, o[1] * inv), hi = __floats2half2_rn(o[2] * inv, o[3] * inv);
