@@ -233,6 +233,10 @@ def decode(tl, c, G, layer=0, scale=None, fused=True):
     (64, 4, 4, 256, [4000, 1, 255]),
     (128, 1, 4, 64, [9000]),
     (128, 8, 4, 128, [33000, 31]),
+    (128, 64, 1, 32, [0, 31, 32, 100, 500]),                 # many short ones: 5 x 64 workgroups
+    (64, 64, 2, 32, [0, 63, 64, 95, 31, 1, 300, 200, 7]),
+    (256, 40, 1, 32, [0, 1, 31, 33, 128, 250, 64]),
+    (32, 128, 1, 32, [3, 62, 0, 63, 1000]),
 ])
 @pytest.mark.parametrize("fused", [True, False])
 def test_decode(tl, d, hkv, G, block, lens, fused):
@@ -320,6 +324,7 @@ def prefill(tl, c, G, counts, layer=0, scale=None, fused=True, commit=False):
     (64, 2, 1, 32, [0, 5, 31], [1, 16, 2]),                 # up to 16 query rows
     (128, 2, 4, 64, [100, 60, 28, 0], [4, 4, 4, 4]),
     (128, 1, 8, 32, [2000, 31], [2, 1]),
+    (128, 64, 4, 32, [0, 30, 31, 61, 100], [4, 4, 1, 3, 2]),
     (32, 2, 8, 32, [0, 0, 62], [2, 1, 2]),
     (256, 1, 2, 32, [70, 31], [8, 3]),
     (64, 2, 1, 32, [0, 0, 0, 40], [17, 31, 32, 33]),         # more

@@ -6,8 +6,8 @@
 // K_t, V_t: the stored whole numbers, ks, vs: the scales of t's group.  Bound by HBM: 2 D
 // bytes a token and kv head.
 //
-// A workgroup of 8 waves (4 at head_dim 256) per (entry, chunk of tiles of 64 tokens, kv head); wave w
-// takes every 8th (4th) tile (half a tile at a time at head_dim 256) and keeps its own running
+// A workgroup of NW waves (8, 4 at head_dim 256, 2 for many short entries) per (entry, chunk of tiles of 64
+// tokens, kv head); wave w takes every NW-th tile (half a tile at a time at head_dim 256) and keeps its own running
 // maximum, sum and output; the next tile is on its way while one is computed.  Tiles lie in
 // memory as the operands that the matrix instructions take, so nothing passes through LDS:
 //   S^T = K Q^T      v_mfma_f32_16x16x32_f16: A = K (token l%16, dims 8(l/16)..+7),
@@ -60,9 +60,8 @@ struct QuantArgs {
 };
 static_assert(sizeof(QuantArgs) <= 4096, "kernel arguments");
 
-template <int D>
-__global__ __launch_bounds__(quant_waves(D) * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(QuantArgs a) {
-    constexpr int NW = quant_waves(D);
+template <int D, int NW>
+__global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(QuantArgs a) {
     constexpr int NG = D <= 128 ? 2 : 1;  // groups of a step
     constexpr int SUB = 2 / NG;           // steps per tile
     constexpr int KS = D / 32, DT = D / 16;
@@ -406,9 +405,8 @@ __global__ __launch_bounds__(kFinishThreads) void quant_finish_kernel(QuantArgs 
 // Floats of the partial maxima and sums, then the outputs at a multiple of 16 bytes.
 size_t part_ml_floats(size_t rows) { return (2 * rows + 3) / 4 * 4; }
 
-template <int D> void launch_one(const QuantArgs &a, int items, hipStream_t stream) {
-    constexpr int         NW = quant_waves(D);
-    auto                 *fn = attn_quant_kernel<D>;
+template <int D, int NW> void launch_one(const QuantArgs &a, int items, hipStream_t stream) {
+    auto                 *fn = attn_quant_kernel<D, NW>;
     static std::once_flag once[64]; // per device
     std::call_once(once[current_device() & 63], [&] {
         HIP_CHECK(hipFuncSetAttribute(reinterpret_cast<const void *>(fn), hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -455,7 +453,11 @@ void launch_attn_quant(const QuantCall &c, const QuantView &v, const QuantPlan &
         a.part_o = l.finish ? workspace + part_ml_floats((size_t)l.items * c.Hkv * a.rows) : nullptr;
         profile_begin(KernelId::AttnQuant, stream);
         if (l.items > 0) {
-            for_head_dim(c.D, [&](auto d) { launch_one<decltype(d)::value>(a, l.items, stream); });
+            for_head_dim(c.D, [&](auto d) {
+                constexpr int D = decltype(d)::value;
+                if (plan.small) launch_one<D, kQuantSmallWaves>(a, l.items, stream);
+                else launch_one<D, quant_waves(D)>(a, l.items, stream);
+            });
             HIP_CHECK(hipGetLastError());
         }
         if (l.finish) {

@@ -47,6 +47,12 @@ void plan_quant(QuantPlan &plan, int G, int Hkv, int D, int cus) {
         consider(lo, k);
     }
     if (work > 2 * n) consider(std::max(waves, share), 1);
+    // More entries than workgroups of all waves fit at once (one a CU, two where registers are few), and short ones:
+    // workgroups of two waves, four times as many. 33 x 32 heads of 128, to 64 tokens 13.8 us, 26.4 with eight
+    // waves, to 800 38.6 and 51.7, to 1500 61.6 and 72.5, to 3000 113 and 110; 90 x 8 9.7 and 19.3, 22.9 and 34.2, 40.9
+    // and 47.0, 79.9 and 74.7; 33 x 32 of 64 7.5 and 13.1, 17.4 and 24.1, 30.4 and 32.3, 61 and 53.  As many as fit: 32 x 8
+    // of 128, to 300 tokens 9.9 and 8.1.
+    plan.small = longest <= 20 && work > n * (D <= 64 ? 2 : 1);
     plan.chunk = (int)std::max<int64_t>(1, std::min<int64_t>(chunk, 1 << 24));
     auto item_tiles = [&](const QuantEntry &e) {
         const int k = quant_items(e.S, plan.chunk);

@@ -66,10 +66,12 @@ struct QuantPlan {
     std::vector<QuantEntry>  entries;
     std::vector<QuantLaunch> launches;
     int                      chunk = 1; // tiles
+    bool                     small = false; // workgroups of kQuantSmallWaves waves
     void                     clear() { entries.clear(), launches.clear(); }
 };
-// Waves of a workgroup.
+// Waves of a workgroup: for most, and for many entries of a few tiles.
 constexpr int quant_waves(int D) { return D <= 128 ? 8 : 4; }
+constexpr int kQuantSmallWaves = 2;
 inline int quant_tiles(int S) { return S / kQuantTile + (S % kQuantTile != 0); }
 inline int quant_items(int S, int chunk) { return (quant_tiles(S) + chunk - 1) / chunk; }
 // Sets item0 of plan.entries (and orders them, longest first), the launches and the chunk length.
