@@ -431,9 +431,12 @@ quant_prefill_kernel(PrefillArgs a) {
 
 constexpr int kMergeThreads = 256, kMergeChunks = 4; // chunks on their way at once
 
-// Workgroup (row tile of a cut entry, kv head; a few rows): D / 4 threads a row.  (A workgroup for every item,
+// Workgroup (row tile of a cut entry, kv head; a few rows): `split` times D / 4 threads a row, which meet in
+// LDS.  (A workgroup for every item,
 // all but a row tile's first leaving at once: 14 us where this takes 8.6, 512 items of 80 row tiles.)
-__global__ __launch_bounds__(kMergeThreads) void quant_prefill_merge_kernel(PrefillArgs a, int D, int ROWS) {
+__global__ __launch_bounds__(kMergeThreads) void quant_prefill_merge_kernel(PrefillArgs a, int D, int ROWS, int split) {
+    __shared__ f32x4  s_o[kMergeThreads];
+    __shared__ float2 s_ml[kMergeThreads];
     const int b = blockIdx.x / a.Hkv, g = blockIdx.x - b * a.Hkv;
     // Row tile b of those of cut entries, in the entries' order.
     int ei = 0, before = 0;
@@ -456,37 +459,53 @@ __global__ __launch_bounds__(kMergeThreads) void quant_prefill_merge_kernel(Pref
         before += __shfl(own, 63);
     }
     const int nch = a.e[ei].nch, rel = (b - before) * nch, item = a.e[ei].item0 + rel;
-    const int per = D / 4, r = blockIdx.y * (kMergeThreads / per) + threadIdx.x / per, d = 4 * (threadIdx.x % per);
+    const int per = D / 4, grp = threadIdx.x / per, part = grp % split, d = 4 * (threadIdx.x % per);
+    const int r = blockIdx.y * (kMergeThreads / per / split) + grp / split;
     const int rows = a.e[ei].nq << a.lgG, rt = (rows + ROWS - 1) / ROWS - 1 - rel / nch, qr = rt * ROWS + r;
-    if (r >= ROWS || qr >= rows) return;
+    const bool there = r < ROWS && qr < rows;
     const int64_t p0 = ((int64_t)item * a.Hkv + g) * ROWS + r, pc = (int64_t)a.Hkv * ROWS;
     float         m = kNone, l = 0.0f;
     f32x4         o = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int c0 = 0; c0 < nch; c0 += kMergeChunks) {
+    auto          raise = [&](float most) {
+        const float by = __builtin_amdgcn_exp2f(m - most);
+        l *= by;
+        o *= by;
+        m = most;
+    };
+    auto join = [&](float2 ml, f32x4 x) { // (ml.x at most m)
+        const float wgt = __builtin_amdgcn_exp2f(ml.x - m);
+        l = fmaf(wgt, ml.y, l);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = fmaf(wgt, x[i], o[i]);
+    };
+    for (int c0 = there ? part : nch; c0 < nch; c0 += kMergeChunks * split) {
         float2 ml[kMergeChunks];
         f32x4  x[kMergeChunks];
 #pragma unroll
         for (int u = 0; u < kMergeChunks; ++u) {
-            const int64_t pr = p0 + min(c0 + u, nch - 1) * pc;
+            const int64_t pr = p0 + min(c0 + u * split, nch - 1) * pc;
             ml[u] = *reinterpret_cast<const float2 *>(a.part_ml + pr * 2);
             x[u] = *reinterpret_cast<const f32x4 *>(a.part_o + pr * D + d);
         }
         float most = m;
 #pragma unroll
         for (int u = 0; u < kMergeChunks; ++u) most = fmaxf(most, ml[u].x);
-        const float before = __builtin_amdgcn_exp2f(m - most);
-        l *= before;
-        o *= before;
-        m = most;
+        raise(most);
 #pragma unroll
-        for (int u = 0; u < kMergeChunks; ++u) {
-            if (c0 + u >= nch) break;
-            const float wgt = __builtin_amdgcn_exp2f(ml[u].x - m);
-            l = fmaf(wgt, ml[u].y, l);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = fmaf(wgt, x[u][i], o[i]);
+        for (int u = 0; u < kMergeChunks; ++u)
+            if (c0 + u * split < nch) join(ml[u], x[u]);
+    }
+    if (split > 1) {
+        s_o[threadIdx.x] = o;
+        s_ml[threadIdx.x] = make_float2(m, l);
+        __syncthreads();
+        for (int k = 1; k < split && part == 0; ++k) {
+            const float2 ml = s_ml[threadIdx.x + k * per];
+            raise(fmaxf(m, ml.x));
+            join(ml, s_o[threadIdx.x + k * per]);
         }
     }
+    if (part != 0 || !there) return;
     const float   inv = 1.0f / (l + 1e-6f);
     const __half2 lo = __floats2half2_rn(o[0] * inv, o[1] * inv), hi = __floats2half2_rn(o[2] * inv, o[3] * inv);
     uint16_t     *op = a.out + ((int64_t)(a.e[ei].tok0 + (qr >> a.lgG)) * a.Hq + (g << a.lgG) + (qr & ((1 << a.lgG) - 1))) * D + d;
@@ -533,12 +552,20 @@ void launch_quant_prefill(const QuantCall &c, const QuantView &v, const QuantPre
         });
         HIP_CHECK(hipGetLastError());
         if (l.parts) {
-            const int rows = kMergeThreads / (c.D / 4);
-            int       row_tiles = 0;
+            int row_tiles = 0, most = 1, split = 1, rows = kMergeThreads / (c.D / 4);
             for (int i = 0; i < l.n; ++i)
-                if (a.e[i].nch > 1) row_tiles += ((a.e[i].nq << a.lgG) + ROWS - 1) / ROWS;
+                if (a.e[i].nch > 1) {
+                    row_tiles += ((a.e[i].nq << a.lgG) + ROWS - 1) / ROWS;
+                    most = std::max(most, a.e[i].nch);
+                }
+            // (while there are few: 3 x 291 tokens of one kv head, to 39 chunks of 15 row tiles, 31 us a call, 37 with one
+            // thread; 100 of 8 heads of 64 over 30000 in 157 chunks 31, 47)
+            while (rows > 1 && split * kMergeChunks < most && (int64_t)row_tiles * c.Hkv * (ROWS / rows) * 2 <= 8 * device_cus()) {
+                split *= 2;
+                rows /= 2;
+            }
             hipLaunchKernelGGL(quant_prefill_merge_kernel, dim3((unsigned)(row_tiles * c.Hkv), (unsigned)((ROWS + rows - 1) / rows)),
-                               dim3(kMergeThreads), 0, stream, a, c.D, ROWS);
+                               dim3(kMergeThreads), 0, stream, a, c.D, ROWS, split);
             HIP_CHECK(hipGetLastError());
         }
         profile_end(KernelId::PrefillQuant, stream);
