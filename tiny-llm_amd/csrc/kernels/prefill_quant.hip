@@ -5,8 +5,8 @@
 // 4 D operations a query row and token, and K and V pass through the CUs once per tile of
 // rows.
 //
-// quant_prefill_kernel: a workgroup of four waves at head_dim 128, two of them a CU, and of eight
-// elsewhere (figures: quant_prefill_waves), per (row tile, chunk of key tiles, kv head);
+// quant_prefill_kernel: a workgroup of four waves at head_dim 128 and of eight elsewhere, two a CU up to
+// head_dim 128 (figures: quant_prefill_waves), per (row tile, chunk of key tiles, kv head);
 // a wave has 32 rows (16 at head_dim 256: tokens x heads of the kv head).  A tile of 64 tokens (32 at
 // head_dim 256) is loaded as stored while the one before is computed, made fp16 once per workgroup and put
 // into one of two LDS buffers as operands, 16 bytes a lane in lane order, so that every LDS access is
@@ -97,7 +97,7 @@ template <bool SMALL> __device__ __forceinline__ void scale_values(u32x4 &x, uin
 }
 
 template <int D>
-__global__ __launch_bounds__(quant_prefill_waves(D) * 64) __attribute__((amdgpu_waves_per_eu(2))) void
+__global__ __launch_bounds__(quant_prefill_waves(D) * 64) __attribute__((amdgpu_waves_per_eu(quant_prefill_waves(D) * quant_prefill_per_cu(D) / 4))) void
 quant_prefill_kernel(PrefillArgs a) {
     constexpr int NW = quant_prefill_waves(D), ROWS = quant_prefill_rows(D);
     constexpr int R = ROWS / NW, NQG = R / 16;                      // rows of a wave, in parts of 16
@@ -258,21 +258,23 @@ quant_prefill_kernel(PrefillArgs a) {
         l_run[j] = 0.0f;
         m_run[j] = kNone;
     }
+
     const f16x8 ones = __builtin_bit_cast(f16x8, u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
 
     // Operands come from LDS in batches, the next one on its way while one is multiplied.  (Left to itself the
     // compiler reads two and waits for them: 607 us where this took 598.)
-    constexpr int NB = NG * KS / 2; // batches of four, of scores and of values
-    f16x8         kf[4], vf[4];
+    // (Two at head_dim 64, and those of the values behind the softmax: 128 registers.)
+    constexpr int BATCH = D == 64 ? 2 : 4, NB = 2 * NG * KS / BATCH; // batches of scores, and of values
+    f16x8         kf[BATCH], vf[BATCH];
     auto scores_batch = [&](int i, int b, f16x8 *f) __attribute__((always_inline)) { // keys 16 tt .., dims 32 st ..
         const f16x8 *k16 = reinterpret_cast<const f16x8 *>(s_k[i % 2]) + lane;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) f[u] = k16[(4 * b + u) * 64];
+        for (int u = 0; u < BATCH; ++u) f[u] = k16[(BATCH * b + u) * 64];
     };
     auto values_batch = [&](int i, int b, f16x8 *f) __attribute__((always_inline)) {
         const f16x8 *v16 = reinterpret_cast<const f16x8 *>(s_v[i % 2]) + lane;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) f[u] = v16[(4 * b + u) * 64];
+        for (int u = 0; u < BATCH; ++u) f[u] = v16[(BATCH * b + u) * 64];
     };
     // (the first batch is in kf, vf)
     auto scores = [&](int i) __attribute__((always_inline)) {
@@ -282,20 +284,20 @@ quant_prefill_kernel(PrefillArgs a) {
             for (int j = 0; j < NQG; ++j) s[j][tt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            f16x8 next[4];
+            f16x8 next[BATCH];
             if (b + 1 < NB) scores_batch(i, b + 1, next);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < BATCH; ++u)
 #pragma unroll
                 for (int j = 0; j < NQG; ++j) {
-                    const int tt = (4 * b + u) / KS, st = (4 * b + u) % KS;
+                    const int tt = (BATCH * b + u) / KS, st = (BATCH * b + u) % KS;
                     s[j][tt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[u], qb[j][st], s[j][tt], 0, 0, 0);
                 }
             __builtin_amdgcn_sched_barrier(0);
             if (b + 1 < NB)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) kf[u] = next[u];
+                for (int u = 0; u < BATCH; ++u) kf[u] = next[u];
         }
     };
     auto softmax = [&](int i) __attribute__((always_inline)) {
@@ -305,12 +307,13 @@ quant_prefill_kernel(PrefillArgs a) {
         for (int k = 0; k < NG; ++k) f[k] = a.scale_log2 * of[k].x;
         if (__builtin_expect(t0 + TILE > all, 0)) { // some score does not count
 #pragma unroll
-            for (int j = 0; j < NQG; ++j)
+            for (int j = 0; j < NQG; ++j) {
+                const int end = seen_by(j) - t0 - 4 * qg;
 #pragma unroll
                 for (int tt = 0; tt < 2 * NG; ++tt)
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        s[j][tt][x] = t0 + 16 * tt + 4 * qg + x < seen_by(j) ? s[j][tt][x] * f[tt >> 1] : -INFINITY;
+                    for (int x = 0; x < 4; ++x) s[j][tt][x] = 16 * tt + x < end ? s[j][tt][x] * f[tt >> 1] : -INFINITY;
+            }
 #pragma unroll
             for (int k = 0; k < NG; ++k) f[k] = 1.0f;
         }
@@ -347,21 +350,21 @@ quant_prefill_kernel(PrefillArgs a) {
         f32x4 sums[NQG][NG];
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            f16x8 next[4];
+            f16x8 next[BATCH];
             if (b + 1 < NB) values_batch(i, b + 1, next);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < BATCH; ++u)
 #pragma unroll
                 for (int j = 0; j < NQG; ++j) {
-                    const int k = (4 * b + u) / DT, dt = (4 * b + u) % DT;
+                    const int k = (BATCH * b + u) / DT, dt = (BATCH * b + u) % DT;
                     if (dt == 0) sums[j][k] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[j][k], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
                     acc[j][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[u], pf[j][k], acc[j][dt], 0, 0, 0);
                 }
             __builtin_amdgcn_sched_barrier(0);
             if (b + 1 < NB)
 #pragma unroll
-                for (int u = 0; u < 4; ++u) vf[u] = next[u];
+                for (int u = 0; u < BATCH; ++u) vf[u] = next[u];
         }
 #pragma unroll
         for (int j = 0; j < NQG; ++j)
@@ -381,8 +384,9 @@ quant_prefill_kernel(PrefillArgs a) {
 #pragma unroll
                 for (int k = 0; k < NG; ++k) of[k] = s_scale[i % 2][k];
                 scores(i);
-                values_batch(i, 0, vf);
+                if (D != 64) values_batch(i, 0, vf);
                 softmax(i);
+                if (D == 64) values_batch(i, 0, vf);
                 values(i);
             }
             if (i + 1 < t_n) stage(i + 1);

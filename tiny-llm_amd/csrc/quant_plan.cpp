@@ -83,7 +83,7 @@ bool plan_quant_prefill(QuantPrefillPlan &plan, int D, int G, int Hkv, int cus) 
     // 110, 236).  A chunk's outputs are written and read again, so where slots run out, only what would take
     // half as long again as the chip's whole work is cut, to that length (longest entry 1.42 and 1.47 times that: 142
     // and 169 us whole, 154 and 177 cut; 1.62 340, 303; 2.3 498, 333; 16 x 300 58 whole, 138 in 2).
-    const int64_t slots = (int64_t)std::max(1, cus) * 8 / quant_prefill_waves(D);
+    const int64_t slots = (int64_t)std::max(1, cus) * quant_prefill_per_cu(D);
     const int     tile = quant_prefill_rows(D);
     auto          keys = [&](const QuantPrefillEntry &e) { return ((int64_t)e.S + quant_prefill_tile(D) - 1) / quant_prefill_tile(D); };
     auto          items = [&](int64_t c) { // of chunks of at most c tiles

@@ -92,12 +92,13 @@ struct QuantPrefillPlan {
     std::vector<QuantPrefillLaunch> launches;
     void                            clear() { entries.clear(), launches.clear(); }
 };
-// Waves and rows of a workgroup, and the tokens of its key tiles.  Four waves and two
-// workgroups a CU at head_dim 128, eight waves and one elsewhere (1 x 8192, 4 x 500 over 3000 .. 6000; 8 heads,
-// groups of 4, eight waves against four: 128 611, 221 against 598, 190 us; 256 1288, 420 against 2704, 825;
-// 64 392, 138 against 396, 154; 32 313, 104 against 289, 114).
+// Waves and rows of a workgroup, workgroups a CU, and the tokens of a key tile.  Four waves and two workgroups at
+// head_dim 128, eight waves elsewhere, two workgroups where 128 registers do (1 x 8192, 4 x 500 over 3000 .. 6000; 8 heads,
+// groups of 4, eight waves against four: 128 611, 221 against 598, 190 us; 256 1288, 420 against 2704, 825; 64
+// 321, 114 against 338, 121; 32 232, 87 against 240, 89.  One workgroup of eight at 64 394, 152, at 32 304, 117).
 constexpr int quant_prefill_waves(int D) { return D == 128 ? 4 : 8; }
 constexpr int quant_prefill_rows(int D) { return quant_prefill_waves(D) * (D <= 128 ? 32 : 16); }
+constexpr int quant_prefill_per_cu(int D) { return D <= 128 ? 2 : 1; }
 constexpr int quant_prefill_tile(int D) { return D <= 128 ? 64 : 32; }
 // Sets nch and item0 of plan.entries and the launches (and orders the
 // entries, longest items first).  False when a launch would have more than 2^32 threads.
