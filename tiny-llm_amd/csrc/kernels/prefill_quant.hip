@@ -23,7 +23,7 @@
 // 8192 tokens, 32 heads over 8 of 128: 557 us, 0.99 PFLOP/s (0.91 on another card, where a large
 // fp16 product takes 1.10 in place of 1.15).  Of a SIMD's cycles MFMA takes 42%, VALU 40%; the LDS is read
 // 40% of the time, without bank conflicts.  What is left are the two waves of a SIMD waiting for each
-// other at barriers and for operands: a third needs 168 registers, and a wave has 226.
+// other at barriers and for operands: a third needs 168 registers, and a wave has 219.
 // Tried and slower: eight waves of which four multiply while four do their softmax (636),
 // one group a step, priorities around the products.
 // quant_prefill_merge_kernel: joins the chunks of entries whose keys were split.
