@@ -13,8 +13,11 @@
 //   S^T = K Q^T      v_mfma_f32_16x16x32_f16: A = K (token l%16, dims 8(l/16)..+7),
 //                    B = Q (row l%16), D = S^T (tokens 4(l/16)+i, row l%16)
 //   O^T += vs V^T P^T  A = V^T (dim l%16, the group's tokens that the lane has weights of),
-//                    B = the weights as they came out; a group's product is scaled in fp32
-// Whole numbers up to 127 are exact in fp16, so the scales are all that rounds them.
+//                    B = the weights as they came out, their upper and then their lower half in
+//                    fp16 (22 bits); a group's product is scaled in fp32
+// Whole numbers up to 127 are exact in fp16, so the scales are all that rounds them.  The weights' lower halves
+// are a second product of the matrix units, which wait for HBM as it is: 64 x 8192 169.4 us with them, 166.8
+// without, 131072 alone 51.3 and 50.6, and without them outputs are 2.9e-4 off, of which their own rounding is 2.1e-4.
 // The open group (fp16, at most 31 tokens), and the one that the call's token closes, is a step of its
 // own of one wave, the one with the fewest others.
 // Measured, 8 kv heads of 128: 64 x 8192 tokens, groups of 4, 161-171 us, 6.3-6.7 TB/s (counters: 1.08 GB read,
@@ -115,6 +118,16 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
             m_run = m_new;
         }
     };
+    auto weigh = [&](float score, f16x8 &hi, f16x8 &lo, int at) __attribute__((always_inline)) { // the weight's 22 bits
+        const float p = __builtin_amdgcn_exp2f(score - m_run);
+        l_run += p;
+        hi[at] = (_Float16)p;
+        lo[at] = (_Float16)(p - (float)hi[at]);
+    };
+    auto times_weights = [](f16x8 v, f16x8 hi, f16x8 lo) __attribute__((always_inline)) {
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(v, hi, __builtin_amdgcn_mfma_f32_16x16x32_f16(v, lo, zero, 0, 0, 0), 0, 0, 0);
+    };
 
     // The wave's steps: step x is half (all) of tile tile_lo + x / SUB * NW + wave.
     const int steps = max(0, (end - tile_lo - wave + NW - 1) / NW) * SUB;
@@ -192,22 +205,17 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
         raise(mloc);
 #pragma unroll
         for (int k = 0; k < NG; ++k) {
-            f16x8 pf;
+            f16x8 hi, lo;
 #pragma unroll
             for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = __builtin_amdgcn_exp2f(s[k][tt][i] - m_run);
-                    l_run += p;
-                    pf[4 * tt + i] = (_Float16)p;
-                }
+                for (int i = 0; i < 4; ++i) weigh(s[k][tt][i], hi, lo, 4 * tt + i);
             // (a group whose scale is NaN is none of the rows' business that see none of it)
             const float by = t0 + 32 * k < bound ? vs[k] : 0.0f;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
                 const u32x4 w = vr[k][dt / 2];
-                const f32x4 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(whole8(w[2 * (dt & 1)], w[2 * (dt & 1) + 1]), pf,
-                                                                      f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+                const f32x4 o = times_weights(whole8(w[2 * (dt & 1)], w[2 * (dt & 1) + 1]), hi, lo);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[dt][i] = fmaf(by, o[i], acc[dt][i]);
             }
@@ -253,15 +261,11 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
                 mloc = fmaxf(mloc, s[tt][i]);
             }
         raise(mloc);
-        f16x8 pf;
+        f16x8 hi, lo;
 #pragma unroll
         for (int tt = 0; tt < 2; ++tt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = __builtin_amdgcn_exp2f(s[tt][i] - m_run);
-                l_run += p;
-                pf[4 * tt + i] = (_Float16)p;
-            }
+            for (int i = 0; i < 4; ++i) weigh(s[tt][i], hi, lo, 4 * tt + i);
         // Values of tokens behind the last are whatever the tile held: 0 times them could be
         // NaN.  The same goes for infinite values that only some of the rows see.
         bool odd = false;
@@ -275,7 +279,7 @@ __global__ __launch_bounds__(NW * 64, D <= 128 ? 2 : 1) void attn_quant_kernel(Q
                 odd |= there && !finite;
                 if (!there || !finite) v[j] = (_Float16)0.0f;
             }
-            const f32x4 o = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pf, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+            const f32x4 o = times_weights(v, hi, lo);
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc[dt][i] = fmaf(group.vs, o[i], acc[dt][i]);
         }
