@@ -135,7 +135,9 @@ int tl_kv_create_paged(const tl_kv_config *cfg, int block_tokens, int num_blocks
  * refuse when the length of one of its sequences changed since its prepare.  tl_kv_advance over
  * less than was appended (drafted tokens that were rejected) may end at a multiple of
  * 32, in the group in which the append began or in the one in which it ended; elsewhere it
- * is refused, the rows of that group being gone.  The first call of a size allocates the
+ * is refused, the rows of that group being gone.  Beyond what was appended it may end
+ * in the group of the last appended token, or anywhere where that one completed its group; elsewhere
+ * it is refused, as the open group's tokens would be lost.  The first call of a size allocates the
  * workspace: make one before a captured one; one batch is used from one stream at a time. */
 int tl_kv_create_quantized(const tl_kv_config *cfg, int block_tokens, int num_blocks, tl_kv_manager **out);
 int tl_kv_is_quantized(const tl_kv_manager *mgr);

@@ -354,11 +354,17 @@ Result<void> KVCacheManager::advanceSeqLen(int seq_id, int num_tokens) {
     if (quantized_) {
         detail::OpenGroup &open = open_[static_cast<size_t>(it->second)];
         if (!open.advance(old_len, new_len)) {
-            const std::string msg = "advanceSeqLen: length " + std::to_string(new_len) + " of sequence " +
-                                    std::to_string(seq_id) + " lies inside the tokens up to " + std::to_string(open.end) +
-                                    " that were appended at once: an 8-bit cache can be cut there at a multiple of " +
-                                    std::to_string(detail::kGroup) +
-                                    ", in the group in which they begin or in the one in which they end";
+            const std::string length = "advanceSeqLen: length " + std::to_string(new_len) + " of sequence " +
+                                       std::to_string(seq_id);
+            const std::string msg =
+                open.leaves_rows(new_len)
+                    ? length + " is beyond the tokens up to " + std::to_string(open.end) +
+                          " that were appended, and in an 8-bit cache the last of them wait in their group of " +
+                          std::to_string(detail::kGroup) + " for those that complete it"
+                    : length + " lies inside the tokens up to " + std::to_string(open.end) +
+                          " that were appended at once: an 8-bit cache can be cut there at a multiple of " +
+                          std::to_string(detail::kGroup) +
+                          ", in the group in which they begin or in the one in which they end";
             TL_LOG_ERROR("%s", msg.c_str());
             return Result<void>::err(msg);
         }

@@ -33,10 +33,14 @@ struct OpenGroup {
     }
     // Tokens that are there, those behind len included, and the tile of their last group.
     std::pair<int, int> held(int len) const { return {end > len ? end : len, end > len ? tiles(len, end - len).second : cur}; }
-    // From length len to length `to`; false (and no change) where that lies inside what one append
-    // brought and the rows that would be open again are gone.
+    // Whether length `to` leaves the group that the last append ended in, whose rows wait in fp16 for those
+    // that complete it: nothing would read them there any more.
+    bool leaves_rows(int to) const { return end % kGroup != 0 && to / kGroup > end / kGroup; }
+    // From length len to length `to`; false (and no change) where that leaves rows behind, or lies
+    // inside what one append brought and the rows that would be open again are gone.
     bool advance(int len, int to) {
         const int g = to / kGroup;
+        if (leaves_rows(to)) return false;
         if (g != len / kGroup && group[1 - cur] == g) {
             cur = 1 - cur;
         } else if (to % kGroup != 0 && to < end && (g != len / kGroup || group[cur] != g)) {
