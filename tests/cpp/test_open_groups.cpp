@@ -94,7 +94,81 @@ static void advance_beyond_what_was_appended() {
     std::puts("ok advance_beyond_what_was_appended");
 }
 
+// Several batches append at one length, in any order, and one of them commits.
+static void advance_over_another_append() {
+    int ok = 0, refused = 0, replaced = 0;
+    for (int it = 0; it < 40000; ++it) {
+        OpenGroup o;
+        Memory    m;
+        int       len = upto(100), last = 0, most = 0;
+        append(o, m, 0, len + 1, 1000);
+        CHECK(o.advance(0, ++len));
+        int n[4];
+        for (int k = 0; k < 4; ++k) n[k] = upto(1) ? 1 + upto(8) : 1 + upto(90);
+        for (int k = 0, count = 1 + upto(4); k < count; ++k) {
+            last = n[upto(3)];
+            most = std::max(most, last);
+            append(o, m, len, last, (k + 2) * 10000);
+        }
+        const int to = len + n[upto(3)];
+        // What an append brought again may be less than what was there before: the rest is gone.
+        const bool gone = to > len + last && to <= len + most;
+        const bool done = o.advance(len, to);
+        if (gone) {
+            CHECK(!done);
+            ++replaced;
+        }
+        if (to == len + last) CHECK(done);
+        if (!done) {
+            ++refused;
+            continue;
+        }
+        ++ok;
+        m.check(to, o.cur);
+    }
+    CHECK(ok > 5000 && refused > 5000 && replaced > 5000);
+    std::puts("ok advance_over_another_append");
+}
+
+// Batches that append to some of the layers only: every layer has to have had the same.
+static void advance_where_layers_differ() {
+    constexpr int L = 3;
+    int           ok = 0, refused = 0;
+    for (int it = 0; it < 40000; ++it) {
+        OpenGroup o;
+        Memory    m[L];
+        int       ends[L] = {}, len = 1 + upto(100);
+        auto      add = [&](int at, int n, unsigned layers, int stamp) {
+            const auto [first, last] = o.tiles(at, n);
+            for (int l = 0; l < L; ++l)
+                if (layers >> l & 1) m[l].append(at, n, first, last, stamp + 1000 * l), ends[l] = at + n;
+            o.append(at, n);
+        };
+        add(0, len + (upto(1) ? 0 : upto(90)), 7, 10000);
+        if (!o.alike(ends, L, 0, len) || !o.advance(0, len)) continue; // (an inside length)
+        int last = 0;
+        for (int k = 0, count = 1 + upto(3); k < count; ++k) {
+            last = 1 + upto(upto(1) ? 8 : 90);
+            add(len, last, upto(1) ? 7u : 1u + (unsigned)upto(6), (k + 2) * 10000);
+            if (upto(2) == 0) { // the same, in all of them
+                add(len, last, 7, (k + 2) * 10000);
+                CHECK(o.alike(ends, L, len, len + last));
+            }
+        }
+        if (!o.alike(ends, L, len, len + last) || !o.advance(len, len + last)) {
+            ++refused;
+            continue;
+        }
+        ++ok;
+        for (int l = 0; l < L; ++l) m[l].check(len + last, o.cur);
+    }
+    CHECK(ok > 5000 && refused > 5000);
+    std::puts("ok advance_where_layers_differ");
+}
+
 int main() {
     advance_beyond_what_was_appended();
+    advance_over_another_append();
+    advance_where_layers_differ();
     return 0;
 }

@@ -41,3 +41,105 @@ def test_lengths_beyond_what_was_appended(tl):
         b.commit(40)
     torch.cuda.synchronize()
     check_first(c, [0, 32, 0, 70])
+
+
+class Prompt:
+    """A prompt of n tokens for sequence 0, and its rows in every layer."""
+
+    def __init__(self, tl, c, n, G=1):
+        self.c, self.n, self.new = c, n, c.new_rows([n])
+        self.b = tl.PrefillBatch(c.mgr, 1, c.hkv * G)
+        self.b.prepare(c.ids[:1], [n])
+        self.kv = [tuple(dev(x[0]) for x in layer) for layer in self.new]
+        self.q = dev(c.rng.standard_normal((n, c.hkv * G, c.d)).astype(np.float16))
+        self.out = torch.zeros_like(self.q)
+
+    def append(self, layer=0, s=0):
+        self.b.append(layer, *(x.data_ptr() for x in self.kv[layer]), s)
+
+    def run(self, layer=0, s=0):
+        self.b.run(layer, self.q.data_ptr(), *(x.data_ptr() for x in self.kv[layer]), self.out.data_ptr(), 0.1, s)
+
+    def attention(self, layer=0, s=0):
+        self.b.attention(layer, self.q.data_ptr(), self.out.data_ptr(), 0.1, s)
+
+    def commit(self):
+        torch.cuda.synchronize()
+        self.b.commit()
+        self.c.note(self.new)
+        self.c.check()
+
+
+def test_a_replayed_append_behind_another_one(tl):
+    """A prompt is captured, another batch appends less to the same sequence, the graph is replayed: the prompt
+    cannot be committed before its append is made again, then it reads back and goes on."""
+    c = QuantCache(tl, [95], 2, 64, seed=32, room=300)
+    a = Prompt(tl, c, 40)
+    a.run()  # (the workspace)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a.run(0, torch.cuda.current_stream().cuda_stream)
+    b = Prompt(tl, c, 1)
+    b.append()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        with pytest.raises(tl.TinyLLMError, match="up to 96 of the last append, which replaced"):
+            a.b.commit()
+    assert c.mgr.getSeqLen(c.ids[0]) == 95
+    a.run()
+    a.commit()
+    c.append([1], "step")
+    c.check()
+
+
+@pytest.mark.parametrize("less", [1, 10, 33, 70])
+def test_an_append_in_between(tl, less):
+    """Without a graph: what the second append replaced is neither committed nor attended to."""
+    c = QuantCache(tl, [95], 2, 64, seed=33, room=300)
+    a, b = Prompt(tl, c, 40), Prompt(tl, c, less)
+    a.append()
+    b.append()
+    if less > 33:  # longer: another group is open
+        with pytest.raises(tl.TinyLLMError, match="lies inside the tokens up to 165"):
+            a.b.commit()
+    else:
+        with pytest.raises(tl.TinyLLMError, match="which replaced one that brought more"):
+            a.b.commit()
+    with pytest.raises(tl.TinyLLMError, match="another append to sequence"):
+        a.attention()
+    r = tl.DecodeBatch(c.mgr, 1, 2)
+    r.prepare_lengths(c.ids, [95 + less])
+    a.append()
+    a.attention()
+    with pytest.raises(tl.TinyLLMError, match="has changed since prepare"):
+        r.attention(0, a.q.data_ptr(), a.out.data_ptr(), 0.1)
+    a.commit()
+    c.append([30])
+    c.check()
+
+
+def test_layers_that_differ(tl):
+    c = QuantCache(tl, [95], 2, 64, seed=34, layers=2, room=300)
+    a, b = Prompt(tl, c, 40), Prompt(tl, c, 10)
+    a.append(0)
+    b.append(0)
+    a.append(1)
+    with pytest.raises(tl.TinyLLMError, match="layers differ"):
+        a.b.commit()
+    r = tl.DecodeBatch(c.mgr, 1, 2)
+    r.prepare_lengths(c.ids, [135])
+    out = torch.zeros((1, 2, 64), dtype=torch.float16, device="cuda")
+    with pytest.raises(tl.TinyLLMError, match="up to 105, has replaced tokens up to 135 of layer 0"):
+        r.attention(0, a.q.data_ptr(), out.data_ptr(), 0.1)
+    r.attention(1, a.q.data_ptr(), out.data_ptr(), 0.1)
+    a.append(0)
+    a.commit()
+    # One layer's token alone: the other's open group would stay behind.
+    c.append([24], "appendKV")
+    x = dev(c.rows(2))
+    assert c.mgr.appendKV(c.ids[0], 0, x.data_ptr(), x.data_ptr(), 2) is None
+    assert "layers differ" in c.mgr.advanceSeqLen(c.ids[0], 2)
+    torch.cuda.synchronize()
+    c.check()

@@ -8,7 +8,7 @@ import pytest
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "tiny-llm_amd", "csrc")
-CHECKS = ["advance_beyond_what_was_appended"]
+CHECKS = ["advance_beyond_what_was_appended", "advance_over_another_append", "advance_where_layers_differ"]
 
 
 def test_open_groups_under_sanitizers(tmp_path):

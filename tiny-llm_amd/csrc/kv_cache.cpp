@@ -121,6 +121,7 @@ Result<std::unique_ptr<KVCacheManager>> KVCacheManager::build(const KVCacheConfi
         if (err != hipSuccess)
             return R::err(std::string("KVCacheManager: scales and open groups: ") + hipGetErrorString(err));
         manager->open_.resize(static_cast<size_t>(config.max_batch_size));
+        manager->appended_end_.resize(static_cast<size_t>(config.max_batch_size) * layers);
     }
     if (manager->blocks_) {
         // Every entry starts at the spare block.
@@ -191,7 +192,10 @@ Result<int> KVCacheManager::allocateSequence(int max_len) {
     slot.max_len = max_len;
     slot.active = true;
     evictions_[static_cast<size_t>(slot_idx)] = Eviction();
-    if (quantized_) open_[static_cast<size_t>(slot_idx)] = detail::OpenGroup();
+    if (quantized_) {
+        open_[static_cast<size_t>(slot_idx)] = detail::OpenGroup();
+        std::fill_n(appended_end_.begin() + static_cast<std::ptrdiff_t>(slot_idx) * config_.num_layers, config_.num_layers, 0);
+    }
     seq_to_slot_[seq_id] = slot_idx;
     return Result<int>::ok(seq_id);
 }
@@ -305,7 +309,7 @@ Result<void> KVCacheManager::appendKV(int seq_id, int layer_idx, const half *new
         const auto [first, last] = openGroup(slot_idx).tiles(write_pos, num_tokens);
         std::vector<detail::QuantAppend> one{{slot_idx, write_pos, num_tokens, 0, first | last << 1, 0}};
         detail::launch_quant_append(quantView(layer_idx), one, config_.num_heads, config_.head_dim, new_k, new_v, stream);
-        noteAppend(slot_idx, num_tokens);
+        noteAppend(slot_idx, layer_idx, 1, num_tokens);
     } else if (!isPaged()) {
         half        *k_cache = memory_pool_ + calculateOffset(slot_idx, layer_idx, false);
         half        *v_cache = memory_pool_ + calculateOffset(slot_idx, layer_idx, true);
@@ -352,22 +356,11 @@ Result<void> KVCacheManager::advanceSeqLen(int seq_id, int num_tokens) {
         }
     }
     if (quantized_) {
-        detail::OpenGroup &open = open_[static_cast<size_t>(it->second)];
-        if (!open.advance(old_len, new_len)) {
-            const std::string length = "advanceSeqLen: length " + std::to_string(new_len) + " of sequence " +
-                                       std::to_string(seq_id);
-            const std::string msg =
-                open.leaves_rows(new_len)
-                    ? length + " is beyond the tokens up to " + std::to_string(open.end) +
-                          " that were appended, and in an 8-bit cache the last of them wait in their group of " +
-                          std::to_string(detail::kGroup) + " for those that complete it"
-                    : length + " lies inside the tokens up to " + std::to_string(open.end) +
-                          " that were appended at once: an 8-bit cache can be cut there at a multiple of " +
-                          std::to_string(detail::kGroup) +
-                          ", in the group in which they begin or in the one in which they end";
+        if (const std::string msg = cannotAdvance(it->second, seq_id, new_len); !msg.empty()) {
             TL_LOG_ERROR("%s", msg.c_str());
             return Result<void>::err(msg);
         }
+        open_[static_cast<size_t>(it->second)].advance(old_len, new_len);
     }
     slot.current_len = new_len;
     TL_LOG_TRACE("advanceSeqLen: seq_id=%d, %d -> %d", seq_id, old_len, slot.current_len);

@@ -17,17 +17,19 @@ constexpr int kQuantBatch = 144; // entries per launch: they travel in the kerne
 constexpr int kQuantPrefillBatch = 112;
 
 // The open group of a slot: which of its two tiles is the current one, the groups whose rows
-// they hold (-1: none), and where the last append ended.
+// they hold (-1: none), where the last append ended, and where the one that went furthest did.
 struct OpenGroup {
     int group[2] = {-1, -1};
     int cur = 0;
     int end = 0;
+    int far = 0;
 
     // The tiles of an append of n tokens behind len: that of the group it begins in, and that of the
     // group it ends in (the other one where that is another group).
     std::pair<int, int> tiles(int len, int n) const { return {cur, len / kGroup == (len + n) / kGroup ? cur : 1 - cur}; }
     void                append(int len, int n) {
         end = len + n;
+        far = end > far ? end : far;
         group[cur] = len / kGroup;
         group[1 - cur] = end / kGroup != len / kGroup && end % kGroup != 0 ? end / kGroup : -1;
     }
@@ -36,11 +38,22 @@ struct OpenGroup {
     // Whether length `to` leaves the group that the last append ended in, whose rows wait in fp16 for those
     // that complete it: nothing would read them there any more.
     bool leaves_rows(int to) const { return end % kGroup != 0 && to / kGroup > end / kGroup; }
-    // From length len to length `to`; false (and no change) where that leaves rows behind, or lies
-    // inside what one append brought and the rows that would be open again are gone.
+    // Whether it is beyond the last append, where an earlier one had brought more: its rows there may
+    // have made room for the last one's.
+    bool replaced(int to) const { return to > end && far > end; }
+    // Whether the layers, whose last appends ended at ends[], can all go from length len to length `to`: the tiles are
+    // told apart by the last append to any of them, so what was appended behind len has to be alike in those that
+    // have some, and the others must not leave rows behind either.
+    bool alike(const int *ends, int layers, int len, int to) const {
+        for (int l = 0; l < layers; ++l)
+            if (ends[l] != end && (ends[l] > len || (ends[l] % kGroup != 0 && to / kGroup > ends[l] / kGroup))) return false;
+        return true;
+    }
+    // From length len to length `to`; false (and no change) where that leaves rows behind, or shows
+    // replaced ones, or lies inside what one append brought and the rows that would be open again are gone.
     bool advance(int len, int to) {
         const int g = to / kGroup;
-        if (leaves_rows(to)) return false;
+        if (leaves_rows(to) || replaced(to)) return false;
         if (g != len / kGroup && group[1 - cur] == g) {
             cur = 1 - cur;
         } else if (to % kGroup != 0 && to < end && (g != len / kGroup || group[cur] != g)) {

@@ -43,8 +43,33 @@ detail::QuantView KVCacheManager::quantView(int layer_idx) const {
 
 const detail::OpenGroup &KVCacheManager::openGroup(int slot) const noexcept { return open_[static_cast<size_t>(slot)]; }
 
-void KVCacheManager::noteAppend(int slot, int n) noexcept {
-    open_[static_cast<size_t>(slot)].append(slots_[static_cast<size_t>(slot)].current_len, n);
+int KVCacheManager::appendedEnd(int slot, int layer) const noexcept {
+    return appended_end_[static_cast<size_t>(slot) * static_cast<size_t>(config_.num_layers) + static_cast<size_t>(layer)];
+}
+
+void KVCacheManager::noteAppend(int slot, int layer_begin, int num_layers, int n) noexcept {
+    const int len = slots_[static_cast<size_t>(slot)].current_len;
+    open_[static_cast<size_t>(slot)].append(len, n);
+    std::fill_n(appended_end_.begin() + static_cast<std::ptrdiff_t>(slot) * config_.num_layers + layer_begin, num_layers, len + n);
+}
+
+std::string KVCacheManager::cannotAdvance(int slot, int seq_id, int to) const {
+    detail::OpenGroup open = open_[static_cast<size_t>(slot)];
+    const int         len = slots_[static_cast<size_t>(slot)].current_len, end = open.end;
+    const int        *ends = &appended_end_[static_cast<size_t>(slot) * static_cast<size_t>(config_.num_layers)];
+    const bool        alike = open.alike(ends, config_.num_layers, len, to);
+    if (alike && open.advance(len, to)) return std::string();
+    const std::string length = "advanceSeqLen: length " + std::to_string(to) + " of sequence " + std::to_string(seq_id);
+    const std::string beyond = length + " is beyond the tokens up to " + std::to_string(end);
+    if (!alike)
+        return length + ": its layers differ in what was appended last, and one of them would lose tokens of its open group";
+    if (open.replaced(to)) return beyond + " of the last append, which replaced one that brought more: append those again";
+    if (open.leaves_rows(to))
+        return beyond + " that were appended, and in an 8-bit cache the last of them wait in their group of " +
+               std::to_string(kGroup) + " for those that complete it";
+    return length + " lies inside the tokens up to " + std::to_string(end) +
+           " that were appended at once: an 8-bit cache can be cut there at a multiple of " + std::to_string(kGroup) +
+           ", in the group in which they begin or in the one in which they end";
 }
 
 namespace detail {
@@ -77,10 +102,6 @@ int QuantStep::items() const {
     return n;
 }
 
-void QuantStep::see(const KVCacheManager &mgr, int32_t id, int32_t slot, bool reads_only) {
-    seen_.push_back({id, slot, mgr.sequence(id)->current_len, reads_only ? held_tokens(mgr, id, slot) : -1});
-}
-
 std::string QuantStep::check(const char *who, const KVCacheManager &mgr, std::initializer_list<const void *> buffers) const {
     for (const Seen &s : seen_) {
         const SequenceCache *sc = mgr.sequence(s.id);
@@ -90,25 +111,33 @@ std::string QuantStep::check(const char *who, const KVCacheManager &mgr, std::in
     return check_quant_call(who, mgr, buffers);
 }
 
-void QuantStep::noteAppends(KVCacheManager &mgr) const {
-    for (const QuantAppend &a : appends) mgr.noteAppend(a.row, a.n);
+std::string QuantStep::checkRead(const char *who, const KVCacheManager &mgr, int layer_idx) const {
+    for (const Seen &s : seen_)
+        if (const int end = mgr.appendedEnd(s.slot, layer_idx); s.end >= 0 && end > s.len && end != s.end)
+            return std::string(who) + ": another append to sequence " + std::to_string(s.id) + ", up to " + std::to_string(end) +
+                   ", has replaced tokens up to " + std::to_string(s.end) + " of layer " + std::to_string(layer_idx);
+    return std::string();
+}
+
+void QuantStep::noteAppends(KVCacheManager &mgr, int layer_begin, int num_layers) const {
+    for (const QuantAppend &a : appends) mgr.noteAppend(a.row, layer_begin, num_layers, a.n);
 }
 
 void QuantStep::prepareDecode(const KVCacheManager &mgr, const std::vector<int32_t> &ids, const std::vector<int32_t> &slots,
                               const std::vector<int32_t> &lens, bool appendable, int num_q_heads) {
     const KVCacheConfig &cfg = mgr.getConfig();
     for (size_t i = 0; i < ids.size(); ++i) {
-        see(mgr, ids[i], slots[i], !appendable);
-        const int S = lens[i], tok = static_cast<int>(i);
+        const int S = lens[i], tok = static_cast<int>(i), len = mgr.sequence(ids[i])->current_len;
         if (appendable) {
             const int tile = mgr.openGroup(slots[i]).cur;
+            seen_.push_back({ids[i], slots[i], len, -1, -1});
             appends.push_back({slots[i], S - 1, 1, tok, tile | tile << 1, 0});
             entries.push_back({slots[i], S, tok, 1, tile, 0});
         } else {
             // A last group that is complete in the cache is read there; what a sequence has
             // advanced over stands as it did then, whatever was appended behind it.
-            const int len = mgr.sequence(ids[i])->current_len;
             auto [held, tile] = mgr.openGroup(slots[i]).held(len);
+            seen_.push_back({ids[i], slots[i], len, held, S > len ? held : -1});
             if (S <= len) {
                 held = len;
                 tile = mgr.openGroup(slots[i]).cur;
@@ -126,10 +155,10 @@ bool QuantStep::preparePrefill(const KVCacheManager &mgr, const std::vector<int3
     const int            group = num_q_heads / cfg.num_heads;
     int                  tok = 0;
     for (size_t i = 0; i < ids.size(); ++i) {
-        see(mgr, ids[i], slots[i], false);
         const int n = counts[i], p0 = mgr.sequence(ids[i])->current_len, S = p0 + n;
         const auto [first, last] = mgr.openGroup(slots[i]).tiles(p0, n);
         const int open = S % kGroup != 0 ? last : -1;
+        seen_.push_back({ids[i], slots[i], p0, -1, open >= 0 && last != first ? S : -1});
         appends.push_back({slots[i], p0, n, tok, first | last << 1, 0});
         entries.push_back({slots[i], S, tok, n, open, 0});
         if (static_cast<int64_t>(n) * group <= kQuantRows) stream.entries.push_back(entries.back());
@@ -152,7 +181,7 @@ Result<void> QuantStep::appendOne(KVCacheManager &mgr, int layer_begin, int num_
         steps = {w.tiles - v.tiles, w.scales - v.scales, w.open - v.open};
     }
     launch_quant_append_one(v, steps, appends, num_layers, cfg.num_heads, cfg.head_dim, new_k, new_v, stream);
-    noteAppends(mgr);
+    noteAppends(mgr, layer_begin, num_layers);
     return Result<void>::ok();
 }
 
@@ -161,13 +190,14 @@ Result<void> QuantStep::append(const char *who, KVCacheManager &mgr, int layer_i
     if (std::string err = check(who, mgr, {new_k, new_v}); !err.empty()) return Result<void>::err(err);
     const KVCacheConfig &cfg = mgr.getConfig();
     launch_quant_append(mgr.quantView(layer_idx), appends, cfg.num_heads, cfg.head_dim, new_k, new_v, stream);
-    noteAppends(mgr);
+    noteAppends(mgr, layer_idx, 1);
     return Result<void>::ok();
 }
 
 Result<void> QuantStep::attention(const char *who, KVCacheManager &mgr, int layer_idx, const half *q, const half *new_k,
                                   const half *new_v, half *out, float scale, int num_q_heads, bool apart, hipStream_t stream) {
     if (std::string err = check(who, mgr, {q, new_k, new_v, out}); !err.empty()) return Result<void>::err(err);
+    if (std::string err = new_k ? std::string() : checkRead(who, mgr, layer_idx); !err.empty()) return Result<void>::err(err);
     const KVCacheConfig &cfg = mgr.getConfig();
     const size_t floats = std::max(quant_workspace_floats(this->stream, cfg.num_heads, cfg.head_dim),
                                    quant_prefill_workspace_floats(prefill, cfg.num_heads, cfg.head_dim));
@@ -189,13 +219,14 @@ Result<void> QuantStep::attention(const char *who, KVCacheManager &mgr, int laye
     c.D = cfg.head_dim;
     if (!this->stream.entries.empty()) launch_attn_quant(c, v, this->stream, ws, stream);
     if (!prefill.entries.empty()) launch_quant_prefill(c, v, prefill, ws, stream);
-    if (new_k) noteAppends(mgr);
+    if (new_k) noteAppends(mgr, layer_idx, 1);
     return Result<void>::ok();
 }
 
 Result<void> QuantStep::gather(KVCacheManager &mgr, int layer_idx, half *k_out, half *v_out, int s_max,
                                hipStream_t stream) {
     if (std::string err = check("DecodeBatch", mgr, {k_out, v_out}); !err.empty()) return Result<void>::err(err);
+    if (std::string err = checkRead("DecodeBatch", mgr, layer_idx); !err.empty()) return Result<void>::err(err);
     const KVCacheConfig &cfg = mgr.getConfig();
     launch_quant_gather(mgr.quantView(layer_idx), entries, cfg.num_heads, cfg.head_dim, s_max, k_out, v_out, stream);
     return Result<void>::ok();

@@ -45,15 +45,16 @@ struct QuantStep {
     Result<void> gather(KVCacheManager &mgr, int layer_idx, half *k_out, half *v_out, int s_max, hipStream_t stream);
 
   private:
-    // The sequences as prepare found them: their lengths and, for a step that only reads,
-    // what they held.
+    // The sequences as prepare found them: their lengths, for a step that only reads what they
+    // held (else -1), and where the last append to a layer has to end (or nothing be behind len) for the
+    // entry's open tile to have its tokens (-1: it is the one that has those before len too).
     struct Seen {
-        int32_t id, slot, len, held;
+        int32_t id, slot, len, held, end;
     };
     std::vector<Seen> seen_;
-    void              see(const KVCacheManager &mgr, int32_t id, int32_t slot, bool reads_only);
     std::string       check(const char *who, const KVCacheManager &mgr, std::initializer_list<const void *> buffers) const;
-    void              noteAppends(KVCacheManager &mgr) const;
+    std::string       checkRead(const char *who, const KVCacheManager &mgr, int layer_idx) const;
+    void              noteAppends(KVCacheManager &mgr, int layer_begin, int num_layers) const;
 };
 
 } // namespace detail

@@ -113,8 +113,12 @@ class KVCacheManager {
     // decode / gather and PrefillBatch::append / attention / prefill write, read and
     // attend to what the cache stands for after the append; q, out, new_k and new_v are 16-byte
     // aligned.  Accounts, projections, eviction and CrossBatch are refused.
-    //   An append replaces what was appended at its position before and not advanced over.
-    // Between prepare and commit of a batch its sequences' lengths must not change (its calls
+    //   An append replaces what was appended at its position before and not advanced over, so
+    // a length beyond the last one is refused where an earlier one brought more, and so is a batch's
+    // commit after another one's append to its sequences that brought less, or to some layers only.
+    // A replayed graph appends again without the host's knowing: after another append to its
+    // sequences, make the calls of the batch again instead.
+    //   Between prepare and commit of a batch its sequences' lengths must not change (its calls
     // refuse).  A sequence may advance over less than was appended (drafted tokens that were
     // rejected), to a multiple of 32, within the group in which the append began or the one
     // in which it ended; elsewhere the rows that the open group needs are gone, and
@@ -156,15 +160,19 @@ class KVCacheManager {
     detail::KvView layerView(int layer_idx, const int32_t *seq_row_dev) const;
     // The same of a pool in 8 bits.
     detail::QuantView quantView(int layer_idx) const;
-    // The open group of a slot of such a pool, and that an append of n tokens to it was queued.
+    // The open group of a slot of such a pool, where the last append to one of its layers ended, and
+    // that an append of n tokens to some of them was queued.
     const detail::OpenGroup &openGroup(int slot) const noexcept;
-    void                     noteAppend(int slot, int n) noexcept;
+    int                      appendedEnd(int slot, int layer) const noexcept;
+    void                     noteAppend(int slot, int layer_begin, int num_layers, int n) noexcept;
 
   private:
     explicit KVCacheManager(const KVCacheConfig &config);
     static Result<std::unique_ptr<KVCacheManager>> build(const KVCacheConfig &config, int block_tokens,
                                                          int num_blocks, bool quantized);
     Result<void> exhausted(int64_t need) const;
+    // Why a slot of a pool in 8 bits cannot have length `to`, "" when it can.
+    std::string cannotAdvance(int slot, int seq_id, int to) const;
 
     size_t calculateOffset(int slot_idx, int layer_idx, bool is_value) const;
     int    findFreeSlot() const;
@@ -200,6 +208,7 @@ class KVCacheManager {
     float2 *scales_ = nullptr;     // [layer][block][kv head][group] (K, V)
     half   *open_tiles_ = nullptr; // [layer][slot][2][kv head][64 D]
     std::vector<detail::OpenGroup> open_;
+    std::vector<int> appended_end_; // [slot][layer]
 };
 
 // A decode step over n sequences of one manager.  prepare() snapshots the
