@@ -246,7 +246,8 @@ int tl_kv_batch_project(tl_kv_batch *batch, int layer, const void *x, int hidden
                         const int8_t *wq, const void *sq, void *q_out, int packed, void *stream);
 /* The commit of InferenceEngine::decodeStep (src/inference_engine.cpp:291):
  * advanceSeqLen(seq_id, num_tokens) for every sequence of the last prepare,
- * in batch order; stops at (and reports) the first failing sequence. */
+ * in batch order; stops at (and reports) the first failing sequence (a pool in
+ * 8 bits: before any of them has advanced, also in tl_kv_prefill_commit). */
 int tl_kv_batch_commit(tl_kv_batch *batch, int num_tokens);
 
 /* ------------------------------------------------------------------------

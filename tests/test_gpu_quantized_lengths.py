@@ -143,3 +143,58 @@ def test_layers_that_differ(tl):
     assert "layers differ" in c.mgr.advanceSeqLen(c.ids[0], 2)
     torch.cuda.synchronize()
     c.check()
+
+
+def test_a_commit_advances_all_or_none(tl):
+    """The second of three sequences refuses: none has advanced, and after its append is made again all do, once."""
+    c = QuantCache(tl, [95, 95, 40], 2, 64, seed=35, room=300)
+    counts = [40, 40, 3]
+    new = c.new_rows(counts)
+    k, v = (dev(np.concatenate(x)) for x in new[0])
+    p = tl.PrefillBatch(c.mgr, 3, 2)
+    p.prepare(c.ids, counts)
+    p.append(0, k.data_ptr(), v.data_ptr())
+    one = tl.PrefillBatch(c.mgr, 1, 2)
+    one.prepare([c.ids[1]], [10])
+    one.append(0, k.data_ptr(), v.data_ptr())
+    with pytest.raises(tl.TinyLLMError, match=f"sequence {c.ids[1]}"):
+        p.commit()
+    assert [c.mgr.getSeqLen(s) for s in c.ids] == [95, 95, 40]
+    p.append(0, k.data_ptr(), v.data_ptr())
+    torch.cuda.synchronize()
+    p.commit()
+    c.note(new)
+    c.check()
+    # steps: 135 and one drafted token more than fits the group of the third
+    b = tl.DecodeBatch(c.mgr, 3, 2)
+    b.prepare(c.ids)
+    b.append(0, 1, k.data_ptr(), v.data_ptr())
+    with pytest.raises(tl.TinyLLMError, match=f"sequence {c.ids[2]}"):
+        b.commit(22)
+    assert [c.mgr.getSeqLen(s) for s in c.ids] == [135, 135, 43]
+    torch.cuda.synchronize()
+    c.check()
+
+
+def test_a_commit_behind_a_release_or_without_blocks(tl):
+    m = tl.KVCacheManager(num_layers=1, num_heads=1, head_dim=64, max_seq_len=256, max_batch_size=3, block_tokens=32, num_blocks=6,
+                          quantized=True)
+    ids = [m.allocateSequence(256)[0] for _ in range(3)]
+    b, p = tl.DecodeBatch(m, 3, 1), tl.PrefillBatch(m, 2, 1)
+    b.prepare(ids)
+    with pytest.raises(tl.TinyLLMError, match="exhausted"):
+        b.commit(96)  # nine blocks
+    assert [m.getSeqLen(s) for s in ids] == [0, 0, 0] and m.freeBlocks() == 3
+    b.commit(64)
+    assert [m.getSeqLen(s) for s in ids] == [64, 64, 64] and m.freeBlocks() == 0
+    assert m.releaseSequence(ids[1]) is None
+    p.prepare([ids[0], ids[2]], [1, 1])
+    with pytest.raises(tl.TinyLLMError, match=f"not found: {ids[1]}"):
+        b.commit(1)
+    assert m.getSeqLen(ids[0]) == 64
+    assert m.releaseSequence(ids[2]) is None
+    with pytest.raises(tl.TinyLLMError, match=f"not found: {ids[2]}"):
+        p.commit()
+    assert m.getSeqLen(ids[0]) == 64
+    with pytest.raises(tl.TinyLLMError, match="positive"):
+        b.commit(0)

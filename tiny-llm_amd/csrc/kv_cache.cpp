@@ -368,6 +368,32 @@ Result<void> KVCacheManager::advanceSeqLen(int seq_id, int num_tokens) {
     return Result<void>::ok();
 }
 
+Result<void> KVCacheManager::advanceAll(const std::vector<int32_t> &ids, const std::vector<int32_t> &num_tokens) {
+    if (quantized_) { // every reason to refuse is looked for before a length changes
+        std::vector<int32_t> rows, lens;
+        for (size_t i = 0; i < ids.size(); ++i) {
+            const int row = slotOf(ids[i]);
+            if (row < 0 || num_tokens[i] <= 0) return advanceSeqLen(ids[i], num_tokens[i]); // refuses
+            const auto &slot = slots_[static_cast<size_t>(row)];
+            rows.push_back(row);
+            lens.push_back(static_cast<int>(std::min<int64_t>(static_cast<int64_t>(slot.current_len) + num_tokens[i], slot.max_len)));
+            if (const std::string msg = cannotAdvance(row, ids[i], lens.back()); !msg.empty()) {
+                TL_LOG_ERROR("%s", msg.c_str());
+                return Result<void>::err(msg);
+            }
+        }
+        if (auto r = reserveSlots(rows.data(), lens.data(), static_cast<int>(rows.size())); r.isErr()) {
+            TL_LOG_ERROR("advanceSeqLen: %s", r.error().c_str());
+            return r;
+        }
+    }
+    for (size_t i = 0; i < ids.size(); ++i) {
+        auto r = advanceSeqLen(ids[i], num_tokens[i]);
+        if (r.isErr()) return r;
+    }
+    return Result<void>::ok();
+}
+
 // getSeqLen / hasSequence / memory statistics (kv_cache.cpp:261-295).
 int KVCacheManager::getSeqLen(int seq_id) const noexcept {
     auto it = seq_to_slot_.find(seq_id);
@@ -702,11 +728,7 @@ Result<void> DecodeBatch::commit(int num_tokens) {
     for (size_t i = 0; i < ids_.size(); ++i)
         if (mgr_.evictionBegun(slot_[i]) && mgr_.slotOf(ids_[i]) == slot_[i])
             return Result<void>::err("DecodeBatch: " + detail::eviction_begun(ids_[i]));
-    for (const int id : ids_) {
-        auto r = mgr_.advanceSeqLen(id, num_tokens);
-        if (r.isErr()) return r;
-    }
-    return Result<void>::ok();
+    return mgr_.advanceAll(ids_, std::vector<int32_t>(ids_.size(), num_tokens));
 }
 
 Result<void> DecodeBatch::prepareLengths(const int *seq_ids, const int *attended, int n,
@@ -1099,11 +1121,7 @@ Result<void> PrefillBatch::commit() {
     for (size_t i = 0; i < ids_.size(); ++i)
         if (mgr_.evictionBegun(slots_[i]) && mgr_.slotOf(ids_[i]) == slots_[i])
             return Result<void>::err("PrefillBatch: " + detail::eviction_begun(ids_[i]));
-    for (size_t i = 0; i < ids_.size(); ++i) {
-        auto r = mgr_.advanceSeqLen(ids_[i], counts_[i]);
-        if (r.isErr()) return r;
-    }
-    return Result<void>::ok();
+    return mgr_.advanceAll(ids_, counts_);
 }
 
 } // namespace tiny_llm

@@ -139,6 +139,9 @@ class KVCacheManager {
     // Maps blocks so that every listed slot holds tokens[i] tokens: all or
     // nothing.
     Result<void> reserveSlots(const int32_t *slots, const int32_t *tokens, int n);
+    // advanceSeqLen of every sequence (each named once) by its num_tokens, in order; a pool in 8 bits
+    // advances all of them or none, others those before the first one that is refused.
+    Result<void> advanceAll(const std::vector<int32_t> &ids, const std::vector<int32_t> &num_tokens);
     // Tokens of the sequence that evictions took from the cache (EvictBatch): the
     // next token's position is getSeqLen + getEvicted.  0 for an unknown sequence.
     int getEvicted(int seq_id) const noexcept;
@@ -255,7 +258,7 @@ class DecodeBatch {
     Result<void> project(int layer_idx, const half *x, int hidden, int group_size, const int8_t *wk,
                          const half *sk, const int8_t *wv, const half *sv, const int8_t *wq,
                          const half *sq, half *q_out, hipStream_t stream, bool packed = false);
-    // advanceSeqLen(seq, num_tokens) for every sequence of the last prepare.
+    // advanceSeqLen(seq, num_tokens) for every sequence of the last prepare (a pool in 8 bits: or for none).
     Result<void> commit(int num_tokens);
 
     int size() const noexcept { return n_; }
@@ -343,7 +346,7 @@ class PrefillBatch {
     // prefill); attention's outputs are not computed.
     Result<void> weights(int layer_idx, const half *q, float scale, int window, const float *weights_in,
                          float *weights_out, hipStream_t stream);
-    // advanceSeqLen(seq, num_tokens[i]) for every sequence of the last prepare.
+    // advanceSeqLen(seq, num_tokens[i]) for every sequence of the last prepare (a pool in 8 bits: or for none).
     Result<void> commit();
 
     int size() const noexcept { return n_; }
