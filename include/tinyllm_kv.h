@@ -132,7 +132,8 @@ int tl_kv_create_paged(const tl_kv_config *cfg, int block_tokens, int num_blocks
  * append.  tl_kv_batch_prepare_lengths: at most the tokens held (appended ones
  * included).  tl_kv_batch_project, accounts, tl_kv_evict_* and tl_kv_cross_* refuse it.
  *   An append replaces what was appended behind the length before.  A batch's calls
- * refuse when the length of one of its sequences changed since its prepare.  tl_kv_advance over
+ * refuse when the length of one of its sequences changed since its prepare, or, where it
+ * attends to appended tokens behind that length, when another append to them had another size.  tl_kv_advance over
  * less than was appended (drafted tokens that were rejected) may end at a multiple of
  * 32, in the group in which the append began or in the one in which it ended; elsewhere it
  * is refused, the rows of that group being gone.  Beyond what was appended it may end

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from quant_ref import QuantCache
+from quant_ref import QuantCache, attend, check_out
 from retention_ref import dev
 
 pytestmark = pytest.mark.gpu
@@ -198,3 +198,41 @@ def test_a_commit_behind_a_release_or_without_blocks(tl):
     assert m.getSeqLen(ids[0]) == 64
     with pytest.raises(tl.TinyLLMError, match="positive"):
         b.commit(0)
+
+
+@pytest.mark.parametrize("lens", [[40, 95, 64], [20, 96, 127]])
+def test_tokens_that_stand_are_read_behind_appends(tl, lens):
+    """A batch that attends to tokens that its sequences have advanced over goes on doing so, whatever is
+    appended behind them; one that attends to appended tokens is refused once those are others."""
+    c = QuantCache(tl, lens, 2, 64, seed=36, hq=8, room=300)
+    att = [n - k for n, k in zip(lens, (0, 3, 64))]
+    q = c.rng.standard_normal((3, 8, 64)).astype(np.float16)
+    dq, out = dev(q), torch.zeros((3, 8, 64), dtype=torch.float16, device="cuda")
+    back = torch.zeros((3, 2, 128, 64), dtype=torch.float16, device="cuda")
+    b, drafts = tl.DecodeBatch(c.mgr, 3, 8), tl.DecodeBatch(c.mgr, 3, 8)
+    b.prepare_lengths(c.ids, att)
+    for counts in ([1, 1, 1], [30, 33, 5], [70, 40, 100]):
+        k, v = dev(c.rows(sum(counts))), dev(c.rows(sum(counts)))
+        p = tl.PrefillBatch(c.mgr, 3, 8)
+        p.prepare(c.ids, counts)
+        p.append(0, k.data_ptr(), v.data_ptr())
+        if counts[0] > 1:
+            with pytest.raises(tl.TinyLLMError, match="has changed since prepare"):
+                drafts.attention(0, dq.data_ptr(), out.data_ptr(), 0.125)
+        drafts.prepare_lengths(c.ids, [n + m for n, m in zip(lens, counts)])
+        out.zero_()
+        b.attention(0, dq.data_ptr(), out.data_ptr(), 0.125)
+        b.gather(0, back.data_ptr(), None, 128)
+        torch.cuda.synchronize()
+        got = out.cpu().numpy()
+        for i, a in enumerate(att):
+            if a == 0:
+                assert not got[i].any() and not back[i].any()
+                continue
+            kk, vv = (x[:a] for x in c.expect(0, i))
+            assert np.array_equal(back[i, :, :a].cpu().numpy(), kk.astype(np.float16).transpose(1, 0, 2))
+            o, mass, err = attend(q[i:i + 1], kk, vv, 0.125, [a - 1])
+            check_out(got[i:i + 1], o, mass, err, a, np.abs(vv).max())
+    assert c.mgr.advanceSeqLen(c.ids[1], 1) is None
+    with pytest.raises(tl.TinyLLMError, match="has changed since prepare"):
+        b.attention(0, dq.data_ptr(), out.data_ptr(), 0.125)

@@ -137,7 +137,7 @@ void QuantStep::prepareDecode(const KVCacheManager &mgr, const std::vector<int32
             // A last group that is complete in the cache is read there; what a sequence has
             // advanced over stands as it did then, whatever was appended behind it.
             auto [held, tile] = mgr.openGroup(slots[i]).held(len);
-            seen_.push_back({ids[i], slots[i], len, held, S > len ? held : -1});
+            seen_.push_back({ids[i], slots[i], len, S > len ? held : -1, S > len ? held : -1});
             if (S <= len) {
                 held = len;
                 tile = mgr.openGroup(slots[i]).cur;

@@ -45,9 +45,10 @@ struct QuantStep {
     Result<void> gather(KVCacheManager &mgr, int layer_idx, half *k_out, half *v_out, int s_max, hipStream_t stream);
 
   private:
-    // The sequences as prepare found them: their lengths, for a step that only reads what they
-    // held (else -1), and where the last append to a layer has to end (or nothing be behind len) for the
-    // entry's open tile to have its tokens (-1: it is the one that has those before len too).
+    // The sequences as prepare found them: their lengths; where a step reads appended tokens that they
+    // have not advanced over, what they held (else -1); and where the last append to a layer has to end (or
+    // nothing be behind len) for the entry's open tile to have its tokens (-1: it is the one that
+    // has those before len too).
     struct Seen {
         int32_t id, slot, len, held, end;
     };
