@@ -236,3 +236,18 @@ def test_tokens_that_stand_are_read_behind_appends(tl, lens):
     assert c.mgr.advanceSeqLen(c.ids[1], 1) is None
     with pytest.raises(tl.TinyLLMError, match="has changed since prepare"):
         b.attention(0, dq.data_ptr(), out.data_ptr(), 0.125)
+
+
+@pytest.mark.parametrize("pool", [dict(), dict(block_tokens=32, num_blocks=8), dict(block_tokens=32, num_blocks=8, quantized=True)])
+def test_counts_at_the_end_of_an_int(tl, pool):
+    """A length and a count whose sum is beyond 2^31 - 1 are an overflow of the cache."""
+    m = tl.KVCacheManager(num_layers=1, num_heads=1, head_dim=64, max_seq_len=128, max_batch_size=2, **pool)
+    s = m.allocateSequence(128)[0]
+    x = torch.zeros((128, 64), dtype=torch.float16, device="cuda")
+    assert m.appendKV(s, 0, x.data_ptr(), x.data_ptr(), 100) is None and m.advanceSeqLen(s, 100) is None
+    for n in (2 ** 31 - 1, 2 ** 31 - 100, 2 ** 31 - 101, 29):
+        assert f"cache overflow. Current: 100, appending: {n}, max: 128" in m.appendKV(s, 0, x.data_ptr(), x.data_ptr(), n)
+        with pytest.raises(tl.TinyLLMError, match="cache overflow"):
+            tl.PrefillBatch(m, 1, 1).prepare([s], [n])
+    assert m.appendKV(s, 0, x.data_ptr(), x.data_ptr(), 28) is None
+    torch.cuda.synchronize()

@@ -282,7 +282,7 @@ Result<void> KVCacheManager::appendKV(int seq_id, int layer_idx, const half *new
     // All layers of a step see the same write position: the length is
     // advanced once after the last layer (kv_cache.cpp:204-208).
     const int write_pos = slot.current_len;
-    if (write_pos + num_tokens > slot.max_len) {
+    if (static_cast<int64_t>(write_pos) + num_tokens > slot.max_len) {
         TL_LOG_ERROR("appendKV: cache overflow. seq_id=%d, write_pos=%d, num_tokens=%d, max_len=%d",
                    seq_id, write_pos, num_tokens, slot.max_len);
         return Result<void>::err("appendKV: cache overflow. Current: " + std::to_string(write_pos) +
