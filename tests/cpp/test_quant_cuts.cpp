@@ -1,5 +1,6 @@
-// How plan_quant_prefill cuts the keys of its entries, on the host under sanitizers: by one length for all
-// of them, into no more chunks than there are tiles, within the slots where the row tiles are, and only where that is so.
+// How plan_quant and plan_quant_prefill cut the work, on the host under sanitizers.  Prompts have their keys cut
+// by one length for all of them, into no more chunks than there are tiles, within the slots where the row tiles
+// are, and only where that is so; steps as was measured faster.
 #include "quant_plan.h"
 
 #include <algorithm>
@@ -20,7 +21,7 @@ using namespace tiny_llm::detail;
 static std::mt19937_64 rng(10);
 static int             upto(int n) { return (int)(rng() % (uint64_t)(n + 1)); }
 
-int main() {
+static void prefill_cuts() {
     int cut = 0, whole = 0, some = 0, fits = 0, rounds = 0;
     for (int it = 0; it < 6000; ++it) {
         const int D = 32 << upto(3), Hkv = 1 << upto(5), G = 1 << upto(3), cus = it % 2 ? 256 : 1 + upto(300);
@@ -75,5 +76,31 @@ int main() {
     }
     CHECK(cut > 1000 && whole > 1000 && some > 300 && fits > 1000 && rounds > 1000);
     std::puts("ok prefill_cuts");
+}
+
+// Decode entries of one length on 256 CUs: whole, or in so many chunks, as was measured faster.
+static void decode_sides() {
+    const struct { int D, Hkv, n, S, items; } sides[] = {
+        {32, 8, 1, 1000, 1},   {64, 8, 1, 1000, 1},   {128, 8, 1, 1000, 1},  {256, 8, 1, 1000, 4},
+        {32, 8, 1, 4000, 8},   {64, 8, 1, 4000, 8},   {128, 8, 1, 4000, 8},  {256, 8, 1, 4000, 16},
+        {32, 8, 16, 1000, 1},  {64, 8, 16, 1000, 1},  {128, 8, 16, 1000, 1}, {256, 8, 16, 1000, 1},
+        {32, 8, 16, 2000, 1},  {64, 8, 16, 2000, 1},  {128, 8, 16, 2000, 1}, {128, 8, 16, 4000, 1},
+        {32, 8, 16, 8000, 2},  {64, 8, 16, 8000, 2},  {128, 8, 16, 8000, 2}, {256, 8, 16, 8000, 2},
+        {32, 8, 28, 6000, 1},  {64, 8, 28, 6000, 1},  {128, 8, 28, 6000, 1}, {256, 8, 24, 6000, 1},
+        {32, 2, 70, 3000, 1},  {128, 2, 70, 3000, 1}, {256, 2, 70, 3000, 1}, {256, 1, 100, 8000, 2},
+    };
+    for (const auto &x : sides) {
+        QuantPlan p;
+        for (int i = 0; i < x.n; ++i) p.entries.push_back({i, x.S + 1, i, 1, 0, 0});
+        plan_quant(p, 4, x.Hkv, x.D, 256);
+        if (quant_items(x.S + 1, p.chunk) != x.items) std::fprintf(stderr, "head_dim %d, %d x %d of %d heads\n", x.D, x.n, x.S, x.Hkv);
+        CHECK(quant_items(x.S + 1, p.chunk) == x.items);
+    }
+    std::puts("ok decode_sides");
+}
+
+int main() {
+    prefill_cuts();
+    decode_sides();
     return 0;
 }

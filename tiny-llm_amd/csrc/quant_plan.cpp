@@ -13,17 +13,30 @@ void plan_quant(QuantPlan &plan, int G, int Hkv, int D, int cus) {
         longest = std::max<int64_t>(longest, quant_tiles(e.S));
     }
     // A workgroup that has a whole entry finishes it; entries in chunks need a second launch, about 3 us
-    // more.  In hundredths of a us (head_dim 128): a tile takes a CU 28, whether one workgroup or two are on it,
-    // and the chip 60 of a CU's share, more where CUs have nothing.  Chunks are the shortest ones that give every CU
-    // one workgroup at most, or two: a few workgroups beyond that would leave their CUs alone with twice the
-    // work.  Beyond two the chip's share is all that counts.
-    // Measured, 8 heads, groups of 4, head_dim 128, whole and cut: 1 x 1000 tokens 10.4, 13.7 us, 1 x 2000 16.0, 12.9,
-    // 1 x 16000 80, 14.6; 16 x 4000 30.1, 33.5, 16 x 16000 98, 91; 64 x 8192 167, 177.  Chunks of a CU's share,
-    // however many, and these: 10 x 100 .. 30000 76, 64; head_dim 64 4 x 28000 .. 32000 34.4, 26.6; 256 16 x 500 ..
-    // 20000 133, 112.
+    // more.  In hundredths of a us: a tile takes a CU `alone`, whether one workgroup or two are on it (what 1 x 4000
+    // takes whole more than 1 x 2000), and the chip 60 of a CU's share at head_dim 128, a quarter more where half of
+    // the CUs have none, a sixth more where some have one workgroup and others two.  Chunks are the shortest ones that
+    // give every CU one workgroup at most, or two: a few workgroups beyond that would leave their CUs alone with twice
+    // the work.  Beyond two the chip's share is all that counts.
+    // Measured, 8 heads, groups of 4, caches beyond the last level's size, us whole and in the shortest chunks of at
+    // most one a CU, of at most two, * what is taken (more of them: profiles/quantized_plan_sides.txt):
+    //   head_dim          32                  64                  128                 256
+    //   1 x 1000          7.4*  9.3  9.5      9.0* 10.7 10.9      12.5* 13.3 13.7     21.0  16.8* 17.1
+    //   1 x 4000          15.1  9.9* 10.0     18.7 11.2* 11.2     27.0  13.8* 14.0    49.7  17.6* 17.7
+    //   16 x 1000         8.1* 10.4 10.6      10.0* 12.4 12.5     14.9* 17.6 18.0     23.5* 26.0  32.7
+    //   16 x 2000         10.7* 12.2 12.2     13.4* 14.7 14.9     20.9* 23.4 25.9     31.6  32.8* 38.0
+    //   16 x 4000         15.7 14.6* 15.8     19.5 20.3* 21.5     32.3* 34.5 39.2     54.2  55.9* 60.9
+    //   16 x 8000         25.9 19.6* 20.3     32.6 29.3* 29.8     52.7 49.6* 54.7     95.9  87.6* 91.3
+    //   16 x 16000        45.4 30.4* 29.9     57.9 48.9* 48.3     97.4 95.0* 92.8     180   165*  167
+    //   28 x 6000         21.4* -    24.3     33.7* -   35.4      62.1* -    65.8     117*  -     117
+    //   40 x 600 .. 8000  26.0* -    24.6     41.7 -    38.2*     66.6 -     64.0*    134   -     131*
+    //   60 x 600 .. 8000  32.7* -    35.1     53.9* -   55.3      92.6 -     95.2*    172   -     165*
+    // With 28 for head_dim 32 and 64 and 112 for 256, 16 x 2000 took the chunks at 32 and 64, 16 x 1000 at 256, and
+    // 70 x 3000 of 2 heads of 256 two a CU, 52.6 for 43.3.  Chunks of a CU's share, however many, and these: 10 x 100 ..
+    // 30000 76, 64; head_dim 64 4 x 28000 .. 32000 34.4, 26.6; 256 16 x 500 .. 20000 133, 112.
     const int64_t n = std::max(1, cus), work = some * Hkv, waves = quant_waves(D);
     const int64_t share = (total * Hkv + n - 1) / n;
-    const int64_t alone = D <= 128 ? 28 : 112, stream = std::max<int64_t>(1, 60 * D / 128);
+    const int64_t alone = D == 32 ? 16 : D == 64 ? 20 : D == 128 ? 28 : 72, stream = std::max<int64_t>(1, 60 * D / 128);
     int64_t       chunk = longest;
     int64_t       least = work <= n ? std::max(alone * longest, stream * total * Hkv / n * (4 * n - work) / (3 * n))
                                     : longest * std::max(alone, stream * 7 / 6);
