@@ -138,7 +138,8 @@ int tl_kv_create_paged(const tl_kv_config *cfg, int block_tokens, int num_blocks
  * 32, in the group in which the append began or in the one in which it ended; elsewhere it
  * is refused, the rows of that group being gone.  Beyond what was appended it may end
  * in the group of the last appended token, or anywhere where that one completed its group; elsewhere
- * it is refused, as the open group's tokens would be lost; and so is a length beyond the last append
+ * it is refused, as the open group's tokens would be lost (tokens that nobody appended
+ * count as zeros in a group that an append completes); and so is a length beyond the last append
  * where an earlier one brought more (a commit after another batch's shorter append to the same
  * sequences), or where layers differ in what was appended last.  A replayed graph appends again without the
  * host's knowing: after another append to its sequences make its batch's calls again.

@@ -251,3 +251,47 @@ def test_counts_at_the_end_of_an_int(tl, pool):
             tl.PrefillBatch(m, 1, 1).prepare([s], [n])
     assert m.appendKV(s, 0, x.data_ptr(), x.data_ptr(), 28) is None
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+@pytest.mark.parametrize("how", ["appendKV", "prefill", "run", "append", "decode"])
+def test_tokens_that_nobody_brought_count_as_zeros(tl, d, how):
+    """A sequence advances over tokens that were not appended, and its group of 32 is completed: what an
+    earlier sequence left in the open group, infinite and large, has no part in the scale of those that were."""
+    big = QuantCache(tl, [31, 60], 2, d, seed=37, hq=2, layers=2, spare=0, room=100)
+    for i in range(2):
+        for layer in range(2):
+            x = torch.full((100, 2, d), float("inf") if i else 60000.0, dtype=torch.float16, device="cuda")
+            big.mgr.appendKV(big.ids[i], layer, x.data_ptr(), x.data_ptr(), 35)
+    torch.cuda.synchronize()
+    for s in big.ids:
+        assert big.mgr.releaseSequence(s) is None
+    c = big
+    c.ids = [c.mgr.allocateSequence(100)[0] for _ in range(2)]
+    c.k, c.v = ([[np.zeros((0, 2, d), np.float16) for _ in range(2)] for _ in range(2)] for _ in range(2))
+    c.append([20, 0])
+    assert c.mgr.advanceSeqLen(c.ids[0], 8) is None and c.mgr.advanceSeqLen(c.ids[1], 60) is None
+    zeros = [tuple([np.zeros((n, 2, d), np.float16) for n in (8, 60)] for _ in range(2)) for _ in range(2)]
+    c.note(zeros)
+    one, steps = how in ("append", "decode"), 4
+    for k in range(steps if one else 1):
+        counts = [1, 1] if one else [9, 4]
+        new = c.new_rows(counts)
+        if how in ("appendKV", "prefill", "append"):
+            c.append(counts, {"append": "step"}.get(how, how), new)
+            continue
+        b = tl.DecodeBatch(c.mgr, 2, 2) if one else tl.PrefillBatch(c.mgr, 2, 2)
+        b.prepare(c.ids) if one else b.prepare(c.ids, counts)
+        for layer in range(2):
+            kk, vv = (dev(np.concatenate(x)) for x in new[layer])
+            q, out = torch.zeros((sum(counts), 2, d), dtype=torch.float16, device="cuda"), torch.zeros_like(kk)
+            (b.decode if one else b.run)(layer, q.data_ptr(), kk.data_ptr(), vv.data_ptr(), out.data_ptr(), 1.0)
+            torch.cuda.synchronize()
+        b.commit(1) if one else b.commit()
+        c.note(new)
+    for layer in range(2):
+        got = c.read(layer)
+        for w in range(2):
+            for i, first in ((0, 0), (1, 32)):  # (the second's first group was never written at all)
+                want = c.expect(layer, i)[w].astype(np.float16).transpose(1, 0, 2)
+                assert np.array_equal(got[w][i][:, first:want.shape[1]], want[:, first:])

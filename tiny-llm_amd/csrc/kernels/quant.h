@@ -46,6 +46,12 @@ struct QuantAppend {
     int     groups() const { return (p0 + n + kGroup - 1) / kGroup - p0 / kGroup; }
 };
 
+// Zeros for the rows lo .. hi - 1 of an open tile that nobody brought, so that they have no part in the scale of
+// the group's others.
+struct QuantRows {
+    int32_t row, tile, lo, hi;
+};
+void launch_quant_zero_rows(const QuantView &v, const std::vector<QuantRows> &entries, int Hkv, int D, hipStream_t stream);
 // Appends new_k / new_v [tokens][Hkv][D]; sets the entries' item0.
 void launch_quant_append(const QuantView &v, std::vector<QuantAppend> &entries, int Hkv, int D, const __half *new_k,
                          const __half *new_v, hipStream_t stream);

@@ -114,6 +114,23 @@ template <int D> __global__ __launch_bounds__(64) void quant_append_one_kernel(A
     if (closes) group.close(a.v.tiles + layer * a.steps.tiles + at * (64 * D), a.v.scales + layer * a.steps.scales + at);
 }
 
+struct ZeroArgs {
+    QuantView v;
+    int       Hkv;
+    QuantRows e[kQuantBatch];
+};
+static_assert(sizeof(ZeroArgs) <= 4096, "kernel arguments");
+
+// A wave per (entry, kv head).
+template <int D> __global__ __launch_bounds__(64) void quant_zero_rows_kernel(ZeroArgs a) {
+    const int i = blockIdx.x / a.Hkv, g = blockIdx.x - i * a.Hkv;
+    uint16_t *tile = open_of<D>(a.v, a.Hkv, a.e[i].row, a.e[i].tile, g);
+    for (int r = a.e[i].lo; r < a.e[i].hi; ++r) {
+        if (threadIdx.x < D / 8) reinterpret_cast<u32x4 *>(tile)[k_piece(r, (int)threadIdx.x)] = u32x4{0u, 0u, 0u, 0u};
+        for (int d = threadIdx.x; d < D; d += 64) tile[32 * D + v_half(r, d)] = 0;
+    }
+}
+
 struct GatherArgs {
     QuantView  v;
     uint16_t  *k_out, *v_out;
@@ -182,6 +199,21 @@ template <int D> __global__ __launch_bounds__(kThreads) void quant_gather_kernel
 }
 
 } // namespace
+
+void launch_quant_zero_rows(const QuantView &v, const std::vector<QuantRows> &entries, int Hkv, int D, hipStream_t stream) {
+    ZeroArgs a{};
+    a.v = v;
+    a.Hkv = Hkv;
+    for (size_t i = 0; i < entries.size();) {
+        const size_t n = std::min<size_t>(kQuantBatch, entries.size() - i);
+        std::memcpy(a.e, entries.data() + i, sizeof(QuantRows) * n);
+        i += n;
+        for_head_dim(D, [&](auto d) {
+            hipLaunchKernelGGL(quant_zero_rows_kernel<decltype(d)::value>, dim3((unsigned)(n * (size_t)Hkv)), dim3(64), 0, stream, a);
+        });
+        HIP_CHECK(hipGetLastError());
+    }
+}
 
 void launch_quant_append(const QuantView &v, std::vector<QuantAppend> &entries, int Hkv, int D, const __half *new_k,
                          const __half *new_v, hipStream_t stream) {

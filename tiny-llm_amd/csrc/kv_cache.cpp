@@ -308,6 +308,7 @@ Result<void> KVCacheManager::appendKV(int seq_id, int layer_idx, const half *new
     if (quantized_) {
         const auto [first, last] = openGroup(slot_idx).tiles(write_pos, num_tokens);
         std::vector<detail::QuantAppend> one{{slot_idx, write_pos, num_tokens, 0, first | last << 1, 0}};
+        detail::zero_unbrought(*this, one, layer_idx, 1, stream);
         detail::launch_quant_append(quantView(layer_idx), one, config_.num_heads, config_.head_dim, new_k, new_v, stream);
         noteAppend(slot_idx, layer_idx, 1, num_tokens);
     } else if (!isPaged()) {

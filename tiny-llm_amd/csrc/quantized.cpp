@@ -87,6 +87,19 @@ int held_tokens(const KVCacheManager &mgr, int seq_id, int slot) {
     return mgr.openGroup(slot).held(mgr.sequence(seq_id)->current_len).first;
 }
 
+void zero_unbrought(const KVCacheManager &mgr, const std::vector<QuantAppend> &appends, int layer_begin, int num_layers,
+                    hipStream_t stream) {
+    const KVCacheConfig &cfg = mgr.getConfig();
+    for (int layer = layer_begin; layer < layer_begin + num_layers; ++layer) {
+        std::vector<QuantRows> rows;
+        for (const QuantAppend &a : appends) {
+            const int group = a.p0 / kGroup * kGroup, lo = std::max(mgr.appendedEnd(a.row, layer), group);
+            if (lo < a.p0) rows.push_back({a.row, a.first_last & 1, lo - group, a.p0 - group});
+        }
+        if (!rows.empty()) launch_quant_zero_rows(mgr.quantView(layer), rows, cfg.num_heads, cfg.head_dim, stream);
+    }
+}
+
 void QuantStep::clear() {
     entries.clear();
     appends.clear();
@@ -180,6 +193,7 @@ Result<void> QuantStep::appendOne(KVCacheManager &mgr, int layer_begin, int num_
         const QuantView w = mgr.quantView(layer_begin + 1);
         steps = {w.tiles - v.tiles, w.scales - v.scales, w.open - v.open};
     }
+    zero_unbrought(mgr, appends, layer_begin, num_layers, stream);
     launch_quant_append_one(v, steps, appends, num_layers, cfg.num_heads, cfg.head_dim, new_k, new_v, stream);
     noteAppends(mgr, layer_begin, num_layers);
     return Result<void>::ok();
@@ -189,6 +203,7 @@ Result<void> QuantStep::append(const char *who, KVCacheManager &mgr, int layer_i
                                hipStream_t stream) {
     if (std::string err = check(who, mgr, {new_k, new_v}); !err.empty()) return Result<void>::err(err);
     const KVCacheConfig &cfg = mgr.getConfig();
+    zero_unbrought(mgr, appends, layer_idx, 1, stream);
     launch_quant_append(mgr.quantView(layer_idx), appends, cfg.num_heads, cfg.head_dim, new_k, new_v, stream);
     noteAppends(mgr, layer_idx, 1);
     return Result<void>::ok();
@@ -207,6 +222,7 @@ Result<void> QuantStep::attention(const char *who, KVCacheManager &mgr, int laye
     float            *ws = work.get(floats);
     const QuantView   v = mgr.quantView(layer_idx);
     // (behind the checks: a refused call has appended nothing)
+    if (new_k) zero_unbrought(mgr, appends, layer_idx, 1, stream);
     if (new_k && apart) launch_quant_append(v, appends, cfg.num_heads, cfg.head_dim, new_k, new_v, stream);
     QuantCall c;
     c.q = q;

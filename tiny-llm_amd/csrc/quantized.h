@@ -19,6 +19,11 @@ std::string check_quant_call(const char *who, const KVCacheManager &mgr, std::in
 // Tokens that a sequence's cache holds, appended ones that it did not advance over included.
 int held_tokens(const KVCacheManager &mgr, int seq_id, int slot);
 
+// Ahead of an append to these layers: what a sequence advanced over in its open group though nobody brought it,
+// behind the last append to the layer, becomes zeros there.
+void zero_unbrought(const KVCacheManager &mgr, const std::vector<QuantAppend> &appends, int layer_begin, int num_layers,
+                    hipStream_t stream);
+
 struct QuantStep {
     std::vector<QuantEntry>  entries; // in the batch's order
     std::vector<QuantAppend> appends;

@@ -123,7 +123,8 @@ class KVCacheManager {
     // rejected), to a multiple of 32, within the group in which the append began or the one
     // in which it ended; elsewhere the rows that the open group needs are gone, and
     // advanceSeqLen refuses.  So it does beyond the group in which the last append ended while
-    // that is open: its tokens are in fp16 there, and would never be read again.
+    // that is open: its tokens are in fp16 there, and would never be read again.  Tokens that a sequence
+    // advanced over though nobody appended them count as zeros in a group that an append completes.
     static Result<std::unique_ptr<KVCacheManager>> createQuantized(const KVCacheConfig &config,
                                                                    int block_tokens, int num_blocks);
     bool   isQuantized() const noexcept { return quantized_; }
