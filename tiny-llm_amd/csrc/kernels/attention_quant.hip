@@ -20,9 +20,9 @@
 // without, 131072 alone 51.3 and 50.6, and without them outputs are 2.9e-4 off, of which their own rounding is 2.1e-4.
 // The open group (fp16, at most 31 tokens), and the one that the call's token closes, is a step of its
 // own of one wave, the one with the fewest others.
-// Measured, 8 kv heads of 128: 64 x 8192 tokens, groups of 4, 161-171 us, 6.3-6.7 TB/s (counters: 1.08 GB read,
-// the cache's own size); 96 ragged ones of 8, 11 million tokens times heads in all 110-116 us and 5 us for the join;
-// 1 x 131072 44 and 5; four sequences of 8 x 64 6.4 us, of which the launch is most.  What did not
+// Measured, 8 kv heads of 128: 64 x 8192 tokens, groups of 4, 163-182 us by clock, a call 169, 6.4 TB/s (counters: 1.08 GB
+// read, the cache's own size); 96 ragged ones of 8, 11 million tokens times heads in all 110-119 us and 5 us for the join;
+// 1 x 131072 42-45 and 5; four sequences of 8 x 64 6.6 us, of which the launch is most.  What did not
 // help: loads that stay in the caches (187 us for 175), one group a step, tiles in another order per workgroup,
 // more workgroups a CU.
 #include "quant_device.h"

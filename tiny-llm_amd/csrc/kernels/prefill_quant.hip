@@ -14,14 +14,18 @@
 //   K   whole numbers, exact in fp16; a group's scale meets the scores, in the softmax's fma
 //   V   times the scale's first 4 bits, exact in fp16 too (7 + 4 bits); what the scale is
 //       more than that, below 1.125 times, meets the weights in the softmax's exponent, and
-//       the row sums are freed of it.  So the weights' rounding to fp16 (2^-11, with errors
-//       of either sign) is all that there is.  Scaling the products instead would cost as
+//       the row sums are freed of it.  Scaling the products instead would cost as
 //       much as the softmax.  (V times the whole scale, rounded: 564 us below in place of 570, and the
 //       error of outputs 3.6e-4 in place of 2.9e-4, of which the outputs' own rounding is 2.1e-4)
+//   P   rounded to fp16, 2^-11 with errors of either sign, and summed as rounded: with V's rounding below
+//       scales of 2^-14 (scale_values) all that there is between the stored numbers and the output's
+//       rounding.  The lower halves as a second product, as in attention_quant.hip, would take the
+//       error from 2.9e-4 to 2.1e-4, and 8192 tokens from 594 us to 782, 4 x 400 .. 512 over 2500 .. 6000 from 181
+//       to 236; at head_dim 64 they do not fit the 128 registers.
 //   S^T = K Q^T, O^T += V^T P^T by v_mfma_f32_16x16x32_f16 as in attention_quant.hip; the row
 //   sums of P by a product with ones
-// 8192 tokens, 32 heads over 8 of 128: 557 us, 0.99 PFLOP/s (0.91 on another card, where a large
-// fp16 product takes 1.10 in place of 1.15).  Of a SIMD's cycles MFMA takes 42%, VALU 40%; the LDS is read
+// 8192 tokens, 32 heads over 8 of 128: 566-618 us by card and clock, 0.89-0.97 PFLOP/s (a large fp16 product takes
+// 1.10-1.17).  Of a SIMD's cycles MFMA takes 38-41%, VALU 37-40%; the LDS is read
 // 40% of the time, without bank conflicts.  What is left are the two waves of a SIMD waiting for each
 // other at barriers and for operands: a third needs 168 registers, and a wave has 219.
 // Tried and slower: eight waves of which four multiply while four do their softmax (636),
@@ -77,8 +81,9 @@ template <int S> __device__ __forceinline__ float xor_lane_max(float x) {
 __device__ __forceinline__ float coarse(float s) { return __uint_as_float(__float_as_uint(s) & 0xFFF00000u); }
 
 // A group's values in fp16 from its whole numbers and a scale of 4 bits: exact where the scale
-// is a normal fp16 number; a smaller one by way of its 2^17-fold (the result is then rounded
-// where it is subnormal).
+// is a normal fp16 number; a smaller one by way of its 2^17-fold.  The result is then rounded
+// where it is subnormal, by at most 2^-25, and the weights' part of 1 (1.125 with the scale's rest) of
+// that in an output is no more than half the last place of the smallest fp16 numbers.
 constexpr uint32_t kLeastHalf = 0x38800000u, kInfinite = 0x7F800000u; // bits of 2^-14, and of infinity
 template <bool SMALL> __device__ __forceinline__ void scale_values(u32x4 &x, uint32_t scale_bits) {
     const bool     twice = SMALL && scale_bits < kLeastHalf;
