@@ -160,7 +160,7 @@ int tl_kv_append(tl_kv_manager *mgr, int seq_id, int layer, const void *new_k, c
 
 int tl_kv_advance(tl_kv_manager *mgr, int seq_id, int num_tokens) {
     if (!mgr) return fail(TL_ERR_INVALID, "tl_kv_advance: null manager");
-    return status(mgr->m->advanceSeqLen(seq_id, num_tokens));
+    return guarded([&] { return status(mgr->m->advanceSeqLen(seq_id, num_tokens)); });
 }
 
 int tl_kv_seq_len(const tl_kv_manager *mgr, int seq_id) { return mgr ? mgr->m->getSeqLen(seq_id) : 0; }
